@@ -491,6 +491,125 @@ int kq_moe_ffn_dev(const kq_moe_ffn* f, const float* xn, float* x, int B, int* s
 #define KQ_FFN_GROUP_LAUNCH 8
 int kq_moe_ffn_last_path(void);
 
+/* ------------------------------------------- around the products
+ * The row operators of a decode step that lie next to its products: the
+ * norm before them (to binary32 or to the int8 rows that they read), products
+ * with 4-bit weights and plain group scales, and the check of drafted tokens
+ * after the LM head.  Device pointers, enqueue only, on any stream; nothing
+ * is allocated and no library scratch is used: what a call needs beside its
+ * operands is device memory that the caller passes (`work`), which calls that
+ * may overlap in time must not share.  -1 with a message on a bad argument
+ * or a launch error.  No counterpart as one call in the reference. */
+
+/* RMS norm of B rows of K values, with the residual's addition before it:
+ *   s = fl(x + resid)                       (x itself when resid is NULL)
+ *   y = fl(s * (sum s^2 / K + eps)^-1/2 * weight)
+ * The squares, their sum and the products are binary64; s and y are rounded
+ * once.  `sum` receives s (NULL: not written), `weight` holds K values (NULL:
+ * ones).  group == 0 writes y; group 16 or 32 writes y as int8 per group of
+ * that many values (K % group == 0), as kq_quantize_x_q8_dev does with the
+ * binary32 y, bit for bit: xq B rows of K bytes, xscale and xsum (may be NULL)
+ * B rows of K / group, and y too unless it is NULL; the rows must then be
+ * finite.  Strides are in elements between rows (0: K).  Any K and alignment
+ * of 4 bytes (16-byte aligned rows are the fast case); xq 4-byte aligned.
+ * sum may be the rows of x or of resid, and y may be too, but not sum's;
+ * otherwise the operands do not overlap. */
+typedef struct kq_rmsnorm {
+    int B, K;
+    float eps;
+    int group;
+    const float* x;
+    const float* resid;
+    const float* weight;
+    float* sum;
+    float* y;
+    int64_t x_stride, resid_stride, sum_stride, y_stride;
+    int8_t* xq;
+    float* xscale;
+    int32_t* xsum;
+} kq_rmsnorm;
+int kq_rmsnorm_dev(const kq_rmsnorm* a, kq_stream stream);
+
+/* A matrix of 4-bit weights with group scales, in planes: row n is K / 2
+ * bytes at q + n * K / 2, weight 2j in the low half of byte j and 2j + 1 in
+ * its high half; each `group` consecutive weights of a row (a multiple of 32
+ * that divides K) share a scale and a zero point:
+ *   w[n][k] = scales[n][k / group] * (q[n][k] - zeros[n][k / group])
+ * scales: N rows of K / group values of scale_type (KQ_TYPE_F16, KQ_TYPE_BF16
+ * or KQ_TYPE_F32); zeros: N rows of K / group bytes, or NULL: all 8.
+ * K % 32 == 0, any N; q is 16-byte aligned, scales to their own size. */
+#define KQ_TYPE_BF16    30      /* of scales only */
+typedef struct kq_w4 {
+    int N, K, group, scale_type;
+    const uint8_t* q;
+    const void* scales;
+    const uint8_t* zeros;
+} kq_w4;
+
+/* y[b] = add[b] + W . x[b] for b < B: B rows of K values, N outputs each
+ * (add NULL: nothing added; it may be y itself).  x and xq are 16-byte
+ * aligned.  work: kq_w4_workspace_bytes of device memory, 256-byte aligned
+ * (0 bytes: may be NULL).
+ * The result is within 2^-20 * sum_k |w_k| max|x| of the exact one, the
+ * maximum over the 32 values of x that k lies in; it does not depend on
+ * other rows' values.  x must be finite. */
+int kq_w4_gemv_dev(const kq_w4* w, const float* x, const float* add, float* y, int B, void* work,
+                   int64_t work_bytes, kq_stream stream);
+
+/* The same product on int8 rows: x[b][k] = xq[b][k] * xscale[b][k / 32], as
+ * kq_rmsnorm_dev (group 32) and kq_quantize_x_q8_dev write them. */
+int kq_w4_gemv_q8_dev(const kq_w4* w, const int8_t* xq, const float* xscale, const float* add,
+                      float* y, int B, void* work, int64_t work_bytes, kq_stream stream);
+
+/* Bytes of workspace the two calls need for B rows (q8 != 0: the second),
+ * or -1. */
+int64_t kq_w4_workspace_bytes(const kq_w4* w, int B, int q8);
+
+/* Verification of drafted tokens (speculative decode) for S sequences: each
+ * has up to T drafted tokens tokens[s][0..n_draft[s]) (n_draft NULL: T each;
+ * values outside 0..T are clamped) and the target's distributions p_i over V
+ * tokens, row i (at target + s * target_seq + i * target_row) being the one
+ * drafted token i is held against, with one more row after the last.
+ *   accepted: token i iff all before it are and u[s][i] * q_i(t) < p_i(t)
+ *   next:     after n accepted tokens of n_draft, drawn with u[s][T] from
+ *             max(p_n - q_n, 0) when n < n_draft (from p_n should that be
+ *             zero everywhere), else from p_n: the lowest v whose running
+ *             sum of weights is above u[s][T] times their total
+ * q_i is the draft's distribution (rows as the target's, T of them), or with
+ * draft NULL all on the drafted token (n-gram drafts): accepted iff u < p,
+ * and the next one is drawn from p without it.
+ * flags 0: the rows are probabilities; KQ_VERIFY_LOGITS: logits, p =
+ * softmax(inv_temp * row), q likewise; KQ_VERIFY_GREEDY: rows of either kind,
+ * draft, u and inv_temp unused: accepted iff the token is its row's maximum
+ * (the lowest of equals), the next one row n's maximum.
+ * Writes n_accept[s] and out[s][0..T]: the accepted tokens, the next one, then
+ * -1.  Computed in binary64 from the binary32 rows.  Tokens outside 0..V-1
+ * are refused; a NaN has no weight; a row with no weight at all (or with an
+ * infinite logit above all) gives next = -1; u >= 1 or NaN draws the last
+ * token with any weight.  u: S rows of T + 1.  Strides are in elements (0:
+ * rows of V, sequences after each other).  T == 0 draws one token from each row. */
+#define KQ_VERIFY_LOGITS 1
+#define KQ_VERIFY_GREEDY 2
+#define KQ_VERIFY_MAX_DRAFT 63
+#define KQ_VERIFY_MAX_ROWS 65535    /* S * (2 T + 1) */
+#define KQ_VERIFY_MAX_VOCAB (1 << 28)
+typedef struct kq_spec_verify {
+    int S, T, V, flags;
+    float inv_temp;
+    const float* target;
+    const float* draft;
+    int64_t target_row, target_seq, draft_row, draft_seq;
+    const int32_t* tokens;
+    const int32_t* n_draft;
+    const float* u;
+    int32_t* n_accept;
+    int32_t* out;
+} kq_spec_verify;
+
+/* Bytes of workspace of a call (256-byte aligned device memory), or -1. */
+int64_t kq_spec_verify_workspace_bytes(const kq_spec_verify* v);
+int kq_spec_verify_dev(const kq_spec_verify* v, void* work, int64_t work_bytes, kq_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

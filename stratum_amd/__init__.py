@@ -32,6 +32,7 @@ TYPE_Q3_K = 11
 TYPE_Q4_K = 12
 TYPE_Q5_K = 13
 TYPE_Q6_K = 14
+TYPE_BF16 = 30     # of group scales only
 TYPE_Q2K_NIB = 42
 # int8-activation mode flag (KQ_INT8_ACT): TYPE_Q4_K | INT8_ACT, and likewise for
 # Q6_K, Q5_K, Q3_K and Q8_0
@@ -59,6 +60,8 @@ EXPORTS = (
     "kq_quantize_x_q8_dev", "kq_softmax_dev", "kq_swiglu_dev", "kq_moe_combine_dev",
     "kq_moe_ffn_workspace_bytes", "kq_moe_ffn_dev", "kq_gemv_multix_mfma_workspace_bytes",
     "kq_reserve_mfma_workspace", "kq_scratch_bytes", "kq_moe_ffn_last_path",
+    "kq_rmsnorm_dev", "kq_w4_gemv_dev", "kq_w4_gemv_q8_dev", "kq_w4_workspace_bytes",
+    "kq_spec_verify_dev", "kq_spec_verify_workspace_bytes",
 )
 # include/kq_gguf.h (bound in stratum_amd/gguf.py)
 GGUF_EXPORTS = (
@@ -182,6 +185,46 @@ class KqMoeFfn(ctypes.Structure):
     ]
 
 
+class KqRmsnorm(ctypes.Structure):
+    """kq_rmsnorm: RMS norm of rows, to binary32 or int8."""
+
+    _fields_ = [
+        ("B", ctypes.c_int), ("K", ctypes.c_int), ("eps", ctypes.c_float),
+        ("group", ctypes.c_int), ("x", ctypes.c_void_p), ("resid", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p), ("sum", ctypes.c_void_p), ("y", ctypes.c_void_p),
+        ("x_stride", ctypes.c_int64), ("resid_stride", ctypes.c_int64),
+        ("sum_stride", ctypes.c_int64), ("y_stride", ctypes.c_int64),
+        ("xq", ctypes.c_void_p), ("xscale", ctypes.c_void_p), ("xsum", ctypes.c_void_p),
+    ]
+
+
+class KqW4(ctypes.Structure):
+    """kq_w4: a matrix of 4-bit weights with group scales, in planes."""
+
+    _fields_ = [
+        ("N", ctypes.c_int), ("K", ctypes.c_int), ("group", ctypes.c_int),
+        ("scale_type", ctypes.c_int), ("q", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+        ("zeros", ctypes.c_void_p),
+    ]
+
+
+# kq_spec_verify flags (include/kq_gemv.h)
+VERIFY_LOGITS, VERIFY_GREEDY = 1, 2
+
+
+class KqSpecVerify(ctypes.Structure):
+    """kq_spec_verify: drafted tokens against the target's distributions."""
+
+    _fields_ = [
+        ("S", ctypes.c_int), ("T", ctypes.c_int), ("V", ctypes.c_int), ("flags", ctypes.c_int),
+        ("inv_temp", ctypes.c_float), ("target", ctypes.c_void_p), ("draft", ctypes.c_void_p),
+        ("target_row", ctypes.c_int64), ("target_seq", ctypes.c_int64),
+        ("draft_row", ctypes.c_int64), ("draft_seq", ctypes.c_int64),
+        ("tokens", ctypes.c_void_p), ("n_draft", ctypes.c_void_p), ("u", ctypes.c_void_p),
+        ("n_accept", ctypes.c_void_p), ("out", ctypes.c_void_p),
+    ]
+
+
 def moe_op(qtype: int, n_out: int, k_in: int, w_ptrs, expert_stride: int, x_ptr: int,
            x_div: int, y_ptrs) -> KqMoeOp:
     op = KqMoeOp()
@@ -258,6 +301,15 @@ def lib() -> ctypes.CDLL:
     L.kq_moe_topk_dev.argtypes = [P, I, I, I, P, P, P]
     L.kq_moe_gemv_dev.argtypes = [ctypes.POINTER(KqMoeOp), P, I, I, I, P]
     L.kq_moe_gemv_routed_dev.argtypes = [ctypes.POINTER(KqMoeOp), P, I, I, I, P, P, P]
+    L.kq_rmsnorm_dev.argtypes = [ctypes.POINTER(KqRmsnorm), P]
+    W4P, VP, LL = ctypes.POINTER(KqW4), ctypes.POINTER(KqSpecVerify), ctypes.c_int64
+    L.kq_w4_gemv_dev.argtypes = [W4P, P, P, P, I, P, LL, P]
+    L.kq_w4_gemv_q8_dev.argtypes = [W4P, P, P, P, P, I, P, LL, P]
+    L.kq_w4_workspace_bytes.argtypes = [W4P, I, I]
+    L.kq_w4_workspace_bytes.restype = LL
+    L.kq_spec_verify_dev.argtypes = [VP, P, LL, P]
+    L.kq_spec_verify_workspace_bytes.argtypes = [VP]
+    L.kq_spec_verify_workspace_bytes.restype = LL
     _LIB = L
     return L
 
@@ -475,3 +527,83 @@ def moe_ffn_dev(f: KqMoeFfn, xn_ptr: int, x_ptr: int, B: int, sel_ptr: int, selw
                 work_ptr: int, work_bytes: int, stream: int | None = None) -> None:
     _check(lib().kq_moe_ffn_dev(ctypes.byref(f), xn_ptr, x_ptr, B, sel_ptr, selw_ptr, work_ptr,
                                 work_bytes, stream), "kq_moe_ffn_dev")
+
+
+def _bytes(n: int, what: str) -> int:
+    if n < 0:
+        msg = lib().kq_last_error().decode(errors="replace")
+        raise RuntimeError(f"{what} failed: {msg}")
+    return n
+
+
+def rmsnorm(B: int, K: int, eps: float, x_ptr: int, resid_ptr: int | None = None,
+            sum_ptr: int | None = None, weight_ptr: int | None = None, y_ptr: int | None = None,
+            group: int = 0, xq_ptr: int | None = None, xscale_ptr: int | None = None,
+            xsum_ptr: int | None = None, x_stride: int = 0, resid_stride: int = 0,
+            sum_stride: int = 0, y_stride: int = 0) -> KqRmsnorm:
+    a = KqRmsnorm()
+    a.B, a.K, a.eps, a.group = B, K, eps, group
+    a.x, a.resid, a.weight, a.sum, a.y = x_ptr, resid_ptr, weight_ptr, sum_ptr, y_ptr
+    a.xq, a.xscale, a.xsum = xq_ptr, xscale_ptr, xsum_ptr
+    a.x_stride, a.resid_stride, a.sum_stride, a.y_stride = (x_stride, resid_stride, sum_stride,
+                                                            y_stride)
+    return a
+
+
+def rmsnorm_dev(a: KqRmsnorm, stream: int | None = None) -> None:
+    """RMS norm of a.B rows, the residual added first (kq_rmsnorm_dev)."""
+    _check(lib().kq_rmsnorm_dev(ctypes.byref(a), stream), "kq_rmsnorm_dev")
+
+
+def w4(N: int, K: int, group: int, scale_type: int, q_ptr: int, scales_ptr: int,
+       zeros_ptr: int | None = None) -> KqW4:
+    w = KqW4()
+    w.N, w.K, w.group, w.scale_type = N, K, group, scale_type
+    w.q, w.scales, w.zeros = q_ptr, scales_ptr, zeros_ptr
+    return w
+
+
+def w4_workspace_bytes(w: KqW4, B: int, q8: bool = False) -> int:
+    return _bytes(lib().kq_w4_workspace_bytes(ctypes.byref(w), B, int(q8)),
+                  "kq_w4_workspace_bytes")
+
+
+def w4_gemv_dev(w: KqW4, x_ptr: int, y_ptr: int, B: int, work_ptr: int | None = None,
+                work_bytes: int = 0, add_ptr: int | None = None, stream: int | None = None) -> None:
+    """B rows of binary32 x times 4-bit weights with group scales."""
+    _check(lib().kq_w4_gemv_dev(ctypes.byref(w), x_ptr, add_ptr, y_ptr, B, work_ptr, work_bytes,
+                                stream), "kq_w4_gemv_dev")
+
+
+def w4_gemv_q8_dev(w: KqW4, xq_ptr: int, xscale_ptr: int, y_ptr: int, B: int,
+                   work_ptr: int | None = None, work_bytes: int = 0, add_ptr: int | None = None,
+                   stream: int | None = None) -> None:
+    """The same on int8 rows with a scale per 32 (kq_rmsnorm_dev, group 32)."""
+    _check(lib().kq_w4_gemv_q8_dev(ctypes.byref(w), xq_ptr, xscale_ptr, add_ptr, y_ptr, B,
+                                   work_ptr, work_bytes, stream), "kq_w4_gemv_q8_dev")
+
+
+def spec_verify(S: int, T: int, V: int, flags: int, target_ptr: int, tokens_ptr: int | None,
+                u_ptr: int | None, n_accept_ptr: int, out_ptr: int, draft_ptr: int | None = None,
+                n_draft_ptr: int | None = None, inv_temp: float = 1.0, target_row: int = 0,
+                target_seq: int = 0, draft_row: int = 0, draft_seq: int = 0) -> KqSpecVerify:
+    v = KqSpecVerify()
+    v.S, v.T, v.V, v.flags, v.inv_temp = S, T, V, flags, inv_temp
+    v.target, v.draft, v.tokens, v.n_draft, v.u = (target_ptr, draft_ptr, tokens_ptr, n_draft_ptr,
+                                                   u_ptr)
+    v.target_row, v.target_seq, v.draft_row, v.draft_seq = (target_row, target_seq, draft_row,
+                                                            draft_seq)
+    v.n_accept, v.out = n_accept_ptr, out_ptr
+    return v
+
+
+def spec_verify_workspace_bytes(v: KqSpecVerify) -> int:
+    return _bytes(lib().kq_spec_verify_workspace_bytes(ctypes.byref(v)),
+                  "kq_spec_verify_workspace_bytes")
+
+
+def spec_verify_dev(v: KqSpecVerify, work_ptr: int, work_bytes: int,
+                    stream: int | None = None) -> None:
+    """Accepted drafted tokens and the token after them (kq_spec_verify_dev)."""
+    _check(lib().kq_spec_verify_dev(ctypes.byref(v), work_ptr, work_bytes, stream),
+           "kq_spec_verify_dev")

@@ -121,6 +121,14 @@ int kqk_launch_mi8_moe(int type, const int* sel, int nm, int E, int nt, int x_di
 int kqk_launch_moe_group(const int* sel, int nm, int E, int nt, int x_div, int mch,
                          const void* w0, const void* w1, float* y0, float* y1, long estride,
                          void* groups, int* ng, hipStream_t st);
+/* the row operators around the products (kq_norm.hip, kq_w4.hip,
+ * kq_verify.hip): arguments checked and strides filled in by kq_step.c */
+int kqk_launch_rmsnorm(const kq_rmsnorm* a, hipStream_t st);
+int64_t kqk_w4_workspace(const kq_w4* w, int B, int q8, int n_cu);
+int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float* xs,
+                  const float* add, float* y, int B, void* work, int n_cu, hipStream_t st);
+int64_t kqk_verify_workspace(const kq_spec_verify* v);
+int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st);
 
 #ifdef __cplusplus
 }

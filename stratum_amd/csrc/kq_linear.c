@@ -235,6 +235,13 @@ static int kq_ready(void) {
     return 0;
 }
 
+/* for kq_step.c: the device is queried; its CU count.  Not exported. */
+__attribute__((visibility("hidden"))) int kq_device(int* n_cu) {
+    if (kq_ready()) return -1;
+    *n_cu = g_kq.n_cu;
+    return 0;
+}
+
 /* The library's own stream, used only by the host-pointer entry points
  * (created at their first call: the device-pointer entry points create
  * nothing).  A blocking stream at the default priority, so it orders with

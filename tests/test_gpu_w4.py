@@ -1,0 +1,256 @@
+"""kq_w4_gemv_dev and kq_w4_gemv_q8_dev against the products in 64 bits.
+
+Bounds, per output, with a = sum_k |s| |q - z| amax_k (amax_k: the largest |x|
+of the 32 values that k lies in): a binary32 x enters with 23 bits below a
+power of two not above 2 amax (an error of at most 2^-23 amax); a block of 32
+products is an integer sum, rounded at most 5 times on its way (its planes'
+sum, the zero point's part, the scales); the blocks' sums are added in any
+order, at most K / 32 additions, then `add`: in all
+(K / 32 + 8) 2^-24 a + 2^-24 |y|."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import stratum_amd as K
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+TYPES = {"f16": (K.TYPE_F16, torch.float16), "bf16": (K.TYPE_BF16, torch.bfloat16), "f32": (K.TYPE_F32, torch.float32)}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    K.lib()
+    yield
+    torch.cuda.synchronize()
+
+
+def st():
+    return torch.cuda.current_stream().cuda_stream
+
+
+class Case:
+    """A matrix, B rows of x, and the exact products (binary64, on the CPU)."""
+
+    def __init__(self, N, Kd, B, g, scale="f16", zeros=False, q8=False, seed=0, xscale=1.0):
+        r = np.random.default_rng(1000 * seed + N + 7 * Kd + 13 * B + g)
+        self.N, self.K, self.B, self.g, self.q8 = N, Kd, B, g, q8
+        q = r.integers(0, 256, (N, Kd // 2), dtype=np.uint8)
+        s = torch.from_numpy((0.004 * np.exp(0.5 * r.standard_normal((N, Kd // g)))).astype(np.float32))
+        s[r.random((N, Kd // g)) < 0.05] *= -1
+        s = s.to(TYPES[scale][1])
+        z = r.integers(0, 16, (N, Kd // g), dtype=np.uint8) if zeros else None
+        x = (r.standard_normal((B, Kd)) * xscale).astype(np.float32)
+        x[:, r.random(Kd) < 0.01] *= 30
+        if Kd > 64:
+            x[:, 32:64] = 0                      # a block of zeros
+        self.dq, self.ds = torch.from_numpy(q).cuda(), s.cuda()
+        self.dz = torch.from_numpy(z).cuda() if zeros else None
+        n = np.stack([q & 15, q >> 4], -1).reshape(N, Kd // g, g).astype(np.float64)
+        n -= 8.0 if z is None else z[:, :, None]
+        self.W = (n * s.double().numpy()[:, :, None]).reshape(N, Kd)
+        amax = np.abs(x).reshape(B, -1, 32).max(-1)
+        if q8:
+            sc = (amax / np.float32(127)).astype(np.float32)
+            xq = np.where(sc[:, :, None] > 0, np.rint(x.reshape(B, -1, 32) / np.where(sc > 0, sc, 1)[:, :, None]), 0)
+            xq = np.clip(xq, -128, 127).astype(np.int8).reshape(B, Kd)
+            if Kd > 64:
+                xq[:, :32] = np.where(r.random((B, 32)) < 0.5, -128, 127)    # the ends of the type
+            x = xq.astype(np.float64) * np.repeat(sc, 32, 1).astype(np.float64)
+            amax = sc * 128.0
+            self.dxq, self.dxs = torch.from_numpy(xq).cuda(), torch.from_numpy(sc).cuda()
+        else:
+            self.dx = torch.from_numpy(x).cuda()
+        self.exact = x.astype(np.float64) @ self.W.T
+        self.a = np.repeat(amax, 32, 1).astype(np.float64) @ np.abs(self.W).T
+        self.desc = K.w4(N, Kd, g, TYPES[scale][0], self.dq.data_ptr(), self.ds.data_ptr(),
+                         self.dz.data_ptr() if zeros else None)
+        self.nb = K.w4_workspace_bytes(self.desc, B, q8)
+        self.work = torch.full((self.nb + 256,), 0xA5, dtype=torch.uint8, device="cuda")
+
+    def call(self, y, add=None, stream=None, work=None):
+        args = (y.data_ptr(), self.B, (self.work if work is None else work).data_ptr(), self.nb,
+                add.data_ptr() if add is not None else None, st() if stream is None else stream)
+        if self.q8:
+            K.w4_gemv_q8_dev(self.desc, self.dxq.data_ptr(), self.dxs.data_ptr(), *args)
+        else:
+            K.w4_gemv_dev(self.desc, self.dx.data_ptr(), *args)
+
+    def tol(self, y):
+        return (self.K / 32 + 8) * 2.0 ** -24 * self.a + 2.0 ** -24 * np.abs(y) + 1e-40
+
+    def check(self, add=None):
+        y = torch.full((self.B * self.N + 32,), float("nan"), device="cuda")
+        self.call(y, add)
+        torch.cuda.synchronize()
+        got = y[:self.B * self.N].cpu().numpy().reshape(self.B, self.N).astype(np.float64)
+        want = self.exact if add is None else self.exact + add.cpu().numpy().reshape(self.B, self.N)
+        bad = ~(np.abs(got - want) <= self.tol(want))
+        assert not bad.any(), (np.argwhere(bad)[:5], got[bad][:5], want[bad][:5])
+        assert torch.isnan(y[self.B * self.N:]).all()
+        assert (self.work[self.nb:] == 0xA5).all()
+        return y
+
+
+SHAPES = [(1, 32, 32), (1, 64, 64), (5, 96, 32), (16, 128, 128), (17, 160, 160), (33, 256, 64), (64, 1024, 32),
+          (100, 1056, 352), (257, 2048, 128), (31, 4096, 4096), (1000, 640, 64), (130, 5120, 128), (40, 17408, 64),
+          (19, 2720, 32), (3000, 512, 256)]
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("N,Kd,g", SHAPES)
+@pytest.mark.parametrize("B", [1, 2, 3, 4, 5, 8])
+def test_products(N, Kd, g, B, q8):
+    Case(N, Kd, B, g, zeros=(N + B) % 2 == 0, q8=q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [6, 7, 9, 12, 15, 16, 17, 31, 32, 33, 48, 63, 64, 65, 130])
+@pytest.mark.parametrize("N,Kd,g", [(77, 352, 32), (208, 1280, 128), (19, 3104, 3104)])
+def test_many_rows(N, Kd, g, B, q8):
+    Case(N, Kd, B, g, zeros=B % 2 == 1, q8=q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("scale", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("g", [32, 64, 96, 128, 192, 256, 384])
+@pytest.mark.parametrize("B", [1, 3, 11])
+def test_groups_and_scale_types(B, g, zeros, scale, q8):
+    Case(53, 2304, B, g, scale, zeros, q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("N,Kd,B", [(151, 57344, 1), (50, 65536, 3), (20, 90112, 9), (7, 131072 + 32, 2), (6, 131072, 20)])
+def test_long_rows(N, Kd, B, q8):
+    Case(N, Kd, B, 32, q8=q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 2, 5, 16])
+def test_many_rows_of_weights(B, q8):
+    """More rows than any grid has waves, the last ones cut off mid-tile."""
+    Case(70001, 64, B, 32, zeros=True, q8=q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 3, 20])
+def test_add(B, q8):
+    c = Case(300, 768, B, 128, q8=q8)
+    add = torch.from_numpy(np.random.default_rng(5).standard_normal(B * 300).astype(np.float32)).cuda()
+    y = c.check(add)
+    over = add.clone()                           # in place
+    c.call(over, over)
+    torch.cuda.synchronize()
+    assert torch.equal(over, y[:B * 300])
+
+
+@pytest.mark.parametrize("xscale", [1e-30, 1e-3, 1e4, 1e30])
+@pytest.mark.parametrize("B", [1, 6])
+def test_far_x(B, xscale):
+    """x far from 1, each block with its own power of two."""
+    Case(64, 1024, B, 64, "f32", xscale=xscale).check()
+
+
+@pytest.mark.parametrize("B", [1, 6])
+def test_wide_blocks(B):
+    """Values of one block of 32 that lie 2^20 apart: the bound counts the largest."""
+    c = Case(64, 512, B, 32)
+    x = c.dx.cpu().numpy()
+    x[:, ::3] *= np.float32(2.0 ** -20)
+    c.dx = torch.from_numpy(x).cuda()
+    c.exact = x.astype(np.float64) @ c.W.T
+    c.a = np.repeat(np.abs(x).reshape(B, -1, 32).max(-1), 32, 1).astype(np.float64) @ np.abs(c.W).T
+    c.check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_rows_do_not_depend_on_each_other(q8):
+    """A non-finite row of x leaves the others' bits alone (within one B)."""
+    for B in (2, 4, 12):
+        c = Case(90, 640, B, 64, q8=q8)
+        y = c.check()[:B * 90].view(B, 90).clone()
+        if q8:
+            c.dxs[1, 3] = float("nan")
+        else:
+            c.dx[1, 100] = float("inf")
+        y2 = torch.empty(B, 90, device="cuda")
+        c.call(y2)
+        torch.cuda.synchronize()
+        keep = [b for b in range(B) if b != 1]
+        assert torch.equal(y[keep].view(torch.int32), y2[keep].view(torch.int32))
+        assert not torch.isfinite(y2[1]).any()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 4, 16])
+def test_same_bits_again_captured_and_on_two_streams(B, q8):
+    """Repeated calls, replays of a graph and overlapping calls on two streams
+    with workspaces of their own give the same bits."""
+    c = [Case(500, 2048, B, 128, q8=q8, seed=i) for i in range(2)]
+    n = B * 500
+    first = [k.check()[:n].clone() for k in c]
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for rnd in range(4):
+        for i in range(2):
+            with torch.cuda.stream(side[i]):
+                y = torch.full((n,), float("nan"), device="cuda")
+                c[i].call(y, stream=side[i].cuda_stream)
+                outs.append((i, y))
+    torch.cuda.synchronize()
+    for i, y in outs:
+        assert torch.equal(y, first[i])
+    graph, ys = torch.cuda.CUDAGraph(), [torch.empty(n, device="cuda") for _ in c]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for k, y in zip(c, ys):
+            k.call(y)
+    for rnd in range(3):
+        for k, y in zip(c, ys):
+            y.fill_(float("nan"))
+            k.work.fill_(rnd)
+        graph.replay()
+        torch.cuda.synchronize()
+        for i, y in enumerate(ys):
+            assert torch.equal(y, first[i])
+            z = torch.empty(n, device="cuda")      # eager work between the replays
+            c[i].call(z)
+            assert torch.equal(z, first[i])
+
+
+def test_norm_to_product():
+    """The norm's int8 rows go to the product as they are."""
+    N, Kd, B = 200, 1024, 5
+    c = Case(N, Kd, B, 128, q8=True)
+    x = torch.randn(B, Kd, device="cuda")
+    K.rmsnorm_dev(K.rmsnorm(B, Kd, 1e-6, x.data_ptr(), group=32, xq_ptr=c.dxq.data_ptr(),
+                            xscale_ptr=c.dxs.data_ptr()), st())
+    torch.cuda.synchronize()
+    sc = c.dxs.cpu().numpy()
+    xv = c.dxq.cpu().numpy().astype(np.float64) * np.repeat(sc, 32, 1)
+    c.exact, c.a = xv @ c.W.T, np.repeat(sc * 128.0, 32, 1) @ np.abs(c.W).T
+    c.check()
+
+
+def test_refuses_a_short_workspace():
+    for B in (1, 8, 16, 64):
+        for q8 in (False, True):
+            c = Case(64, 1024, B, 128, q8=q8)
+            if not c.nb:
+                continue
+            y = torch.full((B, 64), 3.0, device="cuda")
+            for work, nb in ((None, c.nb), (c.work.data_ptr(), c.nb - 1), (c.work.data_ptr() + 16, c.nb)):
+                d = ctypes.byref(c.desc)
+                L = K.lib()
+                rc = (L.kq_w4_gemv_q8_dev(d, c.dxq.data_ptr(), c.dxs.data_ptr(), None, y.data_ptr(), B, work, nb, st())
+                      if q8 else L.kq_w4_gemv_dev(d, c.dx.data_ptr(), None, y.data_ptr(), B, work, nb, st()))
+                assert rc == -1 and b"workspace" in L.kq_last_error()
+            torch.cuda.synchronize()
+            assert (y == 3.0).all()
