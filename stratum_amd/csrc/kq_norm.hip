@@ -25,60 +25,162 @@ __device__ __forceinline__ double wg_sum(double v, double* sm) {
     return v;
 }
 
-// The int8 group of G values that G consecutive lanes hold (one each):
-// kq_quantize_kernel's arithmetic.
-template <int G>
-__device__ __forceinline__ void store_group(const kq_rmsnorm& a, long row, int i, float y) {
-    float amax = fabsf(y);
+template <int V> struct Vec;
+template <> struct Vec<1> { typedef float f __attribute__((ext_vector_type(1))); };
+template <> struct Vec<4> { typedef float f __attribute__((ext_vector_type(4))); };
+
+// The int8 group of G values that G / V consecutive lanes hold (lane t's
+// first is value i): kq_quantize_kernel's arithmetic.
+template <int G, int V>
+__device__ __forceinline__ void store_group(const kq_rmsnorm& a, long row, int i,
+                                            const typename Vec<V>::f y) {
+    float amax = fabsf(y[0]);
 #pragma unroll
-    for (int off = 1; off < G; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+    for (int e = 1; e < V; e++) amax = fmaxf(amax, fabsf(y[e]));
+#pragma unroll
+    for (int off = 1; off < G / V; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
     const float scale = __fdiv_rn(amax, 127.0f);
     const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-    const int q = min(127, max(-128, __float2int_rn(y * inv)));
-    int sum = q;
+    int sum = 0;
+    uint32_t w = 0;
 #pragma unroll
-    for (int off = 1; off < G; off <<= 1) sum += __shfl_xor(sum, off);
+    for (int e = 0; e < V; e++) {
+        const int q = min(127, max(-128, __float2int_rn(y[e] * inv)));
+        sum += q;
+        w |= ((uint32_t)q & 0xffu) << (8 * e);
+    }
+    if (a.xsum) {
+#pragma unroll
+        for (int off = 1; off < G / V; off <<= 1) sum += __shfl_xor(sum, off);
+    }
     if (i >= a.K) return;
-    a.xq[row * a.K + i] = (int8_t)q;
+    if (V == 4)
+        *reinterpret_cast<uint32_t*>(a.xq + row * a.K + i) = w;
+    else
+        a.xq[row * a.K + i] = (int8_t)w;
     if (i % G == 0) {
-        a.xscale[row * (a.K / G) + i / G] = scale;
-        if (a.xsum) a.xsum[row * (a.K / G) + i / G] = sum;
+        const long g = row * (a.K / G) + i / G;
+        a.xscale[g] = scale;
+        if (a.xsum) a.xsum[g] = sum;
     }
 }
 
-__global__ __launch_bounds__(256) void kq_rmsnorm_kernel(kq_rmsnorm a) {
-    __shared__ double sm[4];
+template <int V>
+__device__ __forceinline__ void store_rows(const kq_rmsnorm& a, long row, int i,
+                                           const typename Vec<V>::f y) {
+    if (a.y && i < a.K)
+        *reinterpret_cast<typename Vec<V>::f*>(a.y + row * a.y_stride + i) = y;
+    if (a.group == 32) store_group<32, V>(a, row, i, y);
+    if (a.group == 16) store_group<16, V>(a, row, i, y);
+}
+
+// V consecutive values a lane and step; NV steps hold the row in registers
+// (NV V blockDim >= K), so that it is read once.  NV = 0: rows of any length,
+// read a second time (from `sum`, when that is written: it may be x's rows).
+template <int V, int NV>
+__global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
+    using F = typename Vec<V>::f;
+    // the weights are asked for before the sum, where registers allow it
+    constexpr bool HOLD_W = V * NV <= 16;
+    __shared__ double sm[16];
     const long row = blockIdx.x;
+    const int T = blockDim.x, i0 = V * threadIdx.x, K = a.K;
     const float* x = a.x + row * a.x_stride;
     const float* r = a.resid ? a.resid + row * a.resid_stride : nullptr;
     float* s = a.sum ? a.sum + row * a.sum_stride : nullptr;
-    float* y = a.y ? a.y + row * a.y_stride : nullptr;
+    const F zero = (F)0.0f;
+    F v[NV ? NV : 1], w[NV ? NV : 1];
     double sq = 0.0;
-    for (int i = threadIdx.x; i < a.K; i += 256) {
-        const float v = r ? x[i] + r[i] : x[i];
-        if (s) s[i] = v;
-        sq = sq + (double)v * (double)v;
+    auto take = [&](F t, int i) {
+        if (s) *reinterpret_cast<F*>(s + i) = t;
+#pragma unroll
+        for (int e = 0; e < V; e++) sq = fma((double)t[e], (double)t[e], sq);
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int i = i0 + j * V * T;
+            v[j] = i < K ? *reinterpret_cast<const F*>(x + i) : zero;
+        }
+        if (r) {
+#pragma unroll
+            for (int j = 0; j < NV; j++) {
+                const int i = i0 + j * V * T;
+                if (i < K) v[j] = v[j] + *reinterpret_cast<const F*>(r + i);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int i = i0 + j * V * T;
+            if (HOLD_W && a.weight) w[j] = i < K ? *reinterpret_cast<const F*>(a.weight + i) : zero;
+            if (i < K) take(v[j], i);
+        }
+    } else {
+        for (int i = i0; i < K; i += V * T) {
+            F t = *reinterpret_cast<const F*>(x + i);
+            if (r) t = t + *reinterpret_cast<const F*>(r + i);
+            take(t, i);
+        }
     }
     sq = wg_sum(sq, sm);
-    const double inv = 1.0 / sqrt(sq / (double)a.K + (double)a.eps);
-    for (int i0 = 0; i0 < a.K; i0 += 256) {
-        const int i = i0 + threadIdx.x;
-        float v = 0.0f;
-        if (i < a.K) {
-            v = s ? s[i] : r ? x[i] + r[i] : x[i];
-            const double n = (double)v * inv;
-            v = (float)(a.weight ? n * (double)a.weight[i] : n);
-            if (y) y[i] = v;
+    const double inv = 1.0 / sqrt(sq / (double)K + (double)a.eps);
+    auto finish = [&](F t, F g, int i) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const double n = (double)t[e] * inv;
+            t[e] = (float)(a.weight ? n * (double)g[e] : n);
         }
-        if (a.group == 32) store_group<32>(a, row, i, v);
-        if (a.group == 16) store_group<16>(a, row, i, v);
+        store_rows<V>(a, row, i, t);
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) {
+            const int i = i0 + j * V * T;
+            F g = zero;
+            if (a.weight) g = HOLD_W ? w[j] : i < K ? *reinterpret_cast<const F*>(a.weight + i) : zero;
+            finish(v[j], g, i);
+        }
+    } else {
+        for (int j = 0; j < K; j += V * T) {
+            const int i = i0 + j;
+            F t = zero, g = zero;
+            if (i < K) {
+                t = *reinterpret_cast<const F*>((s ? s : x) + i);
+                if (!s && r) t = t + *reinterpret_cast<const F*>(r + i);
+                if (a.weight) g = *reinterpret_cast<const F*>(a.weight + i);
+            }
+            finish(t, g, i);
+        }
     }
+}
+
+template <int V>
+int launch(const kq_rmsnorm& a, hipStream_t st) {
+    const int nv = (a.K + V - 1) / V;
+    // Few rows: one or two steps on as many lanes as a workgroup has (latency);
+    // else four, in fewer lanes, so that a CU holds several rows.
+    constexpr int MOST = V == 4 ? 4 : 8;       // (8 steps of 4 spill registers)
+    int steps = a.B <= 512 ? 1 : 4;
+    while (steps <= MOST && nv > 1024 * steps) steps *= 2;
+    const dim3 grid((unsigned)a.B);
+    const int per = steps <= MOST ? (nv + steps - 1) / steps : 1024;
+    const dim3 wg((unsigned)((per + 63) / 64 * 64));
+    if (steps == 1) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 1>), grid, wg, 0, st, a);
+    else if (steps == 2) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 2>), grid, wg, 0, st, a);
+    else if (steps == 4) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 4>), grid, wg, 0, st, a);
+    else if (steps == MOST) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, MOST>), grid, wg, 0, st, a);
+    else hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 0>), grid, wg, 0, st, a);
+    return (int)hipGetLastError();
 }
 
 }  // namespace
 
 extern "C" int kqk_launch_rmsnorm(const kq_rmsnorm* a, hipStream_t st) {
     if (a->B < 1 || a->K < 1) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL(kq_rmsnorm_kernel, dim3((unsigned)a->B), dim3(256), 0, st, *a);
-    return (int)hipGetLastError();
+    // four values a load where every row allows it
+    const uintptr_t p = (uintptr_t)a->x | (uintptr_t)a->resid | (uintptr_t)a->weight |
+                        (uintptr_t)a->sum | (uintptr_t)a->y;
+    const int64_t n = a->K | a->x_stride | (a->resid ? a->resid_stride : 0) |
+                      (a->sum ? a->sum_stride : 0) | (a->y ? a->y_stride : 0);
+    return (p & 15) == 0 && (n & 3) == 0 ? launch<4>(*a, st) : launch<1>(*a, st);
 }

@@ -18,12 +18,14 @@ static int misaligned(const void* p, unsigned a) { return ((uintptr_t)p & (a - 1
 
 /* ---------------------------------------------------------------- norm */
 
+#define NORM_MAX_K (1 << 28)
+
 int kq_rmsnorm_dev(const kq_rmsnorm* in, kq_stream stream) {
     static const char who[] = "kq_rmsnorm_dev";
     int n_cu;
     if (!in) return kq_fail("%s: NULL descriptor", who);
     kq_rmsnorm a = *in;
-    if (a.B < 1 || a.K < 1) return kq_fail("%s: B=%d K=%d", who, a.B, a.K);
+    if (a.B < 1 || a.K < 1 || a.K > NORM_MAX_K) return kq_fail("%s: B=%d K=%d", who, a.B, a.K);
     if (!(a.eps >= 0.0f) || isinf(a.eps)) return kq_fail("%s: eps %g", who, (double)a.eps);
     if (a.group != 0 && a.group != 16 && a.group != 32)
         return kq_fail("%s: group %d (0, 16 or 32)", who, a.group);
