@@ -536,8 +536,9 @@ int kq_rmsnorm_dev(const kq_rmsnorm* a, kq_stream stream);
  * that divides K) share a scale and a zero point:
  *   w[n][k] = scales[n][k / group] * (q[n][k] - zeros[n][k / group])
  * scales: N rows of K / group values of scale_type (KQ_TYPE_F16, KQ_TYPE_BF16
- * or KQ_TYPE_F32); zeros: N rows of K / group bytes, or NULL: all 8.
- * K % 32 == 0, any N; q is 16-byte aligned, scales to their own size. */
+ * or KQ_TYPE_F32); zeros: N rows of K / group bytes, the zero point in the
+ * low half (0..15), or NULL: all 8.  K % 32 == 0, K <= 2^20, any N; q is
+ * 16-byte aligned, scales to their own size. */
 #define KQ_TYPE_BF16    30      /* of scales only */
 typedef struct kq_w4 {
     int N, K, group, scale_type;

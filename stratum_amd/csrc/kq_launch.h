@@ -124,6 +124,7 @@ int kqk_launch_moe_group(const int* sel, int nm, int E, int nt, int x_div, int m
 /* the row operators around the products (kq_norm.hip, kq_w4.hip,
  * kq_verify.hip): arguments checked and strides filled in by kq_step.c */
 int kqk_launch_rmsnorm(const kq_rmsnorm* a, hipStream_t st);
+int kqk_w4_set_max_lds(int bytes);
 int64_t kqk_w4_workspace(const kq_w4* w, int B, int q8, int n_cu);
 int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float* xs,
                   const float* add, float* y, int B, void* work, int n_cu, hipStream_t st);

@@ -223,7 +223,7 @@ static int kq_ready(void) {
     g_kq.lds_max = lds > 0 ? lds : 65536;
     if (kqk_set_max_lds(g_kq.lds_max) != 0 || kqk_mx_set_max_lds(g_kq.lds_max) != 0 ||
         kqk_dense_set_max_lds(g_kq.lds_max) != 0 || kqk_mv_set_max_lds(g_kq.lds_max) != 0 ||
-        kqk_mi_set_max_lds(g_kq.lds_max) != 0)
+        kqk_mi_set_max_lds(g_kq.lds_max) != 0 || kqk_w4_set_max_lds(g_kq.lds_max) != 0)
         return kq_fail("cannot raise the LDS limit");
     /* the static scratch of the no-allocation entry point: its address on
      * this device, looked up once now (other devices at their first call) */

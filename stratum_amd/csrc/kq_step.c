@@ -59,10 +59,11 @@ int kq_rmsnorm_dev(const kq_rmsnorm* in, kq_stream stream) {
 
 #define W4_MAX_ROWS (1 << 28)
 #define W4_MAX_BATCH 65535
+#define W4_MAX_K (1 << 20)
 
 static int w4_check(const kq_w4* w, int B, const char* who) {
     if (!w) return kq_fail("%s: NULL descriptor", who);
-    if (w->N < 1 || w->N > W4_MAX_ROWS || w->K < 32 || w->K % 32)
+    if (w->N < 1 || w->N > W4_MAX_ROWS || w->K < 32 || w->K % 32 || w->K > W4_MAX_K)
         return kq_fail("%s: N=%d K=%d (K %% 32 must be 0)", who, w->N, w->K);
     if (w->group < 32 || w->group % 32 || w->K % w->group)
         return kq_fail("%s: group %d of K=%d (a multiple of 32 that divides K)", who, w->group, w->K);

@@ -1,8 +1,8 @@
 """kq_w4_gemv_dev and kq_w4_gemv_q8_dev against the products in 64 bits.
 
 Bounds, per output, with a = sum_k |s| |q - z| amax_k (amax_k: the largest |x|
-of the 32 values that k lies in): a binary32 x enters with 23 bits below a
-power of two not above 2 amax (an error of at most 2^-23 amax); a block of 32
+of the 32 values that k lies in): a binary32 x enters with an error of at most
+2^-22 amax (half a unit of 2^-22 of the power of two above amax); a block of 32
 products is an integer sum, rounded at most 5 times on its way (its planes'
 sum, the zero point's part, the scales); the blocks' sums are added in any
 order, at most K / 32 additions, then `add`: in all
