@@ -43,12 +43,6 @@ __device__ __forceinline__ int group_of(const W4Arg& a, int c) {
     return (int)__umulhi(2u * (unsigned)c + 1u, a.gmagic);
 }
 
-__device__ __forceinline__ float w4_scale(const kq_w4& w, long i) {
-    if (w.scale_type == KQ_TYPE_F16) return __half2float(static_cast<const __half*>(w.scales)[i]);
-    if (w.scale_type == KQ_TYPE_F32) return static_cast<const float*>(w.scales)[i];
-    return __uint_as_float((uint32_t)static_cast<const uint16_t*>(w.scales)[i] << 16);
-}
-
 // What a step loads per 32 weights beside them.  A kernel is compiled for each
 // MODE, because a branch around a load makes every later wait for loads wait
 // for all of them.
@@ -94,6 +88,7 @@ __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel)
 struct X8 {
     uint32_t even[3], odd[3];
     float scale, sum;        // xs; xs * sum of v over the block
+    int isum;                // that sum of v
 };
 
 template <int CTRL>
@@ -135,6 +130,7 @@ __device__ __forceinline__ X8 split_x(const uint4 lo, const uint4 hi) {
     }
     sum += dpp<QUAD_1>(sum);
     sum += dpp<QUAD_2>(sum);
+    o.isum = sum;
     o.sum = o.scale * (float)sum;
     return o;
 }
@@ -334,41 +330,263 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
     }
 }
 
-// One wave per row, a lane per 32 weights, up to 4 streams a pass.
-template <bool Q8>
-__global__ __launch_bounds__(256) void kq_w4_kernel(kq_w4 w, const float* x, const int8_t* xq,
-                                                    const float* xs, const float* add, float* y,
-                                                    int B) {
-    const int row = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (row >= w.N) return;
-    const int b0 = blockIdx.y * 4, nb = min(4, B - b0), nblk = w.K / 32;
-    const uint4* q = reinterpret_cast<const uint4*>(w.q + (long)row * (w.K / 2));
-    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c = lane; c < nblk; c += 64) {
-        const uint4 v = q[c];
-        const long g = (long)row * (w.K / w.group) + (long)c * 32 / w.group;
-        const float s = w4_scale(w, g);
-        const int z = w.zeros ? w.zeros[g] & 15 : 8;
-        const uint32_t d[4] = {v.x, v.y, v.z, v.w};
-        for (int b = 0; b < nb; b++) {
-            float t = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 32; i++) {
-                const float n = (float)((int)((d[i / 8] >> (4 * (i % 8))) & 15) - z);
-                const long at = (long)(b0 + b) * w.K + 32 * c + i;
-                t = fmaf(n, Q8 ? (float)xq[at] : x[at], t);
-            }
-            if (Q8) t = t * xs[(long)(b0 + b) * nblk + c];
-            acc[b] = fmaf(s, t, acc[b]);
+// ---------------------------------------------------- 4 and more streams
+// On the int8 matrix cores: one v_mfma_i32_16x16x32_i8 takes a block of 32 of
+// 16 streams (one digit) against the same block of 16 rows; D[stream 4 (l / 16)
+// + i][row l % 16] in lane l.
+//
+// A wave stays at M windows of 128 weights of the row and walks down the rows
+// 16 at a time, so its streams' x stays in registers in the operand's layout
+// (8 bytes a lane, block and digit).  A lane's 16 bytes of a window are one
+// block of one row; four lane-group swaps bring its four dwords to the four
+// lanes that the operand wants them in.  The digits share an accumulator: what
+// the higher ones gave is shifted by 8 in between.  C0 = -8 sum v makes it sum
+// (q - 8) v; zero points other than 8 are taken off per block with xz.
+// The waves' sums of a step meet in LDS.
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// x of one tile of 16 streams as the kernel reads it, per block: P digits of
+// 64 lanes' 8 bytes (lane 16 q + s: stream s, positions 8 q .. 8 q + 7, the even
+// ones' bytes first), then xs[16], C0[16] and xz[16].
+constexpr int mm_xbytes(int P) { return P * 512; }
+constexpr int MM_META = 192;
+
+// One lane per 8 values: binary32 rows (P = 3) or int8 rows (P = 1) to the layout
+// above, streams past B and blocks past the row's end as zeros.
+template <int P>
+__global__ __launch_bounds__(256) void kq_w4_split_kernel(W4Arg a, int B, int nblkp, uint8_t* xop,
+                                                          uint8_t* meta) {
+    const int i = blockIdx.x * 256 + threadIdx.x;        // [block][stream][4]
+    const int q = i & 3, s = (i >> 2) & 15, b = i >> 6, tile = blockIdx.y, st = tile * 16 + s;
+    if (b >= nblkp) return;
+    const bool on = st < B && b < a.nblk;
+    uint2 o[P];
+    float scale, xz;
+    int sum;
+    if constexpr (P == 3) {
+        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+        if (on) {
+            const uint4* src = reinterpret_cast<const uint4*>(a.x + (long)st * a.w.K + 32L * b + 8 * q);
+            lo = src[0];
+            hi = src[1];
         }
-    }
-    for (int b = 0; b < nb; b++) {
-        float t = acc[b];
+        const X8 v = split_x(lo, hi);
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) t += __shfl_xor(t, off);
-        const long o = (long)(b0 + b) * w.N + row;
-        if (lane == 0) y[o] = add ? add[o] + t : t;
+        for (int p = 0; p < P; p++) o[p] = make_uint2(v.even[p], v.odd[p]);
+        scale = v.scale;
+        xz = v.sum;
+        sum = v.isum;
+    } else {
+        uint2 v = make_uint2(0, 0);
+        if (on) v = *reinterpret_cast<const uint2*>(a.xq + (long)st * a.w.K + 32L * b + 8 * q);
+        o[0] = make_uint2(perm(v.y, v.x, 0x06040200), perm(v.y, v.x, 0x07050301));
+        sum = __builtin_amdgcn_sdot4((int)v.x, 0x01010101, 0, false);
+        sum = __builtin_amdgcn_sdot4((int)v.y, 0x01010101, sum, false);
+        sum += dpp<QUAD_1>(sum);
+        sum += dpp<QUAD_2>(sum);
+        scale = on ? a.xs[(long)st * a.nblk + b] : 0.0f;
+        xz = scale * (float)sum;
     }
+    uint2* const x = reinterpret_cast<uint2*>(xop + ((long)tile * nblkp + b) * mm_xbytes(P));
+#pragma unroll
+    for (int p = 0; p < P; p++) x[p * 64 + 16 * q + s] = o[p];
+    uint32_t* const m = reinterpret_cast<uint32_t*>(meta + ((long)tile * nblkp + b) * MM_META);
+    if (q == 0) m[s] = __float_as_uint(scale);
+    if (q == 1) m[16 + s] = (uint32_t)(-8 * sum);
+    if (q == 2) m[32 + s] = __float_as_uint(xz);
+}
+
+struct MmArg {
+    W4Arg a;
+    int B, ntile;            // streams, tiles of 16
+    int nblkp, nwin;         // blocks and windows of a padded row
+    int nw, ks;              // windows of a workgroup, parts of a row
+    int steps;               // steps of 16 rows of a workgroup
+    const uint8_t* xop;
+    const uint8_t* meta;
+    float* part;             // ks > 1: [ks][B][N]
+};
+
+constexpr int MM_PASS = 2;   // steps between barriers
+constexpr int MM_ROW = 17;   // floats of a row's 16 streams in LDS
+
+constexpr int mm_waves(int P, int M) { return P == 3 ? (M <= 1 ? 4 : M <= 2 ? 3 : 2) : M <= 2 ? 4 : M <= 4 ? 3 : 2; }
+
+// ONE: a window lies in one group (group % 128 == 0)
+template <int P, int M, int MODE, bool ONE>
+__global__ __launch_bounds__(512, mm_waves(P, M)) void kq_w4_mm_kernel(MmArg g) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    const W4Arg& a = g.a;
+    const int tid = threadIdx.x, T = blockDim.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), W = T >> 6;
+    // workgroups of the same rows next to each other: tile, then part of the row
+    const int tile = blockIdx.x % g.ntile, rest = blockIdx.x / g.ntile;
+    const int part = rest % g.ks, w0 = part * g.nw + wave * M;       // first window
+    const long r0 = (long)(rest / g.ks) * g.steps * 16;
+    const int rows = (int)min((long)g.steps * 16, a.w.N - r0);
+    const bool half = a.w.scale_type == KQ_TYPE_F16, zeros = a.w.zeros != nullptr;
+    const int wend = min(g.nwin, (part + 1) * g.nw);                 // windows of this part end here
+
+    const long rowb = 16L * a.nblk, rowsb = (long)a.ngrp * RawScale<MODE>::SB;
+    const auto qp = plane(a.w.q, r0 * rowb, (r0 + rows) * rowb);
+    const auto sp = plane(a.w.scales, r0 * rowsb, (r0 + rows) * rowsb);
+    const auto zp = plane(zeros ? a.w.zeros : a.w.scales, zeros ? r0 * a.ngrp : 0,
+                          zeros ? (r0 + rows) * a.ngrp : 0);
+
+    // scales: lane group q loads window (ONE) or block (else) 4 k + q's
+    constexpr int NS = ONE ? (M + 3) / 4 : M;
+    struct Raw { uint4 q[M]; RawScale<MODE> s[NS]; };
+    uint32_t vq = (uint32_t)n * (uint32_t)rowb + 64u * w0 + 16u * q;
+    int ve[NS];
+#pragma unroll
+    for (int k = 0; k < NS; k++) {
+        const int blk = ONE ? 4 * (w0 + 4 * k + q) : 4 * (w0 + k) + q;
+        ve[k] = n * a.ngrp + min(group_of(a, min(blk, a.nblk - 1)), a.ngrp - 1);
+    }
+    auto load = [&](Raw& t) {
+#pragma unroll
+        for (int j = 0; j < M; j++) {
+            const u32x4 v = __builtin_bit_cast(
+                u32x4, __builtin_amdgcn_raw_buffer_load_b128(qp, (int)(vq + 64u * j), 0, 0));
+            t.q[j] = make_uint4(v.x, v.y, v.z, v.w);
+        }
+#pragma unroll
+        for (int k = 0; k < NS; k++) {
+            t.s[k].load(sp, zp, ve[k]);
+            ve[k] += 16 * a.ngrp;
+        }
+        vq += 16u * (uint32_t)rowb;
+    };
+    Raw cur, nxt;
+    load(cur);
+
+    // this wave's x, and the workgroup's block data to LDS
+    uint2 x[M][4][P];
+#pragma unroll
+    for (int j = 0; j < M; j++)
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+#pragma unroll
+            for (int p = 0; p < P; p++) {
+                x[j][b][p] = make_uint2(0, 0);
+                if (w0 + j < wend)
+                    x[j][b][p] = reinterpret_cast<const uint2*>(
+                        g.xop + ((long)tile * g.nblkp + 4 * (w0 + j) + b) * mm_xbytes(P))[64 * p + lane];
+            }
+    const int mblk = 4 * W * M;                                       // blocks in LDS
+    float* const xsum = reinterpret_cast<float*>(smem + (size_t)mblk * MM_META);
+    for (int i = tid; i < mblk * (MM_META / 16); i += T) {
+        const int b = i / (MM_META / 16), blk = 4 * part * g.nw + b;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (blk < 4 * wend)
+            v = reinterpret_cast<const uint4*>(g.meta + ((long)tile * g.nblkp + blk) * MM_META)[i % (MM_META / 16)];
+        reinterpret_cast<uint4*>(smem)[i] = v;
+    }
+    lds_barrier();
+
+    const int half_floats = MM_PASS * W * 16 * MM_ROW;
+    int at = 0;
+    for (int k0 = 0; k0 < g.steps; k0 += MM_PASS) {
+#pragma unroll 1
+        for (int k = 0; k < MM_PASS; k++) {
+            load(nxt);
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < M; j++) {
+                // dword k of block b, from register k of lane group b to register b of group k
+                const auto p02 = __builtin_amdgcn_permlane32_swap(cur.q[j].x, cur.q[j].z, false, false);
+                const auto p13 = __builtin_amdgcn_permlane32_swap(cur.q[j].y, cur.q[j].w, false, false);
+                const auto b01 = __builtin_amdgcn_permlane16_swap(p02[0], p13[0], false, false);
+                const auto b23 = __builtin_amdgcn_permlane16_swap(p02[1], p13[1], false, false);
+                const uint32_t d[4] = {b01[0], b01[1], b23[0], b23[1]};
+                // the scales of the window or its blocks, to all lane groups
+                const RawScale<MODE>& rs = cur.s[ONE ? j / 4 : j];
+                float sc[4], ze[4];
+                {
+                    const float s = rs.scale(half);
+                    const auto e = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+                    const auto lo = __builtin_amdgcn_permlane32_swap(e[0], e[0], false, false);
+                    const auto hi = __builtin_amdgcn_permlane32_swap(e[1], e[1], false, false);
+                    sc[0] = __uint_as_float(lo[0]); sc[1] = __uint_as_float(hi[0]);
+                    sc[2] = __uint_as_float(lo[1]); sc[3] = __uint_as_float(hi[1]);
+                }
+                if (MODE != M_16) {
+                    const float z = rs.zero(zeros) - 8.0f;
+                    const auto e = __builtin_amdgcn_permlane16_swap(__float_as_uint(z), __float_as_uint(z), false, false);
+                    const auto lo = __builtin_amdgcn_permlane32_swap(e[0], e[0], false, false);
+                    const auto hi = __builtin_amdgcn_permlane32_swap(e[1], e[1], false, false);
+                    ze[0] = __uint_as_float(lo[0]); ze[1] = __uint_as_float(hi[0]);
+                    ze[2] = __uint_as_float(lo[1]); ze[3] = __uint_as_float(hi[1]);
+                }
+                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
+                const uint8_t* mb = smem + (size_t)(4 * (wave * M + j)) * MM_META + 16 * q;
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    const long w = (long)(((uint64_t)((d[b] >> 4) & 0x0f0f0f0fu) << 32) | (d[b] & 0x0f0f0f0fu));
+                    const f32x4 xs = *reinterpret_cast<const f32x4*>(mb + b * MM_META);
+                    const i32x4 c0 = *reinterpret_cast<const i32x4*>(mb + b * MM_META + 64);
+                    i32x4 D;
+                    if constexpr (P == 1) {
+                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][0]), w, c0, 0, 0, 0);
+                    } else {
+                        D = i32x4{0, 0, 0, 0};
+                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][2]), w, D, 0, 0, 0);
+                        D = D << 8;
+                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][1]), w, D, 0, 0, 0);
+                        D = (D << 8) + c0;
+                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][0]), w, D, 0, 0, 0);
+                    }
+                    f32x4 xz;
+                    if (MODE != M_16) xz = *reinterpret_cast<const f32x4*>(mb + b * MM_META + 128);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (ONE) {
+                            t[i] = fmaf(xs[i], (float)D[i], t[i]);
+                            if (MODE != M_16) t[i] = fmaf(-ze[j & 3], xz[i], t[i]);
+                        } else {
+                            float v = xs[i] * (float)D[i];
+                            if (MODE != M_16) v = fmaf(-ze[b], xz[i], v);
+                            acc[i] = fmaf(sc[b], v, acc[i]);
+                        }
+                    }
+                }
+                if (ONE) {
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[i] = fmaf(sc[j & 3], t[i], acc[i]);
+                }
+            }
+            float* o = xsum + at + ((k * W + wave) * 16 + n) * MM_ROW + 4 * q;
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[i] = acc[i];
+            cur = nxt;
+        }
+        lds_barrier();
+        // outputs of the pass: rows next to each other
+        const int nr = min(MM_PASS * 16, rows - k0 * 16);
+        for (int i = tid; i < MM_PASS * 256; i += T) {
+            const int r = i & (MM_PASS * 16 - 1), s = i / (MM_PASS * 16), st = tile * 16 + s;
+            if (r >= nr || st >= g.B) continue;
+            const float* v = xsum + at + ((r >> 4) * W * 16 + (r & 15)) * MM_ROW + s;
+            float sum = v[0];
+            for (int w = 1; w < W; w++) sum = sum + v[w * 16 * MM_ROW];
+            const long o = (long)st * a.w.N + r0 + k0 * 16 + r;
+            if (g.ks > 1) g.part[(long)part * g.B * a.w.N + o] = sum;
+            else a.y[o] = a.add ? a.add[o] + sum : sum;
+        }
+        at = half_floats - at;
+    }
+}
+
+// the parts of rows that were cut, in their order
+__global__ __launch_bounds__(256) void kq_w4_join_kernel(const float* part, const float* add, float* y,
+                                                         long n, int ks) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n) return;
+    float sum = part[i];
+    for (int k = 1; k < ks; k++) sum = sum + part[k * n + i];
+    y[i] = add ? add[i] + sum : sum;
 }
 
 // ------------------------------------------------------------- the plan
@@ -443,6 +661,90 @@ int raise_lds(int bytes) {
     return e ? e : f ? f : g;
 }
 
+// ------------------------------------------------------- matrix-core plan
+
+constexpr int MM_M = 5, MM_W = 8;        // windows of a wave, waves of a workgroup at most
+
+struct MmPlan { int M, W; long lds, grid, xop, meta, part; };
+
+void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
+    const W4Arg& a = g.a;
+    g.ntile = (g.B + 15) / 16;
+    g.nwin = (a.nblk + 3) / 4;
+    g.nblkp = 4 * g.nwin;
+    g.ks = (g.nwin + MM_M * MM_W - 1) / (MM_M * MM_W);
+    g.nw = (g.nwin + g.ks - 1) / g.ks;
+    g.ks = (g.nwin + g.nw - 1) / g.nw;
+    p->M = (g.nw + MM_W - 1) / MM_W;
+    p->W = (g.nw + p->M - 1) / p->M;
+    const long rows16 = (a.w.N + 15) / 16;
+    const long slots = (long)n_cu * mm_waves(P, p->M) * 4 / p->W;
+    long steps = (rows16 * g.ntile * g.ks + slots - 1) / slots;
+    const long most = (1L << 30) / (16L * a.nblk) / 16;        // 32-bit offsets
+    if (steps > most) steps = most;
+    if (steps > rows16) steps = rows16;
+    g.steps = (int)steps;
+    p->grid = (rows16 + steps - 1) / steps * g.ks * g.ntile;
+    p->lds = 4L * p->W * p->M * MM_META + 2L * MM_PASS * p->W * 16 * MM_ROW * 4;
+    p->xop = ((long)g.ntile * g.nblkp * mm_xbytes(P) + 255) & ~255L;
+    p->meta = ((long)g.ntile * g.nblkp * MM_META + 255) & ~255L;
+    p->part = g.ks > 1 ? ((long)g.ks * g.B * a.w.N * 4 + 255) & ~255L : 0;
+}
+
+template <int P, int M, int MODE>
+int launch_mm_m(const MmArg& g, const MmPlan& p, hipStream_t st) {
+    const dim3 grid((unsigned)p.grid), wg((unsigned)(64 * p.W));
+    if (g.a.w.group % 128 == 0)
+        hipLaunchKernelGGL((kq_w4_mm_kernel<P, M, MODE, true>), grid, wg, (size_t)p.lds, st, g);
+    else
+        hipLaunchKernelGGL((kq_w4_mm_kernel<P, M, MODE, false>), grid, wg, (size_t)p.lds, st, g);
+    return (int)hipGetLastError();
+}
+
+template <int P, int M>
+int launch_mm(const MmArg& g, const MmPlan& p, hipStream_t st) {
+    if (g.a.w.scale_type == KQ_TYPE_F32) return launch_mm_m<P, M, M_32Z>(g, p, st);
+    return g.a.w.zeros ? launch_mm_m<P, M, M_16Z>(g, p, st) : launch_mm_m<P, M, M_16>(g, p, st);
+}
+
+template <int P>
+int launch_mm_all(MmArg& g, const MmPlan& p, uint8_t* work, hipStream_t st) {
+    g.xop = work;
+    g.meta = work + p.xop;
+    g.part = reinterpret_cast<float*>(work + p.xop + p.meta);
+    hipLaunchKernelGGL((kq_w4_split_kernel<P>), dim3((unsigned)((g.nblkp * 64 + 255) / 256), (unsigned)g.ntile),
+                       dim3(256), 0, st, g.a, g.B, g.nblkp, work, work + p.xop);
+    int e = (int)hipGetLastError();
+    if (e) return e;
+    switch (p.M) {
+    case 1: e = launch_mm<P, 1>(g, p, st); break;
+    case 2: e = launch_mm<P, 2>(g, p, st); break;
+    case 3: e = launch_mm<P, 3>(g, p, st); break;
+    case 4: e = launch_mm<P, 4>(g, p, st); break;
+    default: e = launch_mm<P, 5>(g, p, st); break;
+    }
+    if (e || g.ks == 1) return e;
+    const long n = (long)g.B * g.a.w.N;
+    hipLaunchKernelGGL(kq_w4_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g.part, g.a.add,
+                       g.a.y, n, g.ks);
+    return (int)hipGetLastError();
+}
+
+bool fill(W4Arg& a, const kq_w4* w) {
+    a.w = *w;
+    a.x = nullptr; a.xq = nullptr; a.xs = nullptr; a.add = nullptr; a.y = nullptr;
+    a.nblk = w->K / 32;
+    a.ngrp = w->K / w->group;
+    a.gmagic = (1u << 31) / (unsigned)(w->group / 32) + 1;
+    a.rs = a.rpw = a.pass = a.tstride = a.red = 0;
+    return w->N >= 1 && w->K >= 32 && w->K % 32 == 0;
+}
+
+// LDS bytes of the walk kernel where it takes the call, else -1.
+long walk_takes(W4Arg& a, int P, int B, int n_cu) {
+    return B <= walk_max_b(P) && a.nblk <= WALK_MAX_BLK ? walk_plan(a, P, B, n_cu) : -1;
+}
+
 }  // namespace
 
 extern "C" {
@@ -457,27 +759,29 @@ int kqk_w4_set_max_lds(int bytes) {
     return 0;
 }
 
-int64_t kqk_w4_workspace(const kq_w4* w, int B, int q8, int n_cu) { return 0; }
+int64_t kqk_w4_workspace(const kq_w4* w, int B, int q8, int n_cu) {
+    MmArg g;
+    MmPlan p;
+    fill(g.a, w);
+    if (walk_takes(g.a, q8 ? 1 : 3, B, n_cu) > 0) return 0;
+    g.B = B;
+    mm_plan(g, q8 ? 1 : 3, n_cu, &p);
+    return p.xop + p.meta + p.part;
+}
 
 int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float* xs,
                   const float* add, float* y, int B, void* work, int n_cu, hipStream_t st) {
-    if (w->N < 1 || w->K < 32 || w->K % 32 || B < 1) return (int)hipErrorInvalidValue;
-    W4Arg a;
-    a.w = *w;
+    MmArg g;
+    MmPlan p;
+    W4Arg& a = g.a;
+    if (!fill(a, w) || B < 1) return (int)hipErrorInvalidValue;
     a.x = x; a.xq = xq; a.xs = xs; a.add = add; a.y = y;
-    a.nblk = w->K / 32;
-    a.ngrp = w->K / w->group;
-    a.gmagic = (1u << 31) / (unsigned)(w->group / 32) + 1;
-    if (B <= walk_max_b(xq ? 1 : 3) && a.nblk <= WALK_MAX_BLK) {
-        const long lds = walk_plan(a, xq ? 1 : 3, B, n_cu);
-        if (lds > 0) return xq ? launch_walk_b<1>(a, B, lds, st) : launch_walk_b<3>(a, B, lds, st);
-    }
-    const dim3 grid((unsigned)((w->N + 3) / 4), (unsigned)((B + 3) / 4));
-    if (xq)
-        hipLaunchKernelGGL(kq_w4_kernel<true>, grid, dim3(256), 0, st, *w, x, xq, xs, add, y, B);
-    else
-        hipLaunchKernelGGL(kq_w4_kernel<false>, grid, dim3(256), 0, st, *w, x, xq, xs, add, y, B);
-    return (int)hipGetLastError();
+    const long lds = walk_takes(a, xq ? 1 : 3, B, n_cu);
+    if (lds > 0) return xq ? launch_walk_b<1>(a, B, lds, st) : launch_walk_b<3>(a, B, lds, st);
+    g.B = B;
+    mm_plan(g, xq ? 1 : 3, n_cu, &p);
+    uint8_t* const ws = static_cast<uint8_t*>(work);
+    return xq ? launch_mm_all<1>(g, p, ws, st) : launch_mm_all<3>(g, p, ws, st);
 }
 
 }
