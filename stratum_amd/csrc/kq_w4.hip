@@ -17,6 +17,7 @@
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
+#include <type_traits>
 
 #include "kq_launch.h"
 
@@ -61,7 +62,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t plane(const void* p, long at, 
 template <int MODE>
 struct RawScale {
     static constexpr int SB = MODE == M_32Z ? 4 : 2;      // bytes of a scale
-    uint32_t s, z;
+    // (as loaded: widening them would wait for them)
+    std::conditional_t<MODE == M_32Z, uint32_t, uint16_t> s;
+    uint8_t z;
     __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t sp, __amdgpu_buffer_rsrc_t zp, int e) {
         if (MODE == M_32Z) s = __builtin_amdgcn_raw_buffer_load_b32(sp, SB * e, 0, 0);
         else s = __builtin_amdgcn_raw_buffer_load_b16(sp, SB * e, 0, 0);
@@ -70,7 +73,7 @@ struct RawScale {
     __device__ __forceinline__ float scale(bool half) const {
         if (MODE == M_32Z) return __uint_as_float(s);
         const float h = __half2float(__ushort_as_half((unsigned short)s));
-        return half ? h : __uint_as_float(s << 16);
+        return half ? h : __uint_as_float((uint32_t)s << 16);
     }
     __device__ __forceinline__ float zero(bool zeros) const {
         return MODE == M_16 || (MODE == M_32Z && !zeros) ? 8.0f : (float)(z & 15);
@@ -88,7 +91,6 @@ __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel)
 struct X8 {
     uint32_t even[3], odd[3];
     float scale, sum;        // xs; xs * sum of v over the block
-    int isum;                // that sum of v
 };
 
 template <int CTRL>
@@ -130,7 +132,6 @@ __device__ __forceinline__ X8 split_x(const uint4 lo, const uint4 hi) {
     }
     sum += dpp<QUAD_1>(sum);
     sum += dpp<QUAD_2>(sum);
-    o.isum = sum;
     o.sum = o.scale * (float)sum;
     return o;
 }
@@ -330,104 +331,137 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
     }
 }
 
-// ---------------------------------------------------- 4 and more streams
-// On the int8 matrix cores: one v_mfma_i32_16x16x32_i8 takes a block of 32 of
-// 16 streams (one digit) against the same block of 16 rows; D[stream 4 (l / 16)
-// + i][row l % 16] in lane l.
+// ------------------------------------------------- more streams
+// On the int8 matrix cores: one v_mfma_i32_16x16x32_i8 takes a block of 32 of 16
+// operand rows against the same block of 16 rows of weights; D[4 (l / 16) +
+// i][weight row l % 16] in register i of lane l.  Streams are laid over the
+// operand rows so that lane group q holds streams q, q + 4, ... (G of them) and
+// nothing else: int8 rows, operand row 4 q + i is stream q + 4 i; binary32 rows,
+// one product per 4 streams, operand row 4 q + i is digit i of stream q + 4 g, so
+// that a lane has the digits it adds up (the fourth row is not read).
 //
-// A wave stays at M windows of 128 weights of the row and walks down the rows
-// 16 at a time, so its streams' x stays in registers in the operand's layout
-// (8 bytes a lane, block and digit).  A lane's 16 bytes of a window are one
-// block of one row; four lane-group swaps bring its four dwords to the four
-// lanes that the operand wants them in.  The digits share an accumulator: what
-// the higher ones gave is shifted by 8 in between.  C0 = -8 sum v makes it sum
-// (q - 8) v; zero points other than 8 are taken off per block with xz.
-// The waves' sums of a step meet in LDS.
+// A workgroup has a part of the row (nw windows of 128 weights), whose x it
+// brings to digits in LDS, and a run of rows.  Its (tile of 16 rows, window)
+// pairs are cut evenly among the waves, wherever that falls: a wave adds up a
+// tile's windows in registers and writes the tile out, or, of a tile that it
+// shares with other waves, leaves its sum in LDS to be joined behind a barrier.
+//
+// A window's weights are loaded in address order (lane 4 r + b: block b of row r;
+// a row to a lane, as the operand wants them, makes every lane of a load a cache
+// access of its own) and change lanes in LDS, in the wave's own 1.5 KB, together
+// with their scales.
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// x of one tile of 16 streams as the kernel reads it, per block: P digits of
-// 64 lanes' 8 bytes (lane 16 q + s: stream s, positions 8 q .. 8 q + 7, the even
-// ones' bytes first), then xs[16], C0[16] and xz[16].
-constexpr int mm_xbytes(int P) { return P * 512; }
-constexpr int MM_META = 192;
-
-// One lane per 8 values: binary32 rows (P = 3) or int8 rows (P = 1) to the layout
-// above, streams past B and blocks past the row's end as zeros.
-template <int P>
-__global__ __launch_bounds__(256) void kq_w4_split_kernel(W4Arg a, int B, int nblkp, uint8_t* xop,
-                                                          uint8_t* meta) {
-    const int i = blockIdx.x * 256 + threadIdx.x;        // [block][stream][4]
-    const int q = i & 3, s = (i >> 2) & 15, b = i >> 6, tile = blockIdx.y, st = tile * 16 + s;
-    if (b >= nblkp) return;
-    const bool on = st < B && b < a.nblk;
-    uint2 o[P];
-    float scale, xz;
-    int sum;
-    if constexpr (P == 3) {
-        uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-        if (on) {
-            const uint4* src = reinterpret_cast<const uint4*>(a.x + (long)st * a.w.K + 32L * b + 8 * q);
-            lo = src[0];
-            hi = src[1];
-        }
-        const X8 v = split_x(lo, hi);
-#pragma unroll
-        for (int p = 0; p < P; p++) o[p] = make_uint2(v.even[p], v.odd[p]);
-        scale = v.scale;
-        xz = v.sum;
-        sum = v.isum;
-    } else {
-        uint2 v = make_uint2(0, 0);
-        if (on) v = *reinterpret_cast<const uint2*>(a.xq + (long)st * a.w.K + 32L * b + 8 * q);
-        o[0] = make_uint2(perm(v.y, v.x, 0x06040200), perm(v.y, v.x, 0x07050301));
-        sum = __builtin_amdgcn_sdot4((int)v.x, 0x01010101, 0, false);
-        sum = __builtin_amdgcn_sdot4((int)v.y, 0x01010101, sum, false);
-        sum += dpp<QUAD_1>(sum);
-        sum += dpp<QUAD_2>(sum);
-        scale = on ? a.xs[(long)st * a.nblk + b] : 0.0f;
-        xz = scale * (float)sum;
-    }
-    uint2* const x = reinterpret_cast<uint2*>(xop + ((long)tile * nblkp + b) * mm_xbytes(P));
-#pragma unroll
-    for (int p = 0; p < P; p++) x[p * 64 + 16 * q + s] = o[p];
-    uint32_t* const m = reinterpret_cast<uint32_t*>(meta + ((long)tile * nblkp + b) * MM_META);
-    if (q == 0) m[s] = __float_as_uint(scale);
-    if (q == 1) m[16 + s] = (uint32_t)(-8 * sum);
-    if (q == 2) m[32 + s] = __float_as_uint(xz);
-}
+// A window's x in LDS: per pair of blocks and lane group P * 4 G entries of 16
+// bytes (8 of either block: the even positions' bytes, then the odd ones'),
+// then xs of its blocks, [block][q][G], and xz likewise, or (ONE) [q][G] of the
+// whole window.
+constexpr int mm_xbytes(int P, int G) { return 512 * P * G; }
+constexpr int mm_window(int P, int G, bool ONE) { return mm_xbytes(P, G) + (ONE ? 80 : 128) * G; }
 
 struct MmArg {
     W4Arg a;
-    int B, ntile;            // streams, tiles of 16
-    int nblkp, nwin;         // blocks and windows of a padded row
-    int nw, ks;              // windows of a workgroup, parts of a row
-    int steps;               // steps of 16 rows of a workgroup
-    const uint8_t* xop;
-    const uint8_t* meta;
+    int B, bt, ntile;        // streams, of a tile of streams; those tiles
+    int nwin, nw, ks;        // windows of a row, of a part; parts
+    int rows;                // of a workgroup
+    int xwaves, xmagic;      // waves that bring a stream's x to LDS; w / xwaves = w * xmagic >> 16
     float* part;             // ks > 1: [ks][B][N]
 };
 
-constexpr int MM_PASS = 2;   // steps between barriers
-constexpr int MM_ROW = 17;   // floats of a row's 16 streams in LDS
-
-constexpr int mm_waves(int P, int M) { return P == 3 ? (M <= 1 ? 4 : M <= 2 ? 3 : 2) : M <= 2 ? 4 : M <= 4 ? 3 : 2; }
+constexpr int MM_W = 16;     // waves
+constexpr int mm_slot(int G) { return 16 * (4 * G + 1); }   // floats of a tile's sums in LDS
+// A wave's own LDS: the sums of the tile that it began with, if others share
+// it; 16 rows of a window, 80 bytes each, and their scales.  What it ends with
+// takes the place of the rows.
+constexpr int MM_ROWB = 80, MM_STAGE = 16 * MM_ROWB + 64 * 8;
+constexpr int mm_wave(int G) { return 4 * mm_slot(G) + MM_STAGE; }
+static_assert(4 * mm_slot(4) <= MM_STAGE);
+constexpr uint32_t FAR = 0x80000000u;    // an offset behind every buffer's end
 
 // ONE: a window lies in one group (group % 128 == 0)
-template <int P, int M, int MODE, bool ONE>
-__global__ __launch_bounds__(512, mm_waves(P, M)) void kq_w4_mm_kernel(MmArg g) {
+// ADD: there is something to add (a load of it in the loop makes waits for
+// weights wait for all of them)
+template <int P, int G, int MODE, bool ONE, bool ADD>
+__global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     extern __shared__ __align__(16) uint8_t smem[];
+    constexpr int T = 64 * MM_W, WB = mm_window(P, G, ONE), XB = mm_xbytes(P, G), E = P * 4 * G;
     const W4Arg& a = g.a;
-    const int tid = threadIdx.x, T = blockDim.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), W = T >> 6;
-    // workgroups of the same rows next to each other: tile, then part of the row
-    const int tile = blockIdx.x % g.ntile, rest = blockIdx.x / g.ntile;
-    const int part = rest % g.ks, w0 = part * g.nw + wave * M;       // first window
-    const long r0 = (long)(rest / g.ks) * g.steps * 16;
-    const int rows = (int)min((long)g.steps * 16, a.w.N - r0);
+    const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // workgroups of the same weights next to each other
+    const int tile = blockIdx.x, part = blockIdx.y, w0 = part * g.nw, nw = min(g.nw, g.nwin - w0);
+    const long r0 = (long)blockIdx.z * g.rows;
+    const int rows = (int)min((long)g.rows, a.w.N - r0), tiles = (rows + 15) / 16;
     const bool half = a.w.scale_type == KQ_TYPE_F16, zeros = a.w.zeros != nullptr;
-    const int wend = min(g.nwin, (part + 1) * g.nw);                 // windows of this part end here
+    const int s0 = tile * g.bt, ns = min(g.bt, g.B - s0);          // streams of this tile
+
+    // x: g.xwaves waves to a stream, a lane 8 values a step.  (What lies in LDS
+    // for streams that are not there only reaches sums that are not theirs.)
+    constexpr int XL = P == 1 ? 1 : 2;
+    const int s = min(wave * g.xmagic >> 16, ns - 1), xstep = g.xwaves * 64;   // (waves left over repeat the last's)
+    const int np = (nw + 1) >> 1, per = np * 32, e0 = w0 * 16;     // (pairs of windows)
+    const int elast = min(a.nblk * 4, e0 + nw * 16) - 1;
+    int e = (wave * g.xmagic >> 16 == s ? (wave - s * g.xwaves) * 64 : 0) + lane;
+    const long st = s0 + s;
+    struct X { uint4 v[XL]; float s; };
+    auto get = [&](int e) {
+        X r;
+        e = min(e0 + e, elast - 3 + (e & 3));
+        if constexpr (P == 1) {
+            const uint2 v = *reinterpret_cast<const uint2*>(a.xq + st * a.w.K + 8L * e);
+            r.v[0] = make_uint4(v.x, v.y, 0, 0);
+            r.s = a.xs[st * a.nblk + (e >> 2)];
+        } else {
+            const uint4* src = reinterpret_cast<const uint4*>(a.x + st * a.w.K + 8L * e);
+            r.v[0] = src[0];
+            r.v[1] = src[1];
+            r.s = 0.0f;
+        }
+        return r;
+    };
+    auto put = [&](int e, X r) {
+        const int b = e >> 2, kq = e & 3;
+        const bool on = e0 + e <= elast, in = e < per;
+#pragma unroll
+        for (int k = 0; k < XL; k++) r.v[k] = on ? r.v[k] : make_uint4(0, 0, 0, 0);
+        uint2 d[P];
+        float scale, xz;
+        if constexpr (P == 1) {
+            const uint32_t x = r.v[0].x, y = r.v[0].y;
+            d[0] = make_uint2(perm(y, x, 0x06040200), perm(y, x, 0x07050301));
+            int sum = __builtin_amdgcn_sdot4((int)x, 0x01010101, 0, false);
+            sum = __builtin_amdgcn_sdot4((int)y, 0x01010101, sum, false);
+            sum += dpp<QUAD_1>(sum);
+            sum += dpp<QUAD_2>(sum);
+            scale = on ? r.s : 0.0f;
+            xz = scale * (float)sum;
+        } else {
+            const X8 v = split_x(r.v[0], r.v[XL - 1]);
+#pragma unroll
+            for (int p = 0; p < P; p++) d[p] = make_uint2(v.even[p], v.odd[p]);
+            scale = v.scale;
+            xz = v.sum;
+        }
+        uint8_t* const w = smem + (size_t)(b >> 2) * WB;
+        const int at = (((b >> 1) & 1) * 4 + kq) * E + s * P;
+        if (in) {
+#pragma unroll
+            for (int p = 0; p < P; p++) reinterpret_cast<uint2*>(w)[(at + p) * 2 + (b & 1)] = d[p];
+        }
+        float* const m = reinterpret_cast<float*>(w + XB) + ((b & 3) * 4 + (s & 3)) * G + (s >> 2);
+        if (in && kq == 0) m[0] = scale;
+        if constexpr (ONE) {                              // 16 lanes hold the window
+            xz = xz + __int_as_float(dpp<HALF_MIRROR>(__float_as_int(xz)));
+            xz = xz + __int_as_float(dpp<MIRROR>(__float_as_int(xz)));
+            if (in && (e & 15) == 1) reinterpret_cast<float*>(w + XB)[16 * G + (s & 3) * G + (s >> 2)] = xz;
+        } else {
+            if (in && kq == 1) m[16 * G] = xz;
+        }
+    };
+    // on its way before the weights, as loads return in order
+    X x0 = get(e), x1 = get(e + xstep);
+    __builtin_amdgcn_sched_barrier(0);
 
     const long rowb = 16L * a.nblk, rowsb = (long)a.ngrp * RawScale<MODE>::SB;
     const auto qp = plane(a.w.q, r0 * rowb, (r0 + rows) * rowb);
@@ -435,147 +469,178 @@ __global__ __launch_bounds__(512, mm_waves(P, M)) void kq_w4_mm_kernel(MmArg g) 
     const auto zp = plane(zeros ? a.w.zeros : a.w.scales, zeros ? r0 * a.ngrp : 0,
                           zeros ? (r0 + rows) * a.ngrp : 0);
 
-    // scales: lane group q loads window (ONE) or block (else) 4 k + q's
-    constexpr int NS = ONE ? (M + 3) / 4 : M;
-    struct Raw { uint4 q[M]; RawScale<MODE> s[NS]; };
-    uint32_t vq = (uint32_t)n * (uint32_t)rowb + 64u * w0 + 16u * q;
-    int ve[NS];
-#pragma unroll
-    for (int k = 0; k < NS; k++) {
-        const int blk = ONE ? 4 * (w0 + 4 * k + q) : 4 * (w0 + k) + q;
-        ve[k] = n * a.ngrp + min(group_of(a, min(blk, a.nblk - 1)), a.ngrp - 1);
-    }
+    // this wave's share: [i0, i1) of tiles x pairs of windows, those fastest
+    const int items = tiles * np, ipw = (items + MM_W - 1) / MM_W;
+    const int i0 = min(wave * ipw, items), i1 = min(i0 + ipw, items);
+    constexpr int NS = ONE ? 1 : 2;
+    struct Raw { uint4 q[2]; RawScale<MODE> s[NS]; };
+    int li = i0, lt = i0 / np, lp = i0 - lt * np;         // the next to load
+    const int ldr = lane >> 2, lb = lane & 3;             // row and block of a lane's load
+    const uint32_t vq = (uint32_t)ldr * (uint32_t)rowb + 16u * lb;
+    const int vs = ldr * a.ngrp;
     auto load = [&](Raw& t) {
+        const uint32_t off = li < i1 ? 0 : FAR;
+        const uint32_t at = (uint32_t)lt * 16u * (uint32_t)rowb + 64u * (uint32_t)(w0 + 2 * lp);
+        const int es = lt * 16 * a.ngrp;
 #pragma unroll
-        for (int j = 0; j < M; j++) {
-            const u32x4 v = __builtin_bit_cast(
-                u32x4, __builtin_amdgcn_raw_buffer_load_b128(qp, (int)(vq + 64u * j), 0, 0));
+        for (int j = 0; j < 2; j++) {
+            const uint32_t o = j && 2 * lp + 1 == nw ? FAR : off;     // (a pair's second may be missing)
+            const u32x4 v = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                qp, (int)(vq + (o | (at + 64u * j))), 0, 0));
             t.q[j] = make_uint4(v.x, v.y, v.z, v.w);
         }
+        // scales: the windows' by the first two lanes of their row, or the blocks'
 #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            t.s[k].load(sp, zp, ve[k]);
-            ve[k] += 16 * a.ngrp;
+        for (int j = 0; j < NS; j++) {
+            const int blk = min(4 * (w0 + 2 * lp + j) + (ONE ? 4 * lb : lb), a.nblk - 1);
+            t.s[j].load(sp, zp, ONE && lb > 1 ? (int)(FAR / 4) : (int)((off / 4) | (uint32_t)(vs + es + group_of(a, blk))));
         }
-        vq += 16u * (uint32_t)rowb;
+        li++;
+        if (++lp == np) { lp = 0; lt++; }
     };
-    Raw cur, nxt;
+    Raw cur;
     load(cur);
 
-    // this wave's x, and the workgroup's block data to LDS
-    uint2 x[M][4][P];
-#pragma unroll
-    for (int j = 0; j < M; j++)
-#pragma unroll
-        for (int b = 0; b < 4; b++)
-#pragma unroll
-            for (int p = 0; p < P; p++) {
-                x[j][b][p] = make_uint2(0, 0);
-                if (w0 + j < wend)
-                    x[j][b][p] = reinterpret_cast<const uint2*>(
-                        g.xop + ((long)tile * g.nblkp + 4 * (w0 + j) + b) * mm_xbytes(P))[64 * p + lane];
-            }
-    const int mblk = 4 * W * M;                                       // blocks in LDS
-    float* const xsum = reinterpret_cast<float*>(smem + (size_t)mblk * MM_META);
-    for (int i = tid; i < mblk * (MM_META / 16); i += T) {
-        const int b = i / (MM_META / 16), blk = 4 * part * g.nw + b;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (blk < 4 * wend)
-            v = reinterpret_cast<const uint4*>(g.meta + ((long)tile * g.nblkp + blk) * MM_META)[i % (MM_META / 16)];
-        reinterpret_cast<uint4*>(smem)[i] = v;
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    do {                                                  // (once whatever the length, lest the loads be moved here)
+        put(e, x0);
+        x0 = get(e + 2 * xstep);
+        put(e + xstep, x1);
+        x1 = get(e + 3 * xstep);
+        e += 2 * xstep;
+    } while (e < per);
     lds_barrier();
+    uint8_t* const own = smem + (size_t)(2 * np) * WB + (size_t)wave * mm_wave(G);
+    uint8_t* const stage = own + 4 * mm_slot(G);
+    const int put_at = ldr * MM_ROWB + 16 * lb, take_at = n * MM_ROWB + 4 * q;
 
-    const int half_floats = MM_PASS * W * 16 * MM_ROW;
-    int at = 0;
-    for (int k0 = 0; k0 < g.steps; k0 += MM_PASS) {
-#pragma unroll 1
-        for (int k = 0; k < MM_PASS; k++) {
-            load(nxt);
-            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    float* const dst = g.ks > 1 ? g.part + (long)part * g.B * a.w.N : a.y;
+    auto out = [&](int s, int r, float v) {               // stream s of the tile, row r of the workgroup
+        if (r >= rows || s >= ns) return;
+        const long o = (long)(s0 + s) * a.w.N + r0 + r;
+        dst[o] = ADD ? a.add[o] + v : v;
+    };
+
+    // this lane's entry of an operand: row n = 4 qs + i
+    const int qs = n >> 2, ni = n & 3;
+    const int entry = P == 1 ? qs + 4 * min(ni, G - 1) : qs * P + min(ni, P - 1);
+    const int xoff = (q * E + entry) * 16, moff = XB + q * G * 4;
+
+    float acc[G];
 #pragma unroll
-            for (int j = 0; j < M; j++) {
-                // dword k of block b, from register k of lane group b to register b of group k
-                const auto p02 = __builtin_amdgcn_permlane32_swap(cur.q[j].x, cur.q[j].z, false, false);
-                const auto p13 = __builtin_amdgcn_permlane32_swap(cur.q[j].y, cur.q[j].w, false, false);
-                const auto b01 = __builtin_amdgcn_permlane16_swap(p02[0], p13[0], false, false);
-                const auto b23 = __builtin_amdgcn_permlane16_swap(p02[1], p13[1], false, false);
-                const uint32_t d[4] = {b01[0], b01[1], b23[0], b23[1]};
-                // the scales of the window or its blocks, to all lane groups
-                const RawScale<MODE>& rs = cur.s[ONE ? j / 4 : j];
-                float sc[4], ze[4];
-                {
-                    const float s = rs.scale(half);
-                    const auto e = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
-                    const auto lo = __builtin_amdgcn_permlane32_swap(e[0], e[0], false, false);
-                    const auto hi = __builtin_amdgcn_permlane32_swap(e[1], e[1], false, false);
-                    sc[0] = __uint_as_float(lo[0]); sc[1] = __uint_as_float(hi[0]);
-                    sc[2] = __uint_as_float(lo[1]); sc[3] = __uint_as_float(hi[1]);
+    for (int k = 0; k < G; k++) acc[k] = 0.0f;
+    int t = i0 / np, w = i0 - t * np, from = w;           // `from`: the tile's first pair here
+    uint32_t* const sl = reinterpret_cast<uint32_t*>(stage + 16 * MM_ROWB);
+    for (int i = i0; i < i1; i++) {
+        uint32_t d[2][4];
+        float sc[2][4], ze[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            // (a wave's LDS accesses are in order)
+            *reinterpret_cast<uint4*>(stage + put_at) = cur.q[j];
+            if (j < NS) {
+                const RawScale<MODE>& r = cur.s[j];
+                if (MODE == M_32Z) reinterpret_cast<uint2*>(sl)[lane] = make_uint2(r.s, r.z);
+                else sl[lane] = MODE == M_16Z ? (uint32_t)r.s | (uint32_t)r.z << 16 : r.s;
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll
+            for (int b = 0; b < 4; b++) d[j][b] = *reinterpret_cast<const uint32_t*>(stage + take_at + 16 * b);
+#pragma unroll
+            for (int b = 0; b < (ONE ? 1 : 4); b++) {
+                RawScale<MODE> r;
+                const int at = 4 * n + (ONE ? j : b);
+                if (MODE == M_32Z) {
+                    const uint2 v = reinterpret_cast<const uint2*>(sl)[at];
+                    r.s = v.x;
+                    r.z = (uint8_t)v.y;
+                } else {
+                    const uint32_t v = sl[at];
+                    r.s = (uint16_t)v;
+                    r.z = (uint8_t)(v >> 16);
                 }
-                if (MODE != M_16) {
-                    const float z = rs.zero(zeros) - 8.0f;
-                    const auto e = __builtin_amdgcn_permlane16_swap(__float_as_uint(z), __float_as_uint(z), false, false);
-                    const auto lo = __builtin_amdgcn_permlane32_swap(e[0], e[0], false, false);
-                    const auto hi = __builtin_amdgcn_permlane32_swap(e[1], e[1], false, false);
-                    ze[0] = __uint_as_float(lo[0]); ze[1] = __uint_as_float(hi[0]);
-                    ze[2] = __uint_as_float(lo[1]); ze[3] = __uint_as_float(hi[1]);
-                }
-                f32x4 t = {0.0f, 0.0f, 0.0f, 0.0f};
-                const uint8_t* mb = smem + (size_t)(4 * (wave * M + j)) * MM_META + 16 * q;
+                sc[j][b] = r.scale(half);
+                ze[j][b] = r.zero(zeros);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        }
+        load(cur);                                     // the next pair's, while this one's are used
 #pragma unroll
-                for (int b = 0; b < 4; b++) {
-                    const long w = (long)(((uint64_t)((d[b] >> 4) & 0x0f0f0f0fu) << 32) | (d[b] & 0x0f0f0f0fu));
-                    const f32x4 xs = *reinterpret_cast<const f32x4*>(mb + b * MM_META);
-                    const i32x4 c0 = *reinterpret_cast<const i32x4*>(mb + b * MM_META + 64);
-                    i32x4 D;
-                    if constexpr (P == 1) {
-                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][0]), w, c0, 0, 0, 0);
-                    } else {
-                        D = i32x4{0, 0, 0, 0};
-                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][2]), w, D, 0, 0, 0);
-                        D = D << 8;
-                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][1]), w, D, 0, 0, 0);
-                        D = (D << 8) + c0;
-                        D = __builtin_amdgcn_mfma_i32_16x16x32_i8(__builtin_bit_cast(long, x[j][b][0]), w, D, 0, 0, 0);
-                    }
-                    f32x4 xz;
-                    if (MODE != M_16) xz = *reinterpret_cast<const f32x4*>(mb + b * MM_META + 128);
+        for (int j = 0; j < 2; j++) {
+            const uint8_t* const xb = smem + (2 * w + j) * WB;
+            const float* const m = reinterpret_cast<const float*>(xb + moff);
+            float sum[G];
+            if (ONE) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (ONE) {
-                            t[i] = fmaf(xs[i], (float)D[i], t[i]);
-                            if (MODE != M_16) t[i] = fmaf(-ze[j & 3], xz[i], t[i]);
+                for (int c = 0; c < G; c++) sum[c] = -ze[j][0] * m[16 * G + c];
+            }
+#pragma unroll
+            for (int b2 = 0; b2 < 2; b2++) {
+                constexpr int NX = P == 1 ? 1 : G;
+                uint4 x[NX];
+#pragma unroll
+                for (int c = 0; c < NX; c++)
+                    x[c] = *reinterpret_cast<const uint4*>(xb + xoff + (b2 * 4 * E + 4 * P * c) * 16);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int b = 2 * b2 + h;
+                    const uint32_t db = d[j][b];
+                    const long wv = (long)(((uint64_t)((db >> 4) & 0x0f0f0f0fu) << 32) | (db & 0x0f0f0f0fu));
+                    int dot[G];
+#pragma unroll
+                    for (int c = 0; c < NX; c++) {
+                        const uint2 xv = h ? make_uint2(x[c].z, x[c].w) : make_uint2(x[c].x, x[c].y);
+                        const i32x4 D = __builtin_amdgcn_mfma_i32_16x16x32_i8(
+                            __builtin_bit_cast(long, xv), wv, i32x4{0, 0, 0, 0}, 0, 0, 0);
+                        if constexpr (P == 1) {
+#pragma unroll
+                            for (int e = 0; e < G; e++) dot[e] = D[e];
                         } else {
-                            float v = xs[i] * (float)D[i];
-                            if (MODE != M_16) v = fmaf(-ze[b], xz[i], v);
-                            acc[i] = fmaf(sc[b], v, acc[i]);
+                            dot[c] = (((D[2] << 8) + D[1]) << 8) + D[0];
                         }
                     }
-                }
-                if (ONE) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) acc[i] = fmaf(sc[j & 3], t[i], acc[i]);
+                    for (int c = 0; c < G; c++) {
+                        const float xs = m[4 * G * b + c];
+                        if (ONE) sum[c] = fmaf(xs, (float)dot[c], sum[c]);
+                        else acc[c] = fmaf(sc[j][b], fmaf(-ze[j][b], m[16 * G + 4 * G * b + c],
+                                                          xs * (float)dot[c]), acc[c]);
+                    }
                 }
             }
-            float* o = xsum + at + ((k * W + wave) * 16 + n) * MM_ROW + 4 * q;
+            if (ONE) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) o[i] = acc[i];
-            cur = nxt;
+                for (int c = 0; c < G; c++) acc[c] = fmaf(sc[j][0], sum[c], acc[c]);
+            }
         }
-        lds_barrier();
-        // outputs of the pass: rows next to each other
-        const int nr = min(MM_PASS * 16, rows - k0 * 16);
-        for (int i = tid; i < MM_PASS * 256; i += T) {
-            const int r = i & (MM_PASS * 16 - 1), s = i / (MM_PASS * 16), st = tile * 16 + s;
-            if (r >= nr || st >= g.B) continue;
-            const float* v = xsum + at + ((r >> 4) * W * 16 + (r & 15)) * MM_ROW + s;
-            float sum = v[0];
-            for (int w = 1; w < W; w++) sum = sum + v[w * 16 * MM_ROW];
-            const long o = (long)st * a.w.N + r0 + k0 * 16 + r;
-            if (g.ks > 1) g.part[(long)part * g.B * a.w.N + o] = sum;
-            else a.y[o] = a.add ? a.add[o] + sum : sum;
+        w++;
+        if (w == np || i + 1 == i1) {                  // the tile's end, or this wave's
+            if (from == 0 && w == np) {
+#pragma unroll
+                for (int c = 0; c < G; c++) out(4 * c + q, t * 16 + n, acc[c]);
+            } else {
+                // the first slot for what began with this wave's first pair
+                float* o = reinterpret_cast<float*>(t * np + from == i0 ? own : stage) + n * (4 * G + 1) + q;
+#pragma unroll
+                for (int c = 0; c < G; c++) o[4 * c] = acc[c];
+            }
+#pragma unroll
+            for (int c = 0; c < G; c++) acc[c] = 0.0f;
+            w = from = 0;
+            t++;
         }
-        at = half_floats - at;
+    }
+    __syncthreads();
+    // shared tiles: their waves' sums in order
+    for (int k = tid / (64 * G); k < tiles; k += T / (64 * G)) {
+        const int wa = k * np / ipw, wb = (k * np + np - 1) / ipw;
+        if (wa == wb) continue;
+        const int r = tid & 15, s = (tid >> 4) % (4 * G);
+        const float* v = reinterpret_cast<const float*>(smem + (size_t)(2 * np) * WB) + r * (4 * G + 1) + s;
+        constexpr int WF = mm_wave(G) / 4;
+        float sum = v[wa * WF + (k * np != wa * ipw ? mm_slot(G) : 0)];
+        for (int x = wa + 1; x <= wb; x++) sum = sum + v[x * WF];
+        out(s, k * 16 + r, sum);
     }
 }
 
@@ -595,6 +660,9 @@ constexpr int WALK_MAX_BLK = 1024;
 constexpr int walk_max_b(int P) { return P == 1 ? 4 : 3; }     // (more spill registers)
 int g_lds_max = 65536;
 
+// a matrix of which a CU's share is one step of 512 lanes
+bool small_matrix(const W4Arg& a, int n_cu) { return ((long)a.w.N + n_cu - 1) / n_cu * a.nblk <= 512; }
+
 // Rows of a step and of a workgroup, steps of a pass, LDS bytes (-1: not
 // taken).  Two workgroups a CU, of as many waves as the registers allow,
 // where the row is short enough; one where the matrix is a step's work of
@@ -602,8 +670,7 @@ int g_lds_max = 65536;
 long walk_plan(W4Arg& a, int P, int NB, int n_cu) {
     const int nblk = a.nblk, waves = 4 * walk_waves(P, NB), D = WALK_D;
     const long N = a.w.N, rowb = 16L * nblk;
-    const bool small = (N + n_cu - 1) / n_cu * nblk <= 512;
-    const int per_cu = nblk <= 32 * waves && !small ? 2 : 1, lanes = 64 * waves / per_cu;
+    const int per_cu = nblk <= 32 * waves && !small_matrix(a, n_cu) ? 2 : 1, lanes = 64 * waves / per_cu;
     const long slots = (long)per_cu * n_cu;
     const long fair = (N + slots - 1) / slots;         // rows of a workgroup, were they cut evenly
     const long fits = (lanes < 1024 ? lanes : 1024) / nblk;
@@ -663,66 +730,55 @@ int raise_lds(int bytes) {
 
 // ------------------------------------------------------- matrix-core plan
 
-constexpr int MM_M = 5, MM_W = 8;        // windows of a wave, waves of a workgroup at most
-
-struct MmPlan { int M, W; long lds, grid, xop, meta, part; };
+struct MmPlan { int G; long lds, runs, part; };
 
 void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
     const W4Arg& a = g.a;
     g.ntile = (g.B + 15) / 16;
+    g.bt = (g.B + g.ntile - 1) / g.ntile;
+    p->G = (g.bt + 3) / 4;
+    if (p->G == 3) p->G = 4;
     g.nwin = (a.nblk + 3) / 4;
-    g.nblkp = 4 * g.nwin;
-    g.ks = (g.nwin + MM_M * MM_W - 1) / (MM_M * MM_W);
+    const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G, a.w.group % 128 == 0);
+    const int most_w = (int)((g_lds_max - own) / wb) & ~1;            // windows that LDS takes, in pairs
+    g.ks = (g.nwin + most_w - 1) / most_w;
     g.nw = (g.nwin + g.ks - 1) / g.ks;
     g.ks = (g.nwin + g.nw - 1) / g.nw;
-    p->M = (g.nw + MM_W - 1) / MM_W;
-    p->W = (g.nw + p->M - 1) / p->M;
-    const long rows16 = (a.w.N + 15) / 16;
-    const long slots = (long)n_cu * mm_waves(P, p->M) * 4 / p->W;
-    long steps = (rows16 * g.ntile * g.ks + slots - 1) / slots;
-    const long most = (1L << 30) / (16L * a.nblk) / 16;        // 32-bit offsets
-    if (steps > most) steps = most;
-    if (steps > rows16) steps = rows16;
-    g.steps = (int)steps;
-    p->grid = (rows16 + steps - 1) / steps * g.ks * g.ntile;
-    p->lds = 4L * p->W * p->M * MM_META + 2L * MM_PASS * p->W * 16 * MM_ROW * 4;
-    p->xop = ((long)g.ntile * g.nblkp * mm_xbytes(P) + 255) & ~255L;
-    p->meta = ((long)g.ntile * g.nblkp * MM_META + 255) & ~255L;
+    long runs = (long)n_cu / ((long)g.ks * g.ntile);                  // one workgroup a CU
+    if (runs < 1) runs = 1;
+    long rows = (a.w.N + runs - 1) / runs;
+    const long most = (1L << 30) / (16L * a.nblk) - 16;               // 32-bit offsets
+    if (rows > most) rows = most;
+    g.rows = (int)rows;
+    p->runs = (a.w.N + rows - 1) / rows;
+    g.xwaves = MM_W / g.bt;
+    g.xmagic = 65536 / g.xwaves + 1;
+    p->lds = (g.nw + 1) / 2 * 2 * wb + own;
     p->part = g.ks > 1 ? ((long)g.ks * g.B * a.w.N * 4 + 255) & ~255L : 0;
 }
 
-template <int P, int M, int MODE>
+template <int P, int G, int MODE>
 int launch_mm_m(const MmArg& g, const MmPlan& p, hipStream_t st) {
-    const dim3 grid((unsigned)p.grid), wg((unsigned)(64 * p.W));
-    if (g.a.w.group % 128 == 0)
-        hipLaunchKernelGGL((kq_w4_mm_kernel<P, M, MODE, true>), grid, wg, (size_t)p.lds, st, g);
-    else
-        hipLaunchKernelGGL((kq_w4_mm_kernel<P, M, MODE, false>), grid, wg, (size_t)p.lds, st, g);
+    if (p.runs > 65535 || g.ks > 65535) return (int)hipErrorInvalidValue;
+    const dim3 grid((unsigned)g.ntile, (unsigned)g.ks, (unsigned)p.runs), wg(64 * MM_W);
+    const bool one = g.a.w.group % 128 == 0, add = g.a.add && g.ks == 1;
+    auto* const k = one ? (add ? kq_w4_mm_kernel<P, G, MODE, true, true> : kq_w4_mm_kernel<P, G, MODE, true, false>)
+                        : (add ? kq_w4_mm_kernel<P, G, MODE, false, true> : kq_w4_mm_kernel<P, G, MODE, false, false>);
+    hipLaunchKernelGGL(k, grid, wg, (size_t)p.lds, st, g);
     return (int)hipGetLastError();
 }
 
-template <int P, int M>
-int launch_mm(const MmArg& g, const MmPlan& p, hipStream_t st) {
-    if (g.a.w.scale_type == KQ_TYPE_F32) return launch_mm_m<P, M, M_32Z>(g, p, st);
-    return g.a.w.zeros ? launch_mm_m<P, M, M_16Z>(g, p, st) : launch_mm_m<P, M, M_16>(g, p, st);
+template <int P, int G>
+int launch_mm_g(const MmArg& g, const MmPlan& p, hipStream_t st) {
+    if (g.a.w.scale_type == KQ_TYPE_F32) return launch_mm_m<P, G, M_32Z>(g, p, st);
+    return g.a.w.zeros ? launch_mm_m<P, G, M_16Z>(g, p, st) : launch_mm_m<P, G, M_16>(g, p, st);
 }
 
 template <int P>
-int launch_mm_all(MmArg& g, const MmPlan& p, uint8_t* work, hipStream_t st) {
-    g.xop = work;
-    g.meta = work + p.xop;
-    g.part = reinterpret_cast<float*>(work + p.xop + p.meta);
-    hipLaunchKernelGGL((kq_w4_split_kernel<P>), dim3((unsigned)((g.nblkp * 64 + 255) / 256), (unsigned)g.ntile),
-                       dim3(256), 0, st, g.a, g.B, g.nblkp, work, work + p.xop);
-    int e = (int)hipGetLastError();
-    if (e) return e;
-    switch (p.M) {
-    case 1: e = launch_mm<P, 1>(g, p, st); break;
-    case 2: e = launch_mm<P, 2>(g, p, st); break;
-    case 3: e = launch_mm<P, 3>(g, p, st); break;
-    case 4: e = launch_mm<P, 4>(g, p, st); break;
-    default: e = launch_mm<P, 5>(g, p, st); break;
-    }
+int launch_mm(MmArg& g, const MmPlan& p, void* work, hipStream_t st) {
+    g.part = static_cast<float*>(work);
+    const int e = p.G == 1 ? launch_mm_g<P, 1>(g, p, st) : p.G == 2 ? launch_mm_g<P, 2>(g, p, st)
+                                                                    : launch_mm_g<P, 4>(g, p, st);
     if (e || g.ks == 1) return e;
     const long n = (long)g.B * g.a.w.N;
     hipLaunchKernelGGL(kq_w4_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g.part, g.a.add,
@@ -740,9 +796,33 @@ bool fill(W4Arg& a, const kq_w4* w) {
     return w->N >= 1 && w->K >= 32 && w->K % 32 == 0;
 }
 
-// LDS bytes of the walk kernel where it takes the call, else -1.
+// LDS bytes of the walk kernel where it takes the call, else -1.  It is ahead
+// with one stream (17408 x 5120 11.5 us against 14.7, int8 rows 11.2 against
+// 13.6) and with two of int8 rows (12.5 / 13.7; 5120 x 17408 13.7 / 18.8), behind
+// with more (binary32, two: 16.2 / 14.8, int8, three: 14.2 / 13.8), but for
+// matrices that are one step of its workgroups, where a launch's latency is what
+// counts (1024 x 1024, int8, four: 4.0 / 4.4).
 long walk_takes(W4Arg& a, int P, int B, int n_cu) {
-    return B <= walk_max_b(P) && a.nblk <= WALK_MAX_BLK ? walk_plan(a, P, B, n_cu) : -1;
+    const bool few = B <= (P == 1 ? 2 : 1) || (B <= walk_max_b(P) && small_matrix(a, n_cu));
+    return few && a.nblk <= WALK_MAX_BLK ? walk_plan(a, P, B, n_cu) : -1;
+}
+
+template <int P, int G, int MODE>
+int raise_mm_m(int bytes) {
+    const void* k[4] = {(const void*)kq_w4_mm_kernel<P, G, MODE, true, true>,
+                        (const void*)kq_w4_mm_kernel<P, G, MODE, true, false>,
+                        (const void*)kq_w4_mm_kernel<P, G, MODE, false, true>,
+                        (const void*)kq_w4_mm_kernel<P, G, MODE, false, false>};
+    for (int i = 0; i < 4; i++) {
+        const int e = (int)hipFuncSetAttribute(k[i], hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e) return e;
+    }
+    return 0;
+}
+template <int P, int G>
+int raise_mm(int bytes) {
+    const int e = raise_mm_m<P, G, M_16>(bytes), f = raise_mm_m<P, G, M_16Z>(bytes), g = raise_mm_m<P, G, M_32Z>(bytes);
+    return e ? e : f ? f : g;
 }
 
 }  // namespace
@@ -751,10 +831,11 @@ extern "C" {
 
 int kqk_w4_set_max_lds(int bytes) {
     g_lds_max = bytes;
-    const int e[7] = {raise_lds<1, 1>(bytes), raise_lds<1, 2>(bytes), raise_lds<1, 3>(bytes),
+    const int e[13] = {raise_lds<1, 1>(bytes), raise_lds<1, 2>(bytes), raise_lds<1, 3>(bytes),
                       raise_lds<1, 4>(bytes), raise_lds<3, 1>(bytes), raise_lds<3, 2>(bytes),
-                      raise_lds<3, 3>(bytes)};
-    for (int i = 0; i < 7; i++)
+                      raise_lds<3, 3>(bytes), raise_mm<1, 1>(bytes), raise_mm<1, 2>(bytes),
+                       raise_mm<1, 4>(bytes), raise_mm<3, 1>(bytes), raise_mm<3, 2>(bytes), raise_mm<3, 4>(bytes)};
+    for (int i = 0; i < 13; i++)
         if (e[i]) return e[i];
     return 0;
 }
@@ -766,7 +847,7 @@ int64_t kqk_w4_workspace(const kq_w4* w, int B, int q8, int n_cu) {
     if (walk_takes(g.a, q8 ? 1 : 3, B, n_cu) > 0) return 0;
     g.B = B;
     mm_plan(g, q8 ? 1 : 3, n_cu, &p);
-    return p.xop + p.meta + p.part;
+    return p.part;
 }
 
 int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float* xs,
@@ -780,8 +861,7 @@ int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float*
     if (lds > 0) return xq ? launch_walk_b<1>(a, B, lds, st) : launch_walk_b<3>(a, B, lds, st);
     g.B = B;
     mm_plan(g, xq ? 1 : 3, n_cu, &p);
-    uint8_t* const ws = static_cast<uint8_t*>(work);
-    return xq ? launch_mm_all<1>(g, p, ws, st) : launch_mm_all<3>(g, p, ws, st);
+    return xq ? launch_mm<1>(g, p, work, st) : launch_mm<3>(g, p, work, st);
 }
 
 }
