@@ -11,8 +11,10 @@
 // and a token changes where one of them moves past u.
 //
 // Launches: the rows' maxima and sums of exponentials per chunk of CH tokens
-// (logits and greedy form); the weights' sums per chunk of the row drawn
-// from; the token.
+// (logits and greedy form); then the weights' sums per chunk of the row drawn
+// from, and, by the workgroup that ends a sequence's last, the token.  (The
+// count of ended ones is cleared by the first launch; probabilities, which need
+// no first launch, draw in a launch of their own instead.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -22,7 +24,9 @@
 
 namespace {
 
-constexpr int CH = 4096, TH = 256, PER = CH / TH;
+constexpr int TH = 256, NJ = 4, CH = 4 * NJ * TH;    // lanes; steps of 4 tokens a lane; tokens of a chunk
+constexpr int SUB = 256, NSUB = CH / SUB;            // a chunk's parts: a wave's step
+constexpr double LOG2E = 1.4426950408889634;
 
 struct VfArg {
     kq_spec_verify v;
@@ -30,8 +34,35 @@ struct VfArg {
     float* pmax;            // [rows][nch]
     double* psum;           // [rows][nch]
     int* parg;              // [rows][nch]
-    double* wsum;           // [S][2][nch]: of max(p - q, 0); of p
+    int nsum;               // nch + nch * NSUB
+    double* wsum;           // [S][nsum]: weights' sums per chunk, then per part of 256 tokens
+    int* ended;             // [S]: workgroups of the second launch that are done
 };
+
+// 2^y for y <= 0, nothing for NaN and below 2^-1000: y = k + r, |r| <= 1/2, and
+// the polynomial of degree 8 that meets 2^r at the nine Chebyshev points of that
+// interval, within 1.1e-12 of it.  k comes as the low bits of y + 1.5 * 2^52 and
+// goes into the exponent as an integer: binary64's round, convert and ldexp
+// instructions take several times a multiply-add's time.  18 instructions a value
+// bound the first launch (240 rows of 151936: with exp() 77 us, with those
+// instructions 34).
+__device__ __forceinline__ double pow2(double y) {
+    constexpr double C[9] = {
+        0x1.0000000000000p+0, 0x1.62e42fef84ceap-1, 0x1.ebfbdff823dddp-3,
+        0x1.c6b08dd6fdf85p-5, 0x1.3b2ab71805844p-7, 0x1.5d8745a62da0ep-10,
+        0x1.4308acadc0000p-13, 0x1.00dc4af70e38ep-16, 0x1.63d109578e38ep-20};
+    constexpr double MAGIC = 0x1.8p52;
+    const double t = y + MAGIC, r = y - (t - MAGIC);
+    double p = C[8];
+#pragma unroll
+    for (int i = 7; i >= 0; i--) p = fma(p, r, C[i]);
+    const int hi = __double2hiint(p) + (__double2loint(t) << 20);
+    return y > -1000.0 ? __hiloint2double(hi, __double2loint(p)) : 0.0;
+}
+
+// 4 values at any 4-byte alignment
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // rows of the chunk tables: target rows first, then the draft's
 __device__ __forceinline__ int trow(const VfArg& a, int s, int i) { return s * (a.v.T + 1) + i; }
@@ -48,87 +79,188 @@ __device__ __forceinline__ const float* draft_row(const VfArg& a, int s, int i) 
     return a.v.draft + s * a.v.draft_seq + i * a.v.draft_row;
 }
 
-// a chunk's maximum, its first place, and the sum of exp((l - max) inv_temp)
+// 4 tokens from k on, `fill` behind the end
+__device__ __forceinline__ f32x4 load4(const float* row, int k, int V, float fill) {
+    f32x4 x;
+    if (k + 4 <= V) {
+        x = *reinterpret_cast<const f32x4u*>(row + k);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = k + e < V ? row[k + e] : fill;
+    }
+    return x;
+}
+
+// a lane's NJ times 4 tokens of a chunk: base + 4 (TH j + tid) .. + 3
+struct Chunk {
+    f32x4 v[NJ];
+    __device__ __forceinline__ void load(const float* row, int base, int V, float fill) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) v[j] = load4(row, base + 4 * (TH * j + (int)threadIdx.x), V, fill);
+    }
+    // the first four; the others move up.  (Loops over j stay loops: their code
+    // is read from memory once a launch, which at few rows is most of its time.)
+    __device__ __forceinline__ f32x4 next() {
+        const f32x4 f = v[0];
+#pragma unroll
+        for (int j = 0; j < NJ - 1; j++) v[j] = v[j + 1];
+        return f;
+    }
+};
+
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+    const int lo = __builtin_amdgcn_mov_dpp(__double2loint(v), CTRL, 0xf, 0xf, false);
+    const int hi = __builtin_amdgcn_mov_dpp(__double2hiint(v), CTRL, 0xf, 0xf, false);
+    return __hiloint2double(hi, lo);
+}
+// sums over 16 lanes and over a wave, in every lane
+__device__ __forceinline__ double sum16(double v) {
+    v = v + dpp<0xB1>(v);                   // quad_perm [1, 0, 3, 2]
+    v = v + dpp<0x4E>(v);                   // quad_perm [2, 3, 0, 1]
+    v = v + dpp<0x141>(v);                  // row_half_mirror
+    return v + dpp<0x140>(v);               // row_mirror
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v = sum16(v);
+    const uint32_t l = (uint32_t)__double2loint(v), h = (uint32_t)__double2hiint(v);
+    const auto l1 = __builtin_amdgcn_permlane16_swap(l, l, false, false);    // rows 0, 0, 2, 2 and 1, 1, 3, 3
+    const auto h1 = __builtin_amdgcn_permlane16_swap(h, h, false, false);
+    v = __hiloint2double((int)h1[0], (int)l1[0]) + __hiloint2double((int)h1[1], (int)l1[1]);
+    const uint32_t m = (uint32_t)__double2loint(v), g = (uint32_t)__double2hiint(v);
+    const auto l2 = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+    const auto h2 = __builtin_amdgcn_permlane32_swap(g, g, false, false);
+    return __hiloint2double((int)h2[0], (int)l2[0]) + __hiloint2double((int)h2[1], (int)l2[1]);
+}
+// what `v` of another lane is, 0 where there is none or the row is not in `ROWS`
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double from(double v) {
+    return __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, ROWS, 0xf, false),
+                            __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+    return fmaxf(v, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), CTRL, 0xf, 0xf, false)));
+}
+__device__ __forceinline__ float max16(float v) {
+    return dpp_max<0x140>(dpp_max<0x141>(dpp_max<0x4E>(dpp_max<0xB1>(v))));
+}
+
+// A chunk's maximum, its first place, and the sum of exp((l - max) inv_temp).
+// BULK: unrolled, for grids that fill the device several times (240 rows of
+// 151936 %%BULK%%; 5 rows, a loop 2.9 us, unrolled 3.4).
+template <bool GREEDY, bool BULK>
 __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
     __shared__ float sm[TH / 64];
     __shared__ int si[TH / 64];
     __shared__ double sd[TH / 64];
     const int T = a.v.T, row = blockIdx.y, nt = a.v.S * (T + 1), tid = threadIdx.x;
+    if (!GREEDY && blockIdx.x == 0 && row < a.v.S && tid == 0) a.ended[row] = 0;
     const bool isd = row >= nt;
     const int s = isd ? (row - nt) / T : row / (T + 1), i = isd ? (row - nt) % T : row % (T + 1);
     if (isd ? i >= drafted(a, s) : i > drafted(a, s)) return;
-    const float* l = isd ? draft_row(a, s, i) : target_row(a, s, i);
-    const int lo = blockIdx.x * CH, hi = min(a.v.V - lo, CH) + lo;
+    const int base = blockIdx.x * CH;
+    Chunk v;
+    v.load(isd ? draft_row(a, s, i) : target_row(a, s, i), base, a.v.V, -INFINITY);
     float m = -INFINITY;
-    int at = 0x7fffffff;
-    for (int k = lo + tid; k < hi; k += TH)
-        if (l[k] > m) { m = l[k]; at = k; }
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const float om = __shfl_xor(m, off);
-        const int oa = __shfl_xor(at, off);
-        if (om > m || (om == m && oa < at)) { m = om; at = oa; }
-    }
-    if ((tid & 63) == 0) { sm[tid >> 6] = m; si[tid >> 6] = at; }
-    __syncthreads();
-    m = sm[0]; at = si[0];
-    for (int k = 1; k < TH / 64; k++)
-        if (sm[k] > m || (sm[k] == m && si[k] < at)) { m = sm[k]; at = si[k]; }
+    for (int j = 0; j < NJ; j++)                                // (a NaN is never the maximum)
+        m = fmaxf(m, fmaxf(fmaxf(v.v[j][0], v.v[j][1]), fmaxf(v.v[j][2], v.v[j][3])));
+    const float mine = m;
+    m = max16(m);
+    m = fmaxf(m, __shfl_xor(m, 16));
+    m = fmaxf(m, __shfl_xor(m, 32));
     const long o = (long)row * a.nch + blockIdx.x;
-    if (tid == 0) { a.pmax[o] = m; a.parg[o] = at; }
-    if (a.v.flags & KQ_VERIFY_GREEDY) return;
+    if (GREEDY) {
+        int at = 0x7fffffff;
+        if (mine == m && m > -INFINITY) {
+#pragma unroll
+            for (int k = 4 * NJ - 1; k >= 0; k--)
+                if (v.v[k / 4][k % 4] == m) at = base + 4 * (TH * (k / 4) + tid) + k % 4;
+        }
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) at = min(at, __shfl_xor(at, off));
+        if ((tid & 63) == 0) { sm[tid >> 6] = m; si[tid >> 6] = at; }
+        __syncthreads();
+        m = sm[0]; at = si[0];
+        for (int k = 1; k < TH / 64; k++)
+            if (sm[k] > m || (sm[k] == m && si[k] < at)) { m = sm[k]; at = si[k]; }
+        if (tid == 0) { a.pmax[o] = m; a.parg[o] = at; }
+        return;
+    }
+    const double c = a.v.inv_temp * LOG2E, mc = m * c;
     double z = 0.0;
-    for (int k = lo + tid; k < hi; k += TH) {
-        const double e = exp(((double)l[k] - (double)m) * (double)a.v.inv_temp);
-        if (e > 0.0) z = z + e;                     // a NaN weighs nothing
-    }
+    if (BULK) {
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) z = z + __shfl_xor(z, off);
-    if ((tid & 63) == 0) sd[tid >> 6] = z;
+        for (int j = 0; j < NJ; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) z = z + pow2(fma((double)v.v[j][e], c, -mc));
+    } else {
+#pragma unroll 1
+        for (int j = 0; j < NJ; j++) {
+            const f32x4 x = v.next();
+#pragma unroll
+            for (int e = 0; e < 4; e++) z = z + pow2(fma((double)x[e], c, -mc));
+        }
+    }
+    z = wave_sum(z);
+    if ((tid & 63) == 0) { sm[tid >> 6] = m; sd[tid >> 6] = z; }
     __syncthreads();
-    if (tid == 0) a.psum[o] = (sd[0] + sd[1]) + (sd[2] + sd[3]);
-}
-
-// one wave: a row's maximum and sum from its chunks
-__device__ __forceinline__ void row_stats(const VfArg& a, int row, float* m, double* z) {
-    const int lane = threadIdx.x & 63;
-    const long o = (long)row * a.nch;
-    float mm = -INFINITY;
-    for (int c = lane; c < a.nch; c += 64) mm = fmaxf(mm, a.pmax[o + c]);
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) mm = fmaxf(mm, __shfl_xor(mm, off));
-    double t = 0.0;
-    for (int c = lane; c < a.nch; c += 64) {
-        const double e = exp(((double)a.pmax[o + c] - (double)mm) * (double)a.v.inv_temp);
-        if (e > 0.0) t = t + e * a.psum[o + c];
+    if (tid < 4) {                          // the waves' sums on one maximum
+        const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
+        z = pow2(((double)sm[tid] - (double)mm) * c) * sd[tid];
+        z = z + dpp<0xB1>(z);
+        z = z + dpp<0x4E>(z);
+        if (tid == 0) {
+            a.pmax[o] = mm;
+            a.psum[o] = z;
+        }
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) t = t + __shfl_xor(t, off);
-    *m = mm;
-    *z = t;
 }
 
-// The weight of token k at the row drawn from, and its p.
+// 16 lanes: a row's maximum and sum from its chunks
+__device__ __forceinline__ void row_stats(const VfArg& a, int row, float* m, double* z) {
+    const int lane = threadIdx.x & 15;
+    const long o = (long)row * a.nch;
+    const double c = a.v.inv_temp * LOG2E;
+    float mm = -INFINITY;
+    double t = 0.0;
+#pragma unroll 1
+    for (int k0 = lane; k0 < a.nch; k0 += 64) {
+        float pm[4], was = mm;
+        double ps[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const bool in = k0 + 16 * k < a.nch;
+            pm[k] = in ? a.pmax[o + k0 + 16 * k] : -INFINITY;
+            ps[k] = in ? a.psum[o + k0 + 16 * k] : 0.0;
+        }
+        mm = fmaxf(fmaxf(fmaxf(mm, pm[0]), pm[1]), fmaxf(pm[2], pm[3]));
+        t = t * pow2(((double)was - (double)mm) * c);
+#pragma unroll
+        for (int k = 0; k < 4; k++) t = fma(pow2(((double)pm[k] - (double)mm) * c), ps[k], t);
+    }
+    const float top = max16(mm);
+    *z = sum16(t * pow2(((double)mm - (double)top) * c));
+    *m = top;
+}
+
+// The weight of a token at the row drawn from.
 struct Drawn {
     const float* p;
     const float* q;         // NULL: one-hot, or nothing refused
     int hot;                // one-hot draft's token, or -1
     bool logits;
-    float pm, qm;
-    double pz, qz, it;      // 1 / sums; inv_temp
-    __device__ __forceinline__ void at(int k, double* r, double* w) const {
-        double pv, qv = 0.0;
+    double pm, qm;
+    double pz, qz, c;       // 1 / sums; inv_temp / ln 2
+    __device__ __forceinline__ double at(int k, float pk, float qk) const {
+        double pv = pk, qv = qk;
         if (logits) {
-            pv = exp(((double)p[k] - (double)pm) * it) * pz;
-            if (q) qv = exp(((double)q[k] - (double)qm) * it) * qz;
-        } else {
-            pv = (double)p[k];
-            if (q) qv = (double)q[k];
+            pv = pow2((pv - pm) * c) * pz;
+            if (q) qv = pow2((qv - qm) * c) * qz;
         }
-        pv = pv > 0.0 ? pv : 0.0;
-        const double d = pv - (qv > 0.0 ? qv : 0.0);
-        *w = pv;
-        *r = k == hot || !(d > 0.0) ? 0.0 : d;
+        pv = fmax(pv, 0.0);                 // (NaN: nothing)
+        return k == hot ? 0.0 : q ? fmax(pv - fmax(qv, 0.0), 0.0) : pv;
     }
 };
 
@@ -139,9 +271,20 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
     __shared__ int sn;
     const int T = a.v.T, nd = drafted(a, s), tid = threadIdx.x;
     const bool lg = a.v.flags & KQ_VERIFY_LOGITS, dr = a.v.draft != nullptr;
-    const double it = a.v.inv_temp;
+    const double c = a.v.inv_temp * LOG2E;
+    // the drafted tokens' own values, asked for before the sums are known
+    int tok = -1;
+    float pt = 0.0f, qt = 0.0f, ut = 0.0f;
+    if (tid < nd) {
+        tok = a.v.tokens[s * T + tid];
+        ut = a.v.u[s * (T + 1) + tid];
+        if (tok >= 0 && tok < a.v.V) {
+            pt = target_row(a, s, tid)[tok];
+            if (dr) qt = draft_row(a, s, tid)[tok];
+        }
+    }
     if (lg) {
-        for (int j = tid >> 6; j < 2 * T + 1; j += TH / 64) {
+        for (int j = tid >> 4; j < 2 * T + 1; j += (int)blockDim.x / 16) {
             const bool isd = j > T;
             const int i = isd ? j - T - 1 : j;
             if (isd ? !dr || i >= nd : i > nd) continue;
@@ -154,19 +297,14 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
         __syncthreads();
     }
     if (tid < 64) {
-        bool no = tid >= nd;
-        if (tid < nd) {
-            const int t = a.v.tokens[s * T + tid];
-            if (t < 0 || t >= a.v.V) {
-                no = true;
-            } else {
-                double p = target_row(a, s, tid)[t], q = dr ? draft_row(a, s, tid)[t] : 1.0;
-                if (lg) {
-                    p = exp((p - (double)mx[tid]) * it) * zs[tid];
-                    if (dr) q = exp((q - (double)mx[T + 1 + tid]) * it) * zs[T + 1 + tid];
-                }
-                no = !((double)a.v.u[s * (T + 1) + tid] * q < p);
+        bool no = tid >= nd || tok < 0 || tok >= a.v.V;
+        if (!no) {
+            double p = pt, q = dr ? qt : 1.0;
+            if (lg) {
+                p = pow2((p - (double)mx[tid]) * c) * zs[tid];
+                if (dr) q = pow2((q - (double)mx[T + 1 + tid]) * c) * zs[T + 1 + tid];
             }
+            no = !((double)ut * q < p);
         }
         const unsigned long long b = __ballot(no);
         if (tid == 0) sn = b ? __ffsll(b) - 1 : 64;
@@ -178,7 +316,7 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
     d.q = n < nd && dr ? draft_row(a, s, n) : nullptr;
     d.hot = n < nd && !dr ? a.v.tokens[s * T + n] : -1;
     d.logits = lg;
-    d.it = it;
+    d.c = c;
     d.pm = lg ? mx[n] : 0.0f;
     d.pz = lg ? zs[n] : 0.0;
     d.qm = lg && d.q ? mx[T + 1 + n] : 0.0f;
@@ -187,131 +325,153 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
     return d;
 }
 
+__device__ __forceinline__ void draw(const VfArg& a, int s, int n, Drawn d);
+
+// DRAW: the sequence's last workgroup draws
+template <bool DRAW>
 __global__ __launch_bounds__(TH) void kq_vf_weights_kernel(VfArg a) {
-    __shared__ double sd[2][TH / 64];
-    const int s = blockIdx.y, tid = threadIdx.x;
+    __shared__ double sd[TH / 64];
+    __shared__ int last;
+    const int s = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CH;
     int n;
     const Drawn d = decide(a, s, &n);
-    const int lo = blockIdx.x * CH, hi = min(a.v.V - lo, CH) + lo;
-    double r = 0.0, w = 0.0;
-    for (int k = lo + tid; k < hi; k += TH) {
-        double rk, wk;
-        d.at(k, &rk, &wk);
-        r = r + rk;
-        w = w + wk;
-    }
+    const float none = d.logits ? -INFINITY : 0.0f;
+    Chunk p, q;
+    p.load(d.p, base, a.v.V, none);
+    if (d.q) q.load(d.q, base, a.v.V, none);
+    // (stores past this XCD's L2, where the last workgroup does not look)
+    double* const sums = a.wsum + (long)s * a.nsum;
+    double* const parts = sums + a.nch + (long)blockIdx.x * NSUB + (tid >> 6);
+    double w = 0.0;
+#pragma unroll 1
+    for (int j = 0; j < NJ; j++) {
+        const f32x4 pv = p.next(), qv = d.q ? q.next() : pv;
+        double wj = 0.0;
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        r = r + __shfl_xor(r, off);
-        w = w + __shfl_xor(w, off);
+        for (int e = 0; e < 4; e++) wj = wj + d.at(base + 4 * (TH * j + tid) + e, pv[e], qv[e]);
+        wj = wave_sum(wj);
+        if ((tid & 63) == 0) __hip_atomic_store(parts + 4 * j, wj, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        w = w + wj;
     }
-    if ((tid & 63) == 0) { sd[0][tid >> 6] = r; sd[1][tid >> 6] = w; }
+    if ((tid & 63) == 0) sd[tid >> 6] = w;
     __syncthreads();
-    if (tid < 2)
-        a.wsum[(2 * (long)s + tid) * a.nch + blockIdx.x] =
-            (sd[tid][0] + sd[tid][1]) + (sd[tid][2] + sd[tid][3]);
+    if (tid == 0) {
+        __hip_atomic_store(sums + blockIdx.x, (sd[0] + sd[1]) + (sd[2] + sd[3]), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+        if (DRAW)
+            last = __hip_atomic_fetch_add(a.ended + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.nch - 1;
+    }
+    if (!DRAW) return;
+    __syncthreads();
+    if (last && tid < 64) draw(a, s, n, d);
 }
 
 // inclusive running sum over a wave's lanes
 __device__ __forceinline__ double wave_scan(double v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const double o = __shfl_up(v, off);
-        if (lane >= off) v = v + o;
-    }
-    return v;
+    v = v + from<0x111, 0xf>(v);            // row_shr 1, 2, 4, 8
+    v = v + from<0x112, 0xf>(v);
+    v = v + from<0x114, 0xf>(v);
+    v = v + from<0x118, 0xf>(v);
+    v = v + from<0x142, 0xa>(v);            // row_bcast 15: a row's end to the next, to rows 1 and 3
+    return v + from<0x143, 0xc>(v);         // row_bcast 31: to rows 2 and 3
 }
 
-// One workgroup per sequence: the chunk in which the running sum passes u
-// times the total, then the token in it.
-__global__ __launch_bounds__(TH) void kq_vf_draw_kernel(VfArg a) {
-    __shared__ double incl[TH];
-    __shared__ double sbase, starget;
-    __shared__ int schunk, sbest, slast;
-    const int s = blockIdx.x, T = a.v.T, tid = threadIdx.x, lane = tid & 63;
+// One step of looking for what a running sum passes `target` in: 64 values, one a
+// lane, after `sum`.  The lane of the first at which it is above the target, else
+// of the last that is not nothing (and `found` stays false); -1 if all are.
+// `base`: the sum before that one.
+__device__ __forceinline__ int passed(double v, double target, double& sum, double& base, bool& found) {
+    const int lane = threadIdx.x & 63;
+    const double in = sum + wave_scan(v);
+    const double prev = from<0x138, 0xf>(in);                  // wave_shr 1, by every lane
+    const double ex = lane ? prev : sum;
+    const unsigned long long over = __ballot(v > 0.0 && in > target), some = __ballot(v > 0.0);
+    sum = __shfl(in, 63);
+    found = over != 0;
+    if (!some) return -1;
+    const int j = over ? __ffsll(over) - 1 : 63 - __clzll(some);
+    base = __shfl(ex, j);
+    return j;
+}
+
+// One wave: the chunk, its part and the token in which the running sum passes u
+// times the total.
+__device__ __forceinline__ void draw(const VfArg& a, int s, int n, Drawn d) {
+    const int T = a.v.T, lane = threadIdx.x & 63;
+    const double* const ws = a.wsum + (long)s * a.nsum;
+    auto sum = [&](int k, int end) {
+        return k < end ? __hip_atomic_load(ws + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0;
+    };
+    const float u = a.v.u[s * (T + 1) + T], none = d.logits ? -INFINITY : 0.0f;
+    // the first 64 chunks' sums stay in registers (most vocabularies have fewer)
+    const double v0 = sum(lane, a.nch);
+    double total = wave_sum(v0);
+#pragma unroll 1
+    for (int c0 = 64; c0 < a.nch; c0 += 64) total = total + wave_sum(sum(c0 + lane, a.nch));
+    double target = (double)u * total, run = 0.0, base = 0.0;
+    bool found = false;
+    int token = -1, k0 = 0, end = 0;         // 256 tokens at a time, [k0, end)
+    if (total > 0.0) {
+        int chunk = passed(v0, target, run, base, found);
+#pragma unroll 1
+        for (int c0 = 64; c0 < a.nch && !found; c0 += 64) {
+            const int j = passed(sum(c0 + lane, a.nch), target, run, base, found);
+            if (j >= 0) chunk = c0 + j;
+        }
+        run = base;
+        const int first = a.nch + chunk * NSUB;
+        const int part = max(0, passed(lane < NSUB ? sum(first + lane, a.nsum) : 0.0, target, run, base, found));
+        k0 = chunk * CH + part * SUB;
+        end = k0 + 1;
+    } else if (d.q || d.hot >= 0) {
+        // Nothing is left of p - q: a token refused though p and q are equal (u =
+        // 1, or values that are no distributions).  From p itself then, by this
+        // wave alone: its sum, and the token.
+        d.q = nullptr;
+        d.hot = -1;
+        end = a.v.V;
+#pragma unroll 1
+        for (int k = 4 * lane; k - 4 * lane < end; k += 256) {
+            const f32x4 pv = load4(d.p, k, a.v.V, none);
+            total = total + wave_sum((d.at(k, pv[0], 0.0f) + d.at(k + 1, pv[1], 0.0f)) +
+                                     (d.at(k + 2, pv[2], 0.0f) + d.at(k + 3, pv[3], 0.0f)));
+        }
+        target = (double)u * total;
+    }
+    run = base;
+    found = false;
+#pragma unroll 1
+    for (; k0 < end && !found; k0 += 256) {
+        const int k = k0 + 4 * lane;         // 4 tokens a lane
+        const f32x4 pv = load4(d.p, k, a.v.V, none), qv = d.q ? load4(d.q, k, a.v.V, none) : pv;
+        double w4[4], w = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w4[e] = d.at(k + e, pv[e], qv[e]);
+            w = w + w4[e];
+        }
+        const int who = passed(w, target, run, base, found);
+        // that lane's token: until the sum is past the target
+        int at = -1;
+        double cum = base;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (w4[e] > 0.0 && !(cum > target)) {
+                cum = cum + w4[e];
+                at = k + e;
+            }
+        if (who >= 0) token = __shfl(at, who);
+    }
+    int* const out = a.v.out + (long)s * (T + 1);
+    if (lane < n) out[lane] = a.v.tokens[s * T + lane];
+    if (lane >= n && lane <= T) out[lane] = lane == n ? token : -1;
+    if (lane == 0) a.v.n_accept[s] = n;
+}
+
+__global__ __launch_bounds__(64) void kq_vf_draw_kernel(VfArg a) {
     int n;
-    const Drawn d = decide(a, s, &n);
-    const double* ws = a.wsum + 2 * (long)s * a.nch;
-    double tot = 0.0;
-    for (int c0 = 0; c0 < a.nch; c0 += 64)
-        tot = tot + __shfl(wave_scan(c0 + lane < a.nch ? ws[c0 + lane] : 0.0), 63);
-    const bool left = tot > 0.0;             // else p itself: p and q are equal here
-    if (!left) ws += a.nch;
-    if (tid < 64) {
-        double base = 0.0, cbase = 0.0, total = 0.0;
-        for (int c0 = 0; c0 < a.nch; c0 += 64)
-            total = total + __shfl(wave_scan(c0 + lane < a.nch ? ws[c0 + lane] : 0.0), 63);
-        const double target = (double)a.v.u[s * (T + 1) + T] * total;
-        int chunk = -1;
-        for (int c0 = 0; c0 < a.nch; c0 += 64) {
-            const double v = c0 + lane < a.nch ? ws[c0 + lane] : 0.0;
-            const double in = base + wave_scan(v);
-            double ex = __shfl_up(in, 1);
-            if (lane == 0) ex = base;
-            const unsigned long long over = __ballot(v > 0.0 && in > target);
-            const unsigned long long some = __ballot(v > 0.0);
-            if (over) {
-                const int j = __ffsll(over) - 1;
-                chunk = c0 + j;
-                cbase = __shfl(ex, j);
-                break;
-            }
-            if (some) {                      // the last one with any weight
-                const int j = 63 - __clzll(some);
-                chunk = c0 + j;
-                cbase = __shfl(ex, j);
-            }
-            base = __shfl(in, 63);
-        }
-        if (tid == 0) {
-            schunk = chunk;
-            sbase = cbase;
-            starget = target;
-            sbest = TH;
-            slast = -1;
-        }
-    }
-    __syncthreads();
-    int token = -1;
-    if (schunk >= 0) {
-        const int lo = schunk * CH + tid * PER, hi = min(a.v.V, lo + PER);
-        double sum = 0.0, v[PER];
-#pragma unroll
-        for (int j = 0; j < PER; j++) {
-            double rk = 0.0, wk = 0.0;
-            if (lo + j < hi) d.at(lo + j, &rk, &wk);
-            v[j] = left ? rk : wk;
-            sum = sum + v[j];
-        }
-        const double ws1 = wave_scan(sum);
-        if (lane == 63) incl[tid >> 6] = ws1;
-        __syncthreads();
-        double before = sbase;
-        for (int k = 0; k < tid >> 6; k++) before = before + incl[k];
-        const double in = before + ws1;
-        __syncthreads();
-        incl[tid] = in;
-        if (sum > 0.0 && in > starget) atomicMin(&sbest, tid);
-        if (sum > 0.0) atomicMax(&slast, tid);
-        __syncthreads();
-        const int who = sbest < TH ? sbest : slast;
-        if (tid == who) {
-            double cum = tid ? incl[tid - 1] : sbase;
-#pragma unroll
-            for (int j = 0; j < PER; j++)
-                if (v[j] > 0.0 && !(cum > starget)) {
-                    cum = cum + v[j];
-                    token = lo + j;
-                }
-            a.v.out[s * (T + 1) + n] = token;
-        }
-    } else if (tid == 0) {
-        a.v.out[s * (T + 1) + n] = -1;
-    }
-    if (tid < n) a.v.out[s * (T + 1) + tid] = a.v.tokens[s * T + tid];
-    if (tid > n && tid <= T) a.v.out[s * (T + 1) + tid] = -1;
-    if (tid == 0) a.v.n_accept[s] = n;
+    const Drawn d = decide(a, blockIdx.x, &n);
+    draw(a, blockIdx.x, n, d);
 }
 
 // The greedy form: a token is accepted iff it is its row's first maximum.
@@ -344,20 +504,23 @@ int64_t layout(const kq_spec_verify* v, VfArg* a, uint8_t* w) {
     const int64_t nch = ((int64_t)v->V + CH - 1) / CH;
     const bool stats = v->flags & (KQ_VERIFY_LOGITS | KQ_VERIFY_GREEDY);
     const int64_t rows = stats ? (int64_t)v->S * (v->T + 1) + (v->draft ? (int64_t)v->S * v->T : 0) : 0;
-    int64_t o[5] = {0};
+    int64_t o[6] = {0};
     o[1] = o[0] + up256(rows * nch * 8);              // psum
     o[2] = o[1] + up256(rows * nch * 4);              // pmax
     o[3] = o[2] + up256(rows * nch * 4);              // parg
-    o[4] = o[3] + up256(2 * (int64_t)v->S * nch * 8); // wsum
+    o[4] = o[3] + up256((int64_t)v->S * nch * (1 + NSUB) * 8);   // wsum
     if (a) {
         a->v = *v;
         a->nch = (int)nch;
+        a->nsum = (int)nch * (1 + NSUB);
         a->psum = (double*)(w + o[0]);
         a->pmax = (float*)(w + o[1]);
         a->parg = (int*)(w + o[2]);
         a->wsum = (double*)(w + o[3]);
+        a->ended = (int*)(w + o[4]);
     }
-    return o[4];
+    o[5] = o[4] + up256((int64_t)v->S * 4);           // ended
+    return o[5];
 }
 
 }  // namespace
@@ -371,16 +534,22 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st) {
         return (int)hipErrorInvalidValue;
     VfArg a;
     layout(v, &a, static_cast<uint8_t*>(work));
-    const bool greedy = v->flags & KQ_VERIFY_GREEDY;
-    if (v->flags & (KQ_VERIFY_LOGITS | KQ_VERIFY_GREEDY)) {
-        const int rows = v->S * (v->T + 1) + (v->draft && !greedy ? v->S * v->T : 0);
-        hipLaunchKernelGGL(kq_vf_stats_kernel, dim3((unsigned)a.nch, (unsigned)rows), dim3(TH), 0, st, a);
+    const bool greedy = v->flags & KQ_VERIFY_GREEDY, logits = v->flags & KQ_VERIFY_LOGITS;
+    const dim3 chunks((unsigned)a.nch, (unsigned)v->S), wg(TH), seqs((unsigned)v->S);
+    if (greedy || logits) {
+        const dim3 grid((unsigned)a.nch, (unsigned)(v->S * (v->T + 1) + (v->draft && !greedy ? v->S * v->T : 0)));
+        const bool bulk = (long)grid.x * grid.y >= 4096;
+        if (greedy) hipLaunchKernelGGL((kq_vf_stats_kernel<true, true>), grid, wg, 0, st, a);
+        else if (bulk) hipLaunchKernelGGL((kq_vf_stats_kernel<false, true>), grid, wg, 0, st, a);
+        else hipLaunchKernelGGL((kq_vf_stats_kernel<false, false>), grid, wg, 0, st, a);
     }
     if (greedy) {
-        hipLaunchKernelGGL(kq_vf_greedy_kernel, dim3((unsigned)v->S), dim3(64), 0, st, a);
+        hipLaunchKernelGGL(kq_vf_greedy_kernel, seqs, dim3(64), 0, st, a);
+    } else if (logits) {
+        hipLaunchKernelGGL(kq_vf_weights_kernel<true>, chunks, wg, 0, st, a);
     } else {
-        hipLaunchKernelGGL(kq_vf_weights_kernel, dim3((unsigned)a.nch, (unsigned)v->S), dim3(TH), 0, st, a);
-        hipLaunchKernelGGL(kq_vf_draw_kernel, dim3((unsigned)v->S), dim3(TH), 0, st, a);
+        hipLaunchKernelGGL(kq_vf_weights_kernel<false>, chunks, wg, 0, st, a);
+        hipLaunchKernelGGL(kq_vf_draw_kernel, seqs, dim3(64), 0, st, a);
     }
     return (int)hipGetLastError();
 }
