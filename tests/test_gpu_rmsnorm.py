@@ -212,3 +212,18 @@ def test_captured_and_on_another_stream():
         torch.cuda.synchronize()
         assert torch.equal(got[0], q) and torch.equal(got[1], sc) and torch.equal(got[2], sm)
         assert np.array_equal(sm.cpu().numpy(), (x * np.float32(i + 1) + r))
+
+
+def test_rows_past_32_bits():
+    """Row strides that put the second row past 2^32 bytes, and the fourth past 2^32 elements."""
+    n, stride = 1000, (1 << 30) + 4
+    buf = torch.empty(4 * stride, device="cuda")
+    rows4 = buf.view(4, stride)[:, :n]
+    x = np.random.default_rng(50).standard_normal((4, n)).astype(np.float32)
+    rows4.copy_(torch.from_numpy(x))
+    y = torch.empty(4, n, device="cuda")
+    K.rmsnorm_dev(K.rmsnorm(4, n, 1e-6, buf.data_ptr(), y_ptr=y.data_ptr(), x_stride=stride), st())
+    K.rmsnorm_dev(K.rmsnorm(4, n, 1e-6, buf.data_ptr(), y_ptr=buf.data_ptr(), x_stride=stride, y_stride=stride), st())
+    torch.cuda.synchronize()
+    check_y(y.cpu().numpy(), want(x, None, None, 1e-6)[1])
+    assert torch.equal(rows4, y)

@@ -376,3 +376,48 @@ def test_decode_step():
         for k in range(S):
             n, want = rule(l[k], None, tk[k], T, uu[k], "logits", 1.0)
             assert na[k].item() == n and out[k].tolist() == want
+
+
+@pytest.mark.parametrize("form", ["logits", "probs", "greedy"])
+def test_rows_past_32_bits(form):
+    """Sequences 2^31 elements apart (8 GiB), the draft's rows 2^30."""
+    S, T, V = 2, 1, 5000
+    target, draft, tokens, nd, u = make(S, T, V, form, form != "greedy", 41)
+    nd[:] = T
+    far, row = (1 << 31) + 8, 1 << 30
+    buf = torch.empty(far + 2 * V, device="cuda")
+    for s in range(S):
+        for i in range(T + 1):
+            buf[s * far + i * V:s * far + (i + 1) * V] = torch.from_numpy(target[s, i]).cuda()
+    dbuf = torch.empty(row + V, device="cuda")
+    if draft is not None:
+        for s in range(S):
+            dbuf[s * row:s * row + V] = torch.from_numpy(draft[s, 0]).cuda()
+    tk, du = torch.from_numpy(tokens).cuda(), torch.from_numpy(u).cuda()
+    na, out = torch.empty(S, dtype=torch.int32, device="cuda"), torch.empty(S, T + 1, dtype=torch.int32, device="cuda")
+    v = K.spec_verify(S, T, V, FLAGS[form], buf.data_ptr(), tk.data_ptr(), du.data_ptr(), na.data_ptr(), out.data_ptr(),
+                      draft_ptr=dbuf.data_ptr() if draft is not None else None, target_seq=far, draft_seq=row)
+    nb = K.spec_verify_workspace_bytes(v)
+    work = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    K.spec_verify_dev(v, work.data_ptr(), nb, st())
+    torch.cuda.synchronize()
+    for s in range(S):
+        n, want = rule(target[s], None if draft is None else draft[s], tokens[s], T, u[s], form, 1.0)
+        assert na[s].item() == n and out[s].tolist() == want
+
+
+@pytest.mark.parametrize("form", ["logits", "probs"])
+@pytest.mark.parametrize("draft", [False, True])
+def test_vocabulary_of_many_chunks(form, draft):
+    """More chunks than a wave has lanes: the draw goes over them 64 at a time."""
+    r = np.random.default_rng(42)
+    S, T, V = 3, 2, 700001
+    target = (1.5 * r.standard_normal((S, T + 1, V))).astype(np.float32)
+    d = (target[:, :T] + 0.5 * r.standard_normal((S, T, V))).astype(np.float32)
+    if form == "probs":
+        target = np.stack([[softmax(v, 1.0) for v in row] for row in target]).astype(np.float32)
+        d = np.stack([[softmax(v, 1.0) for v in row] for row in d]).astype(np.float32)
+    tokens = r.integers(0, V, (S, T)).astype(np.int32)
+    u = np.array([[0.9, 0.1, 0.02], [0.5, 0.9, 0.55], [0.9, 0.9, 0.999]], np.float32)
+    check(target, d if draft else None, tokens, np.array([2, 0, 1], np.int32), u, form)

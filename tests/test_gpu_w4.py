@@ -254,3 +254,32 @@ def test_refuses_a_short_workspace():
                 assert rc == -1 and b"workspace" in L.kq_last_error()
             torch.cuda.synchronize()
             assert (y == 3.0).all()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 3, 8])
+def test_matrices_past_4_gib(B, q8):
+    """Offsets past 32 bits: 2.2 M rows of 4096 weights, 4.5 GB.  Repeats of one small matrix, so that
+    every repeat has to give the same bits."""
+    n, Kd, g, reps = 1103, 4096, 128, 2000
+    c = Case(n, Kd, B, g, zeros=True, q8=q8)
+    first = c.check()[:B * n].view(B, n).clone()
+    N = n * reps
+    q, s, z = c.dq.repeat(reps, 1), c.ds.repeat(reps, 1), c.dz.repeat(reps, 1)
+    assert q.numel() > 1 << 32
+    w = K.w4(N, Kd, g, K.TYPE_F16, q.data_ptr(), s.data_ptr(), z.data_ptr())
+    nb = K.w4_workspace_bytes(w, B, q8)
+    work = torch.empty(max(256, nb), dtype=torch.uint8, device="cuda")
+    y = torch.full((B, N), float("nan"), device="cuda")
+    args = (y.data_ptr(), B, work.data_ptr(), nb)
+    if q8:
+        K.w4_gemv_q8_dev(w, c.dxq.data_ptr(), c.dxs.data_ptr(), *args, stream=st())
+    else:
+        K.w4_gemv_dev(w, c.dx.data_ptr(), *args, stream=st())
+    torch.cuda.synchronize()
+    got = y.view(B, reps, n)
+    # (where a matrix is cut depends on its size, and with it the order of a row's sums)
+    want, tol = torch.from_numpy(c.exact).cuda().view(B, 1, n), torch.from_numpy(c.tol(c.exact)).cuda().view(B, 1, n)
+    assert ((got.double() - want).abs() <= tol).all()
+    if B == 1:
+        assert (got == first.view(B, 1, n)).all()
