@@ -37,27 +37,29 @@ struct VfArg {
     int nsum;               // nch + nch * NSUB
     double* wsum;           // [S][nsum]: weights' sums per chunk, then per part of 256 tokens
     int* ended;             // [S]: workgroups of the second launch that are done
+    double c, far;          // inv_temp / ln 2; 2^(d c) is taken for nothing from d = far = -1000 / c down
 };
 
-// 2^y for y <= 0, nothing for NaN and below 2^-1000: y = k + r, |r| <= 1/2, and
-// the polynomial of degree 8 that meets 2^r at the nine Chebyshev points of that
-// interval, within 1.1e-12 of it.  k comes as the low bits of y + 1.5 * 2^52 and
-// goes into the exponent as an integer: binary64's round, convert and ldexp
-// instructions take several times a multiply-add's time.  18 instructions a value
-// bound the first launch (240 rows of 151936: with exp() 77 us, with those
-// instructions 34).
-__device__ __forceinline__ double pow2(double y) {
+// 2^(d c) for d <= 0, nothing for NaN and below 2^-1000: d c = k + r, |r| <= 1/2,
+// and the polynomial of degree 8 that meets 2^r at the nine Chebyshev points of
+// that interval, within 1.1e-12 of it.  d is the difference of two logits, so it
+// is 0 at the maximum whatever that is (a row of the type's lowest value is a
+// uniform one).  k comes as the low bits of d c + 1.5 * 2^52 and goes into the
+// exponent as an integer.  These 18 binary64 instructions a value bound the first
+// launch (sixteen sequences of seven, 240 rows of 151936, both launches: 57 us,
+// with the library's exp2() 76; one of four, 15 and 18).
+__device__ __forceinline__ double pow2(double d, double c, double far) {
     constexpr double C[9] = {
         0x1.0000000000000p+0, 0x1.62e42fef84ceap-1, 0x1.ebfbdff823dddp-3,
         0x1.c6b08dd6fdf85p-5, 0x1.3b2ab71805844p-7, 0x1.5d8745a62da0ep-10,
         0x1.4308acadc0000p-13, 0x1.00dc4af70e38ep-16, 0x1.63d109578e38ep-20};
     constexpr double MAGIC = 0x1.8p52;
-    const double t = y + MAGIC, r = y - (t - MAGIC);
+    const double t = fma(d, c, MAGIC), r = fma(d, c, -(t - MAGIC));
     double p = C[8];
 #pragma unroll
     for (int i = 7; i >= 0; i--) p = fma(p, r, C[i]);
     const int hi = __double2hiint(p) + (__double2loint(t) << 20);
-    return y > -1000.0 ? __hiloint2double(hi, __double2loint(p)) : 0.0;
+    return d > far ? __hiloint2double(hi, __double2loint(p)) : 0.0;
 }
 
 // 4 values at any 4-byte alignment
@@ -147,8 +149,7 @@ __device__ __forceinline__ float max16(float v) {
 }
 
 // A chunk's maximum, its first place, and the sum of exp((l - max) inv_temp).
-// BULK: unrolled, for grids that fill the device several times (240 rows of
-// 151936 %%BULK%%; 5 rows, a loop 2.9 us, unrolled 3.4).
+// BULK: unrolled, for grids that fill the device several times.
 template <bool GREEDY, bool BULK>
 __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
     __shared__ float sm[TH / 64];
@@ -188,19 +189,19 @@ __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
         if (tid == 0) { a.pmax[o] = m; a.parg[o] = at; }
         return;
     }
-    const double c = a.v.inv_temp * LOG2E, mc = m * c;
+    const double top = m;
     double z = 0.0;
     if (BULK) {
 #pragma unroll
         for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) z = z + pow2(fma((double)v.v[j][e], c, -mc));
+            for (int e = 0; e < 4; e++) z = z + pow2((double)v.v[j][e] - top, a.c, a.far);
     } else {
 #pragma unroll 1
         for (int j = 0; j < NJ; j++) {
             const f32x4 x = v.next();
 #pragma unroll
-            for (int e = 0; e < 4; e++) z = z + pow2(fma((double)x[e], c, -mc));
+            for (int e = 0; e < 4; e++) z = z + pow2((double)x[e] - top, a.c, a.far);
         }
     }
     z = wave_sum(z);
@@ -208,7 +209,7 @@ __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
     __syncthreads();
     if (tid < 4) {                          // the waves' sums on one maximum
         const float mm = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-        z = pow2(((double)sm[tid] - (double)mm) * c) * sd[tid];
+        z = pow2((double)sm[tid] - (double)mm, a.c, a.far) * sd[tid];
         z = z + dpp<0xB1>(z);
         z = z + dpp<0x4E>(z);
         if (tid == 0) {
@@ -222,7 +223,6 @@ __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
 __device__ __forceinline__ void row_stats(const VfArg& a, int row, float* m, double* z) {
     const int lane = threadIdx.x & 15;
     const long o = (long)row * a.nch;
-    const double c = a.v.inv_temp * LOG2E;
     float mm = -INFINITY;
     double t = 0.0;
 #pragma unroll 1
@@ -236,12 +236,12 @@ __device__ __forceinline__ void row_stats(const VfArg& a, int row, float* m, dou
             ps[k] = in ? a.psum[o + k0 + 16 * k] : 0.0;
         }
         mm = fmaxf(fmaxf(fmaxf(mm, pm[0]), pm[1]), fmaxf(pm[2], pm[3]));
-        t = t * pow2(((double)was - (double)mm) * c);
+        t = t * pow2((double)was - (double)mm, a.c, a.far);
 #pragma unroll
-        for (int k = 0; k < 4; k++) t = fma(pow2(((double)pm[k] - (double)mm) * c), ps[k], t);
+        for (int k = 0; k < 4; k++) t = fma(pow2((double)pm[k] - (double)mm, a.c, a.far), ps[k], t);
     }
     const float top = max16(mm);
-    *z = sum16(t * pow2(((double)mm - (double)top) * c));
+    *z = sum16(t * pow2((double)mm - (double)top, a.c, a.far));
     *m = top;
 }
 
@@ -252,12 +252,12 @@ struct Drawn {
     int hot;                // one-hot draft's token, or -1
     bool logits;
     double pm, qm;
-    double pz, qz, c;       // 1 / sums; inv_temp / ln 2
+    double pz, qz, c, far;  // 1 / sums
     __device__ __forceinline__ double at(int k, float pk, float qk) const {
         double pv = pk, qv = qk;
         if (logits) {
-            pv = pow2((pv - pm) * c) * pz;
-            if (q) qv = pow2((qv - qm) * c) * qz;
+            pv = pow2(pv - pm, c, far) * pz;
+            if (q) qv = pow2(qv - qm, c, far) * qz;
         }
         pv = fmax(pv, 0.0);                 // (NaN: nothing)
         return k == hot ? 0.0 : q ? fmax(pv - fmax(qv, 0.0), 0.0) : pv;
@@ -271,7 +271,6 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
     __shared__ int sn;
     const int T = a.v.T, nd = drafted(a, s), tid = threadIdx.x;
     const bool lg = a.v.flags & KQ_VERIFY_LOGITS, dr = a.v.draft != nullptr;
-    const double c = a.v.inv_temp * LOG2E;
     // the drafted tokens' own values, asked for before the sums are known
     int tok = -1;
     float pt = 0.0f, qt = 0.0f, ut = 0.0f;
@@ -301,8 +300,8 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
         if (!no) {
             double p = pt, q = dr ? qt : 1.0;
             if (lg) {
-                p = pow2((p - (double)mx[tid]) * c) * zs[tid];
-                if (dr) q = pow2((q - (double)mx[T + 1 + tid]) * c) * zs[T + 1 + tid];
+                p = pow2(p - (double)mx[tid], a.c, a.far) * zs[tid];
+                if (dr) q = pow2(q - (double)mx[T + 1 + tid], a.c, a.far) * zs[T + 1 + tid];
             }
             no = !((double)ut * q < p);
         }
@@ -316,7 +315,8 @@ __device__ __forceinline__ Drawn decide(const VfArg& a, int s, int* nacc) {
     d.q = n < nd && dr ? draft_row(a, s, n) : nullptr;
     d.hot = n < nd && !dr ? a.v.tokens[s * T + n] : -1;
     d.logits = lg;
-    d.c = c;
+    d.c = a.c;
+    d.far = a.far;
     d.pm = lg ? mx[n] : 0.0f;
     d.pz = lg ? zs[n] : 0.0;
     d.qm = lg && d.q ? mx[T + 1 + n] : 0.0f;
@@ -518,6 +518,8 @@ int64_t layout(const kq_spec_verify* v, VfArg* a, uint8_t* w) {
         a->parg = (int*)(w + o[2]);
         a->wsum = (double*)(w + o[3]);
         a->ended = (int*)(w + o[4]);
+        a->c = v->inv_temp * LOG2E;
+        a->far = -1000.0 / a->c;
     }
     o[5] = o[4] + up256((int64_t)v->S * 4);           // ended
     return o[5];

@@ -227,6 +227,42 @@ def test_nothing_left_of_the_difference():
     assert na.tolist() == [0, 0] and out[:, 0].tolist() == [7, 9]
 
 
+def test_nothing_left_of_the_difference_of_logits():
+    """The same with logits: equal rows, and a draft on the only token that has any weight."""
+    target, draft, tokens, nd, u = make(2, 1, 3000, "logits", True, 14)
+    target[:, 0] = draft[:, 0]
+    nd[:] = 1
+    u[:, 0] = 1.0
+    check(target, draft, tokens, nd, u, "logits")
+    target[:, 0] = -np.inf
+    target[0, 0, 7], target[1, 0, 2999] = -3.0, 400.0
+    tokens[:, 0] = [7, 2999]
+    na, out = run(target, None, tokens, nd, u, "logits")
+    assert na.tolist() == [0, 0] and out[:, 0].tolist() == [7, 2999]
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("it", [1.0, 0.7, 1e-30, 1e30])
+def test_logits_of_any_size(it, draft):
+    """Rows of the type's lowest value alone (uniform), rows masked with it, logits
+    of which neighbours are far apart, large and tiny factors."""
+    V = 5000
+    target, d, tokens, nd, u = make(6, 2, V, "logits", draft, 15)
+    low = np.finfo(np.float32).min
+    nd[:] = 2
+    target[0] = low
+    target[1, :, 5:] = low
+    target[2] = np.float32(1e20)
+    target[2, :, 100:] = np.nextafter(np.float32(1e20), np.float32(0))
+    target[3, :, 10:4990] = low
+    target[3, :, :10] = target[3, :, 4990:] = -low
+    target[4] += np.float32(1e6)
+    if draft:
+        d[1, :, 5:] = low
+        d[5] = low
+    check(target, d, tokens, nd, u, "logits", it=it)
+
+
 def test_greedy_ties():
     """Equal maxima, also across chunks and lanes: the lowest token."""
     V = 9000
