@@ -100,8 +100,8 @@ struct Chunk {
 #pragma unroll
         for (int j = 0; j < NJ; j++) v[j] = load4(row, base + 4 * (TH * j + (int)threadIdx.x), V, fill);
     }
-    // the first four; the others move up.  (Loops over j stay loops: their code
-    // is read from memory once a launch, which at few rows is most of its time.)
+    // the first four; the others move up: for loops over j that stay loops (the
+    // code of long unrolled ones is read from memory in every launch)
     __device__ __forceinline__ f32x4 next() {
         const f32x4 f = v[0];
 #pragma unroll
@@ -149,8 +149,7 @@ __device__ __forceinline__ float max16(float v) {
 }
 
 // A chunk's maximum, its first place, and the sum of exp((l - max) inv_temp).
-// BULK: unrolled, for grids that fill the device several times.
-template <bool GREEDY, bool BULK>
+template <bool GREEDY>
 __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
     __shared__ float sm[TH / 64];
     __shared__ int si[TH / 64];
@@ -191,19 +190,10 @@ __global__ __launch_bounds__(TH) void kq_vf_stats_kernel(VfArg a) {
     }
     const double top = m;
     double z = 0.0;
-    if (BULK) {
 #pragma unroll
-        for (int j = 0; j < NJ; j++)
+    for (int j = 0; j < NJ; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) z = z + pow2((double)v.v[j][e] - top, a.c, a.far);
-    } else {
-#pragma unroll 1
-        for (int j = 0; j < NJ; j++) {
-            const f32x4 x = v.next();
-#pragma unroll
-            for (int e = 0; e < 4; e++) z = z + pow2((double)x[e] - top, a.c, a.far);
-        }
-    }
+        for (int e = 0; e < 4; e++) z = z + pow2((double)v.v[j][e] - top, a.c, a.far);
     z = wave_sum(z);
     if ((tid & 63) == 0) { sm[tid >> 6] = m; sd[tid >> 6] = z; }
     __syncthreads();
@@ -540,10 +530,8 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st) {
     const dim3 chunks((unsigned)a.nch, (unsigned)v->S), wg(TH), seqs((unsigned)v->S);
     if (greedy || logits) {
         const dim3 grid((unsigned)a.nch, (unsigned)(v->S * (v->T + 1) + (v->draft && !greedy ? v->S * v->T : 0)));
-        const bool bulk = (long)grid.x * grid.y >= 4096;
-        if (greedy) hipLaunchKernelGGL((kq_vf_stats_kernel<true, true>), grid, wg, 0, st, a);
-        else if (bulk) hipLaunchKernelGGL((kq_vf_stats_kernel<false, true>), grid, wg, 0, st, a);
-        else hipLaunchKernelGGL((kq_vf_stats_kernel<false, false>), grid, wg, 0, st, a);
+        if (greedy) hipLaunchKernelGGL(kq_vf_stats_kernel<true>, grid, wg, 0, st, a);
+        else hipLaunchKernelGGL(kq_vf_stats_kernel<false>, grid, wg, 0, st, a);
     }
     if (greedy) {
         hipLaunchKernelGGL(kq_vf_greedy_kernel, seqs, dim3(64), 0, st, a);
