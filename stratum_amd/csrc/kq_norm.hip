@@ -157,10 +157,14 @@ __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
 template <int V>
 int launch(const kq_rmsnorm& a, hipStream_t st) {
     const int nv = (a.K + V - 1) / V;
-    // Few rows: one or two steps on as many lanes as a workgroup has (latency);
-    // else four, in fewer lanes, so that a CU holds several rows.
+    // As few steps as there are lanes for (latency: rows of 5120, one of them 4.2 us
+    // against 5.3 with four steps, 512 of them 10.0 / 10.5; rows of 1024 2.5 / 4.1 and
+    // 8.2 / 8.5 for 2048); four in fewer lanes, so that a CU has more rows in flight,
+    // where there are several times the lanes that the device holds (5120: 768 rows
+    // 14.7 / 13.7, 1024 19.0 / 17.1, 4096 53.7 / 52.4; 1024: 4096 rows 14.2 / 13.8), but
+    // not of single values (1056: 512 rows 5.5 / 6.4, 1024 8.8 / 8.3, 4096 26.5 / 28.1).
     constexpr int MOST = V == 4 ? 4 : 8;       // (8 steps of 4 spill registers)
-    int steps = a.B <= 512 ? 1 : 4;
+    int steps = V == 1 || (long)a.B * a.K <= 3 << 20 ? 1 : 4;
     while (steps <= MOST && nv > 1024 * steps) steps *= 2;
     const dim3 grid((unsigned)a.B);
     const int per = steps <= MOST ? (nv + steps - 1) / steps : 1024;
