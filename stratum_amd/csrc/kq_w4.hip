@@ -741,6 +741,8 @@ void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
     g.nwin = (a.nblk + 3) / 4;
     const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G, a.w.group % 128 == 0);
     const int most_w = (int)((g_lds_max - own) / wb) & ~1;            // windows that LDS takes, in pairs
+    // as few parts as x needs: with four, eight streams of binary32 are 5 % faster
+    // (17408 x 5120 22.4 / 21.4 us), int8 rows slower (four 13.4 / 15.6, sixteen 18.0 / 19.3)
     g.ks = (g.nwin + most_w - 1) / most_w;
     g.nw = (g.nwin + g.ks - 1) / g.ks;
     g.ks = (g.nwin + g.nw - 1) / g.nw;
@@ -796,14 +798,22 @@ bool fill(W4Arg& a, const kq_w4* w) {
     return w->N >= 1 && w->K >= 32 && w->K % 32 == 0;
 }
 
-// LDS bytes of the walk kernel where it takes the call, else -1.  It is ahead
-// with one stream (17408 x 5120 11.5 us against 14.7, int8 rows 11.2 against
-// 13.6) and with two of int8 rows (12.5 / 13.7; 5120 x 17408 13.7 / 18.8), behind
-// with more (binary32, two: 16.2 / 14.8, int8, three: 14.2 / 13.8), but for
-// matrices that are one step of its workgroups, where a launch's latency is what
-// counts (1024 x 1024, int8, four: 4.0 / 4.4).
+// LDS bytes of the walk kernel where it takes the call, else -1.  It is ahead of
+// the matrix cores
+// - with one stream (17408 x 5120 11.3 us against 14.8, int8 rows 11.1 / 13.2) and
+//   with two of int8 rows (12.1 / 14.0; 5120 x 17408 14.0 / 19.6);
+// - with three of int8 rows, where a CU has few rows for x, whose way to LDS is
+//   what the other kernel waits for (5120 x 17408 15.8 / 20.4, 5120 x 9216 10.0 / 10.8,
+//   1024 x 5120 4.8 / 5.9; but 5120 x 5120 7.9 / 7.7, 17408 x 17408 39.7 / 37.8);
+// - with as many as it takes, where the matrix is one step of its workgroups and a
+//   launch's latency is what counts (1024 x 1024: four of int8 rows 4.0 / 4.5, three of
+//   binary32 4.6 / 5.1);
+// and behind with more (17408 x 5120: two of binary32 15.6 / 14.8, 5120 x 17408 20.6 /
+// 18.9; four of int8 rows 21.3 / 20.7).
 long walk_takes(W4Arg& a, int P, int B, int n_cu) {
-    const bool few = B <= (P == 1 ? 2 : 1) || (B <= walk_max_b(P) && small_matrix(a, n_cu));
+    const long rows = ((long)a.w.N + n_cu - 1) / n_cu;
+    const bool few = B <= (P == 1 ? 2 : 1) || (P == 1 && B == 3 && a.nblk > 8 * rows) ||
+                     (B <= walk_max_b(P) && small_matrix(a, n_cu));
     return few && a.nblk <= WALK_MAX_BLK ? walk_plan(a, P, B, n_cu) : -1;
 }
 
