@@ -550,10 +550,12 @@ typedef struct kq_w4 {
 /* y[b] = add[b] + W . x[b] for b < B: B rows of K values, N outputs each
  * (add NULL: nothing added; it may be y itself).  x and xq are 16-byte
  * aligned.  work: kq_w4_workspace_bytes of device memory, 256-byte aligned
- * (0 bytes: may be NULL).
- * The result is within 2^-20 * sum_k |w_k| max|x| of the exact one, the
- * maximum over the 32 values of x that k lies in; it does not depend on
- * other rows' values.  x must be finite. */
+ * (0 bytes, as with most sizes: may be NULL).
+ * The result is within (K / 32 + 8) 2^-24 sum_k |w_k| max|x| of the exact one
+ * (and the last rounding's half unit), the maximum over the 32 values of x
+ * that k lies in, counted as 2^-126 where it is less.  A row's bits do not
+ * depend on other rows' values, but on B, as the order of its sum does.  A
+ * row with a value that is not finite gives no finite one. */
 int kq_w4_gemv_dev(const kq_w4* w, const float* x, const float* add, float* y, int B, void* work,
                    int64_t work_bytes, kq_stream stream);
 

@@ -257,6 +257,40 @@ def test_refuses_a_short_workspace():
 
 
 @pytest.mark.parametrize("q8", [False, True])
+def test_refuses_a_short_workspace_for_cut_rows(q8):
+    """Rows that are cut into parts need workspace: without it, with less, unaligned."""
+    for Kd, B in ((40960, 8), (65536, 16)):
+        c = Case(20, Kd, B, 128, q8=q8)
+        assert c.nb >= (2 if not q8 else 0) * 4 * 20 * B and c.nb % 256 == 0
+        if not c.nb:
+            continue
+        y = torch.full((B, 20), 3.0, device="cuda")
+        for work, nb in ((None, c.nb), (c.work.data_ptr(), c.nb - 1), (c.work.data_ptr() + 16, c.nb)):
+            L, d = K.lib(), ctypes.byref(c.desc)
+            rc = (L.kq_w4_gemv_q8_dev(d, c.dxq.data_ptr(), c.dxs.data_ptr(), None, y.data_ptr(), B, work, nb, st())
+                  if q8 else L.kq_w4_gemv_dev(d, c.dx.data_ptr(), None, y.data_ptr(), B, work, nb, st()))
+            assert rc == -1 and b"workspace" in L.kq_last_error()
+        torch.cuda.synchronize()
+        assert (y == 3.0).all()
+        c.check()
+
+
+@pytest.mark.parametrize("B", [1, 2, 6])
+def test_subnormal_x(B):
+    """Blocks of x below 2^-126: half a unit of x's integers is 2^-148 then, as at 2^-126; and per block
+    the three roundings to multiples of 2^-149, the scale (below 1 / 8) and the zero (15) on them."""
+    c = Case(70, 640, B, 64, zeros=True, xscale=1e-40)
+    y = torch.empty(B, 70, device="cuda")
+    c.call(y)
+    torch.cuda.synchronize()
+    xmax = np.maximum(c.dx.cpu().numpy().reshape(B, -1, 32).__abs__().max(-1), 2.0 ** -126)
+    a = np.repeat(xmax, 32, 1).astype(np.float64) @ np.abs(c.W).T
+    tol = (640 / 32 + 8) * 2.0 ** -24 * a + (640 / 32 + 8) * 4 * 2.0 ** -150
+    assert (np.abs(y.cpu().numpy().astype(np.float64) - c.exact) <= tol).all()
+    assert (y != 0).any()
+
+
+@pytest.mark.parametrize("q8", [False, True])
 @pytest.mark.parametrize("B", [1, 3, 8])
 def test_matrices_past_4_gib(B, q8):
     """Offsets past 32 bits: 2.2 M rows of 4096 weights, 4.5 GB.  Repeats of one small matrix, so that
