@@ -320,7 +320,7 @@ __device__ __forceinline__ void draw(const VfArg& a, int s, int n, Drawn d);
 // DRAW: the sequence's last workgroup draws
 template <bool DRAW>
 __global__ __launch_bounds__(TH) void kq_vf_weights_kernel(VfArg a) {
-    __shared__ double sd[TH / 64];
+    __shared__ double sd[TH / 64], ps[NSUB];
     __shared__ int last;
     const int s = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CH;
     int n;
@@ -329,9 +329,8 @@ __global__ __launch_bounds__(TH) void kq_vf_weights_kernel(VfArg a) {
     Chunk p, q;
     p.load(d.p, base, a.v.V, none);
     if (d.q) q.load(d.q, base, a.v.V, none);
-    // (stores past this XCD's L2, where the last workgroup does not look)
     double* const sums = a.wsum + (long)s * a.nsum;
-    double* const parts = sums + a.nch + (long)blockIdx.x * NSUB + (tid >> 6);
+    double* const parts = sums + a.nch + (long)blockIdx.x * NSUB;
     double w = 0.0;
 #pragma unroll 1
     for (int j = 0; j < NJ; j++) {
@@ -340,17 +339,21 @@ __global__ __launch_bounds__(TH) void kq_vf_weights_kernel(VfArg a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) wj = wj + d.at(base + 4 * (TH * j + tid) + e, pv[e], qv[e]);
         wj = wave_sum(wj);
-        if ((tid & 63) == 0) __hip_atomic_store(parts + 4 * j, wj, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if ((tid & 63) == 0) ps[4 * j + (tid >> 6)] = wj;
         w = w + wj;
     }
     if ((tid & 63) == 0) sd[tid >> 6] = w;
     __syncthreads();
-    if (tid == 0) {
-        __hip_atomic_store(sums + blockIdx.x, (sd[0] + sd[1]) + (sd[2] + sd[3]), __ATOMIC_RELAXED,
+    // Stores past this XCD's L2, where the last workgroup does not look; all by the
+    // wave that counts, as its release waits for no other wave's.
+    static_assert(NSUB < 64);
+    if (tid <= NSUB)
+        __hip_atomic_store(tid < NSUB ? parts + tid : sums + blockIdx.x,
+                           tid < NSUB ? ps[tid] : (sd[0] + sd[1]) + (sd[2] + sd[3]), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
-        if (DRAW)
-            last = __hip_atomic_fetch_add(a.ended + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.nch - 1;
-    }
+    __builtin_amdgcn_wave_barrier();
+    if (DRAW && tid == 0)
+        last = __hip_atomic_fetch_add(a.ended + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.nch - 1;
     if (!DRAW) return;
     __syncthreads();
     if (last && tid < 64) draw(a, s, n, d);
