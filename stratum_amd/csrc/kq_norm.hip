@@ -157,14 +157,15 @@ __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
 template <int V>
 int launch(const kq_rmsnorm& a, hipStream_t st) {
     const int nv = (a.K + V - 1) / V;
-    // As few steps as there are lanes for (latency: rows of 5120, one of them 4.2 us
-    // against 5.3 with four steps, 512 of them 10.0 / 10.5; rows of 1024 2.5 / 4.1 and
-    // 8.2 / 8.5 for 2048); four in fewer lanes, so that a CU has more rows in flight,
-    // where there are several times the lanes that the device holds (5120: 768 rows
-    // 14.7 / 13.7, 1024 19.0 / 17.1, 4096 53.7 / 52.4; 1024: 4096 rows 14.2 / 13.8), but
-    // not of single values (1056: 512 rows 5.5 / 6.4, 1024 8.8 / 8.3, 4096 26.5 / 28.1).
+    // One step, on as many lanes as the row has loads, while the device's lanes (2048
+    // on each of 256 CUs) hold all rows; four steps in fewer lanes, which keep more
+    // loads in flight, when they do not.  One step / four, us: rows of 1024 to int8,
+    // one 2.5 / 4.1, 2048 rows 8.2 / 8.5, 4096 14.2 / 13.8; rows of 5120 to binary32,
+    // one 3.1 / 3.4, 512 rows 7.8 / 7.4, 1024 13.5 / 11.2, 4096 36.2 / 33.5; to int8
+    // 4.2 / 5.3, 10.0 / 10.5, 19.0 / 17.1, 53.7 / 52.4; rows of 1153 single values, one
+    // 2.7 / 2.8, 512 rows 4.6 / 4.2, 4096 23.0 / 17.1.
     constexpr int MOST = V == 4 ? 4 : 8;       // (8 steps of 4 spill registers)
-    int steps = V == 1 || (long)a.B * a.K <= 3 << 20 ? 1 : 4;
+    int steps = (long)a.B * nv <= 1 << 19 ? 1 : 4;
     while (steps <= MOST && nv > 1024 * steps) steps *= 2;
     const dim3 grid((unsigned)a.B);
     const int per = steps <= MOST ? (nv + steps - 1) / steps : 1024;
