@@ -14,6 +14,9 @@ wrappers with the reference's argument meaning:
   moe_pack_open / moe_pack_which     (stratum_arch_moe.inc.c:245-313, 506-525)
   moe_topk, moe_topk_dev             moe_topk (stratum_arch_moe.inc.c:368-385)
   moe_gemv_dev(op, sel, B, k, E)     the routed expert GEMVs (:596-603, 808-815, 1135-1205)
+  rmsnorm_dev(a)                     residual + RMS norm, to binary32 or int8 rows
+  w4_gemv_dev / w4_gemv_q8_dev       products with 4-bit weights and group scales
+  spec_verify_dev(v, work, n)        drafted tokens against the target's distributions
 
 There is no CPU fallback: if the library is missing, ``lib()`` raises.
 """
