@@ -30,7 +30,7 @@ constexpr double LOG2E = 1.4426950408889634;
 
 struct VfArg {
     kq_spec_verify v;
-    int nch;                // chunks of a row
+    int nch, cpw;           // chunks of a row; of a workgroup of the second launch
     float* pmax;            // [rows][nch]
     double* psum;           // [rows][nch]
     int* parg;              // [rows][nch]
@@ -322,38 +322,49 @@ template <bool DRAW>
 __global__ __launch_bounds__(TH) void kq_vf_weights_kernel(VfArg a) {
     __shared__ double sd[TH / 64], ps[NSUB];
     __shared__ int last;
-    const int s = blockIdx.y, tid = threadIdx.x, base = blockIdx.x * CH;
+    const int s = blockIdx.y, tid = threadIdx.x;
     int n;
     const Drawn d = decide(a, s, &n);
     const float none = d.logits ? -INFINITY : 0.0f;
-    Chunk p, q;
-    p.load(d.p, base, a.v.V, none);
-    if (d.q) q.load(d.q, base, a.v.V, none);
     double* const sums = a.wsum + (long)s * a.nsum;
-    double* const parts = sums + a.nch + (long)blockIdx.x * NSUB;
-    double w = 0.0;
+    const int end = min(a.nch, ((int)blockIdx.x + 1) * a.cpw);
+    Chunk p, q, pn, qn;
+    pn.load(d.p, blockIdx.x * a.cpw * CH, a.v.V, none);
+    if (d.q) qn.load(d.q, blockIdx.x * a.cpw * CH, a.v.V, none);
 #pragma unroll 1
-    for (int j = 0; j < NJ; j++) {
-        const f32x4 pv = p.next(), qv = d.q ? q.next() : pv;
-        double wj = 0.0;
+    for (int ch = blockIdx.x * a.cpw; ch < end; ch++) {
+        const int base = ch * CH;
+        p = pn;
+        q = qn;
+        if (ch + 1 < end) {                 // the next, while this one is used
+            pn.load(d.p, base + CH, a.v.V, none);
+            if (d.q) qn.load(d.q, base + CH, a.v.V, none);
+        }
+        double w = 0.0;
+#pragma unroll 1
+        for (int j = 0; j < NJ; j++) {
+            const f32x4 pv = p.next(), qv = d.q ? q.next() : pv;
+            double wj = 0.0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) wj = wj + d.at(base + 4 * (TH * j + tid) + e, pv[e], qv[e]);
-        wj = wave_sum(wj);
-        if ((tid & 63) == 0) ps[4 * j + (tid >> 6)] = wj;
-        w = w + wj;
+            for (int e = 0; e < 4; e++) wj = wj + d.at(base + 4 * (TH * j + tid) + e, pv[e], qv[e]);
+            wj = wave_sum(wj);
+            if ((tid & 63) == 0) ps[4 * j + (tid >> 6)] = wj;
+            w = w + wj;
+        }
+        if ((tid & 63) == 0) sd[tid >> 6] = w;
+        __syncthreads();
+        // Stores past this XCD's L2, where the last workgroup does not look; all by the
+        // wave that counts, as its release waits for no other wave's.
+        static_assert(NSUB < 64);
+        if (tid <= NSUB)
+            __hip_atomic_store(tid < NSUB ? sums + a.nch + (long)ch * NSUB + tid : sums + ch,
+                               tid < NSUB ? ps[tid] : (sd[0] + sd[1]) + (sd[2] + sd[3]), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+        if (ch + 1 < end) __syncthreads();
     }
-    if ((tid & 63) == 0) sd[tid >> 6] = w;
-    __syncthreads();
-    // Stores past this XCD's L2, where the last workgroup does not look; all by the
-    // wave that counts, as its release waits for no other wave's.
-    static_assert(NSUB < 64);
-    if (tid <= NSUB)
-        __hip_atomic_store(tid < NSUB ? parts + tid : sums + blockIdx.x,
-                           tid < NSUB ? ps[tid] : (sd[0] + sd[1]) + (sd[2] + sd[3]), __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
     __builtin_amdgcn_wave_barrier();
     if (DRAW && tid == 0)
-        last = __hip_atomic_fetch_add(a.ended + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == a.nch - 1;
+        last = __hip_atomic_fetch_add(a.ended + s, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
     if (!DRAW) return;
     __syncthreads();
     if (last && tid < 64) draw(a, s, n, d);
@@ -530,7 +541,14 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st) {
     VfArg a;
     layout(v, &a, static_cast<uint8_t*>(work));
     const bool greedy = v->flags & KQ_VERIFY_GREEDY, logits = v->flags & KQ_VERIFY_LOGITS;
-    const dim3 chunks((unsigned)a.nch, (unsigned)v->S), wg(TH), seqs((unsigned)v->S);
+    // Where there are many sequences, a workgroup takes several chunks after it has
+    // decided, which each does for itself, and counts itself once (us, 151936 tokens,
+    // one chunk each / this: 32 sequences of 7 111 / 96, 64 of 3 140 / 112, 128 of 2
+    // 280 / 168; 256 of 4 over 32000 135 / 108); few, one, as a chunk more is 3 us more
+    // (one sequence of 4 15.3 / 19.1 with two, sixteen of 7 56.9 / 58.2).
+    const long per = (long)v->S * a.nch / 512;
+    a.cpw = per < 1 ? 1 : per > 6 ? 6 : (int)per;
+    const dim3 chunks((unsigned)((a.nch + a.cpw - 1) / a.cpw), (unsigned)v->S), wg(TH), seqs((unsigned)v->S);
     if (greedy || logits) {
         const dim3 grid((unsigned)a.nch, (unsigned)(v->S * (v->T + 1) + (v->draft && !greedy ? v->S * v->T : 0)));
         if (greedy) hipLaunchKernelGGL(kq_vf_stats_kernel<true>, grid, wg, 0, st, a);

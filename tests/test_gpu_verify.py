@@ -212,6 +212,13 @@ def test_masked_and_odd_rows(form):
         assert na[s] == n and out[s].tolist() == want, (s, na[s], n, out[s], want)
 
 
+@pytest.mark.parametrize("form,draft", [("logits", False), ("logits", True), ("probs", True)])
+@pytest.mark.parametrize("S,V", [(300, 20001), (700, 21000)])
+def test_many_sequences(form, draft, S, V):
+    """Workgroups of two and of six chunks, the last of a row with fewer."""
+    check(*make(S, 1, V, form, draft, 17), form)
+
+
 def test_nothing_left_of_the_difference():
     """u = 1 refuses a token although p equals q: the draw is from p itself."""
     target, draft, tokens, nd, u = make(2, 1, 3000, "probs", True, 12)
