@@ -478,28 +478,47 @@ __global__ __launch_bounds__(64) void kq_vf_draw_kernel(VfArg a) {
     draw(a, blockIdx.x, n, d);
 }
 
-// The greedy form: a token is accepted iff it is its row's first maximum.
-__global__ __launch_bounds__(64) void kq_vf_greedy_kernel(VfArg a) {
-    const int s = blockIdx.x, T = a.v.T, lane = threadIdx.x, nd = drafted(a, s);
-    int n = 0, best = -1;
-    for (; n <= nd; n++) {
-        const long o = (long)trow(a, s, n) * a.nch;
+// The greedy form: a token is accepted iff it is its row's first maximum.  All
+// rows at once, 16 lanes each (row after row until the first refusal, one sequence
+// of 4 drafts, all accepted, took 10.8 us against 6.1, of 63 63.8 against 14.1).
+__global__ __launch_bounds__(TH) void kq_vf_greedy_kernel(VfArg a) {
+    __shared__ int best[KQ_VERIFY_MAX_DRAFT + 1];
+    const int s = blockIdx.x, T = a.v.T, tid = threadIdx.x, nd = drafted(a, s);
+    const int tok = tid < nd ? a.v.tokens[s * T + tid] : -1;
+    for (int i = tid >> 4; i <= nd; i += TH / 16) {
+        const long o = (long)trow(a, s, i) * a.nch;
         float m = -INFINITY;
         int at = 0x7fffffff;
-        for (int c = lane; c < a.nch; c += 64)
-            if (a.pmax[o + c] > m) { m = a.pmax[o + c]; at = a.parg[o + c]; }
+#pragma unroll 1
+        for (int c = tid & 15; c < a.nch; c += 64) {
+            float pm[4];
+            int pa[4];
 #pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
+            for (int k = 0; k < 4; k++) {
+                const bool in = c + 16 * k < a.nch;
+                pm[k] = in ? a.pmax[o + c + 16 * k] : -INFINITY;
+                pa[k] = in ? a.parg[o + c + 16 * k] : 0;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (pm[k] > m) { m = pm[k]; at = pa[k]; }
+        }
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) {
             const float om = __shfl_xor(m, off);
             const int oa = __shfl_xor(at, off);
             if (om > m || (om == m && oa < at)) { m = om; at = oa; }
         }
-        best = at == 0x7fffffff ? -1 : at;
-        if (n == nd || best < 0 || a.v.tokens[s * T + n] != best) break;
+        if ((tid & 15) == 0) best[i] = at == 0x7fffffff ? -1 : at;
     }
-    if (lane < n) a.v.out[s * (T + 1) + lane] = a.v.tokens[s * T + lane];
-    if (lane >= n && lane <= T) a.v.out[s * (T + 1) + lane] = lane == n ? best : -1;
-    if (lane == 0) a.v.n_accept[s] = n;
+    __syncthreads();
+    if (tid >= 64) return;
+    const unsigned long long no = __ballot(tid >= nd || best[tid] < 0 || tok != best[tid]);
+    const int n = __ffsll(no) - 1;                     // (nd <= 63: that lane refuses)
+    int* const out = a.v.out + (long)s * (T + 1);
+    if (tid < n) out[tid] = tok;
+    if (tid >= n && tid <= T) out[tid] = tid == n ? best[n] : -1;
+    if (tid == 0) a.v.n_accept[s] = n;
 }
 
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -555,7 +574,7 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st) {
         else hipLaunchKernelGGL(kq_vf_stats_kernel<false>, grid, wg, 0, st, a);
     }
     if (greedy) {
-        hipLaunchKernelGGL(kq_vf_greedy_kernel, seqs, dim3(64), 0, st, a);
+        hipLaunchKernelGGL(kq_vf_greedy_kernel, seqs, wg, 0, st, a);
     } else if (logits) {
         hipLaunchKernelGGL(kq_vf_weights_kernel<true>, chunks, wg, 0, st, a);
     } else {
