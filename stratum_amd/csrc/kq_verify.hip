@@ -14,7 +14,9 @@
 // (logits and greedy form); then the weights' sums per chunk of the row drawn
 // from, and, by the workgroup that ends a sequence's last, the token.  (The
 // count of ended ones is cleared by the first launch; probabilities, which need
-// no first launch, draw in a launch of their own instead.)
+// no first launch, draw in a launch of their own instead.)  Binary64 instructions
+// bound the first (240 rows of 151936 31 us, 4.7 TB/s), a chain of waits the second
+// (one sequence 9.2 us, sixteen 20).
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

@@ -154,6 +154,9 @@ constexpr int walk_waves(int P, int NB) { return P * NB <= 3 ? 5 : P * NB <= 6 ?
 // registers, and a step's weights are rs neighbouring rows in address order.
 // A lane's term of a row goes to LDS; after a pass of steps a few lanes add up
 // each row's terms, while the next pass goes on with the other half of the buffer.
+// The stream of weights bounds it: 17408 x 5120, one stream, 10.4 us, 4.4 TB/s (a plain
+// read of these bytes: 9); 5120 x 17408 of int8 rows 10.8 us, 4.5 TB/s; the vector
+// ALU is busy for half of that.
 template <int P, int NB, int MODE>
 __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4Arg a) {
     extern __shared__ __align__(16) uint8_t smem[];
@@ -348,8 +351,13 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 //
 // A window's weights are loaded in address order (lane 4 r + b: block b of row r;
 // a row to a lane, as the operand wants them, makes every lane of a load a cache
-// access of its own) and change lanes in LDS, in the wave's own 1.5 KB, together
+// access of its own) and change lanes in LDS, in the wave's own 1.8 KB, together
 // with their scales.
+//
+// No unit is full: 17408 x 5120, sixteen int8 streams, 18.2 us (2.6 TB/s of weights),
+// the vector ALU and the LDS busy for 0.6 of it each, the matrix cores for 0.1; 151936 x
+// 1024, five of binary32, 30 us (3.0 TB/s), 0.6, 0.65 and 0.15.  (Tiles of 32 rows,
+// two operands of weights for one of x, were slower: 20.6 and 29.8 us.)
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
