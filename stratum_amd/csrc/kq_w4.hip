@@ -361,10 +361,13 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// A window's x in LDS: per pair of blocks and lane group P * 4 G entries of 16
-// bytes (8 of either block: the even positions' bytes, then the odd ones'),
-// then xs of its blocks, [block][q][G], and xz likewise, or (ONE) [q][G] of the
-// whole window.
+// A window's x in LDS: 8 places of P * 4 G entries of 16 bytes, for two blocks
+// (pair b2 of the window's) and a lane group each (8 values of either block: the
+// even positions' bytes, then the odd ones'); then xs of its blocks, [block][q][G],
+// and xz likewise, or (ONE) [q][G] of the whole window.  Lane groups q and q ^ 1 are 4
+// places apart, a multiple of 256 bytes: a read of 16 bytes a lane takes lanes of
+// both at once, and so finds them in different banks.
+constexpr int mm_place(int b2, int q) { return (q & 1) * 4 + (q >> 1) * 2 + b2; }
 constexpr int mm_xbytes(int P, int G) { return 512 * P * G; }
 constexpr int mm_window(int P, int G, bool ONE) { return mm_xbytes(P, G) + (ONE ? 80 : 128) * G; }
 
@@ -380,9 +383,9 @@ struct MmArg {
 constexpr int MM_W = 16;     // waves
 constexpr int mm_slot(int G) { return 16 * (4 * G + 1); }   // floats of a tile's sums in LDS
 // A wave's own LDS: the sums of the tile that it began with, if others share
-// it; 16 rows of a window, 80 bytes each, and their scales.  What it ends with
-// takes the place of the rows.
-constexpr int MM_ROWB = 80, MM_STAGE = 16 * MM_ROWB + 64 * 8;
+// it; 16 rows of a window, 64 bytes each, and their scales and zeros.  What it
+// ends with takes the place of the rows.
+constexpr int MM_STAGE = 16 * 64 + 64 * 8;
 constexpr int mm_wave(int G) { return 4 * mm_slot(G) + MM_STAGE; }
 static_assert(4 * mm_slot(4) <= MM_STAGE);
 constexpr uint32_t FAR = 0x80000000u;    // an offset behind every buffer's end
@@ -451,8 +454,9 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
             scale = v.scale;
             xz = v.sum;
         }
+        if (MODE == M_16) xz = -8.0f * xz;                // (the zero of all)
         uint8_t* const w = smem + (size_t)(b >> 2) * WB;
-        const int at = (((b >> 1) & 1) * 4 + kq) * E + s * P;
+        const int at = mm_place((b >> 1) & 1, kq) * E + s * P;
         if (in) {
 #pragma unroll
             for (int p = 0; p < P; p++) reinterpret_cast<uint2*>(w)[(at + p) * 2 + (b & 1)] = d[p];
@@ -520,7 +524,8 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     lds_barrier();
     uint8_t* const own = smem + (size_t)(2 * np) * WB + (size_t)wave * mm_wave(G);
     uint8_t* const stage = own + 4 * mm_slot(G);
-    const int put_at = ldr * MM_ROWB + 16 * lb, take_at = n * MM_ROWB + 4 * q;
+    // (a row's four pieces change places every four rows: no bank conflicts either way)
+    const int put_at = ldr * 64 + 16 * (lb ^ ((ldr >> 2) & 3)), take_at = n * 64 + 4 * q + 16 * ((n >> 2) & 3);
 
     float* const dst = g.ks > 1 ? g.part + (long)part * g.B * a.w.N : a.y;
     auto out = [&](int s, int r, float v) {               // stream s of the tile, row r of the workgroup
@@ -532,13 +537,13 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     // this lane's entry of an operand: row n = 4 qs + i
     const int qs = n >> 2, ni = n & 3;
     const int entry = P == 1 ? qs + 4 * min(ni, G - 1) : qs * P + min(ni, P - 1);
-    const int xoff = (q * E + entry) * 16, moff = XB + q * G * 4;
+    const int xoff = (mm_place(0, q) * E + entry) * 16, moff = XB + q * G * 4;
 
     float acc[G];
 #pragma unroll
     for (int k = 0; k < G; k++) acc[k] = 0.0f;
     int t = i0 / np, w = i0 - t * np, from = w;           // `from`: the tile's first pair here
-    uint32_t* const sl = reinterpret_cast<uint32_t*>(stage + 16 * MM_ROWB);
+    float* const sl = reinterpret_cast<float*>(stage + 16 * 64);
     for (int i = i0; i < i1; i++) {
         uint32_t d[2][4];
         float sc[2][4], ze[2][4];
@@ -548,27 +553,22 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
             *reinterpret_cast<uint4*>(stage + put_at) = cur.q[j];
             if (j < NS) {
                 const RawScale<MODE>& r = cur.s[j];
-                if (MODE == M_32Z) reinterpret_cast<uint2*>(sl)[lane] = make_uint2(r.s, r.z);
-                else sl[lane] = MODE == M_16Z ? (uint32_t)r.s | (uint32_t)r.z << 16 : r.s;
+                if (MODE == M_16) sl[lane] = r.scale(half);
+                else reinterpret_cast<float2*>(sl)[lane] = make_float2(r.scale(half), r.zero(zeros));
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 #pragma unroll
-            for (int b = 0; b < 4; b++) d[j][b] = *reinterpret_cast<const uint32_t*>(stage + take_at + 16 * b);
+            for (int b = 0; b < 4; b++) d[j][b] = *reinterpret_cast<const uint32_t*>(stage + (take_at ^ (16 * b)));
 #pragma unroll
             for (int b = 0; b < (ONE ? 1 : 4); b++) {
-                RawScale<MODE> r;
                 const int at = 4 * n + (ONE ? j : b);
-                if (MODE == M_32Z) {
-                    const uint2 v = reinterpret_cast<const uint2*>(sl)[at];
-                    r.s = v.x;
-                    r.z = (uint8_t)v.y;
+                if (MODE == M_16) {
+                    sc[j][b] = sl[at];
                 } else {
-                    const uint32_t v = sl[at];
-                    r.s = (uint16_t)v;
-                    r.z = (uint8_t)(v >> 16);
+                    const float2 v = reinterpret_cast<const float2*>(sl)[at];
+                    sc[j][b] = v.x;
+                    ze[j][b] = v.y;
                 }
-                sc[j][b] = r.scale(half);
-                ze[j][b] = r.zero(zeros);
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         }
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
             float sum[G];
             if (ONE) {
 #pragma unroll
-                for (int c = 0; c < G; c++) sum[c] = -ze[j][0] * m[16 * G + c];
+                for (int c = 0; c < G; c++) sum[c] = MODE == M_16 ? m[16 * G + c] : -ze[j][0] * m[16 * G + c];
             }
 #pragma unroll
             for (int b2 = 0; b2 < 2; b2++) {
@@ -588,7 +588,7 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                 uint4 x[NX];
 #pragma unroll
                 for (int c = 0; c < NX; c++)
-                    x[c] = *reinterpret_cast<const uint4*>(xb + xoff + (b2 * 4 * E + 4 * P * c) * 16);
+                    x[c] = *reinterpret_cast<const uint4*>(xb + xoff + (mm_place(b2, 0) * E + 4 * P * c) * 16);
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const int b = 2 * b2 + h;
@@ -611,8 +611,11 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                     for (int c = 0; c < G; c++) {
                         const float xs = m[4 * G * b + c];
                         if (ONE) sum[c] = fmaf(xs, (float)dot[c], sum[c]);
-                        else acc[c] = fmaf(sc[j][b], fmaf(-ze[j][b], m[16 * G + 4 * G * b + c],
-                                                          xs * (float)dot[c]), acc[c]);
+                        else {
+                            const float xz = m[16 * G + 4 * G * b + c], d = (float)dot[c];
+                            acc[c] = fmaf(sc[j][b], MODE == M_16 ? fmaf(xs, d, xz) : fmaf(-ze[j][b], xz, xs * d),
+                                          acc[c]);
+                        }
                     }
                 }
             }
@@ -748,7 +751,10 @@ void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
     if (p->G == 3) p->G = 4;
     g.nwin = (a.nblk + 3) / 4;
     const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G, a.w.group % 128 == 0);
-    const int most_w = (int)((g_lds_max - own) / wb) & ~1;            // windows that LDS takes, in pairs
+    int most_w = (int)((g_lds_max - own) / wb) & ~1;                  // windows that LDS takes, in pairs
+    // (two halves of x for as many workgroups each are ahead of all of it for each,
+    // where it fills the LDS: eight streams of binary32, 17408 x 5120 22.1 / 23.5 us)
+    if (P == 3 && p->G == 2 && most_w > 38) most_w = 38;
     // as few parts as x needs: with four, eight streams of binary32 are 5 % faster
     // (17408 x 5120 22.4 / 21.4 us), int8 rows slower (four 13.4 / 15.6, sixteen 18.0 / 19.3)
     g.ks = (g.nwin + most_w - 1) / most_w;
