@@ -354,10 +354,10 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 // access of its own) and change lanes in LDS, in the wave's own 1.8 KB, together
 // with their scales.
 //
-// No unit is full: 17408 x 5120, sixteen int8 streams, 18.2 us (2.6 TB/s of weights),
+// No unit is full: 17408 x 5120, sixteen int8 streams, 17.9 us (2.6 TB/s of weights),
 // the vector ALU and the LDS busy for 0.6 of it each, the matrix cores for 0.1; 151936 x
-// 1024, five of binary32, 30 us (3.0 TB/s), 0.6, 0.65 and 0.15.  (Tiles of 32 rows,
-// two operands of weights for one of x, were slower: 20.6 and 29.8 us.)
+// 1024, five of binary32, 27.6 us (3.3 TB/s), 0.6, 0.6 and 0.15.  (Tiles of 32 rows,
+// two operands of weights for one of x, were slower: 19.1 -> 20.6 and 29.8 -> 29.8 us.)
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
