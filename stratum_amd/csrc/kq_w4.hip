@@ -351,20 +351,20 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 //
 // A window's weights are loaded in address order (lane 4 r + b: block b of row r;
 // a row to a lane, as the operand wants them, makes every lane of a load a cache
-// access of its own) and change lanes in LDS, in the wave's own 1.8 KB, together
+// access of its own) and change lanes in LDS, in the wave's own 1.5 KB, together
 // with their scales.
 //
 // No unit is full: 17408 x 5120, sixteen int8 streams, 17.9 us (2.6 TB/s of weights),
 // the vector ALU and the LDS busy for 0.6 of it each, the matrix cores for 0.1; 151936 x
 // 1024, five of binary32, 27.6 us (3.3 TB/s), 0.6, 0.6 and 0.15.  (Tiles of 32 rows,
-// two operands of weights for one of x, were slower: 19.1 -> 20.6 and 29.8 -> 29.8 us.)
+// two operands of weights for one of x: 19.1 -> 20.6 us the former, the latter the same.)
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // A window's x in LDS: 8 places of P * 4 G entries of 16 bytes, for two blocks
 // (pair b2 of the window's) and a lane group each (8 values of either block: the
 // even positions' bytes, then the odd ones'); then xs of its blocks, [block][q][G],
-// and xz likewise, or (ONE) [q][G] of the whole window.  Lane groups q and q ^ 1 are 4
+// and xz (of MODE M_16 -8 xz) likewise, or (ONE) [q][G] of the whole window.  Lane groups q and q ^ 1 are 4
 // places apart, a multiple of 256 bytes: a read of 16 bytes a lane takes lanes of
 // both at once, and so finds them in different banks.
 constexpr int mm_place(int b2, int q) { return (q & 1) * 4 + (q >> 1) * 2 + b2; }
