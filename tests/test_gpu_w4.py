@@ -257,6 +257,12 @@ def test_refuses_a_short_workspace():
 
 
 @pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("N,Kd,B", [(3, 64, 4097), (1, 32, 65535), (300, 6400, 250)])
+def test_very_many_rows(N, Kd, B, q8):
+    Case(N, Kd, B, 32, zeros=True, q8=q8).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
 def test_refuses_a_short_workspace_for_cut_rows(q8):
     """Rows that are cut into parts need workspace: without it, with less, unaligned."""
     for Kd, B in ((40960, 8), (65536, 16)):
