@@ -12,8 +12,10 @@
 // rows are P = 1 as they come.  Binary32 rows are P = 3: xs is the power of
 // two that puts the block's largest |v| in (2^21, 2^22], so v is off by half a
 // unit, 2^-22 of that largest value, as x's own last bits are from the value
-// it was computed from.  Per block, sum q v (at most 480 * 2^22 < 2^31) is
-// exact; blocks are scaled and added in binary32.
+// it was computed from.  Per block, sum (q - z) v is exact, as is sum q v on its
+// way (at most 480 * 2^22 < 2^31): zero points are taken off in integers, so that
+// weights at theirs give nothing, whatever x is.  Blocks are scaled and added in
+// binary32.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
@@ -75,8 +77,8 @@ struct RawScale {
         const float h = __half2float(__ushort_as_half((unsigned short)s));
         return half ? h : __uint_as_float((uint32_t)s << 16);
     }
-    __device__ __forceinline__ float zero(bool zeros) const {
-        return MODE == M_16 || (MODE == M_32Z && !zeros) ? 8.0f : (float)(z & 15);
+    __device__ __forceinline__ int zero(bool zeros) const {
+        return MODE == M_16 || (MODE == M_32Z && !zeros) ? 8 : z & 15;
     }
 };
 
@@ -90,7 +92,8 @@ __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel)
 // neighbouring lanes hold a block and agree on its scale and sum.
 struct X8 {
     uint32_t even[3], odd[3];
-    float scale, sum;        // xs; xs * sum of v over the block
+    float scale;
+    int sum;                 // of v over the block
 };
 
 template <int CTRL>
@@ -131,8 +134,7 @@ __device__ __forceinline__ X8 split_x(const uint4 lo, const uint4 hi) {
         o.odd[p] = perm(u[3], u[1], s2) | perm(u[7], u[5], s2) << 16;
     }
     sum += dpp<QUAD_1>(sum);
-    sum += dpp<QUAD_2>(sum);
-    o.sum = o.scale * (float)sum;
+    o.sum = sum + dpp<QUAD_2>(sum);
     return o;
 }
 
@@ -154,6 +156,8 @@ constexpr int walk_waves(int P, int NB) { return P * NB <= 3 ? 5 : P * NB <= 6 ?
 // registers, and a step's weights are rs neighbouring rows in address order.
 // A lane's term of a row goes to LDS; after a pass of steps a few lanes add up
 // each row's terms, while the next pass goes on with the other half of the buffer.
+// The zero point: -8 sum v, kept, where it is 8 for all; else z times sum v, in 24
+// bits (binary32 x in two parts, as its sum v has 28).
 // The stream of weights bounds it: 17408 x 5120, one stream, 10.4 us, 4.4 TB/s (a plain
 // read of these bytes: 9); 5120 x 17408 of int8 rows 10.8 us, 4.5 TB/s; the vector
 // ALU is busy for half of that.
@@ -171,7 +175,8 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
     // x is asked for before the weights: loads return in order
     constexpr int XT = 4;               // binary32: up to 4 pieces of 8 values a lane at once
     uint4 xr[P == 1 ? 2 * NB : 2 * XT];
-    float xs[NB], xz[NB];
+    float xs[NB];
+    int xz[NB], xh[NB];                 // sum v, less 4096 xh of it (P > 1); M_16: -8 sum v
     const int xn = NB * nblk * 4;
     if constexpr (P == 1) {
 #pragma unroll
@@ -226,10 +231,10 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                 sum = __builtin_amdgcn_sdot4((int)xe[s][0][i], 0x01010101, sum, false);
                 sum = __builtin_amdgcn_sdot4((int)xo[s][0][i], 0x01010101, sum, false);
             }
-            xz[s] = xs[s] * (float)sum;
+            xz[s] = MODE == M_16 ? -8 * sum : sum;
         }
     } else {
-        // [stream][plane][even, odd][block] of 16 bytes, then {xs, xs sum}
+        // [stream][plane][even, odd][block] of 16 bytes, then {xs, sum v}
         uint32_t* const xp = reinterpret_cast<uint32_t*>(smem);
         float2* const meta = reinterpret_cast<float2*>(smem + (size_t)NB * P * nblk * 32);
         auto put = [&](int i, const uint4 lo, const uint4 hi) {
@@ -241,7 +246,7 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                 d[2 * p * nblk * 4] = v.even[p];
                 d[(2 * p + 1) * nblk * 4] = v.odd[p];
             }
-            if ((e8 & 3) == 0) meta[s * nblk + (e8 >> 2)] = make_float2(v.scale, v.sum);
+            if ((e8 & 3) == 0) meta[s * nblk + (e8 >> 2)] = make_float2(v.scale, __int_as_float(v.sum));
         };
 #pragma unroll
         for (int j = 0; j < XT; j++)
@@ -261,8 +266,10 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                 xo[s][p][0] = o.x; xo[s][p][1] = o.y; xo[s][p][2] = o.z; xo[s][p][3] = o.w;
             }
             const float2 m = meta[s * nblk + c];
+            const int sum = __float_as_int(m.y);
             xs[s] = m.x;
-            xz[s] = m.y;
+            xz[s] = MODE == M_16 ? -8 * sum : sum & 4095;
+            xh[s] = sum >> 12;
         }
         lds_barrier();
     }
@@ -287,7 +294,8 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                         lo[i] = d[i] & 0x0f0f0f0fu;
                         hi[i] = (d[i] >> 4) & 0x0f0f0f0fu;
                     }
-                    const float sc = cur.s.scale(half), ze = cur.s.zero(zeros);
+                    const float sc = cur.s.scale(half);
+                    const int nz = -cur.s.zero(zeros);
 #pragma unroll
                     for (int s = 0; s < NB; s++) {
                         int dot = 0;
@@ -300,7 +308,13 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                                 dot = __builtin_amdgcn_sdot4((int)hi[i], (int)xo[s][p][i], dot, false);
                             }
                         }
-                        if (mine) t[s * tsize] = sc * fmaf(-ze, xz[s], xs[s] * (float)dot);
+                        if (MODE == M_16) {
+                            dot += xz[s];
+                        } else {
+                            dot += __mul24(nz, xz[s]);
+                            if (P > 1) dot += __mul24(nz, xh[s]) * 4096;
+                        }
+                        if (mine) t[s * tsize] = sc * (xs[s] * (float)dot);
                     }
                     t += rs * a.tstride;
                 }
@@ -352,7 +366,10 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 // A window's weights are loaded in address order (lane 4 r + b: block b of row r;
 // a row to a lane, as the operand wants them, makes every lane of a load a cache
 // access of its own) and change lanes in LDS, in the wave's own 1.5 KB, together
-// with their scales.
+// with their scales.  A nibble becomes q - z on its way to the operand: (q - 8) 16,
+// which is the nibble in the byte's high half with its top bit turned (the 16 goes
+// with the digits' joining, or with the scale), or, by a zero point of its row,
+// q + (128 - z), no byte of which carries, with its top bit turned back.
 //
 // No unit is full: 17408 x 5120, sixteen int8 streams, 17.9 us (2.6 TB/s of weights),
 // the vector ALU and the LDS busy for 0.6 of it each, the matrix cores for 0.1; 151936 x
@@ -363,13 +380,12 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 // A window's x in LDS: 8 places of P * 4 G entries of 16 bytes, for two blocks
 // (pair b2 of the window's) and a lane group each (8 values of either block: the
-// even positions' bytes, then the odd ones'); then xs of its blocks, [block][q][G],
-// and xz (of MODE M_16 -8 xz) likewise, or (ONE) [q][G] of the whole window.  Lane groups q and q ^ 1 are 4
-// places apart, a multiple of 256 bytes: a read of 16 bytes a lane takes lanes of
+// even positions' bytes, then the odd ones'); then xs of its blocks, [block][q][G].
+// Lane groups q and q ^ 1 are 4 places apart, a multiple of 256 bytes: a read of 16 bytes a lane takes lanes of
 // both at once, and so finds them in different banks.
 constexpr int mm_place(int b2, int q) { return (q & 1) * 4 + (q >> 1) * 2 + b2; }
 constexpr int mm_xbytes(int P, int G) { return 512 * P * G; }
-constexpr int mm_window(int P, int G, bool ONE) { return mm_xbytes(P, G) + (ONE ? 80 : 128) * G; }
+constexpr int mm_window(int P, int G) { return mm_xbytes(P, G) + 64 * G; }
 
 struct MmArg {
     W4Arg a;
@@ -396,7 +412,7 @@ constexpr uint32_t FAR = 0x80000000u;    // an offset behind every buffer's end
 template <int P, int G, int MODE, bool ONE, bool ADD>
 __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int T = 64 * MM_W, WB = mm_window(P, G, ONE), XB = mm_xbytes(P, G), E = P * 4 * G;
+    constexpr int T = 64 * MM_W, WB = mm_window(P, G), XB = mm_xbytes(P, G), E = P * 4 * G;
     const W4Arg& a = g.a;
     const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, q = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -437,39 +453,24 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
 #pragma unroll
         for (int k = 0; k < XL; k++) r.v[k] = on ? r.v[k] : make_uint4(0, 0, 0, 0);
         uint2 d[P];
-        float scale, xz;
+        float scale;
         if constexpr (P == 1) {
             const uint32_t x = r.v[0].x, y = r.v[0].y;
             d[0] = make_uint2(perm(y, x, 0x06040200), perm(y, x, 0x07050301));
-            int sum = __builtin_amdgcn_sdot4((int)x, 0x01010101, 0, false);
-            sum = __builtin_amdgcn_sdot4((int)y, 0x01010101, sum, false);
-            sum += dpp<QUAD_1>(sum);
-            sum += dpp<QUAD_2>(sum);
             scale = on ? r.s : 0.0f;
-            xz = scale * (float)sum;
         } else {
             const X8 v = split_x(r.v[0], r.v[XL - 1]);
 #pragma unroll
             for (int p = 0; p < P; p++) d[p] = make_uint2(v.even[p], v.odd[p]);
             scale = v.scale;
-            xz = v.sum;
         }
-        if (MODE == M_16) xz = -8.0f * xz;                // (the zero of all)
         uint8_t* const w = smem + (size_t)(b >> 2) * WB;
         const int at = mm_place((b >> 1) & 1, kq) * E + s * P;
         if (in) {
 #pragma unroll
             for (int p = 0; p < P; p++) reinterpret_cast<uint2*>(w)[(at + p) * 2 + (b & 1)] = d[p];
         }
-        float* const m = reinterpret_cast<float*>(w + XB) + ((b & 3) * 4 + (s & 3)) * G + (s >> 2);
-        if (in && kq == 0) m[0] = scale;
-        if constexpr (ONE) {                              // 16 lanes hold the window
-            xz = xz + __int_as_float(dpp<HALF_MIRROR>(__float_as_int(xz)));
-            xz = xz + __int_as_float(dpp<MIRROR>(__float_as_int(xz)));
-            if (in && (e & 15) == 1) reinterpret_cast<float*>(w + XB)[16 * G + (s & 3) * G + (s >> 2)] = xz;
-        } else {
-            if (in && kq == 1) m[16 * G] = xz;
-        }
+        if (in && kq == 0) reinterpret_cast<float*>(w + XB)[((b & 3) * 4 + (s & 3)) * G + (s >> 2)] = scale;
     };
     // on its way before the weights, as loads return in order
     X x0 = get(e), x1 = get(e + xstep);
@@ -546,15 +547,17 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     float* const sl = reinterpret_cast<float*>(stage + 16 * 64);
     for (int i = i0; i < i1; i++) {
         uint32_t d[2][4];
-        float sc[2][4], ze[2][4];
+        float sc[2][4];
+        uint32_t zb[2][4];                             // 128 - z in every byte
 #pragma unroll
         for (int j = 0; j < 2; j++) {
             // (a wave's LDS accesses are in order)
             *reinterpret_cast<uint4*>(stage + put_at) = cur.q[j];
             if (j < NS) {
                 const RawScale<MODE>& r = cur.s[j];
-                if (MODE == M_16) sl[lane] = r.scale(half);
-                else reinterpret_cast<float2*>(sl)[lane] = make_float2(r.scale(half), r.zero(zeros));
+                if (MODE == M_16) sl[lane] = r.scale(half) * (P == 1 ? 0.0625f : 1.0f);
+                else reinterpret_cast<uint2*>(sl)[lane] =
+                    make_uint2(__float_as_uint(r.scale(half)), 0x80808080u - 0x01010101u * (uint32_t)r.zero(zeros));
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
 #pragma unroll
@@ -565,9 +568,9 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                 if (MODE == M_16) {
                     sc[j][b] = sl[at];
                 } else {
-                    const float2 v = reinterpret_cast<const float2*>(sl)[at];
-                    sc[j][b] = v.x;
-                    ze[j][b] = v.y;
+                    const uint2 v = reinterpret_cast<const uint2*>(sl)[at];
+                    sc[j][b] = __uint_as_float(v.x);
+                    zb[j][b] = v.y;
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -580,7 +583,7 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
             float sum[G];
             if (ONE) {
 #pragma unroll
-                for (int c = 0; c < G; c++) sum[c] = MODE == M_16 ? m[16 * G + c] : -ze[j][0] * m[16 * G + c];
+                for (int c = 0; c < G; c++) sum[c] = 0.0f;
             }
 #pragma unroll
             for (int b2 = 0; b2 < 2; b2++) {
@@ -593,7 +596,16 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                 for (int h = 0; h < 2; h++) {
                     const int b = 2 * b2 + h;
                     const uint32_t db = d[j][b];
-                    const long wv = (long)(((uint64_t)((db >> 4) & 0x0f0f0f0fu) << 32) | (db & 0x0f0f0f0fu));
+                    uint32_t lo, hi;
+                    if (MODE == M_16) {
+                        lo = ((db << 4) & 0xf0f0f0f0u) ^ 0x80808080u;
+                        hi = (db & 0xf0f0f0f0u) ^ 0x80808080u;
+                    } else {
+                        const uint32_t z = zb[j][ONE ? 0 : b];
+                        lo = ((db & 0x0f0f0f0fu) + z) ^ 0x80808080u;
+                        hi = (((db >> 4) & 0x0f0f0f0fu) + z) ^ 0x80808080u;
+                    }
+                    const long wv = (long)(((uint64_t)hi << 32) | lo);
                     int dot[G];
 #pragma unroll
                     for (int c = 0; c < NX; c++) {
@@ -604,18 +616,16 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
 #pragma unroll
                             for (int e = 0; e < G; e++) dot[e] = D[e];
                         } else {
-                            dot[c] = (((D[2] << 8) + D[1]) << 8) + D[0];
+                            int top = D[2] * 256 + D[1];
+                            asm("" : "+v"(top));       // (else two shifts and a sum of three)
+                            dot[c] = MODE == M_16 ? top * 16 + (D[0] >> 4) : top * 256 + D[0];
                         }
                     }
 #pragma unroll
                     for (int c = 0; c < G; c++) {
                         const float xs = m[4 * G * b + c];
                         if (ONE) sum[c] = fmaf(xs, (float)dot[c], sum[c]);
-                        else {
-                            const float xz = m[16 * G + 4 * G * b + c], d = (float)dot[c];
-                            acc[c] = fmaf(sc[j][b], MODE == M_16 ? fmaf(xs, d, xz) : fmaf(-ze[j][b], xz, xs * d),
-                                          acc[c]);
-                        }
+                        else acc[c] = fmaf(sc[j][b], xs * (float)dot[c], acc[c]);
                     }
                 }
             }
@@ -750,7 +760,7 @@ void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
     p->G = (g.bt + 3) / 4;
     if (p->G == 3) p->G = 4;
     g.nwin = (a.nblk + 3) / 4;
-    const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G, a.w.group % 128 == 0);
+    const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G);
     int most_w = (int)((g_lds_max - own) / wb) & ~1;                  // windows that LDS takes, in pairs
     // (two halves of x for as many workgroups each are ahead of all of it for each,
     // where it fills the LDS: eight streams of binary32, 17408 x 5120 22.1 / 23.5 us)

@@ -323,3 +323,54 @@ def test_matrices_past_4_gib(B, q8):
     assert ((got.double() - want).abs() <= tol).all()
     if B == 1:
         assert (got == first.view(B, 1, n)).all()
+
+
+def given(c, x=None, nib=None):
+    """The case with other x and other nibbles (N rows of K), and its exact products."""
+    if x is not None:
+        amax = np.abs(x).reshape(c.B, -1, 32).max(-1)
+        if c.q8:
+            sc = (amax / np.float32(127)).astype(np.float32)
+            xq = np.rint(x.reshape(c.B, -1, 32).astype(np.float64) / sc[:, :, None])
+            c.dxq, c.dxs = torch.from_numpy(xq.astype(np.int8).reshape(c.B, c.K)).cuda(), torch.from_numpy(sc).cuda()
+        else:
+            c.dx = torch.from_numpy(x).cuda()
+    if nib is not None:
+        c.dq.copy_(torch.from_numpy((nib[:, ::2] | nib[:, 1::2] << 4).astype(np.uint8)))
+    q = c.dq.cpu().numpy()
+    n = np.stack([q & 15, q >> 4], -1).reshape(c.N, -1, c.g).astype(np.float64)
+    n -= 8.0 if c.dz is None else c.dz.cpu().numpy()[:, :, None]
+    c.W = (n * c.ds.cpu().double().numpy()[:, :, None]).reshape(c.N, c.K)
+    if c.q8:
+        sc = c.dxs.cpu().numpy().astype(np.float64)
+        x, amax = c.dxq.cpu().numpy().astype(np.float64) * np.repeat(sc, 32, 1), sc * 128
+    else:
+        x = c.dx.cpu().numpy().astype(np.float64)
+        amax = np.abs(x).reshape(c.B, -1, 32).max(-1)
+    c.exact, c.a = x @ c.W.T, np.repeat(amax, 32, 1) @ np.abs(c.W).T
+    return c
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 2, 3, 4, 6, 16])
+@pytest.mark.parametrize("g", [32, 128])
+@pytest.mark.parametrize("scale", ["f16", "f32"])
+def test_weights_at_their_zero_point(scale, g, B, q8):
+    """Padded and pruned rows, x of one sign: the bound goes with |q - z|, so rows of which every
+    weight is at its zero point give 0, and one weight in 128 gives no more error than its own."""
+    r = np.random.default_rng(B + g)
+    x = (1 + 0.2 * r.standard_normal((B, 1024))).astype(np.float32) * np.float32(5)
+    for z in (None, 7, 8, 11, 15):
+        c = Case(80, 1024, B, g, scale, z is not None, q8)
+        zero = 8 if z is None else z
+        if z is not None:
+            c.dz.fill_(z)
+        nib = np.full((80, 1024), zero, np.uint8)
+        y = given(c, x, nib).check()
+        assert (y[:B * 80] == 0).all()
+        for k in range(8):
+            nib[np.arange(80), 128 * k + r.integers(0, 128, 80)] ^= 1
+        given(c, nib=nib).check()
+        # near the zero point, most of them on it
+        near = np.clip(zero + np.rint(0.4 * r.standard_normal((80, 1024))), 0, 15).astype(np.uint8)
+        given(c, nib=near).check()
