@@ -552,8 +552,11 @@ typedef struct kq_w4 {
  * aligned.  work: kq_w4_workspace_bytes of device memory, 256-byte aligned
  * (0 bytes, as with most sizes: may be NULL).
  * The result is within (K / 32 + 8) 2^-24 sum_k |w_k| max|x| of the exact one
- * (and the last rounding's half unit), the maximum over the 32 values of x
- * that k lies in, counted as 2^-126 where it is less.  A row's bits do not
+ * (and the last rounding's half unit, and K / 32 of 2^-149), the maximum over
+ * the 32 values of x that k lies in, counted as 2^-126 where it is less: a
+ * weight at its zero point adds nothing, and x may be any finite value as long
+ * as sums of |w x| stay finite.  That holds for scales that are 0 or from 2^-122
+ * to 2^96 in magnitude, as all of binary16 are.  A row's bits do not
  * depend on other rows' values, but on B, as the order of its sum does.  A
  * row with a value that is not finite gives no finite one. */
 int kq_w4_gemv_dev(const kq_w4* w, const float* x, const float* add, float* y, int B, void* work,

@@ -15,7 +15,8 @@
 // it was computed from.  Per block, sum (q - z) v is exact, as is sum q v on its
 // way (at most 480 * 2^22 < 2^31): zero points are taken off in integers, so that
 // weights at theirs give nothing, whatever x is.  Blocks are scaled and added in
-// binary32.
+// binary32, by the weights' scale first: sum (q - z) x passes binary32's range from
+// |x| of 7e35 on, s sum (q - z) v stays in it for scales below 2^96.
 #include <hip/hip_runtime.h>
 #include <hip/hip_fp16.h>
 #include <stdint.h>
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
                             dot += __mul24(nz, xz[s]);
                             if (P > 1) dot += __mul24(nz, xh[s]) * 4096;
                         }
-                        if (mine) t[s * tsize] = sc * (xs[s] * (float)dot);
+                        if (mine) t[s * tsize] = sc * (float)dot * xs[s];
                     }
                     t += rs * a.tstride;
                 }
@@ -580,11 +581,6 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
         for (int j = 0; j < 2; j++) {
             const uint8_t* const xb = smem + (2 * w + j) * WB;
             const float* const m = reinterpret_cast<const float*>(xb + moff);
-            float sum[G];
-            if (ONE) {
-#pragma unroll
-                for (int c = 0; c < G; c++) sum[c] = 0.0f;
-            }
 #pragma unroll
             for (int b2 = 0; b2 < 2; b2++) {
                 constexpr int NX = P == 1 ? 1 : G;
@@ -624,14 +620,9 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
 #pragma unroll
                     for (int c = 0; c < G; c++) {
                         const float xs = m[4 * G * b + c];
-                        if (ONE) sum[c] = fmaf(xs, (float)dot[c], sum[c]);
-                        else acc[c] = fmaf(sc[j][b], xs * (float)dot[c], acc[c]);
+                        acc[c] = fmaf(sc[j][ONE ? 0 : b] * (float)dot[c], xs, acc[c]);
                     }
                 }
-            }
-            if (ONE) {
-#pragma unroll
-                for (int c = 0; c < G; c++) acc[c] = fmaf(sc[j][0], sum[c], acc[c]);
             }
         }
         w++;

@@ -374,3 +374,25 @@ def test_weights_at_their_zero_point(scale, g, B, q8):
         # near the zero point, most of them on it
         near = np.clip(zero + np.rint(0.4 * r.standard_normal((80, 1024))), 0, 15).astype(np.uint8)
         given(c, nib=near).check()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("B", [1, 2, 3, 6, 16])
+@pytest.mark.parametrize("zeros", [False, True])
+def test_x_near_the_largest(zeros, B, q8):
+    """Finite results of x up to binary32's largest: sums of 15 |x| over a block or a window lie past it
+    while those of |w x| (at most 0.3 * 3.4e38, and 0.03 * 256 * 1e37 in the mean) do not."""
+    r = np.random.default_rng(B)
+    for g in (32, 128):
+        for scale in ("f16", "bf16", "f32"):
+            c = Case(48, 256, B, g, scale, zeros, q8)
+            x = (1e37 * r.standard_normal((B, 256))).astype(np.float32)
+            assert np.isfinite(given(c, x).check()[:B * 48].cpu().numpy()).all()
+            x = (1e30 * r.standard_normal((B, 256))).astype(np.float32)
+            x[:, 70] = np.float32(3.4e38)
+            assert np.isfinite(given(c, x).check()[:B * 48].cpu().numpy()).all()
+            if scale != "f16":              # scales far from 1 on either side of x
+                for p in (-90, 90):
+                    c.ds.mul_(2.0 ** p)
+                    given(c, (r.standard_normal((B, 256)) * 2.0 ** -p).astype(np.float32)).check()
+                    c.ds.mul_(2.0 ** -p)
