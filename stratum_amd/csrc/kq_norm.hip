@@ -170,15 +170,32 @@ int launch(const kq_rmsnorm& a, hipStream_t st) {
     constexpr int MOST = V == 4 ? 4 : 8;       // (8 steps of 4 spill registers)
     int steps = (long)a.B * nv <= 1 << 19 ? 1 : 4;
     while (steps <= MOST && nv > 1024 * steps) steps *= 2;
-    const dim3 grid((unsigned)a.B);
     const int per = steps <= MOST ? (nv + steps - 1) / steps : 1024;
     const dim3 wg((unsigned)((per + 63) / 64 * 64));
-    if (steps == 1) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 1>), grid, wg, 0, st, a);
-    else if (steps == 2) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 2>), grid, wg, 0, st, a);
-    else if (steps == 4) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 4>), grid, wg, 0, st, a);
-    else if (steps == MOST) hipLaunchKernelGGL((kq_rmsnorm_kernel<V, MOST>), grid, wg, 0, st, a);
-    else hipLaunchKernelGGL((kq_rmsnorm_kernel<V, 0>), grid, wg, 0, st, a);
-    return (int)hipGetLastError();
+    auto* const k = steps == 1 ? kq_rmsnorm_kernel<V, 1> : steps == 2 ? kq_rmsnorm_kernel<V, 2>
+                  : steps == 4 ? kq_rmsnorm_kernel<V, 4> : steps == MOST ? kq_rmsnorm_kernel<V, MOST>
+                                                                         : kq_rmsnorm_kernel<V, 0>;
+    // A launch of 2^32 lanes or more is cut to their number modulo that without an
+    // error: more rows (2^26 where each takes 64) go in parts.
+    const int most = (int)(0xffffffffu / wg.x);
+    kq_rmsnorm b = a;
+    for (int left = a.B; left > 0; left -= most) {
+        b.B = left < most ? left : most;
+        hipLaunchKernelGGL(k, dim3((unsigned)b.B), wg, 0, st, b);
+        const int e = (int)hipGetLastError();
+        if (e) return e;
+        b.x += most * b.x_stride;
+        if (b.resid) b.resid += most * b.resid_stride;
+        if (b.sum) b.sum += most * b.sum_stride;
+        if (b.y) b.y += most * b.y_stride;
+        if (b.group) {
+            const int64_t groups = (int64_t)most * (b.K / b.group);
+            b.xq += (int64_t)most * b.K;
+            b.xscale += groups;
+            if (b.xsum) b.xsum += groups;
+        }
+    }
+    return 0;
 }
 
 }  // namespace

@@ -227,3 +227,24 @@ def test_rows_past_32_bits():
     torch.cuda.synchronize()
     check_y(y.cpu().numpy(), want(x, None, None, 1e-6)[1])
     assert torch.equal(rows4, y)
+
+
+@pytest.mark.parametrize("group", [0, 16])
+def test_more_rows_than_a_launch_takes(group):
+    """Rows times lanes past 2^32: 64 lanes a row are the fewest, so 2^26 rows and some."""
+    B, n = (1 << 26) + 77, 16 if group else 1
+    x = torch.empty(B, n, device="cuda").uniform_(0.5, 2.0)
+    x[:, ::3] *= -1
+    q, sc = (torch.zeros(B, n, dtype=torch.int8, device="cuda"), torch.zeros(B, device="cuda")) if group else (None, None)
+    y = torch.full((B, n), float("nan"), device="cuda")
+    K.rmsnorm_dev(K.rmsnorm(B, n, 1e-6, x.data_ptr(), y_ptr=y.data_ptr(), group=group,
+                            xq_ptr=q.data_ptr() if group else None, xscale_ptr=sc.data_ptr() if group else None), st())
+    torch.cuda.synchronize()
+    for a in range(0, B, 1 << 24):
+        d = x[a:a + (1 << 24)].double()
+        want = d / torch.sqrt((d * d).mean(1, keepdim=True) + np.float64(np.float32(1e-6)))
+        got = y[a:a + (1 << 24)].double()
+        assert ((got - want).abs() <= want.abs() * (2.0 ** -24 * (1 + 2.0 ** -20) + 24 * 2.0 ** -53)).all()
+        if group:
+            s = sc[a:a + (1 << 24), None].double()
+            assert ((q[a:a + (1 << 24)].double() * s - got).abs() <= s * (0.5 + 2.0 ** -16)).all()
