@@ -656,14 +656,16 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
     }
 }
 
-// the parts of rows that were cut, in their order
+// the parts of rows that were cut, in their order (a launch of 2^32 lanes or more is
+// cut to their number modulo that without an error, so the lanes step over the rest)
+constexpr long JOIN_WGS = 1L << 22;
 __global__ __launch_bounds__(256) void kq_w4_join_kernel(const float* part, const float* add, float* y,
                                                          long n, int ks) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    float sum = part[i];
-    for (int k = 1; k < ks; k++) sum = sum + part[k * n + i];
-    y[i] = add ? add[i] + sum : sum;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
+        float sum = part[i];
+        for (int k = 1; k < ks; k++) sum = sum + part[k * n + i];
+        y[i] = add ? add[i] + sum : sum;
+    }
 }
 
 // ------------------------------------------------------------- the plan
@@ -798,8 +800,9 @@ int launch_mm(MmArg& g, const MmPlan& p, void* work, hipStream_t st) {
                                                                     : launch_mm_g<P, 4>(g, p, st);
     if (e || g.ks == 1) return e;
     const long n = (long)g.B * g.a.w.N;
-    hipLaunchKernelGGL(kq_w4_join_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, g.part, g.a.add,
-                       g.a.y, n, g.ks);
+    const long wgs = (n + 255) / 256;
+    hipLaunchKernelGGL(kq_w4_join_kernel, dim3((unsigned)(wgs < JOIN_WGS ? wgs : JOIN_WGS)), dim3(256), 0, st,
+                       g.part, g.a.add, g.a.y, n, g.ks);
     return (int)hipGetLastError();
 }
 

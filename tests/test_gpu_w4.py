@@ -396,3 +396,30 @@ def test_x_near_the_largest(zeros, B, q8):
                     c.ds.mul_(2.0 ** p)
                     given(c, (r.standard_normal((B, 256)) * 2.0 ** -p).astype(np.float32)).check()
                     c.ds.mul_(2.0 ** -p)
+
+
+def test_more_outputs_of_cut_rows_than_a_launch_has_lanes():
+    """2^32 and more outputs of rows in two parts, which a launch of its own joins (50 GB): seven rows of x
+    over and over, so that every repeat has to give the same bits, the first of them the bound's."""
+    n, Kd, g, m = 337, 2560, 128, 7
+    reps, B = 195, 65534
+    c = Case(n, Kd, m, g)
+    N = n * reps
+    assert N * B > 1 << 32
+    q, s = c.dq.repeat(reps, 1), c.ds.repeat(reps, 1)
+    x = c.dx.repeat(B // m, 1).contiguous()
+    w = K.w4(N, Kd, g, K.TYPE_F16, q.data_ptr(), s.data_ptr())
+    nb = K.w4_workspace_bytes(w, B)
+    assert nb >= 2 * 4 * N * B
+    work = torch.empty(nb, dtype=torch.uint8, device="cuda")
+    y = torch.full((B, N), float("nan"), device="cuda")
+    K.w4_gemv_dev(w, x.data_ptr(), y.data_ptr(), B, work.data_ptr(), nb, stream=st())
+    torch.cuda.synchronize()
+    del work
+    got = y[:m].cpu().numpy().reshape(m, reps, n).astype(np.float64)
+    assert (np.abs(got - c.exact[:, None]) <= c.tol(c.exact)[:, None]).all()
+    for a in range(0, B, 700):
+        part = y[a:a + 700].view(-1, m, N)
+        assert (part == y[:m]).all()
+    del y, part
+    torch.cuda.empty_cache()
