@@ -754,12 +754,12 @@ void mm_plan(MmArg& g, int P, int n_cu, MmPlan* p) {
     if (p->G == 3) p->G = 4;
     g.nwin = (a.nblk + 3) / 4;
     const long own = (long)MM_W * mm_wave(p->G), wb = mm_window(P, p->G);
-    int most_w = (int)((g_lds_max - own) / wb) & ~1;                  // windows that LDS takes, in pairs
-    // (two halves of x for as many workgroups each are ahead of all of it for each,
-    // where it fills the LDS: eight streams of binary32, 17408 x 5120 22.1 / 23.5 us)
-    if (P == 3 && p->G == 2 && most_w > 38) most_w = 38;
-    // as few parts as x needs: with four, eight streams of binary32 are 5 % faster
-    // (17408 x 5120 22.4 / 21.4 us), int8 rows slower (four 13.4 / 15.6, sixteen 18.0 / 19.3)
+    const int most_w = (int)((g_lds_max - own) / wb) & ~1;                  // windows that LDS takes, in pairs
+    // as few parts as x needs.  Eight streams of binary32 in one part / in two, us: 11008
+    // rows of 4096 12.5 / 13.3, of 5120 15.1 / 15.6; 65536 rows of 5120 44.9 / 48.6, 17408
+    // 19.6 / 19.2, 5120 12.7 / 12.0 (what two gain where a CU has few rows, x's way to LDS,
+    // is less than the join's launch costs elsewhere); int8 rows in one / four, 17408 x
+    // 5120, four streams 13.4 / 15.6, sixteen 18.0 / 19.3
     g.ks = (g.nwin + most_w - 1) / most_w;
     g.nw = (g.nwin + g.ks - 1) / g.ks;
     g.ks = (g.nwin + g.nw - 1) / g.nw;

@@ -423,3 +423,15 @@ def test_more_outputs_of_cut_rows_than_a_launch_has_lanes():
         assert (part == y[:m]).all()
     del y, part
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("g", [32, 64, 128])
+def test_workspace_only_where_x_does_not_fit(g, q8):
+    """With eight rows the waves' own LDS is 33 KB and a window of 128 values 3200 bytes (int8 1152), so
+    that 160 KB hold 40 windows of them; none of these needs a workspace."""
+    for N in (5120, 17408, 65536):
+        for Kd in (128, 4096, 4992, 5120):
+            for B in (1, 2, 5, 8):
+                assert K.w4_workspace_bytes(K.w4(N, Kd, g, K.TYPE_F16, 256, 256), B, q8) == 0
+    assert K.w4_workspace_bytes(K.w4(5120, 40960, g, K.TYPE_F16, 256, 256), 8, q8) > 0
