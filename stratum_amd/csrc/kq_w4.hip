@@ -552,7 +552,8 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
         uint32_t zb[2][4];                             // 128 - z in every byte
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            // (a wave's LDS accesses are in order)
+            // A wave's LDS accesses are in order; the fences keep the compiler's order of what
+            // its lanes write and others of them read, both ways.
             *reinterpret_cast<uint4*>(stage + put_at) = cur.q[j];
             if (j < NS) {
                 const RawScale<MODE>& r = cur.s[j];
@@ -560,7 +561,7 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                 else reinterpret_cast<uint2*>(sl)[lane] =
                     make_uint2(__float_as_uint(r.scale(half)), 0x80808080u - 0x01010101u * (uint32_t)r.zero(zeros));
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
             for (int b = 0; b < 4; b++) d[j][b] = *reinterpret_cast<const uint32_t*>(stage + (take_at ^ (16 * b)));
 #pragma unroll
@@ -574,7 +575,7 @@ __global__ __launch_bounds__(64 * MM_W) void kq_w4_mm_kernel(MmArg g) {
                     zb[j][b] = v.y;
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
         load(cur);                                     // the next pair's, while this one's are used
 #pragma unroll
