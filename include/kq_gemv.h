@@ -592,7 +592,7 @@ int64_t kq_w4_workspace_bytes(const kq_w4* w, int B, int q8);
  * -1.  Computed in binary64 from the binary32 rows.  Tokens outside 0..V-1
  * are refused; a NaN has no weight; a row with no weight at all (or with an
  * infinite logit above all) gives next = -1; u >= 1 or NaN draws the last
- * token with any weight.  u: S rows of T + 1.  Strides are in elements (0:
+ * token with any weight, u <= 0 the first.  u: S rows of T + 1.  Strides are in elements (0:
  * rows of V, sequences after each other).  T == 0 draws one token from each row. */
 #define KQ_VERIFY_LOGITS 1
 #define KQ_VERIFY_GREEDY 2

@@ -457,12 +457,14 @@ __device__ __forceinline__ void draw(const VfArg& a, int s, int n, Drawn d) {
             w = w + w4[e];
         }
         const int who = passed(w, target, run, base, found);
-        // that lane's token: until the sum is past the target
+        // that lane's token: until the sum is past the target, its first with any weight
+        // where the sum before it is already (a negative u; or a last bit, as lanes'
+        // running sums are added up in orders of their own)
         int at = -1;
         double cum = base;
 #pragma unroll
         for (int e = 0; e < 4; e++)
-            if (w4[e] > 0.0 && !(cum > target)) {
+            if (w4[e] > 0.0 && (at < 0 || !(cum > target))) {
                 cum = cum + w4[e];
                 at = k + e;
             }

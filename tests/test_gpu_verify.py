@@ -464,3 +464,28 @@ def test_vocabulary_of_many_chunks(form, draft):
     tokens = r.integers(0, V, (S, T)).astype(np.int32)
     u = np.array([[0.9, 0.1, 0.02], [0.5, 0.9, 0.55], [0.9, 0.9, 0.999]], np.float32)
     check(target, d if draft else None, tokens, np.array([2, 0, 1], np.int32), u, form)
+
+
+@pytest.mark.parametrize("form", ["logits", "probs"])
+@pytest.mark.parametrize("draft", [False, True])
+def test_u_below_zero(form, draft):
+    """u below zero draws the first token with any weight, as u = 0 does."""
+    target, d, tokens, nd, u = make(4, 2, 9000, form, draft, 51)
+    nd[:] = [0, 2, 0, 2]
+    u[:, :2] = [[0, 0], [0, 0], [0, 0], [2, 2]]          # the last refuses its first token
+    target[:, :, :4100] = -np.inf if form == "logits" else 0.0
+    tokens[:] = [4100, 8000]
+    u[:, 2] = [-0.0, -1e-30, -3.0, -np.inf]
+    na, out = run(target, d, tokens, nd, u, form)
+    assert na.tolist() == [0, 2, 0, 0] if not draft else na[0] == na[2] == na[3] == 0
+    for s in range(4):
+        n = na[s]
+        if form == "logits":
+            p = softmax(target[s, n], 1.0)
+            q = softmax(d[s, n], 1.0) if draft and n < nd[s] else 0.0
+        else:
+            p, q = target[s, n].astype(np.float64), d[s, n].astype(np.float64) if draft and n < nd[s] else 0.0
+        w = np.maximum(p - q, 0)
+        if not draft and n < nd[s]:
+            w[tokens[s, n]] = 0
+        assert out[s, n] == np.flatnonzero(w)[0]
