@@ -489,3 +489,16 @@ def test_u_below_zero(form, draft):
         if not draft and n < nd[s]:
             w[tokens[s, n]] = 0
         assert out[s, n] == np.flatnonzero(w)[0]
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_empty_row_after_accepted_tokens(draft):
+    """Logits of -inf everywhere at the second drafted token, and in the row after the last:
+    what lies before is accepted (u = 0), nothing can be drawn there."""
+    target, d, tokens, nd, u = make(3, 2, 6000, "logits", draft, 52)
+    u[:], nd[:] = 0.0, 2
+    u[:, 2] = 0.5
+    target[0, 1], target[1, 2], target[2, 1, :] = -np.inf, -np.inf, np.nan
+    na, out = run(target, d, tokens, nd, u, "logits")
+    assert na.tolist() == [1, 2, 1]
+    assert out.tolist() == [[tokens[0, 0], -1, -1], [*tokens[1], -1], [tokens[2, 0], -1, -1]]
