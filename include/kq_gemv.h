@@ -589,11 +589,17 @@ int64_t kq_w4_workspace_bytes(const kq_w4* w, int B, int q8);
  * draft, u and inv_temp unused: accepted iff the token is its row's maximum
  * (the lowest of equals), the next one row n's maximum.
  * Writes n_accept[s] and out[s][0..T]: the accepted tokens, the next one, then
- * -1.  Computed in binary64 from the binary32 rows.  Tokens outside 0..V-1
- * are refused; a NaN has no weight; a row with no weight at all (or with an
- * infinite logit above all) gives next = -1; u >= 1 or NaN draws the last
- * token with any weight, u <= 0 the first.  u: S rows of T + 1.  Strides are in elements (0:
- * rows of V, sequences after each other).  T == 0 draws one token from each row. */
+ * -1.  Computed in binary64 from the binary32 rows; of logits, p and q are
+ * within 6e-12 of their values (exponentials within 1.1e-12, of which a
+ * weight, its chunk's and its row's sum have five; a few more 1.1e-12 where V
+ * is above 262144), and less than 2^-1000 of a row's largest counts as nothing.
+ * p - q has the sum of both errors, so u decides another token than exact
+ * values would only where it lies that near to a border.  Tokens outside
+ * 0..V-1 are refused; a NaN has no weight; a row with no weight at all (or
+ * with an infinite logit above all) gives next = -1; u >= 1 or NaN draws the
+ * last token with any weight, u <= 0 the first.  u: S rows of T + 1.  Strides
+ * are in elements (0: rows of V, sequences after each other).  T == 0 draws
+ * one token from each row. */
 #define KQ_VERIFY_LOGITS 1
 #define KQ_VERIFY_GREEDY 2
 #define KQ_VERIFY_MAX_DRAFT 63

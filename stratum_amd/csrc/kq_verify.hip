@@ -8,7 +8,9 @@
 // whose running sum of weights is above u times their total.
 //
 // All of it is binary64: a running sum over 150 K tokens has as many borders,
-// and a token changes where one of them moves past u.
+// and a token changes where one of them moves past u.  Of logits the weights are
+// good to 6e-12 (pow2() below), which moves borders by a ten-thousandth of a
+// binary32 u's step (2^-24).
 //
 // Launches: the rows' maxima and sums of exponentials per chunk of CH tokens
 // (logits and greedy form); then the weights' sums per chunk of the row drawn
@@ -47,7 +49,9 @@ struct VfArg {
 // that interval, within 1.1e-12 of it.  d is the difference of two logits, so it
 // is 0 at the maximum whatever that is (a row of the type's lowest value is a
 // uniform one).  k comes as the low bits of d c + 1.5 * 2^52 and goes into the
-// exponent as an integer.  These 18 binary64 instructions a value bound the first
+// exponent as an integer.  A weight has five of them on its way: its own, and four
+// in its row's sum, to the maximum of a wave, a chunk, a lane's chunks and the row (one
+// more per 64 chunks after the first).  These 18 binary64 instructions a value bound the first
 // launch (sixteen sequences of seven, 240 rows of 151936, both launches: 57 us,
 // with the library's exp2() 76; one of four, 15 and 18).
 __device__ __forceinline__ double pow2(double d, double c, double far) {

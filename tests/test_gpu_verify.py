@@ -502,3 +502,31 @@ def test_empty_row_after_accepted_tokens(draft):
     na, out = run(target, d, tokens, nd, u, "logits")
     assert na.tolist() == [1, 2, 1]
     assert out.tolist() == [[tokens[0, 0], -1, -1], [*tokens[1], -1], [tokens[2, 0], -1, -1]]
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("S,T,V", [(6, 2, 50), (6, 5, 1000), (4, 3, 20001)])
+def test_logits_with_their_error(S, T, V, draft):
+    """A weight is within 6e-12 of p's (five exponentials of 1.1e-12 on its way, include/kq_gemv.h), so p - q
+    within 6e-12 (p + q), and a running sum of it within 1.2e-11, and V 2^-52 of the total: u lies further from
+    every border that decides something, and then the tokens are equal."""
+    for seed in range(4):
+        target, d, tokens, nd, u = make(S, T, V, "logits", draft, 60 + seed)
+        for s in range(S):
+            n = 0
+            while True:
+                p = softmax(target[s, n], 1.25)
+                if n == nd[s]:
+                    w = p
+                    break
+                t = tokens[s, n]
+                q = softmax(d[s, n], 1.25) if draft else np.eye(1, V, t)[0]
+                a = np.float64(u[s, n]) * q[t]
+                assert abs(a - p[t]) > 6e-12 * (a + p[t])
+                if not a < p[t]:
+                    w = np.maximum(p - q, 0)
+                    break
+                n += 1
+            cum = np.cumsum(w)
+            assert np.abs(cum - np.float64(u[s, T]) * cum[-1]).min() > 2 * 1.2e-11 + V * 2.0 ** -52 * cum[-1]
+        check(target, d, tokens, nd, u, "logits", it=1.25)
