@@ -83,8 +83,6 @@ __device__ __forceinline__ void store_rows(const kq_rmsnorm& a, long row, int i,
 template <int V, int NV>
 __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
     using F = typename Vec<V>::f;
-    // the weights are asked for before the sum, where registers allow it
-    constexpr bool HOLD_W = V * NV <= 16;
     __shared__ double sm[16];
     const long row = blockIdx.x;
     const int T = blockDim.x, i0 = V * threadIdx.x, K = a.K;
@@ -115,7 +113,8 @@ __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int i = i0 + j * V * T;
-            if (HOLD_W && a.weight) w[j] = i < K ? *reinterpret_cast<const F*>(a.weight + i) : zero;
+            // (the weights are asked for before the sum)
+            if (a.weight) w[j] = i < K ? *reinterpret_cast<const F*>(a.weight + i) : zero;
             if (i < K) take(v[j], i);
         }
     } else {
@@ -139,9 +138,7 @@ __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
 #pragma unroll
         for (int j = 0; j < NV; j++) {
             const int i = i0 + j * V * T;
-            F g = zero;
-            if (a.weight) g = HOLD_W ? w[j] : i < K ? *reinterpret_cast<const F*>(a.weight + i) : zero;
-            finish(v[j], g, i);
+            finish(v[j], a.weight ? w[j] : zero, i);
         }
     } else {
         for (int j = 0; j < K; j += V * T) {
@@ -160,13 +157,14 @@ __global__ __launch_bounds__(1024) void kq_rmsnorm_kernel(kq_rmsnorm a) {
 template <int V>
 int launch(const kq_rmsnorm& a, hipStream_t st) {
     const int nv = (a.K + V - 1) / V;
-    // One step, on as many lanes as the row has loads, while the device's lanes (2048
-    // on each of 256 CUs) hold all rows; four steps in fewer lanes, which keep more
-    // loads in flight, when they do not.  One step / four, us: rows of 1024 to int8,
-    // one 2.5 / 4.1, 2048 rows 8.2 / 8.5, 4096 14.2 / 13.8; rows of 5120 to binary32,
-    // one 3.1 / 3.4, 512 rows 7.8 / 7.4, 1024 13.5 / 11.2, 4096 36.2 / 33.5; to int8
-    // 4.2 / 5.3, 10.0 / 10.5, 19.0 / 17.1, 53.7 / 52.4; rows of 1153 single values, one
-    // 2.7 / 2.8, 512 rows 4.6 / 4.2, 4096 23.0 / 17.1.
+    // As few steps as 1024 lanes allow (one up to 1024 loads a row) while the device's
+    // lanes (2048 on each of 256 CUs) hold all rows; four steps in fewer lanes, which
+    // keep more loads in flight, when they do not.  One step / four, us: rows of 1024
+    // to int8, one 2.5 / 4.1, 2048 rows 8.2 / 8.5, 4096 14.2 / 13.8.  Two steps (of 1280
+    // or 1153 loads) / four: rows of 5120 to binary32, one 3.1 / 3.4, 512 rows 7.8 / 7.4,
+    // 1024 13.5 / 11.2, 4096 36.2 / 33.5; to int8 4.2 / 5.3, 10.0 / 10.5, 19.0 / 17.1,
+    // 53.7 / 52.4; rows of 1153 single values, one 2.7 / 2.8, 512 rows 4.6 / 4.2, 4096
+    // 23.0 / 17.1.
     constexpr int MOST = V == 4 ? 4 : 8;       // (8 steps of 4 spill registers)
     int steps = (long)a.B * nv <= 1 << 19 ? 1 : 4;
     while (steps <= MOST && nv > 1024 * steps) steps *= 2;
