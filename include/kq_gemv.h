@@ -493,9 +493,9 @@ int kq_moe_ffn_last_path(void);
 
 /* ------------------------------------------- around the products
  * The row operators of a decode step that lie next to its products: the
- * norm before them (to binary32 or to the int8 rows that they read), products
- * with 4-bit weights and plain group scales, and the check of drafted tokens
- * after the LM head.  Device pointers, enqueue only, on any stream; nothing
+ * norm before them (to binary32, which every product reads, or to int8 rows,
+ * which those of this section read), products with 4-bit weights and plain
+ * group scales, and the check of drafted tokens after the LM head.  Device pointers, enqueue only, on any stream; nothing
  * is allocated and no library scratch is used: what a call needs beside its
  * operands is device memory that the caller passes (`work`), which calls that
  * may overlap in time must not share.  -1 with a message on a bad argument

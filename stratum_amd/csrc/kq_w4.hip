@@ -159,8 +159,8 @@ constexpr int walk_waves(int P, int NB) { return P * NB <= 3 ? 5 : P * NB <= 6 ?
 // each row's terms, while the next pass goes on with the other half of the buffer.
 // The zero point: -8 sum v, kept, where it is 8 for all; else z times sum v, in 24
 // bits (binary32 x in two parts, as its sum v has 28).
-// The stream of weights bounds it: 17408 x 5120, one stream, 10.4 us, 4.4 TB/s (a plain
-// read of these bytes: 9); 5120 x 17408 of int8 rows 10.8 us, 4.5 TB/s; the vector
+// The stream of weights bounds it: 17408 x 5120, one stream, 10.7 us, 4.3 TB/s (a plain
+// read of these bytes: 9); 5120 x 17408 of int8 rows 10.6 us, 4.6 TB/s; the vector
 // ALU is busy for half of that.
 template <int P, int NB, int MODE>
 __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4Arg a) {
@@ -372,10 +372,12 @@ __global__ __launch_bounds__(1024, walk_waves(P, NB)) void kq_w4_walk_kernel(W4A
 // with the digits' joining, or with the scale), or, by a zero point of its row,
 // q + (128 - z), no byte of which carries, with its top bit turned back.
 //
-// No unit is full: 17408 x 5120, sixteen int8 streams, 17.9 us (2.6 TB/s of weights),
-// the vector ALU and the LDS busy for 0.6 of it each, the matrix cores for 0.1; 151936 x
-// 1024, five of binary32, 27.6 us (3.3 TB/s), 0.6, 0.6 and 0.15.  (Tiles of 32 rows,
-// two operands of weights for one of x: 19.1 -> 20.6 us the former, the latter the same.)
+// No unit is full: 17408 x 5120, sixteen int8 streams, 17.7 us (2.7 TB/s of weights),
+// the vector ALU and the LDS busy for half of it each, the matrix cores for 0.1; a
+// workgroup's 68 rows are five tiles (15 % of whose rows are not there), 100 pairs on 16
+// waves, and every workgroup brings x to LDS.  151936 x 1024, five of binary32, 24.9 us
+// (3.6 TB/s), 0.6, 0.55 and 0.2.  (Tiles of 32 rows, two operands of weights for one of
+// x, when these took 19.1 and 27.6 us: 20.6 us the former, the latter the same.)
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -819,16 +821,16 @@ bool fill(W4Arg& a, const kq_w4* w) {
 
 // LDS bytes of the walk kernel where it takes the call, else -1.  It is ahead of
 // the matrix cores
-// - with one stream (17408 x 5120 11.3 us against 14.8, int8 rows 11.1 / 13.2) and
-//   with two of int8 rows (12.1 / 14.0; 5120 x 17408 14.0 / 19.6);
+// - with one stream (17408 x 5120 11.3 us against 13.9, int8 rows 11.1 / 12.8) and
+//   with two of int8 rows (12.0 / 12.9; 5120 x 17408 12.7 / 14.4);
 // - with three of int8 rows, where a CU has few rows for x, whose way to LDS is
-//   what the other kernel waits for (5120 x 17408 15.8 / 20.4, 5120 x 9216 10.0 / 10.8,
-//   1024 x 5120 4.8 / 5.9; but 5120 x 5120 7.9 / 7.7, 17408 x 17408 39.7 / 37.8);
+//   what the other kernel waits for (5120 x 17408 14.4 / 15.2, 5120 x 9216 9.9 / 10.5,
+//   1024 x 5120 4.8 / 5.8; but 5120 x 5120 7.8 / 7.5, 17408 x 17408 39.5 / 37.4);
 // - with as many as it takes, where the matrix is one step of its workgroups and a
 //   launch's latency is what counts (1024 x 1024: four of int8 rows 4.0 / 4.5, three of
-//   binary32 4.6 / 5.1);
-// and behind with more (17408 x 5120: two of binary32 15.6 / 14.8, 5120 x 17408 20.6 /
-// 18.9; four of int8 rows 21.3 / 20.7).
+//   binary32 4.7 / 4.9);
+// and behind with more (17408 x 5120: two of binary32 16.4 / 14.2, 5120 x 17408 20.6 /
+// 16.1; four of int8 rows 17.3 / 13.4).
 long walk_takes(W4Arg& a, int P, int B, int n_cu) {
     const long rows = ((long)a.w.N + n_cu - 1) / n_cu;
     const bool few = B <= (P == 1 ? 2 : 1) || (P == 1 && B == 3 && a.nblk > 8 * rows) ||
