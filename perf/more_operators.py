@@ -368,7 +368,7 @@ def _bind(st):
         plan = KQ.kv_plan(S, c["page"], st["pages"], at(st["cached"]), new_ptr=at(st["new"]), start_ptr=at(st["start"]),
                           lens_ptr=at(st["lens"]), shape=shape, list_ptr=at(st["list"]), list_bytes=nb)
         st["cache"] = [cache(st["kv"][i], st["scale"][i], st["pages"]) for i in range(c["n"])]
-        st["desc"] = [plan] + [KQ.paged_attn(shape, st["cache"][i], at(st["q"][i]), at(out[i]), at(st["table"]),
+        st["desc"] = [plan] + [KQ.paged_attn(shape, st["cache"][i], at(st["q"][i]), at(out[i]), N, at(st["table"]),
                                              st["table"].shape[1], at(st["start"]), at(st["lens"]), D ** -0.5,
                                              list_ptr=at(st["list"]), list_bytes=nb) for i in range(c["n"])]
         st["calls"] = [(lib.kq_kv_plan_dev, (ctypes.byref(plan), stream))] + [
