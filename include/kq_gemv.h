@@ -622,6 +622,164 @@ typedef struct kq_spec_verify {
 int64_t kq_spec_verify_workspace_bytes(const kq_spec_verify* v);
 int kq_spec_verify_dev(const kq_spec_verify* v, void* work, int64_t work_bytes, kq_stream stream);
 
+/* ------------------------------------------- attention over a paged cache
+ * What lies between a step's QKV products and its O product: the pages of its
+ * new tokens, the rotation of queries and keys with the store into the cache, and
+ * the attention of the new tokens over what is cached.  Device pointers, enqueue
+ * only, on any stream; nothing is allocated and no library scratch is used.  -1
+ * with a message on a bad argument or a launch error.  No counterpart as one call
+ * in the reference, whose cache is one row of memory per sequence.
+ *
+ * A token's slot is its page's number times `page` plus its place in the page.
+ * A kernel never follows a slot, page or row number out of the operands' bounds:
+ * what it says of such numbers stands with each call. */
+
+/* The keys and values of one layer: n_pages pages of `page` tokens, n_kv heads of
+ * D values each (D % 8 == 0, at most 256; n_pages * page < 2^31).  The row of
+ * token t of page p for head h starts p * page_stride + h * head_stride +
+ * t * token_stride elements behind k and v (0: D, page rows, n_kv heads; a multiple
+ * of 8 otherwise), which are 16-byte aligned.  KQ_TYPE_F16, KQ_TYPE_BF16, or
+ * KQ_TYPE_I8: a row is int8 times its scale, k_scale and v_scale being n_pages x
+ * n_kv x page binary32 values. */
+#define KQ_TYPE_I8      24      /* of caches only */
+#define KQ_KV_MAX_D     256
+#define KQ_KV_MAX_ROWS  (1 << 22)       /* token rows of one call of kq_kv_store_dev */
+typedef struct kq_kv_cache {
+    int type, n_pages, page, n_kv, D;
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    int64_t page_stride, head_stride, token_stride;
+} kq_kv_cache;
+
+/* The sizes of an attention call: S sequences of at most T new tokens each, n_q
+ * heads of queries (n_q % n_kv == 0, n_q <= KQ_ATTN_MAX_HEADS), and the window: a
+ * token sees itself and the window - 1 tokens before it (0: all before it). */
+#define KQ_ATTN_MAX_SEQS 65535
+#define KQ_ATTN_MAX_NEW 64          /* KQ_VERIFY_MAX_DRAFT drafted tokens and the one before them */
+#define KQ_ATTN_MAX_HEADS 1024
+typedef struct kq_attn_shape {
+    int S, T, n_q, n_kv, D, window;
+} kq_attn_shape;
+
+/* A step's block tables, slots and positions, and the list of work of its
+ * attention, from the requests' lengths; one launch.  Sequence s has cached[s]
+ * tokens in the cache, n_new[s] new ones (NULL: one each) and held[s] pages (NULL: as
+ * many as its cached tokens fill), the first entries of its row of `table`
+ * (table_stride entries each).  A sequence that needs more pages than it holds
+ * gets them from the end of free_pages[0..*n_free): in the order of sequences, as
+ * long as what all of them up to it need is there, and all it needs or none.  Tables
+ * too narrow for a sequence count as no pages for it, and it takes none.
+ *   table       the new pages' entries, the others stay as they are
+ *   held_out    pages held now (may be held)
+ *   n_free_out  free pages left (may be n_free); free_pages stays as it is
+ *   start       S + 1: the first row of each sequence's new tokens, and their number
+ *   lens        cached + new, 0 where pages are missing
+ *   pos, slot   of each new token: its position, and its slot (-1 where pages are
+ *               missing, or its page is not in 0..n_pages-1); N entries at most
+ *   n_short     one value: the sequences whose pages are missing
+ * Any output may be NULL.  table NULL: no pages are dealt with (free_pages, n_free,
+ * held, held_out, n_free_out, slot and n_short are NULL then).  Lengths below 0
+ * count as 0, above 2^30 - 1 as that; the new tokens are fewer than 2^31.
+ * list (NULL: none, shape unused): kq_kv_list_bytes of device memory, 256-byte
+ * aligned, filled for kq_paged_attn_dev calls of this shape (whose S is the
+ * plan's), until the lengths change: equal shares of the keys to read.  Sequences
+ * of no or more than T new tokens have none. */
+#define KQ_KV_MAX_PAGE 65536
+typedef struct kq_kv_plan {
+    int S, page, n_pages, table_stride;
+    const int32_t* cached;
+    const int32_t* n_new;
+    const int32_t* held;
+    int32_t* table;
+    const int32_t* free_pages;
+    const int32_t* n_free;
+    int32_t* held_out;
+    int32_t* n_free_out;
+    int32_t* start;
+    int32_t* lens;
+    int N;
+    int32_t* pos;
+    int32_t* slot;
+    int32_t* n_short;
+    kq_attn_shape shape;
+    void* list;
+    int64_t list_bytes;
+} kq_kv_plan;
+int kq_kv_plan_dev(const kq_kv_plan* p, kq_stream stream);
+
+/* Bytes of the list of a shape, or -1. */
+int64_t kq_kv_list_bytes(const kq_attn_shape* s);
+
+/* Rotates queries and keys, and stores keys and values in their slots; one launch.
+ * Row i < N (i < *n_tokens, a device value, unless that is NULL) has n_kv heads of D
+ * values at k + i * k_stride and v + i * v_stride, and n_q heads at q + i * q_stride
+ * (q NULL: none).  The first `rot` values of each head of q and k (even, 0: none, at
+ * most D) turn in pairs (j, j + rot / 2), or (2j, 2j + 1) where `interleaved`:
+ *   (a, b) -> (a cos - b sin, b cos + a sin), angle = pos[i] * freq[j],
+ * in binary64, rounded once to binary32 (freq: rot / 2 binary32 values).  q goes to
+ * q_out + i * q_out_stride (which may be q, with its stride).  The rows of k and v
+ * are rounded to the cache's type, to nearest; to int8 with scale = max|x| / 127 of
+ * the row, as kq_quantize_x_q8_dev does with a group, bit for bit (they must then
+ * be finite).  Slots are distinct; a slot outside 0..n_pages * page - 1 is not
+ * written.  Rows are 16-byte aligned, strides multiples of 4 (0: rows of their
+ * heads). */
+typedef struct kq_kv_store {
+    kq_kv_cache cache;
+    int N;
+    const int32_t* n_tokens;
+    const int32_t* slot;
+    const float* k;
+    const float* v;
+    int64_t k_stride, v_stride;
+    const int32_t* pos;
+    int rot, interleaved;
+    const float* freq;
+    int n_q;
+    const float* q;
+    float* q_out;
+    int64_t q_stride, q_out_stride;
+} kq_kv_store;
+int kq_kv_store_dev(const kq_kv_store* a, kq_stream stream);
+
+/* Attention of each sequence's new tokens over its cached ones (their own keys and
+ * values are in the cache already).  Sequence s has lens[s] tokens, the last n of
+ * which are new, n = start[s + 1] - start[s], with queries in rows start[s].. of q
+ * (start NULL: one each, row s); query head h reads the cache's head h / (n_q / n_kv).
+ *   out = sum_j p_j v_j,  p = softmax over the keys j that the token sees of scale q . k_j
+ * q and out: N rows of n_q heads of D binary32 values, q_stride and out_stride
+ * elements apart (0: n_q * D; multiples of 4), 16-byte aligned; they do not overlap.
+ * table: S rows of table_stride page numbers.  Keys past the table, and keys
+ * on pages outside 0..n_pages-1, are not seen; a token that sees no key gets zeros.
+ * What a token does not see does not reach it, whatever it holds.  Sequences of more
+ * than T new tokens, rows of none and rows outside 0..N-1 are left as they are.
+ * Products are exact to 2^-21 of their operands or better and summed in binary32.
+ * list: as kq_kv_plan_dev wrote it for this shape and these lengths, NULL: a
+ * workgroup takes a whole sequence (short ones; with few and long ones most of the
+ * device idles).  Calls that share a list must not overlap in time, nor calls that
+ * share a workspace (kq_paged_attn_workspace_bytes, 256-byte aligned; without a
+ * list: NULL). */
+typedef struct kq_paged_attn {
+    kq_attn_shape shape;
+    kq_kv_cache cache;
+    float scale;
+    int N;
+    const float* q;
+    float* out;
+    int64_t q_stride, out_stride;
+    const int32_t* table;
+    int table_stride;
+    const int32_t* start;
+    const int32_t* lens;
+    void* list;
+    int64_t list_bytes;
+} kq_paged_attn;
+int kq_paged_attn_dev(const kq_paged_attn* a, void* work, int64_t work_bytes, kq_stream stream);
+
+/* Bytes of workspace of a call with a list, or -1. */
+int64_t kq_paged_attn_workspace_bytes(const kq_attn_shape* s);
+
 #ifdef __cplusplus
 }
 #endif

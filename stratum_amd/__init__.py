@@ -17,6 +17,9 @@ wrappers with the reference's argument meaning:
   rmsnorm_dev(a)                     residual + RMS norm, to binary32 or int8 rows
   w4_gemv_dev / w4_gemv_q8_dev       products with 4-bit weights and group scales
   spec_verify_dev(v, work, n)        drafted tokens against the target's distributions
+  kv_plan_dev(p)                     block tables, slots and positions of a step's tokens
+  kv_store_dev(a)                    rotary embedding, keys and values into a paged cache
+  paged_attn_dev(a, work, n)         attention of new tokens over a paged cache
 
 There is no CPU fallback: if the library is missing, ``lib()`` raises.
 """
@@ -35,7 +38,8 @@ TYPE_Q3_K = 11
 TYPE_Q4_K = 12
 TYPE_Q5_K = 13
 TYPE_Q6_K = 14
-TYPE_BF16 = 30     # of group scales only
+TYPE_I8 = 24       # of caches only
+TYPE_BF16 = 30     # of group scales and caches only
 TYPE_Q2K_NIB = 42
 # int8-activation mode flag (KQ_INT8_ACT): TYPE_Q4_K | INT8_ACT, and likewise for
 # Q6_K, Q5_K, Q3_K and Q8_0
@@ -65,6 +69,8 @@ EXPORTS = (
     "kq_reserve_mfma_workspace", "kq_scratch_bytes", "kq_moe_ffn_last_path",
     "kq_rmsnorm_dev", "kq_w4_gemv_dev", "kq_w4_gemv_q8_dev", "kq_w4_workspace_bytes",
     "kq_spec_verify_dev", "kq_spec_verify_workspace_bytes",
+    "kq_kv_plan_dev", "kq_kv_list_bytes", "kq_kv_store_dev", "kq_paged_attn_dev",
+    "kq_paged_attn_workspace_bytes",
 )
 # include/kq_gguf.h (bound in stratum_amd/gguf.py)
 GGUF_EXPORTS = (
@@ -228,6 +234,63 @@ class KqSpecVerify(ctypes.Structure):
     ]
 
 
+class KqKvCache(ctypes.Structure):
+    """kq_kv_cache: the paged keys and values of one layer."""
+
+    _fields_ = [
+        ("type", ctypes.c_int), ("n_pages", ctypes.c_int), ("page", ctypes.c_int),
+        ("n_kv", ctypes.c_int), ("D", ctypes.c_int), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("page_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+        ("token_stride", ctypes.c_int64),
+    ]
+
+
+class KqAttnShape(ctypes.Structure):
+    """kq_attn_shape: the sizes of an attention call."""
+
+    _fields_ = [(n, ctypes.c_int) for n in ("S", "T", "n_q", "n_kv", "D", "window")]
+
+
+class KqKvPlan(ctypes.Structure):
+    """kq_kv_plan: block tables, slots and positions of a step's new tokens."""
+
+    _fields_ = [
+        ("S", ctypes.c_int), ("page", ctypes.c_int), ("n_pages", ctypes.c_int),
+        ("table_stride", ctypes.c_int)] + [(n, ctypes.c_void_p) for n in (
+            "cached", "n_new", "held", "table", "free_pages", "n_free", "held_out", "n_free_out",
+            "start", "lens")] + [
+        ("N", ctypes.c_int), ("pos", ctypes.c_void_p), ("slot", ctypes.c_void_p),
+        ("n_short", ctypes.c_void_p), ("shape", KqAttnShape), ("list", ctypes.c_void_p),
+        ("list_bytes", ctypes.c_int64),
+    ]
+
+
+class KqKvStore(ctypes.Structure):
+    """kq_kv_store: rotary embedding, and keys and values into the cache."""
+
+    _fields_ = [
+        ("cache", KqKvCache), ("N", ctypes.c_int), ("n_tokens", ctypes.c_void_p),
+        ("slot", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("pos", ctypes.c_void_p),
+        ("rot", ctypes.c_int), ("interleaved", ctypes.c_int), ("freq", ctypes.c_void_p),
+        ("n_q", ctypes.c_int), ("q", ctypes.c_void_p), ("q_out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64), ("q_out_stride", ctypes.c_int64),
+    ]
+
+
+class KqPagedAttn(ctypes.Structure):
+    """kq_paged_attn: attention of new tokens over a paged cache."""
+
+    _fields_ = [
+        ("shape", KqAttnShape), ("cache", KqKvCache), ("scale", ctypes.c_float),
+        ("N", ctypes.c_int), ("q", ctypes.c_void_p), ("out", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64), ("table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int), ("start", ctypes.c_void_p), ("lens", ctypes.c_void_p),
+        ("list", ctypes.c_void_p), ("list_bytes", ctypes.c_int64),
+    ]
+
+
 def moe_op(qtype: int, n_out: int, k_in: int, w_ptrs, expert_stride: int, x_ptr: int,
            x_div: int, y_ptrs) -> KqMoeOp:
     op = KqMoeOp()
@@ -313,6 +376,14 @@ def lib() -> ctypes.CDLL:
     L.kq_spec_verify_dev.argtypes = [VP, P, LL, P]
     L.kq_spec_verify_workspace_bytes.argtypes = [VP]
     L.kq_spec_verify_workspace_bytes.restype = LL
+    SP = ctypes.POINTER(KqAttnShape)
+    L.kq_kv_plan_dev.argtypes = [ctypes.POINTER(KqKvPlan), P]
+    L.kq_kv_list_bytes.argtypes = [SP]
+    L.kq_kv_list_bytes.restype = LL
+    L.kq_kv_store_dev.argtypes = [ctypes.POINTER(KqKvStore), P]
+    L.kq_paged_attn_dev.argtypes = [ctypes.POINTER(KqPagedAttn), P, LL, P]
+    L.kq_paged_attn_workspace_bytes.argtypes = [SP]
+    L.kq_paged_attn_workspace_bytes.restype = LL
     _LIB = L
     return L
 
@@ -610,3 +681,89 @@ def spec_verify_dev(v: KqSpecVerify, work_ptr: int, work_bytes: int,
     """Accepted drafted tokens and the token after them (kq_spec_verify_dev)."""
     _check(lib().kq_spec_verify_dev(ctypes.byref(v), work_ptr, work_bytes, stream),
            "kq_spec_verify_dev")
+
+
+def kv_cache(qtype: int, n_pages: int, page: int, n_kv: int, D: int, k_ptr: int, v_ptr: int,
+             k_scale_ptr: int | None = None, v_scale_ptr: int | None = None, page_stride: int = 0,
+             head_stride: int = 0, token_stride: int = 0) -> KqKvCache:
+    c = KqKvCache()
+    c.type, c.n_pages, c.page, c.n_kv, c.D = qtype, n_pages, page, n_kv, D
+    c.k, c.v, c.k_scale, c.v_scale = k_ptr, v_ptr, k_scale_ptr, v_scale_ptr
+    c.page_stride, c.head_stride, c.token_stride = page_stride, head_stride, token_stride
+    return c
+
+
+def attn_shape(S: int, T: int, n_q: int, n_kv: int, D: int, window: int = 0) -> KqAttnShape:
+    s = KqAttnShape()
+    s.S, s.T, s.n_q, s.n_kv, s.D, s.window = S, T, n_q, n_kv, D, window
+    return s
+
+
+def kv_list_bytes(s: KqAttnShape) -> int:
+    return _bytes(lib().kq_kv_list_bytes(ctypes.byref(s)), "kq_kv_list_bytes")
+
+
+def kv_plan(S: int, page: int, n_pages: int, cached_ptr: int, new_ptr: int | None = None,
+            held_ptr: int | None = None, table_ptr: int | None = None, table_stride: int = 0,
+            free_ptr: int | None = None, n_free_ptr: int | None = None,
+            held_out_ptr: int | None = None, n_free_out_ptr: int | None = None,
+            start_ptr: int | None = None, lens_ptr: int | None = None, N: int = 0,
+            pos_ptr: int | None = None, slot_ptr: int | None = None, short_ptr: int | None = None,
+            shape: KqAttnShape | None = None, list_ptr: int | None = None,
+            list_bytes: int = 0) -> KqKvPlan:
+    p = KqKvPlan()
+    p.S, p.page, p.n_pages, p.table_stride, p.N = S, page, n_pages, table_stride, N
+    p.cached, p.n_new, p.held, p.table = cached_ptr, new_ptr, held_ptr, table_ptr
+    p.free_pages, p.n_free, p.held_out, p.n_free_out = (free_ptr, n_free_ptr, held_out_ptr,
+                                                        n_free_out_ptr)
+    p.start, p.lens, p.pos, p.slot, p.n_short = start_ptr, lens_ptr, pos_ptr, slot_ptr, short_ptr
+    if shape is not None:
+        p.shape = shape
+    p.list, p.list_bytes = list_ptr, list_bytes
+    return p
+
+
+def kv_plan_dev(p: KqKvPlan, stream: int | None = None) -> None:
+    """Block tables, slots and positions of a step's new tokens (kq_kv_plan_dev)."""
+    _check(lib().kq_kv_plan_dev(ctypes.byref(p), stream), "kq_kv_plan_dev")
+
+
+def kv_store(cache: KqKvCache, N: int, slot_ptr: int, k_ptr: int, v_ptr: int, k_stride: int = 0,
+             v_stride: int = 0, n_tokens_ptr: int | None = None, pos_ptr: int | None = None,
+             rot: int = 0, interleaved: bool = False, freq_ptr: int | None = None, n_q: int = 0,
+             q_ptr: int | None = None, q_stride: int = 0, q_out_ptr: int | None = None,
+             q_out_stride: int = 0) -> KqKvStore:
+    a = KqKvStore()
+    a.cache, a.N, a.n_tokens, a.slot, a.pos = cache, N, n_tokens_ptr, slot_ptr, pos_ptr
+    a.k, a.v, a.k_stride, a.v_stride = k_ptr, v_ptr, k_stride, v_stride
+    a.rot, a.interleaved, a.freq = rot, int(interleaved), freq_ptr
+    a.n_q, a.q, a.q_out, a.q_stride, a.q_out_stride = n_q, q_ptr, q_out_ptr, q_stride, q_out_stride
+    return a
+
+
+def kv_store_dev(a: KqKvStore, stream: int | None = None) -> None:
+    """Rotated queries and keys; keys and values into their slots (kq_kv_store_dev)."""
+    _check(lib().kq_kv_store_dev(ctypes.byref(a), stream), "kq_kv_store_dev")
+
+
+def paged_attn(shape: KqAttnShape, cache: KqKvCache, q_ptr: int, out_ptr: int, N: int,
+               table_ptr: int, table_stride: int, start_ptr: int | None, lens_ptr: int,
+               scale: float, list_ptr: int | None = None, list_bytes: int = 0, q_stride: int = 0,
+               out_stride: int = 0) -> KqPagedAttn:
+    a = KqPagedAttn()
+    a.shape, a.cache, a.scale, a.N, a.q, a.out = shape, cache, scale, N, q_ptr, out_ptr
+    a.q_stride, a.out_stride, a.table, a.table_stride = q_stride, out_stride, table_ptr, table_stride
+    a.start, a.lens, a.list, a.list_bytes = start_ptr, lens_ptr, list_ptr, list_bytes
+    return a
+
+
+def paged_attn_workspace_bytes(s: KqAttnShape) -> int:
+    return _bytes(lib().kq_paged_attn_workspace_bytes(ctypes.byref(s)),
+                  "kq_paged_attn_workspace_bytes")
+
+
+def paged_attn_dev(a: KqPagedAttn, work_ptr: int | None = None, work_bytes: int = 0,
+                   stream: int | None = None) -> None:
+    """Attention of new tokens over a paged cache (kq_paged_attn_dev)."""
+    _check(lib().kq_paged_attn_dev(ctypes.byref(a), work_ptr, work_bytes, stream),
+           "kq_paged_attn_dev")

@@ -130,6 +130,26 @@ int kqk_launch_w4(const kq_w4* w, const float* x, const int8_t* xq, const float*
                   const float* add, float* y, int B, void* work, int n_cu, hipStream_t st);
 int64_t kqk_verify_workspace(const kq_spec_verify* v);
 int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st);
+/* attention over a paged cache (kq_kv.hip, kq_attn.hip): arguments checked and
+ * strides filled in by kq_kv.c.  The list of work, in ints: their number, then from
+ * KQK_LIST_HEAD on `cap` items of KQK_ITEM, then a counter for each sequence, head of
+ * keys and block of rows, 0 between calls.  An item: sequence, first key, key behind
+ * its last, number and index among the sequence's items, the first of their partial
+ * results. */
+#define KQK_LIST_HEAD 8
+#define KQK_ITEM 8
+typedef struct {
+    int budget;              /* items beyond one a sequence */
+    int cap;                 /* S + budget */
+    int parts;               /* partial results at most: of sequences with several items */
+    int blocks;              /* of query rows, in each sequence and head of keys */
+    int64_t counters;
+} kqk_attn_sizes;
+void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z);
+int64_t kqk_attn_workspace(const kq_attn_shape* s, int n_cu);
+int kqk_launch_attn(const kq_paged_attn* a, const kqk_attn_sizes* z, void* work, hipStream_t st);
+int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, hipStream_t st);
+int kqk_launch_kv_store(const kq_kv_store* a, int n_cu, hipStream_t st);
 
 #ifdef __cplusplus
 }
