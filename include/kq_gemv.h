@@ -638,11 +638,12 @@ int kq_spec_verify_dev(const kq_spec_verify* v, void* work, int64_t work_bytes, 
  * D values each (D % 8 == 0, at most 256; n_pages * page < 2^31).  The row of
  * token t of page p for head h starts p * page_stride + h * head_stride +
  * t * token_stride elements behind k and v (0: D, page rows, n_kv heads; a multiple
- * of 8 otherwise), which are 16-byte aligned.  KQ_TYPE_F16, KQ_TYPE_BF16, or
+ * of 8 otherwise, between tokens at most KQ_KV_MAX_TOKEN_STRIDE), which are 16-byte aligned.  KQ_TYPE_F16, KQ_TYPE_BF16, or
  * KQ_TYPE_I8: a row is int8 times its scale, k_scale and v_scale being n_pages x
  * n_kv x page binary32 values. */
 #define KQ_TYPE_I8      24      /* of caches only */
 #define KQ_KV_MAX_D     256
+#define KQ_KV_MAX_TOKEN_STRIDE (1 << 24)
 #define KQ_KV_MAX_ROWS  (1 << 22)       /* token rows of one call of kq_kv_store_dev */
 typedef struct kq_kv_cache {
     int type, n_pages, page, n_kv, D;
@@ -754,7 +755,9 @@ int kq_kv_store_dev(const kq_kv_store* a, kq_stream stream);
  * on pages outside 0..n_pages-1, are not seen; a token that sees no key gets zeros.
  * What a token does not see does not reach it, whatever it holds.  Sequences of more
  * than T new tokens, rows of none and rows outside 0..N-1 are left as they are.
- * Products are exact to 2^-21 of their operands or better and summed in binary32.
+ * Queries and weights enter the products with 22 bits or more (of values below 2^-17 of
+ * a head's largest query, or of a row's largest weight, fewer), keys and values as
+ * they are; sums are binary32.
  * list: as kq_kv_plan_dev wrote it for this shape and these lengths, NULL: a
  * workgroup takes a whole sequence (short ones; with few and long ones most of the
  * device idles).  Calls that share a list must not overlap in time, nor calls that

@@ -2,108 +2,847 @@
 //
 //   out = sum_j p_j v_j,  p = softmax over the keys j that a token sees of scale q . k_j
 //
-// One wave per token and query head: 64 keys at a time, a key's product in each
-// lane, then the values, D / 64 of them in each lane.
-#include <hip/hip_bf16.h>
+// The rows of a sequence and a head of keys are its new tokens' queries of the G =
+// n_q / n_kv heads that read it; a workgroup takes 16 RT of them and an item of the
+// list (a share of the sequence's keys), each of its waves every NW-th step of 32
+// keys.  One pass, with a running maximum m and sum l of each row:
+//   S^T = K Q^T   16 keys x 16 rows a matrix instruction, K as it lies in the cache
+//                 (a lane has 8 values of one key), Q^T from LDS
+//   p = 2^(S - m), in the layout that S^T has: 8 keys of a row a lane, which is that
+//                 of the second product's right operand if the keys of a step are
+//                 taken in the order 4 g + j, 16 + 4 g + j (lane group g)
+//   O^T = V^T P^T a lane loads 8 (or 4) neighbouring values of those 8 keys; an
+//                 operand for value t of each is one byte permutation a register
+// so that keys and values go from memory to registers and matrix cores without LDS.
+// Queries and weights are binary32: as two binary16 numbers (22 bits, queries with a
+// power of two a row, weights times 2^9) where keys are binary16 or int8, as three
+// bfloat16 numbers (24 bits) where they are bfloat16.  Matrix work is far from full,
+// so that the further products are free.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
 #include "kq_launch.h"
 
-#pragma clang fp contract(off)
-
 namespace {
 
-template <int TYPE>
-__device__ __forceinline__ float value(const void* p, long i) {
-    if constexpr (TYPE == KQ_TYPE_F16) return __half2float(static_cast<const __half*>(p)[i]);
-    if constexpr (TYPE == KQ_TYPE_BF16)
-        return __uint_as_float((uint32_t)static_cast<const uint16_t*>(p)[i] << 16);
-    return (float)static_cast<const int8_t*>(p)[i];
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+struct __attribute__((aligned(4))) F4 { float v[4]; };    // four floats at any 4-byte address
+
+struct AttnArg {
+    const uint8_t* k;
+    const uint8_t* v;
+    const float* ks;
+    const float* vs;
+    const float* q;
+    float* out;
+    const int* table;
+    const int* start;
+    const int* lens;
+    const int* items;           // NULL: workgroup x is sequence x
+    const int* count;
+    int* counter;
+    float* part;                // partial results: parts x n_kv x R rows of D
+    float2* ml;                 // and their maximum and sum
+    int64_t page_b, head_b, tok_b, q_stride, out_stride;      // cache strides in bytes
+    uint64_t div;               // page / 16 by multiplication
+    float qscale;               // scale log2 e
+    int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts;
+};
+
+__device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
+    return __builtin_amdgcn_perm(hi, lo, sel);
+}
+
+// Maximum (sum) over the four lanes of a row: lanes c, 16 + c, 32 + c, 48 + c.
+__device__ __forceinline__ float max4(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sum4(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
+// Two binary32 values as 16-bit ones in NP registers whose sum they are.
+template <int NP>
+__device__ __forceinline__ void split(float a, float b, uint32_t* o) {
+    if constexpr (NP == 2) {
+        const f16x2 h = {(_Float16)a, (_Float16)b};
+        const f16x2 l = {(_Float16)(a - (float)h[0]), (_Float16)(b - (float)h[1])};
+        o[0] = __builtin_bit_cast(uint32_t, h);
+        o[1] = __builtin_bit_cast(uint32_t, l);
+    } else {
+        // by truncation: 8 bits each, nothing is left over
+        const uint32_t top = 0xffff0000u;
+        o[0] = perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & top);
+        b -= __uint_as_float(__float_as_uint(b) & top);
+        o[1] = perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+        a -= __uint_as_float(__float_as_uint(a) & top);
+        b -= __uint_as_float(__float_as_uint(b) & top);
+        o[2] = perm(__float_as_uint(b), __float_as_uint(a), 0x07060302);
+    }
+}
+
+// Bytes e and e + 1 of x, and byte e of x and of y, as binary16 integers: 1024 + 128
+// + the value by its bits, less 1152.
+__device__ __forceinline__ uint32_t halves(uint32_t u) {
+    const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+    return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u ^ 0x64806480u) - off);
+}
+
+template <int NP>
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (NP == 2)
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// DM: values of a head at most (D itself where EXACT); TILED: the page is a multiple
+// of 16 tokens, so that 16 keys lie on one page; RT: tiles of 16 rows; NW: waves.
+template <int TYPE, int DM, bool EXACT, bool TILED, int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
+    constexpr int NP = TYPE == KQ_TYPE_BF16 ? 3 : 2;      // numbers for a query or weight
+    constexpr int ES = TYPE == KQ_TYPE_I8 ? 1 : 2;
+    constexpr int NCH = DM / 32;                          // steps of 32 values of the first product
+    constexpr int W = DM >= 128 ? 8 : 4;                  // values a lane of a key in the second
+    constexpr int NB = DM / (16 * W);
+    constexpr int VW = W * ES / 4;                        // registers of W values
+    constexpr int OS = 16 * W + 4;                        // a row of a block of values in LDS
+    constexpr int QB = NP * RT * 16 * DM * 2, OB = NW * 16 * OS * 4;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[QB > OB ? QB : OB];
+    __shared__ float2 s_ml[NW][16 * RT];
+    __shared__ float s_inv[16 * RT];
+    __shared__ int s_last;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const int c = lane & 15, g = lane >> 4, h = blockIdx.y, D = EXACT ? DM : a.D, G = a.G;
+    int s = blockIdx.x, k0 = 0, k1, num = 1, idx = 0, part = 0, row0, n, len;
+    if (a.items) {
+        if (s >= min(a.cap, *a.count)) return;
+        const int* const it = a.items + s * KQK_ITEM;
+        s = it[0];
+        k0 = it[1];
+        k1 = it[2];
+        num = it[3] >> 16;
+        idx = it[3] & 0xffff;
+        part = it[4];
+        row0 = it[5];
+        n = it[6];
+        len = it[7];
+        if (s < 0 || s >= a.S || k0 < 0 || num < 1 || (num > 1 && (part < 0 || idx >= num || part > a.parts - num)))
+            return;
+    } else {
+        row0 = a.start ? a.start[s] : s;
+        n = a.start ? a.start[s + 1] - row0 : 1;
+        k1 = len = a.lens[s];
+        if (a.window) k0 = max(0, len - n + 1 - a.window) & ~31;
+    }
+    if (n < 1 || n > a.T) return;
+    const int rows = n * G, first = blockIdx.z * 16 * RT;   // of this sequence; of this workgroup
+    if (first >= rows) return;
+    const int* const table = a.table + (int64_t)s * a.table_stride;
+    k0 &= ~31;
+    k1 = (int)min((int64_t)min(k1, 0x7fff0000), (int64_t)a.table_stride * a.page);
+
+    // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
+    constexpr int QP = 16 * RT / (4 * NW) > 0 ? 16 * RT / (4 * NW) : 1;      // rows a 16 lanes take
+    constexpr int QO = (DM / 8 + 15) / 16;
+    f32x4 qv[QP][QO][2];
+#pragma unroll
+    for (int i = 0; i < QP; i++) {
+        const int r = (tid >> 4) + 4 * NW * i, row = first + r;
+        const int64_t tok = (int64_t)row0 + row / G;
+        const bool on = r < 16 * RT && row < rows && tok >= 0 && tok < a.N;
+        const float* const q = a.q + tok * a.q_stride + (int64_t)(h * G + row % G) * D;
+#pragma unroll
+        for (int o = 0; o < QO; o++) {
+            const int d = 8 * (c + 16 * o);
+            qv[i][o][0] = qv[i][o][1] = (f32x4)0.0f;
+            if (on && d < D) {
+                qv[i][o][0] = *reinterpret_cast<const f32x4*>(q + d);
+                qv[i][o][1] = *reinterpret_cast<const f32x4*>(q + d + 4);
+            }
+        }
+    }
+
+    // ---- where a step's keys lie
+    const uint8_t* const kh = a.k + h * a.head_b;
+    const uint8_t* const vh = a.v + h * a.head_b;
+    int pg[2];                                              // pages of the next step's keys
+    auto fetch = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            if constexpr (TILED) {
+                const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
+            } else {
+                const uint32_t b = (uint32_t)(kb + 16 * t + c) / (uint32_t)a.page;
+                pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
+            }
+        }
+    };
+    u32x4 kr[2][NCH], vr[8][NB];
+    float ksr[8], vsr[8];
+    bool have[2];                                           // the keys' pages are pages
+    const uint8_t* vp[8];
+    int64_t sp[2];
+    const uint32_t klane = TILED ? c * (uint32_t)a.tok_b + 8 * ES * g : 8 * ES * g;
+    const uint32_t vlane = (TILED ? 4 * g * (uint32_t)a.tok_b : 0u) + W * ES * c;
+    auto octet = [&](int ch) { return EXACT || 32 * ch + 8 * g < D; };
+    auto load_k = [&](int kb) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const uint8_t* p;
+            if constexpr (TILED) {
+                int page = uniform(pg[t]);
+                have[t] = (uint32_t)page < (uint32_t)a.n_pages;
+                page = have[t] ? page : 0;
+                const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                const int at = have[t] ? kb + 16 * t - (int)(b * (uint32_t)a.page) : 0;
+                const int64_t o = page * a.page_b + at * a.tok_b;
+                p = kh + o;
+#pragma unroll
+                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + o + j * a.tok_b;
+                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
+            } else {
+                have[t] = (uint32_t)pg[t] < (uint32_t)a.n_pages;
+                const int page = have[t] ? pg[t] : 0, at = have[t] ? (kb + 16 * t + c) % a.page : 0;
+                const int64_t o = page * a.page_b + at * a.tok_b;
+                p = kh + o;
+#pragma unroll
+                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + __shfl(o, 4 * g + j);
+                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
+            }
+#pragma unroll
+            for (int ch = 0; ch < NCH; ch++) {
+                if (!EXACT && 32 * ch >= D) continue;
+                const uint8_t* const x = p + (klane + (octet(ch) ? 32 * ES * ch : -8 * ES * g));
+                if constexpr (ES == 2) {
+                    kr[t][ch] = *reinterpret_cast<const u32x4*>(x);
+                } else {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+                    kr[t][ch][0] = y[0];
+                    kr[t][ch][1] = y[1];
+                }
+            }
+            if constexpr (TYPE == KQ_TYPE_I8) {
+                if constexpr (TILED) {
+                    const F4 x = *reinterpret_cast<const F4*>(a.ks + sp[t] + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) ksr[4 * t + j] = x.v[j];
+                } else {
+                    ksr[t] = a.ks[sp[t]];
+                }
+            }
+        }
+    };
+    auto load_v = [&]() {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                const uint8_t* const x = vp[j] + (EXACT || W * c + 16 * W * b < D ? vlane + 16 * W * ES * b
+                                                                                 : vlane - W * ES * c);
+                if constexpr (VW == 4) {
+                    vr[j][b] = *reinterpret_cast<const u32x4*>(x);
+                } else if constexpr (VW == 2) {
+                    const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+                    vr[j][b][0] = y[0];
+                    vr[j][b][1] = y[1];
+                } else {
+                    vr[j][b][0] = *reinterpret_cast<const uint32_t*>(x);
+                }
+            }
+        if constexpr (TYPE == KQ_TYPE_I8) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if constexpr (TILED) {
+                    const F4 x = *reinterpret_cast<const F4*>(a.vs + sp[t] + 4 * g);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) vsr[4 * t + j] = x.v[j];
+                } else {
+                    vsr[t] = a.vs[sp[t]];
+                }
+            }
+        }
+    };
+
+    int kb = k0 + 32 * wave;
+    const bool any = kb < k1;
+    if (any) {
+        fetch(kb);
+        load_k(kb);
+        load_v();
+        if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
+    }
+
+    uint32_t* const ql = reinterpret_cast<uint32_t*>(lds);
+#pragma unroll
+    for (int i = 0; i < QP; i++) {
+        const int r = (tid >> 4) + 4 * NW * i;
+        if (r >= 16 * RT) continue;
+        float inv = 1.0f, f = 1.0f;
+        float top = 0.0f;
+#pragma unroll
+        for (int o = 0; o < QO; o++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                qv[i][o][0][e] *= a.qscale;
+                qv[i][o][1][e] *= a.qscale;
+                top = fmaxf(top, fmaxf(fabsf(qv[i][o][0][e]), fabsf(qv[i][o][1][e])));
+            }
+        if constexpr (NP == 2) {
+            // the row times a power of two, its largest value from 2^13 to 2^14
+#pragma unroll
+            for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+            if (top > 0.0f && top < INFINITY) {
+                const int e = min(126, 140 - (int)(__float_as_uint(top) >> 23));
+                f = __uint_as_float((uint32_t)(127 + e) << 23);
+                inv = __uint_as_float((uint32_t)(127 - e) << 23);
+            }
+            if (c == 0) s_inv[r] = inv;
+        }
+#pragma unroll
+        for (int o = 0; o < QO; o++) {
+            if (DM % 128 && c + 16 * o >= DM / 8) continue;
+            u32x4 w[NP];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t p[NP];
+                split<NP>(qv[i][o][e >> 1][2 * (e & 1)] * f, qv[i][o][e >> 1][2 * (e & 1) + 1] * f, p);
+#pragma unroll
+                for (int j = 0; j < NP; j++) w[j][e] = p[j];
+            }
+#pragma unroll
+            for (int j = 0; j < NP; j++)
+                reinterpret_cast<u32x4*>(ql)[((j * RT + r / 16) * (DM / 8) + c + 16 * o) * 16 + r % 16] = w[j];
+        }
+    }
+    __syncthreads();
+
+    // ---- rows of this lane: the keys they see, [lo, hi)
+    int lo[RT], hi[RT];
+    float inv[RT], m[RT], l[RT];
+    f32x4 acc[RT][NB][W];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = first + 16 * rt + c, last = len - n + row / G;
+        // (rows behind the last one see everything: their sums are nobody's)
+        lo[rt] = row < rows && a.window ? last + 1 - a.window : 0;
+        hi[rt] = row < rows ? min(last + 1, k1) : k1;
+        inv[rt] = NP == 2 ? s_inv[16 * rt + c] : 1.0f;
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int t = 0; t < W; t++) acc[rt][b][t] = (f32x4)0.0f;
+    }
+    int ve = 0;                             // int8: the sums' exponent
+    (void)ve;
+    // steps within [all_lo, all_hi) are seen by all rows
+    const int row_n = min(rows, first + 16 * RT) - 1;
+    const int all_hi = min(k1, len - n + first / G + 1);
+    const int all_lo = a.window ? len - n + row_n / G + 1 - a.window : 0;
+
+    // ---- steps
+    // An infinity or NaN among the values would reach rows that do not see its key, and
+    // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
+    // number they are taken again without such values, which are then added alone.
+    bool careful = false;
+#pragma unroll 1
+    while (true) {
+#pragma unroll 1
+    for (; kb < k1; kb += 32 * NW) {
+        const bool ok0 = have[0], ok1 = have[1];
+        const bool full = TILED ? kb >= all_lo && kb + 32 <= all_hi && ok0 && ok1
+                                : kb >= all_lo && kb + 32 <= all_hi && __all(ok0 && ok1);
+        // (read in each step: the compiler would keep more queries than there are registers)
+        uint32_t qat = lane;
+        if constexpr (DM * RT > 128) asm volatile("" : "+v"(qat));
+        f32x4 sc[RT][2];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = (f32x4)0.0f;
+#pragma unroll
+        for (int ch = 0; ch < NCH; ch++) {
+            if (!EXACT && 32 * ch >= D) continue;
+            u32x4 x[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                x[t] = kr[t][ch];
+                if constexpr (TYPE == KQ_TYPE_I8) {
+                    const uint32_t y0 = kr[t][ch][0], y1 = kr[t][ch][1];
+                    x[t][0] = halves(perm(0, y0, 0x0c010c00));
+                    x[t][1] = halves(perm(0, y0, 0x0c030c02));
+                    x[t][2] = halves(perm(0, y1, 0x0c010c00));
+                    x[t][3] = halves(perm(0, y1, 0x0c030c02));
+                }
+                if (!EXACT && !octet(ch)) x[t] = (u32x4)0u;
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int j = 0; j < NP; j++) {
+                    const u32x4 y = reinterpret_cast<const u32x4*>(ql)[((j * RT + rt) * (DM / 8) + 4 * ch) * 16 + qat];
+                    sc[rt][0] = mfma<NP>(x[0], y, sc[rt][0]);
+                    sc[rt][1] = mfma<NP>(x[1], y, sc[rt][1]);
+                }
+        }
+        float kscale[8], vscale[8];
+        if constexpr (TYPE == KQ_TYPE_I8) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                kscale[j] = TILED ? ksr[j] : __shfl(ksr[j >> 2], 4 * g + (j & 3));
+                vscale[j] = TILED ? vsr[j] : __shfl(vsr[j >> 2], 4 * g + (j & 3));
+            }
+        }
+        // which of the lane's keys are there at all, bit j: key 16 (j / 4) + 4 g + j % 4
+        uint32_t there = 0xff;
+        if (!full) {
+            uint32_t p;
+            if constexpr (TILED) {
+                p = (ok0 ? 0x0f : 0) | (ok1 ? 0xf0 : 0);
+            } else {
+                const unsigned long long b0 = __ballot(ok0), b1 = __ballot(ok1);
+                p = (uint32_t)((b0 >> (4 * g)) & 15) | (uint32_t)((b1 >> (4 * g)) & 15) << 4;
+            }
+            there = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+                if (key < k1 && (p >> j & 1)) there |= 1u << j;
+            }
+            if constexpr (TYPE == KQ_TYPE_I8) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) vscale[j] = there >> j & 1 ? vscale[j] : 0.0f;
+            }
+        }
+        // the next step's keys are asked for as soon as this one's are used
+        const int nb = kb + 32 * NW;
+        u32x4 vc[8][NB];
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+#pragma unroll
+            for (int b = 0; b < NB; b++) vc[j][b] = vr[j][b];
+        if (nb < k1) {
+            load_k(nb);
+            if (nb + 32 * NW < k1) fetch(nb + 32 * NW);
+        }
+        // weights
+        if constexpr (TYPE == KQ_TYPE_I8) {
+            // the sums are kept times a power of two that is near the largest scale so far
+            float top = fabsf(vscale[0]);
+#pragma unroll
+            for (int j = 1; j < 8; j++) top = fmaxf(top, fabsf(vscale[j]));
+            const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
+            if (e > ve) {
+                const float f = ve ? __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23) : 0.0f;
+                ve = e;
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int t = 0; t < W; t++) acc[rt][b][t] *= f;
+            }
+            const float f = __uint_as_float((uint32_t)(254 - max(1, ve)) << 23);
+#pragma unroll
+            for (int j = 0; j < 8; j++) vscale[j] *= f;
+        }
+        float x[RT][8], top[RT];
+        bool far = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                x[rt][j] = sc[rt][j >> 2][j & 3];
+                if constexpr (NP == 2) x[rt][j] *= inv[rt];
+                if constexpr (TYPE == KQ_TYPE_I8) x[rt][j] *= kscale[j];
+            }
+            if (!full) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+                    x[rt][j] = key >= lo[rt] && key < hi[rt] && (there >> j & 1) ? x[rt][j] : -INFINITY;
+                }
+            }
+            top[rt] = x[rt][0];
+#pragma unroll
+            for (int j = 1; j < 8; j++) top[rt] = fmaxf(top[rt], x[rt][j]);
+            top[rt] = max4(top[rt]);
+            far |= top[rt] > m[rt] + 5.0f;
+        }
+        // (2^5 above the maximum that the weights are taken from before that is moved)
+        if (__any(far)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const float nm = fmaxf(m[rt], top[rt]), f = nm == -INFINITY ? 1.0f : exp2_(m[rt] - nm);
+                m[rt] = nm;
+                l[rt] *= f;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int t = 0; t < W; t++) acc[rt][b][t] *= f;
+            }
+        }
+        u32x4 w[RT][NP];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
+            // with int8 values' scales below 2^16)
+            const float base = (m[rt] == -INFINITY ? 0.0f : m[rt]) - (NP == 2 ? 9.0f : 0.0f);
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                float p = exp2_(x[rt][j] - base), q = exp2_(x[rt][j + 1] - base);
+                sum += p + q;
+                if constexpr (TYPE == KQ_TYPE_I8) {
+                    p *= vscale[j];
+                    q *= vscale[j + 1];
+                }
+                uint32_t o[NP];
+                split<NP>(p, q, o);
+#pragma unroll
+                for (int e = 0; e < NP; e++) w[rt][e][j >> 1] = o[e];
+            }
+            l[rt] += sum;
+        }
+        // values
+        if (!full) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const uint32_t keep = there >> j & 1 ? 0xffffffffu : 0u;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int e = 0; e < VW; e++) vc[j][b][e] &= keep;
+            }
+        }
+        auto operand = [&](const u32x4 (&x)[8][NB], int b, int t) {
+            u32x4 o;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if constexpr (ES == 2) {
+                    o[j] = perm(x[2 * j + 1][b][t >> 1], x[2 * j][b][t >> 1], t & 1 ? 0x07060302 : 0x05040100);
+                } else {
+                    const uint32_t e = t & 3;
+                    o[j] = halves(perm(x[2 * j + 1][b][t >> 2], x[2 * j][b][t >> 2], 0x0c000c00u | e | (4 + e) << 16));
+                }
+            }
+            return o;
+        };
+        if (ES == 2 && careful) {
+            constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int e = 0; e < VW; e++) {
+                        const uint32_t v = vc[j][b][e];
+                        if ((v & 0x7fff) >= NONE) vc[j][b][e] &= 0xffff0000u;
+                        if ((v >> 16 & 0x7fff) >= NONE) vc[j][b][e] &= 0xffffu;
+                    }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (!EXACT && 16 * W * b >= D) continue;
+#pragma unroll
+            for (int t = 0; t < W; t++) {
+                const u32x4 x = operand(vc, b, t);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int j = 0; j < NP; j++) acc[rt][b][t] = mfma<NP>(x, w[rt][j], acc[rt][b][t]);
+            }
+        }
+        if (nb < k1) load_v();
+    }
+
+    if (ES == 1 || careful) break;
+    float none = 0.0f;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int t = 0; t < W; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) none = fmaf(acc[rt][b][t][i], 0.0f, none);
+    if (!__any(none != 0.0f)) break;
+    careful = true;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        m[rt] = -INFINITY;
+        l[rt] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int t = 0; t < W; t++) acc[rt][b][t] = (f32x4)0.0f;
+    }
+    kb = k0 + 32 * wave;
+    fetch(kb);
+    load_k(kb);
+    load_v();
+    if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
+    }
+    if (careful) {
+#pragma unroll 1
+        for (kb = k0 + 32 * wave; kb < k1; kb += 32 * NW) {
+#pragma unroll 1
+            for (int key = kb; key < min(kb + 32, k1); key++) {
+                const int page = table[key / a.page];
+                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                const uint8_t* const x = vh + page * a.page_b + key % a.page * a.tok_b;
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+#pragma unroll
+                        for (int t = 0; t < W; t++) {
+                            const int d = 16 * W * b + W * (4 * g + i) + t;
+                            const uint32_t u = reinterpret_cast<const uint16_t*>(x)[EXACT ? d : min(d, D - 1)];
+                            float y;
+                            if constexpr (TYPE == KQ_TYPE_F16) y = __half2float(__ushort_as_half(u));
+                            else y = __uint_as_float(u << 16);
+                            y = __builtin_isfinite(y) ? 0.0f : y;
+#pragma unroll
+                            for (int rt = 0; rt < RT; rt++)
+                                acc[rt][b][t][i] += key >= lo[rt] && key < hi[rt] ? y : 0.0f;
+                        }
+            }
+        }
+    }
+
+    // ---- the waves' sums
+    __syncthreads();                        // (queries have been read)
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        l[rt] = sum4(l[rt]);
+        if (g == 0) s_ml[wave][16 * rt + c] = make_float2(m[rt], l[rt]);
+    }
+    __syncthreads();
+    float* const ol = reinterpret_cast<float*>(lds);
+    const int64_t prow = ((int64_t)(part + idx) * a.n_kv + h) * a.R + first;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        if (first + 16 * rt >= rows) continue;
+        float top = s_ml[0][16 * rt + c].x;
+#pragma unroll
+        for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][16 * rt + c].x);
+        float f = exp2_(m[rt] - (top == -INFINITY ? 0.0f : top));
+        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)max(1, ve) << 23);
+        const int live = min(16, rows - first - 16 * rt);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            if (!EXACT && 16 * W * b >= D) continue;
+            if (rt || b) __syncthreads();
+            if (c < live) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int t = 0; t < W; t += 4)
+                        *reinterpret_cast<f32x4*>(ol + (wave * 16 + c) * OS + W * (4 * g + i) + t) =
+                            (f32x4){acc[rt][b][t][i], acc[rt][b][t + 1][i], acc[rt][b][t + 2][i], acc[rt][b][t + 3][i]} * f;
+            }
+            __syncthreads();
+            for (int e = tid; e < live * 4 * W; e += 64 * NW) {
+                const int r = e / (4 * W), d = e % (4 * W) * 4;
+                if (!EXACT && 16 * W * b + d >= D) continue;
+                f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
+                float mm = s_ml[0][16 * rt + r].x;
+#pragma unroll
+                for (int i = 1; i < NW; i++) {
+                    y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
+                    mm = fmaxf(mm, s_ml[i][16 * rt + r].x);
+                }
+                const float base = mm == -INFINITY ? 0.0f : mm;
+                float ll = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NW; i++) ll += s_ml[i][16 * rt + r].y * exp2_(s_ml[i][16 * rt + r].x - base);
+                const int row = first + 16 * rt + r;
+                if (num == 1) {
+                    const int64_t tok = (int64_t)row0 + row / G;
+                    if (tok >= 0 && tok < a.N)
+                        *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + 16 * W * b + d) =
+                            ll == 0.0f ? (f32x4)0.0f : y / ll;
+                } else {
+                    float* const o = a.part + (prow + 16 * rt + r) * D + 16 * W * b + d;
+#pragma unroll
+                    for (int i = 0; i < 4; i += 2)
+                        __hip_atomic_store(reinterpret_cast<uint64_t*>(o + i),
+                                           (uint64_t)__float_as_uint(y[i]) | (uint64_t)__float_as_uint(y[i + 1]) << 32,
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    if (b == 0 && d == 0)
+                        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.ml + prow + 16 * rt + r),
+                                           (uint64_t)__float_as_uint(mm) | (uint64_t)__float_as_uint(ll) << 32,
+                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+            }
+        }
+    }
+    if (num == 1) return;
+
+    // ---- a sequence's last workgroup joins the partial results
+    __threadfence();                        // each wave's stores, before the count
+    __syncthreads();
+    if (tid == 0) {
+        int* const p = a.counter + ((int64_t)s * a.n_kv + h) * gridDim.z + blockIdx.z;
+        s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == num - 1;
+        if (s_last) __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!s_last) return;
+    auto get = [](const void* p) {
+        const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
+    };
+    const int64_t step = (int64_t)a.n_kv * a.R, from = ((int64_t)part * a.n_kv + h) * a.R;
+    const int live = min(rows - first, 16 * RT), pairs = D / 2;
+    for (int e = tid; e < live * pairs; e += 64 * NW) {
+        const int row = first + e / pairs, d = e % pairs * 2;
+        float mm = -INFINITY;
+        for (int i = 0; i < num; i++) mm = fmaxf(mm, get(a.ml + from + i * step + row).x);
+        const float base = mm == -INFINITY ? 0.0f : mm;
+        float ll = 0.0f, x = 0.0f, y = 0.0f;
+        for (int i = 0; i < num; i++) {
+            const float2 t = get(a.ml + from + i * step + row), o = get(a.part + (from + i * step + row) * D + d);
+            const float f = exp2_(t.x - base);
+            ll += t.y * f;
+            x += o.x * f;
+            y += o.y * f;
+        }
+        const int64_t tok = (int64_t)row0 + row / G;
+        if (tok >= 0 && tok < a.N)
+            *reinterpret_cast<float2*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) =
+                ll == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x / ll, y / ll);
+    }
+}
+
+typedef void (*Kernel)(AttnArg);
+
+// Waves of a workgroup, and tiles of rows at most: a lane holds 64 registers of keys
+// and values and 32 of sums a tile for each 128 values of a head.
+template <int DM, int RT> constexpr int NWV = DM == 256 || DM * RT > 256 ? 4 : 8;
+constexpr int most_tiles(int D) { return D > 128 ? 2 : 4; }
+
+template <int TYPE, int DM, bool EXACT, bool TILED>
+Kernel by_rows(int rt, int* nw) {
+    constexpr int M = most_tiles(DM);
+    *nw = rt == 1 ? NWV<DM, 1> : rt == 2 ? NWV<DM, 2> : NWV<DM, M>;
+    return rt == 1   ? kq_attn_kernel<TYPE, DM, EXACT, TILED, 1, NWV<DM, 1>>
+           : rt == 2 ? kq_attn_kernel<TYPE, DM, EXACT, TILED, 2, NWV<DM, 2>>
+                     : kq_attn_kernel<TYPE, DM, EXACT, TILED, M, NWV<DM, M>>;
 }
 
 template <int TYPE>
-__global__ __launch_bounds__(64) void kq_attn_kernel(kq_paged_attn a) {
-    const kq_kv_cache& c = a.cache;
-    const int s = blockIdx.x, h = blockIdx.y, t = blockIdx.z, lane = threadIdx.x, D = c.D;
-    const int hk = h / (a.shape.n_q / a.shape.n_kv);
-    const int row0 = a.start ? a.start[s] : s, n = a.start ? a.start[s + 1] - row0 : 1;
-    const long row = (long)row0 + t;
-    if (n < 1 || n > a.shape.T || t >= n || row < 0 || row >= a.N) return;
-    const int last = a.lens[s] - n + t;                   // the last key it sees
-    const int from = a.shape.window ? max(0, last + 1 - a.shape.window) : 0;
-    const int end = (int)min((long)last + 1, (long)a.table_stride * c.page);
-    __shared__ float q[KQ_KV_MAX_D];
-    __shared__ float ps[64];
-    __shared__ long at[64];
-    for (int d = lane; d < D; d += 64) q[d] = a.q[row * a.q_stride + (long)h * D + d] * a.scale;
-    __syncthreads();
-    float m = -INFINITY, l = 0.0f, o[KQ_KV_MAX_D / 64] = {};
-    for (int j0 = from; j0 < end; j0 += 64) {
-        const int j = j0 + lane;
-        long where = -1, sc = 0;
-        if (j < end) {
-            const int page = a.table[(long)s * a.table_stride + j / c.page], i = j % c.page;
-            if (page >= 0 && page < c.n_pages) {
-                where = page * c.page_stride + hk * c.head_stride + i * c.token_stride;
-                sc = ((long)page * c.n_kv + hk) * c.page + i;
-            }
-        }
-        float x = -INFINITY;
-        if (where >= 0) {
-            x = 0.0f;
-            for (int d = 0; d < D; d++) x = fmaf(q[d], value<TYPE>(c.k, where + d), x);
-            if (TYPE == KQ_TYPE_I8) x *= c.k_scale[sc];
-        }
-        float top = x;
-        for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-        const float nm = fmaxf(m, top);
-        float p = where >= 0 ? expf(x - nm) : 0.0f, sum = p;
-        for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-        const float f = nm == m ? 1.0f : expf(m - nm);
-        l = l * f + sum;
-        m = nm;
-        if (TYPE == KQ_TYPE_I8 && where >= 0) p *= c.v_scale[sc];
-        ps[lane] = p;
-        at[lane] = where;
-        __syncthreads();
-        for (int e = 0; e < KQ_KV_MAX_D / 64; e++) {
-            const int d = lane + 64 * e;
-            if (d >= D) break;
-            o[e] *= f;
-            for (int k = 0; k < 64; k++)
-                if (at[k] >= 0) o[e] = fmaf(ps[k], value<TYPE>(c.v, at[k] + d), o[e]);
-        }
-        __syncthreads();
-    }
-    for (int e = 0; e < KQ_KV_MAX_D / 64; e++) {
-        const int d = lane + 64 * e;
-        if (d < D) a.out[row * a.out_stride + (long)h * D + d] = l == 0.0f ? 0.0f : o[e] / l;
-    }
+Kernel pick(int D, bool tiled, int rt, int* nw) {
+    if (!tiled) return D <= 128 ? by_rows<TYPE, 128, false, false>(rt, nw) : by_rows<TYPE, 256, false, false>(rt, nw);
+    if (D == 64) return by_rows<TYPE, 64, true, true>(rt, nw);
+    if (D == 128) return by_rows<TYPE, 128, true, true>(rt, nw);
+    if (D == 256) return by_rows<TYPE, 256, true, true>(rt, nw);
+    return D < 128 ? by_rows<TYPE, 128, false, true>(rt, nw) : by_rows<TYPE, 256, false, true>(rt, nw);
 }
+
+int tiles(const kq_attn_shape* s) {
+    const int rows = s->T * (s->n_q / s->n_kv);
+    return rows <= 16 ? 1 : rows <= 32 ? 2 : most_tiles(s->D);
+}
+
+int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 }  // namespace
 
 extern "C" {
 
 void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
-    z->blocks = 1;
+    const int rows = s->T * (s->n_q / s->n_kv), rb = 16 * tiles(s);
+    z->blocks = (rows + rb - 1) / rb;
     const int per = s->n_kv * z->blocks;
-    z->budget = (4 * n_cu + per - 1) / per;
+    z->budget = (2 * n_cu + per - 1) / per;
     z->cap = s->S + z->budget;
     z->parts = 2 * z->budget;
     z->counters = (int64_t)s->S * per;
 }
 
-int64_t kqk_attn_workspace(const kq_attn_shape* s, int n_cu) { return 0; }
+int64_t kqk_attn_workspace(const kq_attn_shape* s, int n_cu) {
+    kqk_attn_sizes z;
+    kqk_attn_plan(s, n_cu, &z);
+    const int64_t rows = (int64_t)z.parts * s->n_kv * s->T * (s->n_q / s->n_kv);
+    return up256(rows * s->D * 4) + up256(rows * 8);
+}
 
-int kqk_launch_attn(const kq_paged_attn* a, const kqk_attn_sizes* z, void* work, hipStream_t st) {
-    auto* const k = a->cache.type == KQ_TYPE_F16    ? kq_attn_kernel<KQ_TYPE_F16>
-                    : a->cache.type == KQ_TYPE_BF16 ? kq_attn_kernel<KQ_TYPE_BF16>
-                                                    : kq_attn_kernel<KQ_TYPE_I8>;
-    hipLaunchKernelGGL(k, dim3((unsigned)a->shape.S, (unsigned)a->shape.n_q, (unsigned)a->shape.T),
-                       dim3(64), 0, st, *a);
+int kqk_launch_attn(const kq_paged_attn* p, const kqk_attn_sizes* z, void* work, hipStream_t st) {
+    const kq_kv_cache& c = p->cache;
+    const kq_attn_shape& s = p->shape;
+    const int es = c.type == KQ_TYPE_I8 ? 1 : 2;
+    AttnArg a = {};
+    a.k = (const uint8_t*)c.k;
+    a.v = (const uint8_t*)c.v;
+    a.ks = c.k_scale;
+    a.vs = c.v_scale;
+    a.q = p->q;
+    a.out = p->out;
+    a.table = p->table;
+    a.start = p->start;
+    a.lens = p->lens;
+    a.page_b = c.page_stride * es;
+    a.head_b = c.head_stride * es;
+    a.tok_b = c.token_stride * es;
+    a.q_stride = p->q_stride;
+    a.out_stride = p->out_stride;
+    a.qscale = (float)(p->scale * 1.4426950408889634);
+    a.S = s.S;
+    a.T = s.T;
+    a.G = s.n_q / s.n_kv;
+    a.R = s.T * a.G;
+    a.n_kv = s.n_kv;
+    a.D = s.D;
+    a.window = s.window;
+    a.N = p->N;
+    a.page = c.page;
+    a.n_pages = c.n_pages;
+    a.table_stride = p->table_stride;
+    a.cap = z->cap;
+    a.parts = z->parts;
+    const bool tiled = c.page % 16 == 0;
+    if (tiled) {
+        // (b d = 2^40 + e with e < d = page / 16 <= 2^12: tiles below 2^27 are divided exactly)
+        const uint64_t d = c.page / 16;
+        a.div = (((uint64_t)1 << 40) + d - 1) / d;
+    }
+    if (p->list) {
+        a.count = (const int*)p->list;
+        a.items = a.count + KQK_LIST_HEAD;
+        a.counter = (int*)p->list + KQK_LIST_HEAD + (int64_t)z->cap * KQK_ITEM;
+        const int64_t rows = (int64_t)z->parts * s.n_kv * a.R;
+        a.part = (float*)work;
+        a.ml = (float2*)((uint8_t*)work + up256(rows * s.D * 4));
+    }
+    int nw = 0;
+    const int rt = tiles(&s);
+    const Kernel k = c.type == KQ_TYPE_F16    ? pick<KQ_TYPE_F16>(s.D, tiled, rt, &nw)
+                     : c.type == KQ_TYPE_BF16 ? pick<KQ_TYPE_BF16>(s.D, tiled, rt, &nw)
+                                              : pick<KQ_TYPE_I8>(s.D, tiled, rt, &nw);
+    const dim3 grid((unsigned)(p->list ? z->cap : s.S), (unsigned)s.n_kv, (unsigned)z->blocks);
+    hipLaunchKernelGGL(k, grid, dim3(64 * nw), 0, st, a);
     return (int)hipGetLastError();
 }
 

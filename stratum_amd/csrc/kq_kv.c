@@ -42,7 +42,7 @@ static int cache_check(kq_kv_cache* c, const char* who) {
     if (!c->head_stride) c->head_stride = c->token_stride * c->page;
     if (!c->page_stride) c->page_stride = c->head_stride * c->n_kv;
     if (c->token_stride < c->D || c->head_stride < c->D || c->page_stride < c->D ||
-        (c->token_stride | c->head_stride | c->page_stride) % 8)
+        c->token_stride > KQ_KV_MAX_TOKEN_STRIDE || (c->token_stride | c->head_stride | c->page_stride) % 8)
         return kq_fail("%s: cache strides %lld, %lld, %lld", who, (long long)c->page_stride,
                        (long long)c->head_stride, (long long)c->token_stride);
     return 0;

@@ -98,7 +98,7 @@ __device__ __forceinline__ int items_of(int keys, int share) {
 __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(PlanArg a) {
     __shared__ long long sm[PT / 64];
     __shared__ int first_tok[PT], first_page[PT], first_item[PT], first_part[PT];
-    __shared__ int s_cached[PT], s_held[PT], s_from[PT], s_end[PT];
+    __shared__ int s_cached[PT], s_held[PT], s_from[PT], s_end[PT], s_fresh[PT];
     __shared__ bool s_ok[PT];
     const kq_kv_plan& p = a.p;
     const int tid = threadIdx.x;
@@ -141,6 +141,7 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(PlanArg a) {
         s_held[tid] = q.held;
         s_from[tid] = from;
         s_end[tid] = end;
+        s_fresh[tid] = q.fresh;
         s_ok[tid] = ok;
         if (s < p.S) {
             if (p.start) p.start[s] = (int)(tok0 + tok);
@@ -181,9 +182,11 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(PlanArg a) {
             o[0] = s0 + i;
             o[1] = s_from[i] + idx * per;
             o[2] = min(s_end[i], s_from[i] + (idx + 1) * per);
-            o[3] = num;
-            o[4] = idx;
-            o[5] = part0 + first_part[i];
+            o[3] = num << 16 | idx;
+            o[4] = part0 + first_part[i];
+            o[5] = (int)(tok0 + first_tok[i]);
+            o[6] = s_fresh[i];
+            o[7] = s_end[i];
         }
         tok0 += ntok;
         page0 += npage;

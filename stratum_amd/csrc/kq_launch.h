@@ -134,8 +134,8 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st);
  * strides filled in by kq_kv.c.  The list of work, in ints: their number, then from
  * KQK_LIST_HEAD on `cap` items of KQK_ITEM, then a counter for each sequence, head of
  * keys and block of rows, 0 between calls.  An item: sequence, first key, key behind
- * its last, number and index among the sequence's items, the first of their partial
- * results. */
+ * its last, number (upper half) and index among the sequence's items, the first of
+ * their partial results, the sequence's first row, new tokens and length. */
 #define KQK_LIST_HEAD 8
 #define KQK_ITEM 8
 typedef struct {

@@ -9,7 +9,14 @@ are then within factors of exp(+-e) and of the power's own error (2 u), so that 
 is within 2 e + 4 u of its value; the products with the values are good to 2^-21, and
 sums over L keys (and the joins, fewer than L) are off by at most (2 L + 64) u of the
 sum of p|v|, as is the weights' sum of itself.  Together, times sum p|v|:
-    2 e + 2^-20 + (4 L + 200) u."""
+    2 e + 2^-20 + (4 L + 200) u.
+With binary16 and int8 caches a weight is two binary16 numbers, of 2^9 times the weight
+(and of its value's scale over the largest one's power of two), whose last step is 2^-24:
+2^-25 / 2^9 = 2^-34 of the row's largest weight (the one that has not more than 2^5 on
+the base they are taken from, so it is no less than the base's) and of the largest
+scale go missing at most, times a value each: L 2^-34 max|v| in all.  Queries likewise: two
+binary16 numbers of the row times a power of two that puts its largest from 2^13 on, so
+2^-25 / 2^13 = 2^-38 of that one, times sum |scale k_d|, is added to e."""
 import numpy as np
 import pytest
 
@@ -181,6 +188,11 @@ class Case:
                 pv = torch.matmul(p, v.abs()).reshape(self.n_q, D)
                 e = X.amax(-1) * (2.0 ** -21 + (D + 8) * U) + 4 * U * x.abs().amax(-1)
                 tol = pv * (2 * e.reshape(self.n_q, 1) + 2.0 ** -20 + (4 * len(keys) + 200) * U) + 2.0 ** -126
+                if self.t != K.TYPE_BF16:
+                    e = e + 2.0 ** -38 * q.abs().amax(-1) * k.abs().sum(-1).amax(-1, keepdim=True)
+                    top = v.abs().amax((1, 2)).repeat_interleave(G).reshape(self.n_q, 1)
+                    tol = pv * (2 * e.reshape(self.n_q, 1) + 2.0 ** -20 + (4 * len(keys) + 200) * U) + \
+                        len(keys) * 2.0 ** -34 * top + 2.0 ** -126
                 bad = ~((got[r] - want).abs() <= tol)
                 assert not bad.any(), (s, i, int(bad.sum()), float((got[r] - want).abs().max()), float(tol.max()))
         rest = out[:, self.n_q * D:]

@@ -198,10 +198,11 @@ def test_list(S, T, n_kv, window, longest, new):
     at = part = 0
     for s in want:
         lo = max(0, lens[s] - n[s] + 1 - window) & ~31 if window and lens[s] else 0
-        num = items[at][3]
+        num = items[at][3] >> 16
         for i in range(num):
             it = items[at + i]
-            assert it[0] == s and it[1] == lo and it[3] == num and it[4] == i and it[5] == part
+            assert it[0] == s and it[1] == lo and it[3] == num << 16 | i and it[4] == part
+            assert it[5] == o["start"][s] and it[6] == n[s] and it[7] == lens[s]
             assert it[1] <= it[2] and (it[2] == lens[s]) == (i == num - 1) and it[1] % 32 == 0
             assert num == 1 or it[2] > it[1]
             lo = it[2]

@@ -85,7 +85,7 @@ CACHES = [(dict(qtype=K.TYPE_F32), "cache type 0"), (dict(qtype=12), "cache type
           (dict(qtype=K.TYPE_I8), "scales"), (dict(qtype=K.TYPE_I8, k_scale_ptr=P), "scales"),
           (dict(qtype=K.TYPE_I8, k_scale_ptr=P, v_scale_ptr=P + 2), "scales"), (dict(k_scale_ptr=P), "not int8"),
           (dict(token_stride=56), "strides"), (dict(token_stride=68), "strides"), (dict(head_stride=-64), "strides"),
-          (dict(page_stride=100), "strides")]
+          (dict(page_stride=100), "strides"), (dict(token_stride=(1 << 24) + 8), "strides")]
 
 
 @pytest.mark.parametrize("kw,word", CACHES)
