@@ -701,11 +701,15 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
     if (num == 1) return;
 
     // ---- a sequence's last workgroup joins the partial results
-    __threadfence();                        // each wave's stores, before the count
+    // The results and the count are device-scope atomics, which go past the caches that
+    // another XCD does not see: once a wave's stores are acknowledged they are there for
+    // all, and the barrier puts every wave's before the count.  (A release fence instead
+    // writes back the L2, in each of hundreds of workgroups.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) {
         int* const p = a.counter + ((int64_t)s * a.n_kv + h) * gridDim.z + blockIdx.z;
-        s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == num - 1;
+        s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == num - 1;
         if (s_last) __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
     __syncthreads();
@@ -714,25 +718,59 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
         const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
     };
-    const int64_t step = (int64_t)a.n_kv * a.R, from = ((int64_t)part * a.n_kv + h) * a.R;
-    const int live = min(rows - first, 16 * RT), pairs = D / 2;
-    for (int e = tid; e < live * pairs; e += 64 * NW) {
-        const int row = first + e / pairs, d = e % pairs * 2;
-        float mm = -INFINITY;
-        for (int i = 0; i < num; i++) mm = fmaxf(mm, get(a.ml + from + i * step + row).x);
-        const float base = mm == -INFINITY ? 0.0f : mm;
-        float ll = 0.0f, x = 0.0f, y = 0.0f;
-        for (int i = 0; i < num; i++) {
-            const float2 t = get(a.ml + from + i * step + row), o = get(a.part + (from + i * step + row) * D + d);
-            const float f = exp2_(t.x - base);
-            ll += t.y * f;
-            x += o.x * f;
-            y += o.y * f;
+    // Rows and quads of values over the lanes, and where those are fewer, the parts too;
+    // each part's weight 2^(m - max) once, for as many rows at a time as LDS has room.
+    const int64_t step = (int64_t)a.n_kv * a.R, from = ((int64_t)part * a.n_kv + h) * a.R + first;
+    constexpr int ROOM = sizeof(lds) / 4 - 64 * NW * 4;
+    float* const wl = ol + 64 * NW * 4;
+    const int live = min(rows - first, 16 * RT), quads = D / 4, at_once = max(1, min(live, ROOM / num));
+    for (int r0 = 0; r0 < live; r0 += at_once) {
+        const int nr = min(at_once, live - r0);
+        __syncthreads();
+        for (int r = wave; r < nr; r += NW) {
+            const float2* const p = a.ml + from + r0 + r;
+            float top = -INFINITY, sum = 0.0f;
+            for (int i = lane; i < num; i += 64) {
+                const float2 t = get(p + i * step);
+                top = fmaxf(top, t.x);
+            }
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+            const float base = top == -INFINITY ? 0.0f : top;
+            for (int i = lane; i < num; i += 64) {
+                const float2 t = get(p + i * step);
+                sum += t.y * exp2_(t.x - base);
+            }
+#pragma unroll
+            for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
+            for (int i = lane; i < num; i += 64)
+                wl[r * num + i] = sum == 0.0f ? 0.0f : exp2_(get(p + i * step).x - base) / sum;
         }
-        const int64_t tok = (int64_t)row0 + row / G;
-        if (tok >= 0 && tok < a.N)
-            *reinterpret_cast<float2*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) =
-                ll == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(x / ll, y / ll);
+        __syncthreads();
+        const int units = nr * quads;
+        int ways = 1;
+        while (2 * ways * units <= 64 * NW && 2 * ways <= num) ways *= 2;
+        for (int e0 = 0; e0 < units * ways; e0 += 64 * NW) {
+            const int e = e0 + tid, u = e % units, way = e / units, r = u / quads, d = u % quads * 4;
+            f32x4 y = (f32x4)0.0f;
+            if (way < ways) {
+                const float* const p = a.part + (from + r0 + r) * D + d;
+#pragma unroll 8
+                for (int i = way; i < num; i += ways) {
+                    const float2 t0 = get(p + i * step * D), t1 = get(p + i * step * D + 2);
+                    y += (f32x4){t0.x, t0.y, t1.x, t1.y} * wl[r * num + i];
+                }
+            }
+            if (ways > 1) {                 // (a single round then)
+                *reinterpret_cast<f32x4*>(ol + 4 * tid) = y;
+                __syncthreads();
+                for (int i = 1; i < ways && way == 0; i++) y += *reinterpret_cast<const f32x4*>(ol + 4 * (tid + i * units));
+            }
+            const int row = first + r0 + r;
+            const int64_t tok = (int64_t)row0 + row / G;
+            if (way == 0 && tok >= 0 && tok < a.N)
+                *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) = y;
+        }
     }
 }
 

@@ -13,72 +13,98 @@
 namespace {
 
 // ------------------------------------------------------------------ plan
+//
+// One workgroup: a sequence a lane (more in rounds), sums over them by lanes' shifts,
+// then new pages, new tokens and the attention's items over all lanes, each of which
+// finds its sequence by bisection in LDS.  A chain of latencies bounds it: lengths,
+// sums, the pages that slots lie on.
 
-constexpr int PT = 1024;            // lanes of the plan's one workgroup
+constexpr int PT = 1024;            // lanes at most
 constexpr int MOST = (1 << 30) - 1; // of a length
 
 struct PlanArg {
     kq_kv_plan p;
     int budget, cap;
-    long long counters;
+    int counters;
     int* items;                     // KQK_ITEM each
     int* count;
     int* counter;
 };
 
 struct Seq {
-    int cached, fresh, held, from, end;  // keys [from, end) are read by its new tokens
-    long long need;                      // pages
-    bool narrow;
+    uint32_t cached, fresh, held, need, from, end;   // keys [from, end) are read by its new tokens
+    bool narrow, attended;
 };
 
-__device__ __forceinline__ int clamped(int v, int most) { return min(max(v, 0), most); }
+__device__ __forceinline__ uint32_t clamped(int v, int most) { return (uint32_t)min(max(v, 0), most); }
+__device__ __forceinline__ uint32_t plus(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
 
-__device__ __forceinline__ Seq load_seq(const kq_kv_plan& p, int s) {
+__device__ __forceinline__ Seq load_seq(const PlanArg& a, int s) {
+    const kq_kv_plan& p = a.p;
     Seq q = {};
     if (s >= p.S) return q;
-    q.cached = clamped(p.cached[s], MOST);
-    q.fresh = p.n_new ? clamped(p.n_new[s], MOST) : 1;
+    const int cached = p.cached[s], fresh = p.n_new ? p.n_new[s] : 1, held = p.held ? p.held[s] : 0;
+    q.cached = clamped(cached, MOST);
+    q.fresh = clamped(fresh, MOST);
     q.end = q.cached + q.fresh;
     if (p.table) {
-        const int pages = (q.end + p.page - 1) / p.page;
-        q.held = p.held ? clamped(p.held[s], p.table_stride)
-                        : min((q.cached + p.page - 1) / p.page, p.table_stride);
-        q.narrow = pages > p.table_stride;
-        q.need = q.narrow ? 0 : max(0, pages - q.held);
+        const uint32_t page = (uint32_t)p.page, pages = (q.end + page - 1) / page;
+        q.held = p.held ? clamped(held, p.table_stride)
+                        : min((q.cached + page - 1) / page, (uint32_t)p.table_stride);
+        q.narrow = pages > (uint32_t)p.table_stride;
+        q.need = q.narrow || pages <= q.held ? 0 : pages - q.held;
     }
     const int w = p.shape.window;
-    q.from = w ? max(0, q.cached + 1 - w) & ~31 : 0;
+    q.from = w && (int)q.cached + 1 > w ? (q.cached + 1 - w) & ~31u : 0;
+    q.attended = a.items && q.fresh >= 1 && q.fresh <= (uint32_t)p.shape.T;
     return q;
 }
 
-__device__ __forceinline__ bool attended(const PlanArg& a, const Seq& q) {
-    return a.items && q.fresh >= 1 && q.fresh <= a.p.shape.T;
+// A step of a sum over the lanes before: DPP row_shr by 1 to 8, then a row's last lane
+// to the next row and the second row's to the upper half.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t scan_step(uint32_t x) {
+    return plus(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    x = scan_step<0x111, 0xf>(x);
+    x = scan_step<0x112, 0xf>(x);
+    x = scan_step<0x114, 0xf>(x);
+    x = scan_step<0x118, 0xf>(x);
+    x = scan_step<0x142, 0xa>(x);
+    return scan_step<0x143, 0xc>(x);
 }
 
-// The sum before each lane's value over the workgroup, and all of it.
-__device__ __forceinline__ long long wg_scan(long long v, long long* sm, long long* total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    long long in = v;
+// N sums (that stay at 2^32 - 1 from there on) over the lanes before each and over all.
+template <int N>
+__device__ __forceinline__ void wg_scan(const uint32_t (&v)[N], uint32_t (*sm)[4], uint32_t (&before)[N],
+                                        uint32_t (&all)[N]) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    uint32_t in[N];
 #pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const long long o = __shfl_up(in, off);
-        if (lane >= off) in += o;
-    }
-    __syncthreads();                      // (the last scan's sums have been read)
-    if (lane == 63) sm[wave] = in;
+    for (int i = 0; i < N; i++) in[i] = wave_scan(v[i]);
+    if (lane == 63)
+#pragma unroll
+        for (int i = 0; i < N; i++) sm[wave][i] = in[i];
     __syncthreads();
-    long long before = 0, all = 0;
-    for (int i = 0; i < PT / 64; i++) {
-        if (i < wave) before += sm[i];
-        all += sm[i];
+#pragma unroll
+    for (int i = 0; i < N; i++) before[i] = all[i] = 0;
+    for (int w = 0; w < waves; w++)
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            if (w == wave) before[i] = all[i];
+            all[i] = plus(all[i], sm[w][i]);
+        }
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        // (the lane before's inclusive sum: exact also where sums stay at their most)
+        const uint32_t prev = (uint32_t)__shfl_up((int)in[i], 1);
+        before[i] = plus(before[i], lane ? prev : 0);
     }
-    *total = all;
-    return before + in - v;
 }
 
 // The last i < n with first[i] <= v (first[0] is 0, the values ascend).
-__device__ __forceinline__ int owner(const int* first, int n, int v) {
+__device__ __forceinline__ int owner(const uint32_t* first, int n, uint32_t v) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -88,55 +114,58 @@ __device__ __forceinline__ int owner(const int* first, int n, int v) {
     return lo;
 }
 
-__device__ __forceinline__ int items_of(int keys, int share) {
+// How many items keys take where one has at most `share`, and the keys of each.
+__device__ __forceinline__ uint32_t items_of(uint32_t keys, uint32_t share, uint32_t* per) {
+    *per = max(keys, 1u);
     if (keys <= share) return 1;
-    const int n = (keys + share - 1) / share;
-    const int per = ((keys + n - 1) / n + 31) & ~31;
-    return (keys + per - 1) / per;
+    const uint32_t n = (keys + share - 1) / share;
+    *per = ((keys + n - 1) / n + 31) & ~31u;
+    return (keys + *per - 1) / *per;
 }
 
-__global__ __launch_bounds__(PT) void kq_kv_plan_kernel(PlanArg a) {
-    __shared__ long long sm[PT / 64];
-    __shared__ int first_tok[PT], first_page[PT], first_item[PT], first_part[PT];
-    __shared__ int s_cached[PT], s_held[PT], s_from[PT], s_end[PT], s_fresh[PT];
+__global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
+    __shared__ uint32_t sm[3][PT / 64][4];
+    __shared__ uint32_t first_tok[PT], first_page[PT], first_item[PT], s_cached[PT], s_held[PT], s_from[PT],
+        s_end[PT], s_fresh[PT], s_part[PT];
     __shared__ bool s_ok[PT];
     const kq_kv_plan& p = a.p;
-    const int tid = threadIdx.x;
-    const long long room = p.table ? max(0, *p.n_free) : 0;
-    for (long long i = tid; i < a.counters; i += PT) a.counter[i] = 0;
-    int share = 0x7fffffc0;
+    const int tid = threadIdx.x, T = blockDim.x;
+    const uint32_t room = p.table ? (uint32_t)max(0, *p.n_free) : 0;
+    Seq q = load_seq(a, tid);
+    for (int i = tid; i < a.counters; i += T) a.counter[i] = 0;
+    uint32_t share = 0x7fffffc0u;
     if (a.items && a.budget) {
-        long long keys = 0, all;
-        for (int s0 = 0; s0 < p.S; s0 += PT) {
-            const Seq q = load_seq(p, s0 + tid);
-            if (s0 + tid < p.S && attended(a, q)) keys += q.end - q.from;
+        // keys in units of 32, their lower and upper 16 bits
+        uint32_t units[2] = {0, 0}, before[2], all[2];
+        for (int s0 = 0; s0 < p.S; s0 += T) {
+            const Seq r = s0 ? load_seq(a, s0 + tid) : q;
+            const uint32_t n = r.attended ? (r.end - r.from + 31) / 32 : 0;
+            units[0] += n & 0xffff;
+            units[1] += n >> 16;
         }
-        wg_scan(keys, sm, &all);
-        share = (int)min((long long)share, max(64ll, ((all + a.budget - 1) / a.budget + 31) & ~31ll));
+        wg_scan<2>(units, sm[0], before, all);
+        const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
+        uint32_t n = (uint32_t)((double)total / (double)a.budget);
+        while ((uint64_t)n * (uint32_t)a.budget < total) n++;
+        share = min(share, max(64u, min(n, 0x3ffffffu) * 32));
     }
-    long long tok0 = 0, page0 = 0, taken = 0, shorts = 0;
-    int item0 = 0, part0 = 0;
-    for (int s0 = 0; s0 < p.S; s0 += PT) {
-        const int s = s0 + tid, n = min(PT, p.S - s0);
-        const Seq q = load_seq(p, s);
-        long long ntok, npage, nitem, npart, nshort, last;
-        const long long tok = wg_scan(s < p.S ? q.fresh : 0, sm, &ntok);
-        const long long pg = wg_scan(q.need, sm, &npage);
-        const bool ok = !q.narrow && (q.need == 0 || page0 + pg + q.need <= room);
-        const int from = ok ? q.from : 0, end = ok ? q.end : 0;
-        const int items = s < p.S && attended(a, q) ? items_of(end - from, share) : 0;
-        const int item = (int)wg_scan(items, sm, &nitem);
-        const int parts = items > 1 ? items : 0;
-        const int part = (int)wg_scan(parts, sm, &npart);
-        wg_scan(s < p.S && !ok, sm, &nshort);
-        wg_scan(ok ? q.need : 0, sm, &last);
+    uint32_t tok0 = 0, page0 = 0, taken = 0, shorts = 0, item0 = 0, part0 = 0;
+    for (int s0 = 0; s0 < p.S; s0 += T) {
+        const int s = s0 + tid, n = min(T, p.S - s0);
+        if (s0) q = load_seq(a, s);
+        uint32_t b1[2], n1[2], b2[4], n2[4], per;
+        const uint32_t v1[2] = {q.fresh, q.need};
+        wg_scan<2>(v1, sm[1], b1, n1);
+        const bool ok = !q.narrow && (q.need == 0 || plus(plus(page0, b1[1]), q.need) <= room);
+        const uint32_t from = ok ? q.from : 0, end = ok ? q.end : 0;
+        const uint32_t items = q.attended ? items_of(end - from, share, &per) : 0, parts = items > 1 ? items : 0;
         // (pages run out once: those who get theirs are the first that need any)
-        taken += last;
-        shorts += nshort;
-        first_tok[tid] = (int)min(tok, 0x7fffffffll);
-        first_page[tid] = (int)min(pg, 0x7fffffffll);
-        first_item[tid] = item;
-        first_part[tid] = part;
+        const uint32_t v2[4] = {items, parts, s < p.S && !ok ? 1u : 0u, ok ? q.need : 0u};
+        wg_scan<4>(v2, sm[2], b2, n2);
+        first_tok[tid] = b1[0];
+        first_page[tid] = b1[1];
+        first_item[tid] = b2[0];
+        s_part[tid] = b2[1];
         s_cached[tid] = q.cached;
         s_held[tid] = q.held;
         s_from[tid] = from;
@@ -144,61 +173,57 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(PlanArg a) {
         s_fresh[tid] = q.fresh;
         s_ok[tid] = ok;
         if (s < p.S) {
-            if (p.start) p.start[s] = (int)(tok0 + tok);
-            if (p.lens) p.lens[s] = ok ? q.end : 0;
-            if (p.held_out) p.held_out[s] = q.held + (ok ? (int)q.need : 0);
+            if (p.start) p.start[s] = (int)(tok0 + b1[0]);
+            if (p.lens) p.lens[s] = ok ? (int)q.end : 0;
+            if (p.held_out) p.held_out[s] = (int)(q.held + (ok ? q.need : 0));
         }
         __syncthreads();
         // new pages, from the end of the free ones
         if (p.table)
-            for (long long e = tid; e < npage && page0 + e < room; e += PT) {
-                const int i = owner(first_page, n, (int)e);
+            for (uint32_t e = tid; e < n1[1] && plus(page0, e) < room; e += T) {
+                const int i = owner(first_page, n, e);
                 if (s_ok[i])
-                    p.table[(long long)(s0 + i) * p.table_stride + s_held[i] + (int)(e - first_page[i])] =
+                    p.table[(int64_t)(s0 + i) * p.table_stride + s_held[i] + (e - first_page[i])] =
                         p.free_pages[room - 1 - (page0 + e)];
             }
         // new tokens
         if (p.pos || p.slot)
-            for (long long t = tid; t < ntok && tok0 + t < p.N; t += PT) {
-                const int i = owner(first_tok, n, (int)t);
-                const int pos = s_cached[i] + (int)(t - first_tok[i]);
-                if (p.pos) p.pos[tok0 + t] = pos;
+            for (uint32_t t = tid; t < n1[0] && plus(tok0, t) < (uint32_t)p.N; t += T) {
+                const int i = owner(first_tok, n, t);
+                const uint32_t pos = s_cached[i] + (t - first_tok[i]);
+                if (p.pos) p.pos[tok0 + t] = (int)pos;
                 if (!p.slot) continue;
                 int slot = -1;
                 if (s_ok[i]) {
-                    const int b = pos / p.page, more = b - s_held[i];
-                    const int page = more < 0 ? p.table[(long long)(s0 + i) * p.table_stride + b]
-                                              : p.free_pages[room - 1 - (page0 + first_page[i] + more)];
-                    if (page >= 0 && page < p.n_pages) slot = page * p.page + (pos - b * p.page);
+                    const uint32_t b = pos / (uint32_t)p.page;
+                    const int page = b < s_held[i] ? p.table[(int64_t)(s0 + i) * p.table_stride + b]
+                                                   : p.free_pages[room - 1 - (page0 + first_page[i] + (b - s_held[i]))];
+                    if ((uint32_t)page < (uint32_t)p.n_pages) slot = page * p.page + (int)(pos - b * (uint32_t)p.page);
                 }
                 p.slot[tok0 + t] = slot;
             }
         // the attention's items
-        for (long long e = tid; e < nitem && item0 + e < a.cap; e += PT) {
-            const int i = owner(first_item, n, (int)e), idx = (int)e - first_item[i];
-            const int keys = s_end[i] - s_from[i], num = items_of(keys, share);
-            const int per = ((keys + num - 1) / num + 31) & ~31;
-            int* const o = a.items + (item0 + e) * KQK_ITEM;
-            o[0] = s0 + i;
-            o[1] = s_from[i] + idx * per;
-            o[2] = min(s_end[i], s_from[i] + (idx + 1) * per);
-            o[3] = num << 16 | idx;
-            o[4] = part0 + first_part[i];
-            o[5] = (int)(tok0 + first_tok[i]);
-            o[6] = s_fresh[i];
-            o[7] = s_end[i];
+        for (uint32_t e = tid; e < n2[0] && item0 + e < (uint32_t)a.cap; e += T) {
+            const int i = owner(first_item, n, e);
+            const uint32_t idx = e - first_item[i], num = items_of(s_end[i] - s_from[i], share, &per);
+            int4* const o = reinterpret_cast<int4*>(a.items + (int64_t)(item0 + e) * KQK_ITEM);
+            o[0] = make_int4(s0 + i, (int)(s_from[i] + idx * per), (int)min(s_end[i], s_from[i] + (idx + 1) * per),
+                             (int)(num << 16 | idx));
+            o[1] = make_int4((int)(part0 + s_part[i]), (int)(tok0 + first_tok[i]), (int)s_fresh[i], (int)s_end[i]);
         }
-        tok0 += ntok;
-        page0 += npage;
-        item0 += (int)nitem;
-        part0 += (int)npart;
+        tok0 = plus(tok0, n1[0]);
+        page0 = plus(page0, n1[1]);
+        item0 += n2[0];
+        part0 += n2[1];
+        shorts += n2[2];
+        taken += n2[3];
         __syncthreads();
     }
     if (tid == 0) {
         if (p.start) p.start[p.S] = (int)tok0;
         if (p.n_free_out) *p.n_free_out = (int)(room - taken);
         if (p.n_short) *p.n_short = (int)shorts;
-        if (a.items) *a.count = min(item0, a.cap);
+        if (a.items) *a.count = min((int)item0, a.cap);
     }
 }
 
@@ -294,12 +319,15 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
     if (p->list) {
         a.budget = z->budget;
         a.cap = z->cap;
-        a.counters = z->counters;
+        a.counters = (int)z->counters;
         a.count = (int*)p->list;
         a.items = a.count + KQK_LIST_HEAD;
         a.counter = a.items + (long)z->cap * KQK_ITEM;
     }
-    hipLaunchKernelGGL(kq_kv_plan_kernel, dim3(1), dim3(PT), 0, st, a);
+    // a lane for each sequence, and for each new token that there may be
+    int lanes = p->S > p->N ? p->S : p->N;
+    lanes = lanes > PT ? PT : (lanes + 63) / 64 * 64;
+    hipLaunchKernelGGL(kq_kv_plan_kernel, dim3(1), dim3((unsigned)lanes), 0, st, a);
     return (int)hipGetLastError();
 }
 
