@@ -101,6 +101,11 @@ __device__ __forceinline__ uint32_t halves(uint32_t u) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u ^ 0x64806480u) - off);
 }
 
+template <int TYPE>
+__device__ __forceinline__ float value(uint32_t u) {
+    return TYPE == KQ_TYPE_F16 ? __half2float(__ushort_as_half((unsigned short)u)) : __uint_as_float(u << 16);
+}
+
 template <int NP>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     if constexpr (NP == 2)
@@ -117,7 +122,7 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // DM: values of a head at most (D itself where EXACT); TILED: the page is a multiple
 // of 16 tokens, so that 16 keys lie on one page; RT: tiles of 16 rows; NW: waves.
 template <int TYPE, int DM, bool EXACT, bool TILED, int RT, int NW>
-__global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT > 256 ? 1 : 2))) void kq_attn_kernel(const AttnArg a) {
     constexpr int NP = TYPE == KQ_TYPE_BF16 ? 3 : 2;      // numbers for a query or weight
     constexpr int ES = TYPE == KQ_TYPE_I8 ? 1 : 2;
     constexpr int NCH = DM / 32;                          // steps of 32 values of the first product
@@ -129,7 +134,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[QB > OB ? QB : OB];
     __shared__ float2 s_ml[NW][16 * RT];
     __shared__ float s_inv[16 * RT];
-    __shared__ int s_last;
+    __shared__ int s_last, s_bad;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4, h = blockIdx.y, D = EXACT ? DM : a.D, G = a.G;
@@ -294,6 +299,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
     }
 
     uint32_t* const ql = reinterpret_cast<uint32_t*>(lds);
+    if (tid == 0) s_bad = 0;
 #pragma unroll
     for (int i = 0; i < QP; i++) {
         const int r = (tid >> 4) + 4 * NW * i;
@@ -405,6 +411,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
                     sc[rt][1] = mfma<NP>(x[1], y, sc[rt][1]);
                 }
         }
+        __builtin_amdgcn_sched_barrier(0);
         float kscale[8], vscale[8];
         if constexpr (TYPE == KQ_TYPE_I8) {
 #pragma unroll
@@ -436,11 +443,6 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
         }
         // the next step's keys are asked for as soon as this one's are used
         const int nb = kb + 32 * NW;
-        u32x4 vc[8][NB];
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-#pragma unroll
-            for (int b = 0; b < NB; b++) vc[j][b] = vr[j][b];
         if (nb < k1) {
             load_k(nb);
             if (nb + 32 * NW < k1) fetch(nb + 32 * NW);
@@ -524,6 +526,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
             }
             l[rt] += sum;
         }
+        __builtin_amdgcn_sched_barrier(0);
         // values
         if (!full) {
 #pragma unroll
@@ -532,7 +535,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int e = 0; e < VW; e++) vc[j][b][e] &= keep;
+                    for (int e = 0; e < VW; e++) vr[j][b][e] &= keep;
             }
         }
         auto operand = [&](const u32x4 (&x)[8][NB], int b, int t) {
@@ -556,9 +559,9 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int e = 0; e < VW; e++) {
-                        const uint32_t v = vc[j][b][e];
-                        if ((v & 0x7fff) >= NONE) vc[j][b][e] &= 0xffff0000u;
-                        if ((v >> 16 & 0x7fff) >= NONE) vc[j][b][e] &= 0xffffu;
+                        const uint32_t v = vr[j][b][e];
+                        if ((v & 0x7fff) >= NONE) vr[j][b][e] &= 0xffff0000u;
+                        if ((v >> 16 & 0x7fff) >= NONE) vr[j][b][e] &= 0xffffu;
                     }
         }
 #pragma unroll
@@ -566,11 +569,12 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
             if (!EXACT && 16 * W * b >= D) continue;
 #pragma unroll
             for (int t = 0; t < W; t++) {
-                const u32x4 x = operand(vc, b, t);
+                const u32x4 x = operand(vr, b, t);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
 #pragma unroll
                     for (int j = 0; j < NP; j++) acc[rt][b][t] = mfma<NP>(x, w[rt][j], acc[rt][b][t]);
+                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
         if (nb < k1) load_v();
@@ -603,33 +607,7 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
     load_v();
     if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
     }
-    if (careful) {
-#pragma unroll 1
-        for (kb = k0 + 32 * wave; kb < k1; kb += 32 * NW) {
-#pragma unroll 1
-            for (int key = kb; key < min(kb + 32, k1); key++) {
-                const int page = table[key / a.page];
-                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                const uint8_t* const x = vh + page * a.page_b + key % a.page * a.tok_b;
-#pragma unroll
-                for (int b = 0; b < NB; b++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-#pragma unroll
-                        for (int t = 0; t < W; t++) {
-                            const int d = 16 * W * b + W * (4 * g + i) + t;
-                            const uint32_t u = reinterpret_cast<const uint16_t*>(x)[EXACT ? d : min(d, D - 1)];
-                            float y;
-                            if constexpr (TYPE == KQ_TYPE_F16) y = __half2float(__ushort_as_half(u));
-                            else y = __uint_as_float(u << 16);
-                            y = __builtin_isfinite(y) ? 0.0f : y;
-#pragma unroll
-                            for (int rt = 0; rt < RT; rt++)
-                                acc[rt][b][t][i] += key >= lo[rt] && key < hi[rt] ? y : 0.0f;
-                        }
-            }
-        }
-    }
+    if (careful) s_bad = 1;
 
     // ---- the waves' sums
     __syncthreads();                        // (queries have been read)
@@ -641,6 +619,22 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
     __syncthreads();
     float* const ol = reinterpret_cast<float*>(lds);
     const int64_t prow = ((int64_t)(part + idx) * a.n_kv + h) * a.R + first;
+    // (row of the workgroup, value)
+    auto store_out = [&](int r, int d, f32x4 y) {
+        const int row = first + r;
+        const int64_t tok = (int64_t)row0 + row / G;
+        if (tok >= 0 && tok < a.N)
+            *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) = y;
+    };
+    // (row of the partial results)
+    auto put = [](void* p, float lo, float hi) {
+        __hip_atomic_store(static_cast<uint64_t*>(p), (uint64_t)__float_as_uint(lo) | (uint64_t)__float_as_uint(hi) << 32,
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
+    auto store_part = [&](int64_t row, int d, f32x4 y) {
+        put(a.part + row * D + d, y[0], y[1]);
+        put(a.part + row * D + d + 2, y[2], y[3]);
+    };
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         if (first + 16 * rt >= rows) continue;
@@ -678,107 +672,109 @@ __global__ __launch_bounds__(64 * NW) void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                 for (int i = 0; i < NW; i++) ll += s_ml[i][16 * rt + r].y * exp2_(s_ml[i][16 * rt + r].x - base);
                 const int row = first + 16 * rt + r;
-                if (num == 1) {
-                    const int64_t tok = (int64_t)row0 + row / G;
-                    if (tok >= 0 && tok < a.N)
-                        *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + 16 * W * b + d) =
-                            ll == 0.0f ? (f32x4)0.0f : y / ll;
-                } else {
-                    float* const o = a.part + (prow + 16 * rt + r) * D + 16 * W * b + d;
+                if (ES == 2 && s_bad) {
+                    // values that are no numbers, for the rows that see them
+                    const int last = len - n + row / G, end = min(last + 1, k1);
+#pragma unroll 1
+                    for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
+                        const int page = table[key / a.page];
+                        if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                        const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b +
+                                                                        2 * (16 * W * b + d));
 #pragma unroll
-                    for (int i = 0; i < 4; i += 2)
-                        __hip_atomic_store(reinterpret_cast<uint64_t*>(o + i),
-                                           (uint64_t)__float_as_uint(y[i]) | (uint64_t)__float_as_uint(y[i + 1]) << 32,
-                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    if (b == 0 && d == 0)
-                        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.ml + prow + 16 * rt + r),
-                                           (uint64_t)__float_as_uint(mm) | (uint64_t)__float_as_uint(ll) << 32,
-                                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                        for (int i = 0; i < 4; i++) {
+                            const float z = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
+                            y[i] += __builtin_isfinite(z) ? 0.0f : z;
+                        }
+                    }
+                }
+                if (num == 1)
+                    store_out(16 * rt + r, 16 * W * b + d, ll == 0.0f ? (f32x4)0.0f : y / ll);
+                else {
+                    store_part(prow + 16 * rt + r, 16 * W * b + d, y);
+                    if (b == 0 && d == 0) put(a.ml + prow + 16 * rt + r, mm, ll);
                 }
             }
         }
     }
     if (num == 1) return;
 
-    // ---- a sequence's last workgroup joins the partial results
-    // The results and the count are device-scope atomics, which go past the caches that
-    // another XCD does not see: once a wave's stores are acknowledged they are there for
-    // all, and the barrier puts every wave's before the count.  (A release fence instead
-    // writes back the L2, in each of hundreds of workgroups.)
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    if (tid == 0) {
-        int* const p = a.counter + ((int64_t)s * a.n_kv + h) * gridDim.z + blockIdx.z;
-        s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == num - 1;
-        if (s_last) __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    if (!s_last) return;
+    // ---- partial results are joined by the last workgroup of each eight, theirs by the
+    // last of these.  Results and counts are device-scope atomics, which go past the
+    // caches that another XCD does not see: once a wave's stores are acknowledged they are
+    // there for all, and the barrier puts every wave's before the count.  (A release fence
+    // instead writes back the L2, in each of hundreds of workgroups: 64 ragged streams
+    // took 233 us with it, 124 without.)
+    const int live = min(rows - first, 16 * RT), quads = D / 4;
+    auto last_of = [&](int slot, int n) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (tid == 0) {
+            int* const p = a.counter + ((int64_t)(part + slot) * a.n_kv + h) * gridDim.z + blockIdx.z;
+            s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+            if (s_last) __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        return s_last != 0;
+    };
     auto get = [](const void* p) {
         const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
     };
-    // Rows and quads of values over the lanes, and where those are fewer, the parts too;
-    // each part's weight 2^(m - max) once, for as many rows at a time as LDS has room.
-    const int64_t step = (int64_t)a.n_kv * a.R, from = ((int64_t)part * a.n_kv + h) * a.R + first;
-    constexpr int ROOM = sizeof(lds) / 4 - 64 * NW * 4;
-    float* const wl = ol + 64 * NW * 4;
-    const int live = min(rows - first, 16 * RT), quads = D / 4, at_once = max(1, min(live, ROOM / num));
-    for (int r0 = 0; r0 < live; r0 += at_once) {
-        const int nr = min(at_once, live - r0);
-        __syncthreads();
-        for (int r = wave; r < nr; r += NW) {
-            const float2* const p = a.ml + from + r0 + r;
-            float top = -INFINITY, sum = 0.0f;
-            for (int i = lane; i < num; i += 64) {
-                const float2 t = get(p + i * step);
-                top = fmaxf(top, t.x);
-            }
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-            const float base = top == -INFINITY ? 0.0f : top;
-            for (int i = lane; i < num; i += 64) {
-                const float2 t = get(p + i * step);
-                sum += t.y * exp2_(t.x - base);
-            }
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) sum += __shfl_xor(sum, off);
-            for (int i = lane; i < num; i += 64)
-                wl[r * num + i] = sum == 0.0f ? 0.0f : exp2_(get(p + i * step).x - base) / sum;
-        }
-        __syncthreads();
-        const int units = nr * quads;
-        int ways = 1;
-        while (2 * ways * units <= 64 * NW && 2 * ways <= num) ways *= 2;
-        for (int e0 = 0; e0 < units * ways; e0 += 64 * NW) {
-            const int e = e0 + tid, u = e % units, way = e / units, r = u / quads, d = u % quads * 4;
+    // n results, `by` apart from slot `from` on, to the first's place or, `end`, to out
+    auto join = [&](int from, int by, int n, bool end) {
+        const int64_t row1 = ((int64_t)(part + from) * a.n_kv + h) * a.R + first, step = (int64_t)by * a.n_kv * a.R;
+        for (int e = tid; e < live * quads; e += 64 * NW) {
+            const int r = e / quads, d = e % quads * 4;
             f32x4 y = (f32x4)0.0f;
-            if (way < ways) {
-                const float* const p = a.part + (from + r0 + r) * D + d;
-#pragma unroll 8
-                for (int i = way; i < num; i += ways) {
-                    const float2 t0 = get(p + i * step * D), t1 = get(p + i * step * D + 2);
-                    y += (f32x4){t0.x, t0.y, t1.x, t1.y} * wl[r * num + i];
+            float top = -INFINITY, sum = 0.0f;
+#pragma unroll 1
+            for (int i0 = 0; i0 < n; i0 += 8) {
+                float2 t[8], o[8][2];
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int64_t at = row1 + r + min(i0 + i, n - 1) * step;
+                    t[i] = get(a.ml + at);
+                    o[i][0] = get(a.part + at * D + d);
+                    o[i][1] = get(a.part + at * D + d + 2);
+                }
+                float nm = top;
+#pragma unroll
+                for (int i = 0; i < 8; i++) nm = fmaxf(nm, t[i].x);
+                const float base = nm == -INFINITY ? 0.0f : nm, f = exp2_(top - base);
+                top = nm;
+                y *= f;
+                sum *= f;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (i0 + i >= n) break;
+                    const float w = exp2_(t[i].x - base);
+                    y += (f32x4){o[i][0].x, o[i][0].y, o[i][1].x, o[i][1].y} * w;
+                    sum += t[i].y * w;
                 }
             }
-            if (ways > 1) {                 // (a single round then)
-                *reinterpret_cast<f32x4*>(ol + 4 * tid) = y;
-                __syncthreads();
-                for (int i = 1; i < ways && way == 0; i++) y += *reinterpret_cast<const f32x4*>(ol + 4 * (tid + i * units));
+            if (end) {
+                store_out(r, d, sum == 0.0f ? (f32x4)0.0f : y / sum);
+            } else {
+                store_part(row1 + r, d, y);
+                if (d == 0) s_ml[0][r] = make_float2(top, sum);
             }
-            const int row = first + r0 + r;
-            const int64_t tok = (int64_t)row0 + row / G;
-            if (way == 0 && tok >= 0 && tok < a.N)
-                *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) = y;
         }
-    }
+        if (end) return;
+        __syncthreads();                    // (all lanes have read the maximum and sum of their row)
+        if (tid < live) put(a.ml + row1 + tid, s_ml[0][tid].x, s_ml[0][tid].y);
+    };
+    const int group = idx & ~7, of = min(8, num - group);
+    if (!last_of(group, of)) return;
+    join(group, 1, of, num <= 8);
+    if (num > 8 && last_of(1, (num + 7) / 8)) join(0, 8, (num + 7) / 8, true);
 }
 
 typedef void (*Kernel)(AttnArg);
 
 // Waves of a workgroup, and tiles of rows at most: a lane holds 64 registers of keys
 // and values and 32 of sums a tile for each 128 values of a head.
-template <int DM, int RT> constexpr int NWV = DM == 256 || DM * RT > 256 ? 4 : 8;
+template <int DM, int RT> constexpr int NWV = 4;
 constexpr int most_tiles(int D) { return D > 128 ? 2 : 4; }
 
 template <int TYPE, int DM, bool EXACT, bool TILED>
@@ -817,7 +813,7 @@ void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
     z->budget = (2 * n_cu + per - 1) / per;
     z->cap = s->S + z->budget;
     z->parts = 2 * z->budget;
-    z->counters = (int64_t)s->S * per;
+    z->counters = (int64_t)z->parts * per;
 }
 
 int64_t kqk_attn_workspace(const kq_attn_shape* s, int n_cu) {

@@ -132,10 +132,10 @@ int64_t kqk_verify_workspace(const kq_spec_verify* v);
 int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st);
 /* attention over a paged cache (kq_kv.hip, kq_attn.hip): arguments checked and
  * strides filled in by kq_kv.c.  The list of work, in ints: their number, then from
- * KQK_LIST_HEAD on `cap` items of KQK_ITEM, then a counter for each sequence, head of
- * keys and block of rows, 0 between calls.  An item: sequence, first key, key behind
- * its last, number (upper half) and index among the sequence's items, the first of
- * their partial results, the sequence's first row, new tokens and length. */
+ * KQK_LIST_HEAD on `cap` items of KQK_ITEM, then counters, 0 between calls: of each
+ * partial result's place, head of keys and block of rows.  An item: sequence, first key,
+ * key behind its last, number (upper half) and index among the sequence's items, the
+ * place of their first partial result, the sequence's first row, new tokens and length. */
 #define KQK_LIST_HEAD 8
 #define KQK_ITEM 8
 typedef struct {
