@@ -129,12 +129,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     constexpr int W = DM >= 128 ? 8 : 4;                  // values a lane of a key in the second
     constexpr int NB = DM / (16 * W);
     constexpr int VW = W * ES / 4;                        // registers of W values
-    constexpr int OS = 16 * W + 4;                        // a row of a block of values in LDS
+    constexpr int OS = DM + 4;                            // a row of sums in LDS
     constexpr int QB = NP * RT * 16 * DM * 2, OB = NW * 16 * OS * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[QB > OB ? QB : OB];
     __shared__ float2 s_ml[NW][16 * RT];
+    __shared__ float2 s_all[16 * RT];
     __shared__ float s_inv[16 * RT];
-    __shared__ int s_last, s_bad;
+    __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4, h = blockIdx.y, D = EXACT ? DM : a.D, G = a.G;
@@ -166,6 +167,19 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     k0 &= ~31;
     k1 = (int)min((int64_t)min(k1, 0x7fff0000), (int64_t)a.table_stride * a.page);
 
+    const uint8_t* const kh = a.k + h * a.head_b;
+    const uint8_t* const vh = a.v + h * a.head_b;
+    int lo[RT], hi[RT];                     // the keys that a lane's rows see
+    float m[RT], l[RT];
+    f32x4 acc[RT][NB][W];
+    int ve = 0;                             // int8: the sums' exponent
+    // An infinity or NaN among the values would reach rows that do not see its key, and
+    // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
+    // number all are taken again without such values, which are then added alone.
+    bool careful = false;
+#pragma unroll 1
+    while (true) {
+
     // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
     constexpr int QP = 16 * RT / (4 * NW) > 0 ? 16 * RT / (4 * NW) : 1;      // rows a 16 lanes take
     constexpr int QO = (DM / 8 + 15) / 16;
@@ -188,8 +202,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     }
 
     // ---- where a step's keys lie
-    const uint8_t* const kh = a.k + h * a.head_b;
-    const uint8_t* const vh = a.v + h * a.head_b;
     int pg[2];                                              // pages of the next step's keys
     auto fetch = [&](int kb) {
 #pragma unroll
@@ -299,7 +311,6 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     }
 
     uint32_t* const ql = reinterpret_cast<uint32_t*>(lds);
-    if (tid == 0) s_bad = 0;
 #pragma unroll
     for (int i = 0; i < QP; i++) {
         const int r = (tid >> 4) + 4 * NW * i;
@@ -343,10 +354,8 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     }
     __syncthreads();
 
-    // ---- rows of this lane: the keys they see, [lo, hi)
-    int lo[RT], hi[RT];
-    float inv[RT], m[RT], l[RT];
-    f32x4 acc[RT][NB][W];
+    // ---- rows of this lane
+    float inv[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int row = first + 16 * rt + c, last = len - n + row / G;
@@ -361,20 +370,13 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
 #pragma unroll
             for (int t = 0; t < W; t++) acc[rt][b][t] = (f32x4)0.0f;
     }
-    int ve = 0;                             // int8: the sums' exponent
-    (void)ve;
+    ve = 0;
     // steps within [all_lo, all_hi) are seen by all rows
     const int row_n = min(rows, first + 16 * RT) - 1;
     const int all_hi = min(k1, len - n + first / G + 1);
     const int all_lo = a.window ? len - n + row_n / G + 1 - a.window : 0;
 
     // ---- steps
-    // An infinity or NaN among the values would reach rows that do not see its key, and
-    // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
-    // number they are taken again without such values, which are then added alone.
-    bool careful = false;
-#pragma unroll 1
-    while (true) {
 #pragma unroll 1
     for (; kb < k1; kb += 32 * NW) {
         const bool ok0 = have[0], ok1 = have[1];
@@ -580,37 +582,23 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         if (nb < k1) load_v();
     }
 
-    if (ES == 1 || careful) break;
     float none = 0.0f;
+    if constexpr (ES == 2) {
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int t = 0; t < W; t++)
+                for (int t = 0; t < W; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) none = fmaf(acc[rt][b][t][i], 0.0f, none);
-    if (!__any(none != 0.0f)) break;
+                    for (int i = 0; i < 4; i++) none = fmaf(acc[rt][b][t][i], 0.0f, none);
+    }
+    // (a barrier: queries have been read)
+    if (!__syncthreads_or(none != 0.0f) || careful) break;
     careful = true;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        m[rt] = -INFINITY;
-        l[rt] = 0.0f;
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-            for (int t = 0; t < W; t++) acc[rt][b][t] = (f32x4)0.0f;
     }
-    kb = k0 + 32 * wave;
-    fetch(kb);
-    load_k(kb);
-    load_v();
-    if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
-    }
-    if (careful) s_bad = 1;
 
     // ---- the waves' sums
-    __syncthreads();                        // (queries have been read)
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         l[rt] = sum4(l[rt]);
@@ -635,6 +623,16 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         put(a.part + row * D + d, y[0], y[1]);
         put(a.part + row * D + d + 2, y[2], y[3]);
     };
+    if (tid < 16 * RT) {
+        float top = s_ml[0][tid].x, sum = 0.0f;
+#pragma unroll
+        for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][tid].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int i = 0; i < NW; i++) sum += s_ml[i][tid].y * exp2_(s_ml[i][tid].x - base);
+        s_all[tid] = make_float2(top, sum);
+    }
+    const int quads = D / 4;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         if (first + 16 * rt >= rows) continue;
@@ -643,57 +641,45 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][16 * rt + c].x);
         float f = exp2_(m[rt] - (top == -INFINITY ? 0.0f : top));
         if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)max(1, ve) << 23);
-        const int live = min(16, rows - first - 16 * rt);
+        const int here = min(16, rows - first - 16 * rt);
+        if (rt) __syncthreads();
+        if (c < here) {
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-            if (!EXACT && 16 * W * b >= D) continue;
-            if (rt || b) __syncthreads();
-            if (c < live) {
+            for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int t = 0; t < W; t += 4)
-                        *reinterpret_cast<f32x4*>(ol + (wave * 16 + c) * OS + W * (4 * g + i) + t) =
+                        *reinterpret_cast<f32x4*>(ol + (wave * 16 + c) * OS + 16 * W * b + W * (4 * g + i) + t) =
                             (f32x4){acc[rt][b][t][i], acc[rt][b][t + 1][i], acc[rt][b][t + 2][i], acc[rt][b][t + 3][i]} * f;
-            }
-            __syncthreads();
-            for (int e = tid; e < live * 4 * W; e += 64 * NW) {
-                const int r = e / (4 * W), d = e % (4 * W) * 4;
-                if (!EXACT && 16 * W * b + d >= D) continue;
-                f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
-                float mm = s_ml[0][16 * rt + r].x;
+        }
+        __syncthreads();
+        for (int e = tid; e < here * quads; e += 64 * NW) {
+            const int r = e / quads, d = e % quads * 4;
+            f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
 #pragma unroll
-                for (int i = 1; i < NW; i++) {
-                    y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
-                    mm = fmaxf(mm, s_ml[i][16 * rt + r].x);
-                }
-                const float base = mm == -INFINITY ? 0.0f : mm;
-                float ll = 0.0f;
-#pragma unroll
-                for (int i = 0; i < NW; i++) ll += s_ml[i][16 * rt + r].y * exp2_(s_ml[i][16 * rt + r].x - base);
-                const int row = first + 16 * rt + r;
-                if (ES == 2 && s_bad) {
-                    // values that are no numbers, for the rows that see them
-                    const int last = len - n + row / G, end = min(last + 1, k1);
+            for (int i = 1; i < NW; i++) y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
+            if (ES == 2 && careful) {
+                // values that are no numbers, for the rows that see them
+                const int last = len - n + (first + 16 * rt + r) / G, end = min(last + 1, k1);
 #pragma unroll 1
-                    for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
-                        const int page = table[key / a.page];
-                        if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                        const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b +
-                                                                        2 * (16 * W * b + d));
+                for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
+                    const int page = table[key / a.page];
+                    if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                    const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b + 2 * d);
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float z = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
-                            y[i] += __builtin_isfinite(z) ? 0.0f : z;
-                        }
+                    for (int i = 0; i < 4; i++) {
+                        const float z = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
+                        y[i] += __builtin_isfinite(z) ? 0.0f : z;
                     }
                 }
-                if (num == 1)
-                    store_out(16 * rt + r, 16 * W * b + d, ll == 0.0f ? (f32x4)0.0f : y / ll);
-                else {
-                    store_part(prow + 16 * rt + r, 16 * W * b + d, y);
-                    if (b == 0 && d == 0) put(a.ml + prow + 16 * rt + r, mm, ll);
-                }
+            }
+            const float2 all = s_all[16 * rt + r];
+            if (num == 1) {
+                store_out(16 * rt + r, d, all.y == 0.0f ? (f32x4)0.0f : y / all.y);
+            } else {
+                store_part(prow + 16 * rt + r, d, y);
+                if (d == 0) put(a.ml + prow + 16 * rt + r, all.x, all.y);
             }
         }
     }
@@ -705,7 +691,7 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     // there for all, and the barrier puts every wave's before the count.  (A release fence
     // instead writes back the L2, in each of hundreds of workgroups: 64 ragged streams
     // took 233 us with it, 124 without.)
-    const int live = min(rows - first, 16 * RT), quads = D / 4;
+    const int live = min(rows - first, 16 * RT);
     auto last_of = [&](int slot, int n) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
@@ -721,43 +707,62 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
     };
+    constexpr int JU = RT * DM >= 256 ? 4 : 2;   // quads of values that a lane has in flight
     // n results, `by` apart from slot `from` on, to the first's place or, `end`, to out
     auto join = [&](int from, int by, int n, bool end) {
         const int64_t row1 = ((int64_t)(part + from) * a.n_kv + h) * a.R + first, step = (int64_t)by * a.n_kv * a.R;
-        for (int e = tid; e < live * quads; e += 64 * NW) {
-            const int r = e / quads, d = e % quads * 4;
-            f32x4 y = (f32x4)0.0f;
-            float top = -INFINITY, sum = 0.0f;
+        for (int e0 = tid; e0 < live * quads; e0 += 64 * NW * JU) {
+            f32x4 y[JU];
+            float top[JU], sum[JU];
+#pragma unroll
+            for (int u = 0; u < JU; u++) {
+                y[u] = (f32x4)0.0f;
+                top[u] = -INFINITY;
+                sum[u] = 0.0f;
+            }
 #pragma unroll 1
             for (int i0 = 0; i0 < n; i0 += 8) {
-                float2 t[8], o[8][2];
+                float2 t[JU][8], o[JU][8][2];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const int64_t at = row1 + r + min(i0 + i, n - 1) * step;
-                    t[i] = get(a.ml + at);
-                    o[i][0] = get(a.part + at * D + d);
-                    o[i][1] = get(a.part + at * D + d + 2);
+                for (int u = 0; u < JU; u++) {
+                    const int e = min(e0 + 64 * NW * u, live * quads - 1), r = e / quads, d = e % quads * 4;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int64_t at = row1 + r + min(i0 + i, n - 1) * step;
+                        t[u][i] = get(a.ml + at);
+                        o[u][i][0] = get(a.part + at * D + d);
+                        o[u][i][1] = get(a.part + at * D + d + 2);
+                    }
                 }
-                float nm = top;
 #pragma unroll
-                for (int i = 0; i < 8; i++) nm = fmaxf(nm, t[i].x);
-                const float base = nm == -INFINITY ? 0.0f : nm, f = exp2_(top - base);
-                top = nm;
-                y *= f;
-                sum *= f;
+                for (int u = 0; u < JU; u++) {
+                    float nm = top[u];
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    if (i0 + i >= n) break;
-                    const float w = exp2_(t[i].x - base);
-                    y += (f32x4){o[i][0].x, o[i][0].y, o[i][1].x, o[i][1].y} * w;
-                    sum += t[i].y * w;
+                    for (int i = 0; i < 8; i++) nm = fmaxf(nm, t[u][i].x);
+                    const float base = nm == -INFINITY ? 0.0f : nm, f = exp2_(top[u] - base);
+                    top[u] = nm;
+                    y[u] *= f;
+                    sum[u] *= f;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float w = exp2_(t[u][i].x - base);
+                        if (i0 + i < n) {
+                            y[u] += (f32x4){o[u][i][0].x, o[u][i][0].y, o[u][i][1].x, o[u][i][1].y} * w;
+                            sum[u] += t[u][i].y * w;
+                        }
+                    }
                 }
             }
-            if (end) {
-                store_out(r, d, sum == 0.0f ? (f32x4)0.0f : y / sum);
-            } else {
-                store_part(row1 + r, d, y);
-                if (d == 0) s_ml[0][r] = make_float2(top, sum);
+#pragma unroll
+            for (int u = 0; u < JU; u++) {
+                const int e = e0 + 64 * NW * u, r = e / quads, d = e % quads * 4;
+                if (e >= live * quads) continue;
+                if (end) {
+                    store_out(r, d, sum[u] == 0.0f ? (f32x4)0.0f : y[u] / sum[u]);
+                } else {
+                    store_part(row1 + r, d, y[u]);
+                    if (d == 0) s_ml[0][r] = make_float2(top[u], sum[u]);
+                }
             }
         }
         if (end) return;
