@@ -3,9 +3,9 @@
 //   out = sum_j p_j v_j,  p = softmax over the keys j that a token sees of scale q . k_j
 //
 // The rows of a sequence and a head of keys are its new tokens' queries of the G =
-// n_q / n_kv heads that read it; a workgroup takes 16 RT of them and an item of the
-// list (a share of the sequence's keys), each of its waves every NW-th step of 32
-// keys.  One pass, with a running maximum m and sum l of each row:
+// n_q / n_kv heads that read it; a workgroup takes 16 of them and an item of the list
+// (a share of the sequence's keys), each of its waves every fourth step of 32 keys (64 of
+// few bytes).  One pass, with a running maximum m and sum l of each row:
 //   S^T = K Q^T   16 keys x 16 rows a matrix instruction, K as it lies in the cache
 //                 (a lane has 8 values of one key), Q^T from LDS
 //   p = 2^(S - m), in the layout that S^T has: 8 keys of a row a lane, which is that
@@ -32,6 +32,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef u32x4 u32x4a __attribute__((aligned(8)));
 struct __attribute__((aligned(4))) F4 { float v[4]; };    // four floats at any 4-byte address
 
 struct AttnArg {
@@ -50,9 +51,9 @@ struct AttnArg {
     float* part;                // partial results: parts x n_kv x R rows of D
     float2* ml;                 // and their maximum and sum
     int64_t page_b, head_b, tok_b, q_stride, out_stride;      // cache strides in bytes
-    uint64_t div;               // page / 16 by multiplication
+    uint64_t div, kv_div, blocks_div;    // page / 16, n_kv and 8 blocks by multiplication
     float qscale;               // scale log2 e
-    int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts;
+    int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts, blocks;
 };
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
@@ -116,32 +117,45 @@ __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+constexpr int NW = 4;           // waves of a workgroup
+
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // DM: values of a head at most (D itself where EXACT); TILED: the page is a multiple
-// of 16 tokens, so that 16 keys lie on one page; RT: tiles of 16 rows; NW: waves.
-template <int TYPE, int DM, bool EXACT, bool TILED, int RT, int NW>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT > 256 ? 1 : 2))) void kq_attn_kernel(const AttnArg a) {
+// of 16 tokens, so that 16 keys lie on one page.
+template <int TYPE, int DM, bool EXACT, bool TILED>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(2)))
+void kq_attn_kernel(const AttnArg a) {
     constexpr int NP = TYPE == KQ_TYPE_BF16 ? 3 : 2;      // numbers for a query or weight
     constexpr int ES = TYPE == KQ_TYPE_I8 ? 1 : 2;
     constexpr int NCH = DM / 32;                          // steps of 32 values of the first product
+    // tiles of 32 keys in a step: two where one has few bytes to wait for
+    constexpr int NS = DM * ES <= 128 ? 2 : 1, KEYS = 32 * NS;
+    constexpr bool WIDE = TYPE == KQ_TYPE_I8 && EXACT;    // int8 keys in loads of 16
     constexpr int W = DM >= 128 ? 8 : 4;                  // values a lane of a key in the second
     constexpr int NB = DM / (16 * W);
     constexpr int VW = W * ES / 4;                        // registers of W values
     constexpr int OS = DM + 4;                            // a row of sums in LDS
-    constexpr int QB = NP * RT * 16 * DM * 2, OB = NW * 16 * OS * 4;
+    constexpr int QB = NP * 16 * DM * 2, OB = NW * 16 * OS * 4;
     __shared__ __attribute__((aligned(16))) uint8_t lds[QB > OB ? QB : OB];
-    __shared__ float2 s_ml[NW][16 * RT];
-    __shared__ float2 s_all[16 * RT];
-    __shared__ float s_inv[16 * RT];
+    __shared__ float2 s_ml[NW][16], s_all[16];
+    __shared__ float s_inv[16];
     __shared__ int s_last;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const int c = lane & 15, g = lane >> 4, h = blockIdx.y, D = EXACT ? DM : a.D, G = a.G;
-    int s = blockIdx.x, k0 = 0, k1, num = 1, idx = 0, part = 0, row0, n, len;
+    const int c = lane & 15, g = lane >> 4, D = EXACT ? DM : a.D, G = a.G;
+    // Item after item, of each all heads and blocks of rows: those beyond the list's come
+    // last (head after head instead, 64 workgroups with 64 more in front of each other's
+    // took 22.6 us for 17.3).  Blocks of rows of one item and head are eight workgroups
+    // apart, which puts them on one XCD, in whose L2 the keys are.
+    const int eight = (int)((uint64_t)blockIdx.x * a.blocks_div >> 40), rest = blockIdx.x - 8 * a.blocks * eight;
+    const int z = rest >> 3, pair = 8 * eight + (rest & 7);
+    int s = (int)((uint64_t)(uint32_t)pair * a.kv_div >> 40);
+    const int h = pair - s * a.n_kv;
+    int k0 = 0, k1, num = 1, idx = 0, part = 0, row0, n, len;
+    if (s >= (a.items ? min(a.cap, *a.count) : a.S)) return;
     if (a.items) {
-        if (s >= min(a.cap, *a.count)) return;
         const int* const it = a.items + s * KQK_ITEM;
         s = it[0];
         k0 = it[1];
@@ -158,20 +172,20 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         row0 = a.start ? a.start[s] : s;
         n = a.start ? a.start[s + 1] - row0 : 1;
         k1 = len = a.lens[s];
-        if (a.window) k0 = max(0, len - n + 1 - a.window) & ~31;
+        if (a.window) k0 = max(0, len - n + 1 - a.window);
     }
     if (n < 1 || n > a.T) return;
-    const int rows = n * G, first = blockIdx.z * 16 * RT;   // of this sequence; of this workgroup
-    if (first >= rows) return;
+    const int first = 16 * z, live = min(16, n * G - first);      // rows of this workgroup
+    if (live <= 0) return;
     const int* const table = a.table + (int64_t)s * a.table_stride;
     k0 &= ~31;
     k1 = (int)min((int64_t)min(k1, 0x7fff0000), (int64_t)a.table_stride * a.page);
-
     const uint8_t* const kh = a.k + h * a.head_b;
     const uint8_t* const vh = a.v + h * a.head_b;
-    int lo[RT], hi[RT];                     // the keys that a lane's rows see
-    float m[RT], l[RT];
-    f32x4 acc[RT][NB][W];
+
+    int lo, hi;                             // the keys that a lane's row sees
+    float m, l;
+    f32x4 acc[NB][W];
     int ve = 0;                             // int8: the sums' exponent
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
@@ -179,344 +193,312 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
     bool careful = false;
 #pragma unroll 1
     while (true) {
-
-    // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
-    constexpr int QP = 16 * RT / (4 * NW) > 0 ? 16 * RT / (4 * NW) : 1;      // rows a 16 lanes take
-    constexpr int QO = (DM / 8 + 15) / 16;
-    f32x4 qv[QP][QO][2];
+        // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
+        constexpr int QO = (DM / 8 + 15) / 16;
+        const int qr = tid >> 4;            // 16 lanes a row
+        f32x4 qv[QO][2];
+        {
+            const int64_t tok = (int64_t)row0 + (first + qr) / G;
+            const bool on = qr < live && tok >= 0 && tok < a.N;
+            const float* const q = a.q + tok * a.q_stride + (int64_t)(h * G + (first + qr) % G) * D;
 #pragma unroll
-    for (int i = 0; i < QP; i++) {
-        const int r = (tid >> 4) + 4 * NW * i, row = first + r;
-        const int64_t tok = (int64_t)row0 + row / G;
-        const bool on = r < 16 * RT && row < rows && tok >= 0 && tok < a.N;
-        const float* const q = a.q + tok * a.q_stride + (int64_t)(h * G + row % G) * D;
-#pragma unroll
-        for (int o = 0; o < QO; o++) {
-            const int d = 8 * (c + 16 * o);
-            qv[i][o][0] = qv[i][o][1] = (f32x4)0.0f;
-            if (on && d < D) {
-                qv[i][o][0] = *reinterpret_cast<const f32x4*>(q + d);
-                qv[i][o][1] = *reinterpret_cast<const f32x4*>(q + d + 4);
-            }
-        }
-    }
-
-    // ---- where a step's keys lie
-    int pg[2];                                              // pages of the next step's keys
-    auto fetch = [&](int kb) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            if constexpr (TILED) {
-                const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
-                pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
-            } else {
-                const uint32_t b = (uint32_t)(kb + 16 * t + c) / (uint32_t)a.page;
-                pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
-            }
-        }
-    };
-    u32x4 kr[2][NCH], vr[8][NB];
-    float ksr[8], vsr[8];
-    bool have[2];                                           // the keys' pages are pages
-    const uint8_t* vp[8];
-    int64_t sp[2];
-    const uint32_t klane = TILED ? c * (uint32_t)a.tok_b + 8 * ES * g : 8 * ES * g;
-    const uint32_t vlane = (TILED ? 4 * g * (uint32_t)a.tok_b : 0u) + W * ES * c;
-    auto octet = [&](int ch) { return EXACT || 32 * ch + 8 * g < D; };
-    auto load_k = [&](int kb) {
-#pragma unroll
-        for (int t = 0; t < 2; t++) {
-            const uint8_t* p;
-            if constexpr (TILED) {
-                int page = uniform(pg[t]);
-                have[t] = (uint32_t)page < (uint32_t)a.n_pages;
-                page = have[t] ? page : 0;
-                const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
-                const int at = have[t] ? kb + 16 * t - (int)(b * (uint32_t)a.page) : 0;
-                const int64_t o = page * a.page_b + at * a.tok_b;
-                p = kh + o;
-#pragma unroll
-                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + o + j * a.tok_b;
-                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
-            } else {
-                have[t] = (uint32_t)pg[t] < (uint32_t)a.n_pages;
-                const int page = have[t] ? pg[t] : 0, at = have[t] ? (kb + 16 * t + c) % a.page : 0;
-                const int64_t o = page * a.page_b + at * a.tok_b;
-                p = kh + o;
-#pragma unroll
-                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + __shfl(o, 4 * g + j);
-                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
-            }
-#pragma unroll
-            for (int ch = 0; ch < NCH; ch++) {
-                if (!EXACT && 32 * ch >= D) continue;
-                const uint8_t* const x = p + (klane + (octet(ch) ? 32 * ES * ch : -8 * ES * g));
-                if constexpr (ES == 2) {
-                    kr[t][ch] = *reinterpret_cast<const u32x4*>(x);
-                } else {
-                    const u32x2 y = *reinterpret_cast<const u32x2*>(x);
-                    kr[t][ch][0] = y[0];
-                    kr[t][ch][1] = y[1];
+            for (int o = 0; o < QO; o++) {
+                const int d = 8 * (c + 16 * o);
+                qv[o][0] = qv[o][1] = (f32x4)0.0f;
+                if (on && d < D) {
+                    qv[o][0] = *reinterpret_cast<const f32x4*>(q + d);
+                    qv[o][1] = *reinterpret_cast<const f32x4*>(q + d + 4);
                 }
             }
-            if constexpr (TYPE == KQ_TYPE_I8) {
+        }
+
+        // ---- where a step's keys lie
+        int pg[2 * NS];                     // pages of the next step's keys
+        auto fetch = [&](int kb) {
+#pragma unroll
+            for (int t = 0; t < 2 * NS; t++) {
+                uint32_t b;
+                if constexpr (TILED) b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                else b = (uint32_t)(kb + 16 * t + c) / (uint32_t)a.page;
+                pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
+            }
+        };
+        u32x4 kr[2 * NS][WIDE ? NCH / 2 : NCH], vr[8 * NS][NB];
+        float ksr[8 * NS], vsr[8 * NS];
+        bool have[2 * NS];                  // the keys' pages are pages
+        const uint8_t* vp[8 * NS];
+        int64_t sp[2 * NS];
+        const uint32_t klane = (TILED ? c * (uint32_t)a.tok_b : 0u) + (WIDE ? 16 : 8 * ES) * g;
+        const uint32_t vlane = (TILED ? 4 * g * (uint32_t)a.tok_b : 0u) + W * ES * c;
+        auto octet = [&](int ch) { return EXACT || 32 * ch + 8 * g < D; };
+        auto load_k = [&](int kb) {
+#pragma unroll
+            for (int t = 0; t < 2 * NS; t++) {
+                // (a key that is not there is read as the first one of the first page)
+                int page = TILED ? uniform(pg[t]) : pg[t], at;
+                have[t] = (uint32_t)page < (uint32_t)a.n_pages;
+                page = have[t] ? page : 0;
                 if constexpr (TILED) {
+                    const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                    at = kb + 16 * t - (int)(b * (uint32_t)a.page);
+                } else {
+                    at = (int)((uint32_t)(kb + 16 * t + c) % (uint32_t)a.page);
+                }
+                at = have[t] ? at : 0;
+                const int64_t o = page * a.page_b + at * a.tok_b;
+#pragma unroll
+                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + (TILED ? o + j * a.tok_b : (int64_t)__shfl(o, 4 * g + j));
+                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
+#pragma unroll
+                for (int ch = 0; ch < NCH; ch++) {
+                    if (!EXACT && 32 * ch >= D) continue;
+                    const uint8_t* const x = kh + o + (klane + (WIDE || octet(ch) ? 32 * ES * ch : -8 * ES * g));
+                    if constexpr (WIDE) {
+                        if (ch % 2 == 0) kr[t][ch / 2] = *reinterpret_cast<const u32x4a*>(x);
+                    } else if constexpr (ES == 2) {
+                        kr[t][ch] = *reinterpret_cast<const u32x4*>(x);
+                    } else {
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+                        kr[t][ch][0] = y[0];
+                        kr[t][ch][1] = y[1];
+                    }
+                }
+                if constexpr (TYPE == KQ_TYPE_I8 && TILED) {
                     const F4 x = *reinterpret_cast<const F4*>(a.ks + sp[t] + 4 * g);
 #pragma unroll
                     for (int j = 0; j < 4; j++) ksr[4 * t + j] = x.v[j];
-                } else {
+                } else if constexpr (TYPE == KQ_TYPE_I8) {
                     ksr[t] = a.ks[sp[t]];
                 }
             }
-        }
-    };
-    auto load_v = [&]() {
+        };
+        auto load_v = [&]() {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
+            for (int j = 0; j < 8 * NS; j++)
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-                const uint8_t* const x = vp[j] + (EXACT || W * c + 16 * W * b < D ? vlane + 16 * W * ES * b
-                                                                                 : vlane - W * ES * c);
-                if constexpr (VW == 4) {
-                    vr[j][b] = *reinterpret_cast<const u32x4*>(x);
-                } else if constexpr (VW == 2) {
-                    const u32x2 y = *reinterpret_cast<const u32x2*>(x);
-                    vr[j][b][0] = y[0];
-                    vr[j][b][1] = y[1];
-                } else {
-                    vr[j][b][0] = *reinterpret_cast<const uint32_t*>(x);
+                for (int b = 0; b < NB; b++) {
+                    const uint8_t* const x = vp[j] + (EXACT || W * c + 16 * W * b < D ? vlane + 16 * W * ES * b
+                                                                                     : vlane - W * ES * c);
+                    if constexpr (VW == 4) {
+                        vr[j][b] = *reinterpret_cast<const u32x4*>(x);
+                    } else if constexpr (VW == 2) {
+                        const u32x2 y = *reinterpret_cast<const u32x2*>(x);
+                        vr[j][b][0] = y[0];
+                        vr[j][b][1] = y[1];
+                    } else {
+                        vr[j][b][0] = *reinterpret_cast<const uint32_t*>(x);
+                    }
+                }
+            if constexpr (TYPE == KQ_TYPE_I8) {
+#pragma unroll
+                for (int t = 0; t < 2 * NS; t++) {
+                    if constexpr (TILED) {
+                        const F4 x = *reinterpret_cast<const F4*>(a.vs + sp[t] + 4 * g);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) vsr[4 * t + j] = x.v[j];
+                    } else {
+                        vsr[t] = a.vs[sp[t]];
+                    }
                 }
             }
-        if constexpr (TYPE == KQ_TYPE_I8) {
+        };
+
+        int kb = k0 + KEYS * wave;
+        if (kb < k1) {
+            fetch(kb);
+            load_k(kb);
+            load_v();
+            if (kb + KEYS * NW < k1) fetch(kb + KEYS * NW);
+        }
+
+        u32x4* const ql = reinterpret_cast<u32x4*>(lds);
+        {
+            float inv = 1.0f, f = 1.0f, top = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
-                if constexpr (TILED) {
-                    const F4 x = *reinterpret_cast<const F4*>(a.vs + sp[t] + 4 * g);
+            for (int o = 0; o < QO; o++)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) vsr[4 * t + j] = x.v[j];
-                } else {
-                    vsr[t] = a.vs[sp[t]];
+                for (int e = 0; e < 4; e++) {
+                    qv[o][0][e] *= a.qscale;
+                    qv[o][1][e] *= a.qscale;
+                    top = fmaxf(top, fmaxf(fabsf(qv[o][0][e]), fabsf(qv[o][1][e])));
                 }
+            if constexpr (NP == 2) {
+                // the row times a power of two, its largest value from 2^13 to 2^14
+#pragma unroll
+                for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
+                if (top > 0.0f && top < INFINITY) {
+                    const int e = min(126, 140 - (int)(__float_as_uint(top) >> 23));
+                    f = __uint_as_float((uint32_t)(127 + e) << 23);
+                    inv = __uint_as_float((uint32_t)(127 - e) << 23);
+                }
+                if (c == 0) s_inv[qr] = inv;
+            }
+#pragma unroll
+            for (int o = 0; o < QO; o++) {
+                if (DM % 128 && c + 16 * o >= DM / 8) continue;
+                u32x4 w[NP];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    uint32_t p[NP];
+                    split<NP>(qv[o][e >> 1][2 * (e & 1)] * f, qv[o][e >> 1][2 * (e & 1) + 1] * f, p);
+#pragma unroll
+                    for (int j = 0; j < NP; j++) w[j][e] = p[j];
+                }
+#pragma unroll
+                for (int j = 0; j < NP; j++) ql[(j * (DM / 8) + c + 16 * o) * 16 + qr] = w[j];
             }
         }
-    };
+        __syncthreads();
 
-    int kb = k0 + 32 * wave;
-    const bool any = kb < k1;
-    if (any) {
-        fetch(kb);
-        load_k(kb);
-        load_v();
-        if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
-    }
-
-    uint32_t* const ql = reinterpret_cast<uint32_t*>(lds);
-#pragma unroll
-    for (int i = 0; i < QP; i++) {
-        const int r = (tid >> 4) + 4 * NW * i;
-        if (r >= 16 * RT) continue;
-        float inv = 1.0f, f = 1.0f;
-        float top = 0.0f;
-#pragma unroll
-        for (int o = 0; o < QO; o++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                qv[i][o][0][e] *= a.qscale;
-                qv[i][o][1][e] *= a.qscale;
-                top = fmaxf(top, fmaxf(fabsf(qv[i][o][0][e]), fabsf(qv[i][o][1][e])));
-            }
-        if constexpr (NP == 2) {
-            // the row times a power of two, its largest value from 2^13 to 2^14
-#pragma unroll
-            for (int off = 1; off < 16; off <<= 1) top = fmaxf(top, __shfl_xor(top, off));
-            if (top > 0.0f && top < INFINITY) {
-                const int e = min(126, 140 - (int)(__float_as_uint(top) >> 23));
-                f = __uint_as_float((uint32_t)(127 + e) << 23);
-                inv = __uint_as_float((uint32_t)(127 - e) << 23);
-            }
-            if (c == 0) s_inv[r] = inv;
+        // ---- the lane's row (those behind the last see everything: their sums are nobody's)
+        {
+            const int last = len - n + (first + c) / G;
+            lo = c < live && a.window ? last + 1 - a.window : 0;
+            hi = c < live ? min(last + 1, k1) : k1;
         }
-#pragma unroll
-        for (int o = 0; o < QO; o++) {
-            if (DM % 128 && c + 16 * o >= DM / 8) continue;
-            u32x4 w[NP];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                uint32_t p[NP];
-                split<NP>(qv[i][o][e >> 1][2 * (e & 1)] * f, qv[i][o][e >> 1][2 * (e & 1) + 1] * f, p);
-#pragma unroll
-                for (int j = 0; j < NP; j++) w[j][e] = p[j];
-            }
-#pragma unroll
-            for (int j = 0; j < NP; j++)
-                reinterpret_cast<u32x4*>(ql)[((j * RT + r / 16) * (DM / 8) + c + 16 * o) * 16 + r % 16] = w[j];
-        }
-    }
-    __syncthreads();
-
-    // ---- rows of this lane
-    float inv[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        const int row = first + 16 * rt + c, last = len - n + row / G;
-        // (rows behind the last one see everything: their sums are nobody's)
-        lo[rt] = row < rows && a.window ? last + 1 - a.window : 0;
-        hi[rt] = row < rows ? min(last + 1, k1) : k1;
-        inv[rt] = NP == 2 ? s_inv[16 * rt + c] : 1.0f;
-        m[rt] = -INFINITY;
-        l[rt] = 0.0f;
+        const float inv = NP == 2 ? s_inv[c] : 1.0f;
+        m = -INFINITY;
+        l = 0.0f;
+        ve = 0;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int t = 0; t < W; t++) acc[rt][b][t] = (f32x4)0.0f;
-    }
-    ve = 0;
-    // steps within [all_lo, all_hi) are seen by all rows
-    const int row_n = min(rows, first + 16 * RT) - 1;
-    const int all_hi = min(k1, len - n + first / G + 1);
-    const int all_lo = a.window ? len - n + row_n / G + 1 - a.window : 0;
+            for (int t = 0; t < W; t++) acc[b][t] = (f32x4)0.0f;
+        // keys within [all_lo, all_hi) are seen by all rows
+        const int all_hi = min(k1, len - n + first / G + 1);
+        const int all_lo = a.window ? len - n + (first + live - 1) / G + 1 - a.window : 0;
 
-    // ---- steps
+        // ---- steps
 #pragma unroll 1
-    for (; kb < k1; kb += 32 * NW) {
-        const bool ok0 = have[0], ok1 = have[1];
-        const bool full = TILED ? kb >= all_lo && kb + 32 <= all_hi && ok0 && ok1
-                                : kb >= all_lo && kb + 32 <= all_hi && __all(ok0 && ok1);
-        // (read in each step: the compiler would keep more queries than there are registers)
-        uint32_t qat = lane;
-        if constexpr (DM * RT > 128) asm volatile("" : "+v"(qat));
-        f32x4 sc[RT][2];
+        for (; kb < k1; kb += KEYS * NW) {
+            bool ok[2 * NS], all_ok = true;
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) sc[rt][0] = sc[rt][1] = (f32x4)0.0f;
-#pragma unroll
-        for (int ch = 0; ch < NCH; ch++) {
-            if (!EXACT && 32 * ch >= D) continue;
-            u32x4 x[2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                x[t] = kr[t][ch];
-                if constexpr (TYPE == KQ_TYPE_I8) {
-                    const uint32_t y0 = kr[t][ch][0], y1 = kr[t][ch][1];
-                    x[t][0] = halves(perm(0, y0, 0x0c010c00));
-                    x[t][1] = halves(perm(0, y0, 0x0c030c02));
-                    x[t][2] = halves(perm(0, y1, 0x0c010c00));
-                    x[t][3] = halves(perm(0, y1, 0x0c030c02));
-                }
-                if (!EXACT && !octet(ch)) x[t] = (u32x4)0u;
+            for (int t = 0; t < 2 * NS; t++) {
+                ok[t] = have[t];
+                all_ok &= ok[t];
             }
+            const bool full = kb >= all_lo && kb + KEYS <= all_hi && (TILED ? all_ok : __all(all_ok));
+            // (queries are read in each step: the compiler would keep them in registers)
+            uint32_t qat = WIDE ? 32 * g + c : lane;
+            asm volatile("" : "+v"(qat));
+            f32x4 sc[2 * NS];
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
+            for (int t = 0; t < 2 * NS; t++) sc[t] = (f32x4)0.0f;
+#pragma unroll
+            for (int ch = 0; ch < NCH; ch++) {
+                if (!EXACT && 32 * ch >= D) continue;
+                u32x4 x[2 * NS];
+#pragma unroll
+                for (int t = 0; t < 2 * NS; t++) {
+                    if constexpr (TYPE == KQ_TYPE_I8) {
+                        const uint32_t y0 = WIDE ? kr[t][ch / 2][2 * (ch & 1)] : kr[t][ch][0];
+                        const uint32_t y1 = WIDE ? kr[t][ch / 2][2 * (ch & 1) + 1] : kr[t][ch][1];
+                        x[t][0] = halves(perm(0, y0, 0x0c010c00));
+                        x[t][1] = halves(perm(0, y0, 0x0c030c02));
+                        x[t][2] = halves(perm(0, y1, 0x0c010c00));
+                        x[t][3] = halves(perm(0, y1, 0x0c030c02));
+                    } else {
+                        x[t] = kr[t][ch];
+                    }
+                    if (!EXACT && !octet(ch)) x[t] = (u32x4)0u;
+                }
+                // (a lane's 8 values of chunk ch are the (4 ch + g)th of the row, WIDE: the
+                // (8 (ch / 2) + 2 g + ch % 2)th)
 #pragma unroll
                 for (int j = 0; j < NP; j++) {
-                    const u32x4 y = reinterpret_cast<const u32x4*>(ql)[((j * RT + rt) * (DM / 8) + 4 * ch) * 16 + qat];
-                    sc[rt][0] = mfma<NP>(x[0], y, sc[rt][0]);
-                    sc[rt][1] = mfma<NP>(x[1], y, sc[rt][1]);
+                    const u32x4 y = ql[(j * (DM / 8) + (WIDE ? 8 * (ch / 2) + (ch & 1) : 4 * ch)) * 16 + qat];
+#pragma unroll
+                    for (int t = 0; t < 2 * NS; t++) sc[t] = mfma<NP>(x[t], y, sc[t]);
                 }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        float kscale[8], vscale[8];
-        if constexpr (TYPE == KQ_TYPE_I8) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                kscale[j] = TILED ? ksr[j] : __shfl(ksr[j >> 2], 4 * g + (j & 3));
-                vscale[j] = TILED ? vsr[j] : __shfl(vsr[j >> 2], 4 * g + (j & 3));
             }
-        }
-        // which of the lane's keys are there at all, bit j: key 16 (j / 4) + 4 g + j % 4
-        uint32_t there = 0xff;
-        if (!full) {
-            uint32_t p;
-            if constexpr (TILED) {
-                p = (ok0 ? 0x0f : 0) | (ok1 ? 0xf0 : 0);
-            } else {
-                const unsigned long long b0 = __ballot(ok0), b1 = __ballot(ok1);
-                p = (uint32_t)((b0 >> (4 * g)) & 15) | (uint32_t)((b1 >> (4 * g)) & 15) << 4;
-            }
-            there = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-                if (key < k1 && (p >> j & 1)) there |= 1u << j;
-            }
+            __builtin_amdgcn_sched_barrier(0);
+            float kscale[8 * NS], vscale[8 * NS];
             if constexpr (TYPE == KQ_TYPE_I8) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) vscale[j] = there >> j & 1 ? vscale[j] : 0.0f;
+                for (int j = 0; j < 8 * NS; j++) {
+                    kscale[j] = TILED ? ksr[j] : __shfl(ksr[j >> 2], 4 * g + (j & 3));
+                    vscale[j] = TILED ? vsr[j] : __shfl(vsr[j >> 2], 4 * g + (j & 3));
+                }
             }
-        }
-        // the next step's keys are asked for as soon as this one's are used
-        const int nb = kb + 32 * NW;
-        if (nb < k1) {
-            load_k(nb);
-            if (nb + 32 * NW < k1) fetch(nb + 32 * NW);
-        }
-        // weights
-        if constexpr (TYPE == KQ_TYPE_I8) {
-            // the sums are kept times a power of two that is near the largest scale so far
-            float top = fabsf(vscale[0]);
+            // which of the lane's keys are there at all, bit j: key 16 (j / 4) + 4 g + j % 4
+            uint32_t there = (1u << 8 * NS) - 1;
+            if (!full) {
+                uint32_t p = 0;
 #pragma unroll
-            for (int j = 1; j < 8; j++) top = fmaxf(top, fabsf(vscale[j]));
-            const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
-            if (e > ve) {
-                const float f = ve ? __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23) : 0.0f;
-                ve = e;
+                for (int t = 0; t < 2 * NS; t++)
+                    p |= (TILED ? (ok[t] ? 15u : 0u) : (uint32_t)(__ballot(ok[t]) >> (4 * g)) & 15u) << (4 * t);
+                there = 0;
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
+                for (int j = 0; j < 8 * NS; j++) {
+                    const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
+                    if (key < k1 && (p >> j & 1)) there |= 1u << j;
+                }
+                if constexpr (TYPE == KQ_TYPE_I8) {
+#pragma unroll
+                    for (int j = 0; j < 8 * NS; j++) vscale[j] = there >> j & 1 ? vscale[j] : 0.0f;
+                }
+            }
+            // the next step's keys are asked for as soon as this one's are used
+            const int nb = kb + KEYS * NW;
+            if (nb < k1) {
+                load_k(nb);
+                if (nb + KEYS * NW < k1) fetch(nb + KEYS * NW);
+            }
+            // weights
+            if constexpr (TYPE == KQ_TYPE_I8) {
+                // the sums are kept times a power of two that is near the largest scale so far
+                float top = fabsf(vscale[0]);
+#pragma unroll
+                for (int j = 1; j < 8 * NS; j++) top = fmaxf(top, fabsf(vscale[j]));
+                const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
+                if (e > ve) {
+                    const float f = ve ? __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23) : 0.0f;
+                    ve = e;
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
-                        for (int t = 0; t < W; t++) acc[rt][b][t] *= f;
+                        for (int t = 0; t < W; t++) acc[b][t] *= f;
+                }
+                const float f = __uint_as_float((uint32_t)(254 - max(1, ve)) << 23);
+#pragma unroll
+                for (int j = 0; j < 8 * NS; j++) vscale[j] *= f;
             }
-            const float f = __uint_as_float((uint32_t)(254 - max(1, ve)) << 23);
+            float x[8 * NS];
 #pragma unroll
-            for (int j = 0; j < 8; j++) vscale[j] *= f;
-        }
-        float x[RT][8], top[RT];
-        bool far = false;
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                x[rt][j] = sc[rt][j >> 2][j & 3];
-                if constexpr (NP == 2) x[rt][j] *= inv[rt];
-                if constexpr (TYPE == KQ_TYPE_I8) x[rt][j] *= kscale[j];
+            for (int j = 0; j < 8 * NS; j++) {
+                x[j] = sc[j >> 2][j & 3];
+                if constexpr (NP == 2) x[j] *= inv;
+                if constexpr (TYPE == KQ_TYPE_I8) x[j] *= kscale[j];
             }
             if (!full) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < 8 * NS; j++) {
                     const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
-                    x[rt][j] = key >= lo[rt] && key < hi[rt] && (there >> j & 1) ? x[rt][j] : -INFINITY;
+                    x[j] = key >= lo && key < hi && (there >> j & 1) ? x[j] : -INFINITY;
                 }
             }
-            top[rt] = x[rt][0];
+            float top = x[0];
 #pragma unroll
-            for (int j = 1; j < 8; j++) top[rt] = fmaxf(top[rt], x[rt][j]);
-            top[rt] = max4(top[rt]);
-            far |= top[rt] > m[rt] + 5.0f;
-        }
-        // (2^5 above the maximum that the weights are taken from before that is moved)
-        if (__any(far)) {
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                const float nm = fmaxf(m[rt], top[rt]), f = nm == -INFINITY ? 1.0f : exp2_(m[rt] - nm);
-                m[rt] = nm;
-                l[rt] *= f;
+            for (int j = 1; j < 8 * NS; j++) top = fmaxf(top, x[j]);
+            top = max4(top);
+            // (2^5 above the maximum that the weights are taken from before that is moved)
+            if (__any(top > m + 5.0f)) {
+                const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.0f : exp2_(m - nm);
+                m = nm;
+                l *= f;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int t = 0; t < W; t++) acc[rt][b][t] *= f;
+                    for (int t = 0; t < W; t++) acc[b][t] *= f;
             }
-        }
-        u32x4 w[RT][NP];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
             // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
             // with int8 values' scales below 2^16)
-            const float base = (m[rt] == -INFINITY ? 0.0f : m[rt]) - (NP == 2 ? 9.0f : 0.0f);
-            float sum = 0.0f;
+            u32x4 w[NS][NP];
+            const float base = (m == -INFINITY ? 0.0f : m) - (NP == 2 ? 9.0f : 0.0f);
 #pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                float p = exp2_(x[rt][j] - base), q = exp2_(x[rt][j + 1] - base);
-                sum += p + q;
+            for (int j = 0; j < 8 * NS; j += 2) {
+                float p = exp2_(x[j] - base), q = exp2_(x[j + 1] - base);
+                l += p + q;
                 if constexpr (TYPE == KQ_TYPE_I8) {
                     p *= vscale[j];
                     q *= vscale[j + 1];
@@ -524,95 +506,107 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
                 uint32_t o[NP];
                 split<NP>(p, q, o);
 #pragma unroll
-                for (int e = 0; e < NP; e++) w[rt][e][j >> 1] = o[e];
+                for (int e = 0; e < NP; e++) w[j >> 3][e][j >> 1 & 3] = o[e];
             }
-            l[rt] += sum;
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        // values
-        if (!full) {
+            __builtin_amdgcn_sched_barrier(0);
+            // values
+            if (!full) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const uint32_t keep = there >> j & 1 ? 0xffffffffu : 0u;
+                for (int j = 0; j < 8 * NS; j++) {
+                    const uint32_t keep = there >> j & 1 ? 0xffffffffu : 0u;
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int e = 0; e < VW; e++) vr[j][b][e] &= keep;
-            }
-        }
-        auto operand = [&](const u32x4 (&x)[8][NB], int b, int t) {
-            u32x4 o;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if constexpr (ES == 2) {
-                    o[j] = perm(x[2 * j + 1][b][t >> 1], x[2 * j][b][t >> 1], t & 1 ? 0x07060302 : 0x05040100);
-                } else {
-                    const uint32_t e = t & 3;
-                    o[j] = halves(perm(x[2 * j + 1][b][t >> 2], x[2 * j][b][t >> 2], 0x0c000c00u | e | (4 + e) << 16));
+                        for (int e = 0; e < VW; e++) vr[j][b][e] &= keep;
                 }
             }
-            return o;
-        };
-        if (ES == 2 && careful) {
-            constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
+            if (ES == 2 && careful) {
+                constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
 #pragma unroll
-            for (int j = 0; j < 8; j++)
+                for (int j = 0; j < 8 * NS; j++)
 #pragma unroll
-                for (int b = 0; b < NB; b++)
+                    for (int b = 0; b < NB; b++)
 #pragma unroll
-                    for (int e = 0; e < VW; e++) {
-                        const uint32_t v = vr[j][b][e];
-                        if ((v & 0x7fff) >= NONE) vr[j][b][e] &= 0xffff0000u;
-                        if ((v >> 16 & 0x7fff) >= NONE) vr[j][b][e] &= 0xffffu;
-                    }
-        }
-#pragma unroll
-        for (int b = 0; b < NB; b++) {
-            if (!EXACT && 16 * W * b >= D) continue;
-#pragma unroll
-            for (int t = 0; t < W; t++) {
-                const u32x4 x = operand(vr, b, t);
-#pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-                    for (int j = 0; j < NP; j++) acc[rt][b][t] = mfma<NP>(x, w[rt][j], acc[rt][b][t]);
-                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                        for (int e = 0; e < VW; e++) {
+                            const uint32_t v = vr[j][b][e];
+                            if ((v & 0x7fff) >= NONE) vr[j][b][e] &= 0xffff0000u;
+                            if ((v >> 16 & 0x7fff) >= NONE) vr[j][b][e] &= 0xffffu;
+                        }
             }
-        }
-        if (nb < k1) load_v();
-    }
-
-    float none = 0.0f;
-    if constexpr (ES == 2) {
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++)
+            for (int b = 0; b < NB; b++) {
+                if (!EXACT && 16 * W * b >= D) continue;
+#pragma unroll
+                for (int t = 0; t < W; t++) {
+#pragma unroll
+                    for (int i = 0; i < NS; i++) {
+                        u32x4 v;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            const u32x4 v0 = vr[8 * i + 2 * j][b], v1 = vr[8 * i + 2 * j + 1][b];
+                            if constexpr (ES == 2)
+                                v[j] = perm(v1[t >> 1], v0[t >> 1], t & 1 ? 0x07060302 : 0x05040100);
+                            else
+                                v[j] = halves(perm(v1[t >> 2], v0[t >> 2], 0x0c000c00u | (t & 3) | (4 + (t & 3)) << 16));
+                        }
+#pragma unroll
+                        for (int j = 0; j < NP; j++) acc[b][t] = mfma<NP>(v, w[i][j], acc[b][t]);
+                    }
+                    // (in few registers: the compiler would make all operands first)
+                    if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (nb < k1) load_v();
+        }
+
+        float none = 0.0f;
+        if constexpr (ES == 2) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int t = 0; t < W; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) none = fmaf(acc[rt][b][t][i], 0.0f, none);
-    }
-    // (a barrier: queries have been read)
-    if (!__syncthreads_or(none != 0.0f) || careful) break;
-    careful = true;
+                    for (int i = 0; i < 4; i++) none = fmaf(acc[b][t][i], 0.0f, none);
+        }
+        // (a barrier: queries have been read)
+        if (!__syncthreads_or(none != 0.0f) || careful) break;
+        careful = true;
     }
 
     // ---- the waves' sums
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        l[rt] = sum4(l[rt]);
-        if (g == 0) s_ml[wave][16 * rt + c] = make_float2(m[rt], l[rt]);
-    }
+    l = sum4(l);
+    if (g == 0) s_ml[wave][c] = make_float2(m, l);
     __syncthreads();
     float* const ol = reinterpret_cast<float*>(lds);
-    const int64_t prow = ((int64_t)(part + idx) * a.n_kv + h) * a.R + first;
-    // (row of the workgroup, value)
+    const int quads = D / 4;
+    {
+        float top = s_ml[0][c].x, sum = 0.0f;
+#pragma unroll
+        for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][c].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        if (tid < 16) {
+#pragma unroll
+            for (int i = 0; i < NW; i++) sum += s_ml[i][c].y * exp2_(s_ml[i][c].x - base);
+            s_all[c] = make_float2(top, sum);
+        }
+        float f = exp2_(m - base);
+        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)max(1, ve) << 23);
+        if (c < live) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int t = 0; t < W; t += 4)
+                        *reinterpret_cast<f32x4*>(ol + (wave * 16 + c) * OS + 16 * W * b + W * (4 * g + i) + t) =
+                            (f32x4){acc[b][t][i], acc[b][t + 1][i], acc[b][t + 2][i], acc[b][t + 3][i]} * f;
+        }
+    }
+    __syncthreads();
     auto store_out = [&](int r, int d, f32x4 y) {
-        const int row = first + r;
-        const int64_t tok = (int64_t)row0 + row / G;
+        const int64_t tok = (int64_t)row0 + (first + r) / G;
         if (tok >= 0 && tok < a.N)
-            *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + row % G) * D + d) = y;
+            *reinterpret_cast<f32x4*>(a.out + tok * a.out_stride + (int64_t)(h * G + (first + r) % G) * D + d) = y;
     };
     // (row of the partial results)
     auto put = [](void* p, float lo, float hi) {
@@ -623,81 +617,49 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         put(a.part + row * D + d, y[0], y[1]);
         put(a.part + row * D + d + 2, y[2], y[3]);
     };
-    if (tid < 16 * RT) {
-        float top = s_ml[0][tid].x, sum = 0.0f;
+    const int64_t prow = ((int64_t)(part + idx) * a.n_kv + h) * a.R + first;
+    for (int e = tid; e < live * quads; e += 64 * NW) {
+        const int r = e / quads, d = e % quads * 4;
+        f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
 #pragma unroll
-        for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][tid].x);
-        const float base = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int i = 0; i < NW; i++) sum += s_ml[i][tid].y * exp2_(s_ml[i][tid].x - base);
-        s_all[tid] = make_float2(top, sum);
-    }
-    const int quads = D / 4;
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-        if (first + 16 * rt >= rows) continue;
-        float top = s_ml[0][16 * rt + c].x;
-#pragma unroll
-        for (int i = 1; i < NW; i++) top = fmaxf(top, s_ml[i][16 * rt + c].x);
-        float f = exp2_(m[rt] - (top == -INFINITY ? 0.0f : top));
-        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)max(1, ve) << 23);
-        const int here = min(16, rows - first - 16 * rt);
-        if (rt) __syncthreads();
-        if (c < here) {
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++)
-#pragma unroll
-                    for (int t = 0; t < W; t += 4)
-                        *reinterpret_cast<f32x4*>(ol + (wave * 16 + c) * OS + 16 * W * b + W * (4 * g + i) + t) =
-                            (f32x4){acc[rt][b][t][i], acc[rt][b][t + 1][i], acc[rt][b][t + 2][i], acc[rt][b][t + 3][i]} * f;
-        }
-        __syncthreads();
-        for (int e = tid; e < here * quads; e += 64 * NW) {
-            const int r = e / quads, d = e % quads * 4;
-            f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
-#pragma unroll
-            for (int i = 1; i < NW; i++) y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
-            if (ES == 2 && careful) {
-                // values that are no numbers, for the rows that see them
-                const int last = len - n + (first + 16 * rt + r) / G, end = min(last + 1, k1);
+        for (int i = 1; i < NW; i++) y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
+        if (ES == 2 && careful) {
+            // values that are no numbers, for the rows that see them
+            const int last = len - n + (first + r) / G, end = min(last + 1, k1);
 #pragma unroll 1
-                for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
-                    const int page = table[key / a.page];
-                    if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                    const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b + 2 * d);
+            for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
+                const int page = table[key / a.page];
+                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
+                const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b + 2 * d);
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float z = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
-                        y[i] += __builtin_isfinite(z) ? 0.0f : z;
-                    }
+                for (int i = 0; i < 4; i++) {
+                    const float v = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
+                    y[i] += __builtin_isfinite(v) ? 0.0f : v;
                 }
             }
-            const float2 all = s_all[16 * rt + r];
-            if (num == 1) {
-                store_out(16 * rt + r, d, all.y == 0.0f ? (f32x4)0.0f : y / all.y);
-            } else {
-                store_part(prow + 16 * rt + r, d, y);
-                if (d == 0) put(a.ml + prow + 16 * rt + r, all.x, all.y);
-            }
+        }
+        const float2 all = s_all[r];
+        if (num == 1) {
+            store_out(r, d, all.y == 0.0f ? (f32x4)0.0f : y / all.y);
+        } else {
+            store_part(prow + r, d, y);
+            if (d == 0) put(a.ml + prow + r, all.x, all.y);
         }
     }
     if (num == 1) return;
 
-    // ---- partial results are joined by the last workgroup of each eight, theirs by the
-    // last of these.  Results and counts are device-scope atomics, which go past the
-    // caches that another XCD does not see: once a wave's stores are acknowledged they are
-    // there for all, and the barrier puts every wave's before the count.  (A release fence
-    // instead writes back the L2, in each of hundreds of workgroups: 64 ragged streams
-    // took 233 us with it, 124 without.)
-    const int live = min(rows - first, 16 * RT);
-    auto last_of = [&](int slot, int n) {
+    // ---- Partial results are joined by the last workgroup, or, where that would be long, by
+    // the last of each eight and theirs by the last of these.  Results and counts are
+    // device-scope atomics, which go past the caches that another XCD does not see: once
+    // a wave's stores are acknowledged they are there for all, and the barrier puts every
+    // wave's before the count.  (A release fence instead writes back the L2, in each of
+    // hundreds of workgroups: 64 ragged streams took 233 us with it, 124 without.)
+    auto last_of = [&](int slot, int of) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (tid == 0) {
-            int* const p = a.counter + ((int64_t)(part + slot) * a.n_kv + h) * gridDim.z + blockIdx.z;
-            s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+            int* const p = a.counter + ((int64_t)(part + slot) * a.n_kv + h) * a.blocks + z;
+            s_last = __hip_atomic_fetch_add(p, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == of - 1;
             if (s_last) __hip_atomic_store(p, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
         __syncthreads();
@@ -707,9 +669,10 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
         const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
     };
-    constexpr int JU = RT * DM >= 256 ? 4 : 2;   // quads of values that a lane has in flight
+    // JU quads of JN results that a lane has in flight
+    constexpr int JU = 2, JN = 8, FLAT = 12288;
     // n results, `by` apart from slot `from` on, to the first's place or, `end`, to out
-    auto join = [&](int from, int by, int n, bool end) {
+    auto join = [&](int from, int by, int of, bool end) {
         const int64_t row1 = ((int64_t)(part + from) * a.n_kv + h) * a.R + first, step = (int64_t)by * a.n_kv * a.R;
         for (int e0 = tid; e0 < live * quads; e0 += 64 * NW * JU) {
             f32x4 y[JU];
@@ -721,14 +684,14 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
                 sum[u] = 0.0f;
             }
 #pragma unroll 1
-            for (int i0 = 0; i0 < n; i0 += 8) {
-                float2 t[JU][8], o[JU][8][2];
+            for (int i0 = 0; i0 < of; i0 += JN) {
+                float2 t[JU][JN], o[JU][JN][2];
 #pragma unroll
                 for (int u = 0; u < JU; u++) {
                     const int e = min(e0 + 64 * NW * u, live * quads - 1), r = e / quads, d = e % quads * 4;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const int64_t at = row1 + r + min(i0 + i, n - 1) * step;
+                    for (int i = 0; i < JN; i++) {
+                        const int64_t at = row1 + r + min(i0 + i, of - 1) * step;
                         t[u][i] = get(a.ml + at);
                         o[u][i][0] = get(a.part + at * D + d);
                         o[u][i][1] = get(a.part + at * D + d + 2);
@@ -738,15 +701,15 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
                 for (int u = 0; u < JU; u++) {
                     float nm = top[u];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) nm = fmaxf(nm, t[u][i].x);
+                    for (int i = 0; i < JN; i++) nm = fmaxf(nm, t[u][i].x);
                     const float base = nm == -INFINITY ? 0.0f : nm, f = exp2_(top[u] - base);
                     top[u] = nm;
                     y[u] *= f;
                     sum[u] *= f;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) {
+                    for (int i = 0; i < JN; i++) {
                         const float w = exp2_(t[u][i].x - base);
-                        if (i0 + i < n) {
+                        if (i0 + i < of) {
                             y[u] += (f32x4){o[u][i][0].x, o[u][i][0].y, o[u][i][1].x, o[u][i][1].y} * w;
                             sum[u] += t[u][i].y * w;
                         }
@@ -761,48 +724,30 @@ __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(DM * RT
                     store_out(r, d, sum[u] == 0.0f ? (f32x4)0.0f : y[u] / sum[u]);
                 } else {
                     store_part(row1 + r, d, y[u]);
-                    if (d == 0) s_ml[0][r] = make_float2(top[u], sum[u]);
+                    if (d == 0) s_all[r] = make_float2(top[u], sum[u]);
                 }
             }
         }
         if (end) return;
         __syncthreads();                    // (all lanes have read the maximum and sum of their row)
-        if (tid < live) put(a.ml + row1 + tid, s_ml[0][tid].x, s_ml[0][tid].y);
+        if (tid < live) put(a.ml + row1 + tid, s_all[tid].x, s_all[tid].y);
     };
-    const int group = idx & ~7, of = min(8, num - group);
+    const bool flat = num <= 8 || live * quads * num <= FLAT;
+    const int group = flat ? 0 : idx & ~7, of = flat ? num : min(8, num - group);
     if (!last_of(group, of)) return;
-    join(group, 1, of, num <= 8);
-    if (num > 8 && last_of(1, (num + 7) / 8)) join(0, 8, (num + 7) / 8, true);
+    join(group, 1, of, flat);
+    if (!flat && last_of(1, (num + 7) / 8)) join(0, 8, (num + 7) / 8, true);
 }
 
 typedef void (*Kernel)(AttnArg);
 
-// Waves of a workgroup, and tiles of rows at most: a lane holds 64 registers of keys
-// and values and 32 of sums a tile for each 128 values of a head.
-template <int DM, int RT> constexpr int NWV = 4;
-constexpr int most_tiles(int D) { return D > 128 ? 2 : 4; }
-
-template <int TYPE, int DM, bool EXACT, bool TILED>
-Kernel by_rows(int rt, int* nw) {
-    constexpr int M = most_tiles(DM);
-    *nw = rt == 1 ? NWV<DM, 1> : rt == 2 ? NWV<DM, 2> : NWV<DM, M>;
-    return rt == 1   ? kq_attn_kernel<TYPE, DM, EXACT, TILED, 1, NWV<DM, 1>>
-           : rt == 2 ? kq_attn_kernel<TYPE, DM, EXACT, TILED, 2, NWV<DM, 2>>
-                     : kq_attn_kernel<TYPE, DM, EXACT, TILED, M, NWV<DM, M>>;
-}
-
 template <int TYPE>
-Kernel pick(int D, bool tiled, int rt, int* nw) {
-    if (!tiled) return D <= 128 ? by_rows<TYPE, 128, false, false>(rt, nw) : by_rows<TYPE, 256, false, false>(rt, nw);
-    if (D == 64) return by_rows<TYPE, 64, true, true>(rt, nw);
-    if (D == 128) return by_rows<TYPE, 128, true, true>(rt, nw);
-    if (D == 256) return by_rows<TYPE, 256, true, true>(rt, nw);
-    return D < 128 ? by_rows<TYPE, 128, false, true>(rt, nw) : by_rows<TYPE, 256, false, true>(rt, nw);
-}
-
-int tiles(const kq_attn_shape* s) {
-    const int rows = s->T * (s->n_q / s->n_kv);
-    return rows <= 16 ? 1 : rows <= 32 ? 2 : most_tiles(s->D);
+Kernel pick(int D, bool tiled) {
+    if (!tiled) return D <= 128 ? kq_attn_kernel<TYPE, 128, false, false> : kq_attn_kernel<TYPE, 256, false, false>;
+    if (D == 64) return kq_attn_kernel<TYPE, 64, true, true>;
+    if (D == 128) return kq_attn_kernel<TYPE, 128, true, true>;
+    if (D == 256) return kq_attn_kernel<TYPE, 256, true, true>;
+    return D < 128 ? kq_attn_kernel<TYPE, 128, false, true> : kq_attn_kernel<TYPE, 256, false, true>;
 }
 
 int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
@@ -812,10 +757,10 @@ int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 extern "C" {
 
 void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
-    const int rows = s->T * (s->n_q / s->n_kv), rb = 16 * tiles(s);
-    z->blocks = (rows + rb - 1) / rb;
+    z->blocks = (s->T * (s->n_q / s->n_kv) + 15) / 16;
     const int per = s->n_kv * z->blocks;
     z->budget = (2 * n_cu + per - 1) / per;
+    z->few = 32 * n_cu / per;
     z->cap = s->S + z->budget;
     z->parts = 2 * z->budget;
     z->counters = (int64_t)z->parts * per;
@@ -875,13 +820,16 @@ int kqk_launch_attn(const kq_paged_attn* p, const kqk_attn_sizes* z, void* work,
         a.part = (float*)work;
         a.ml = (float2*)((uint8_t*)work + up256(rows * s.D * 4));
     }
-    int nw = 0;
-    const int rt = tiles(&s);
-    const Kernel k = c.type == KQ_TYPE_F16    ? pick<KQ_TYPE_F16>(s.D, tiled, rt, &nw)
-                     : c.type == KQ_TYPE_BF16 ? pick<KQ_TYPE_BF16>(s.D, tiled, rt, &nw)
-                                              : pick<KQ_TYPE_I8>(s.D, tiled, rt, &nw);
-    const dim3 grid((unsigned)(p->list ? z->cap : s.S), (unsigned)s.n_kv, (unsigned)z->blocks);
-    hipLaunchKernelGGL(k, grid, dim3(64 * nw), 0, st, a);
+    const Kernel k = c.type == KQ_TYPE_F16    ? pick<KQ_TYPE_F16>(s.D, tiled)
+                     : c.type == KQ_TYPE_BF16 ? pick<KQ_TYPE_BF16>(s.D, tiled)
+                                              : pick<KQ_TYPE_I8>(s.D, tiled);
+    // (below 2^23 workgroups, n_kv and blocks at most 2^10 and 2^8: exact)
+    a.blocks = z->blocks;
+    a.kv_div = (((uint64_t)1 << 40) + s.n_kv - 1) / s.n_kv;
+    a.blocks_div = (((uint64_t)1 << 40) + 8 * z->blocks - 1) / (8 * z->blocks);
+    const int64_t pairs = (int64_t)(p->list ? z->cap : s.S) * s.n_kv;
+    const dim3 grid((unsigned)((pairs + 7) / 8 * 8 * z->blocks));
+    hipLaunchKernelGGL(k, grid, dim3(64 * NW), 0, st, a);
     return (int)hipGetLastError();
 }
 

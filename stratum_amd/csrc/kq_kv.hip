@@ -24,7 +24,7 @@ constexpr int MOST = (1 << 30) - 1; // of a length
 
 struct PlanArg {
     kq_kv_plan p;
-    int budget, cap;
+    int budget, cap, few;           // (kqk_attn_sizes)
     int counters;
     int* items;                     // KQK_ITEM each
     int* count;
@@ -123,6 +123,13 @@ __device__ __forceinline__ uint32_t items_of(uint32_t keys, uint32_t share, uint
     return (keys + *per - 1) / *per;
 }
 
+__device__ __forceinline__ void put_item(const PlanArg& a, uint32_t at, int s, uint32_t from, uint32_t to, uint32_t num,
+                                         uint32_t idx, uint32_t part, uint32_t row, uint32_t fresh, uint32_t len) {
+    int4* const o = reinterpret_cast<int4*>(a.items + (int64_t)at * KQK_ITEM);
+    o[0] = make_int4(s, (int)from, (int)to, (int)(num << 16 | idx));
+    o[1] = make_int4((int)part, (int)row, (int)fresh, (int)len);
+}
+
 __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
     __shared__ uint32_t sm[3][PT / 64][4];
     __shared__ uint32_t first_tok[PT], first_page[PT], first_item[PT], s_cached[PT], s_held[PT], s_from[PT],
@@ -147,7 +154,7 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
         uint32_t n = (uint32_t)((double)total / (double)a.budget);
         while ((uint64_t)n * (uint32_t)a.budget < total) n++;
-        share = min(share, max(64u, min(n, 0x3ffffffu) * 32));
+        share = min(share, max(total * 32 <= (uint64_t)a.few ? 128u : 256u, min(n, 0x3ffffffu) * 32));
     }
     uint32_t tok0 = 0, page0 = 0, taken = 0, shorts = 0, item0 = 0, part0 = 0;
     for (int s0 = 0; s0 < p.S; s0 += T) {
@@ -164,8 +171,14 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         wg_scan<4>(v2, sm[2], b2, n2);
         first_tok[tid] = b1[0];
         first_page[tid] = b1[1];
-        first_item[tid] = b2[0];
+        // (items: first those of sequences with several, which are the longer ones)
+        const uint32_t single = items == 1 ? 1 : 0;
+        first_item[tid] = b2[1];
         s_part[tid] = b2[1];
+        if (single) {
+            const uint32_t e = item0 + n2[1] + (b2[0] - b2[1]);
+            if (e < (uint32_t)a.cap) put_item(a, e, s, from, end, 1, 0, 0, tok0 + b1[0], q.fresh, end);
+        }
         s_cached[tid] = q.cached;
         s_held[tid] = q.held;
         s_from[tid] = from;
@@ -203,13 +216,11 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
                 p.slot[tok0 + t] = slot;
             }
         // the attention's items
-        for (uint32_t e = tid; e < n2[0] && item0 + e < (uint32_t)a.cap; e += T) {
+        for (uint32_t e = tid; e < n2[1] && item0 + e < (uint32_t)a.cap; e += T) {
             const int i = owner(first_item, n, e);
             const uint32_t idx = e - first_item[i], num = items_of(s_end[i] - s_from[i], share, &per);
-            int4* const o = reinterpret_cast<int4*>(a.items + (int64_t)(item0 + e) * KQK_ITEM);
-            o[0] = make_int4(s0 + i, (int)(s_from[i] + idx * per), (int)min(s_end[i], s_from[i] + (idx + 1) * per),
-                             (int)(num << 16 | idx));
-            o[1] = make_int4((int)(part0 + s_part[i]), (int)(tok0 + first_tok[i]), (int)s_fresh[i], (int)s_end[i]);
+            put_item(a, item0 + e, s0 + i, s_from[i] + idx * per, min(s_end[i], s_from[i] + (idx + 1) * per), num, idx,
+                     part0 + s_part[i], tok0 + first_tok[i], s_fresh[i], s_end[i]);
         }
         tok0 = plus(tok0, n1[0]);
         page0 = plus(page0, n1[1]);
@@ -319,6 +330,7 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
     if (p->list) {
         a.budget = z->budget;
         a.cap = z->cap;
+        a.few = z->few;
         a.counters = (int)z->counters;
         a.count = (int*)p->list;
         a.items = a.count + KQK_LIST_HEAD;

@@ -195,20 +195,23 @@ def test_list(S, T, n_kv, window, longest, new):
     count, items = lst[0], lst[8:8 + 8 * lst[0]].reshape(-1, 8)
     n, lens = np.maximum(a[1], 0), o["lens"][:S]
     want = [s for s in range(S) if 1 <= n[s] <= T]
-    at = part = 0
+    parts = []
     for s in want:
         lo = max(0, lens[s] - n[s] + 1 - window) & ~31 if window and lens[s] else 0
-        num = items[at][3] >> 16
-        for i in range(num):
-            it = items[at + i]
-            assert it[0] == s and it[1] == lo and it[3] == num << 16 | i and it[4] == part
+        mine = items[items[:, 0] == s]
+        num = len(mine)
+        assert num >= 1
+        if num > 1:
+            parts += range(mine[0][4], mine[0][4] + num)
+        for i, it in enumerate(mine):
+            assert it[1] == lo and it[3] == num << 16 | i and (num == 1 or it[4] == mine[0][4])
             assert it[5] == o["start"][s] and it[6] == n[s] and it[7] == lens[s]
             assert it[1] <= it[2] and (it[2] == lens[s]) == (i == num - 1) and it[1] % 32 == 0
             assert num == 1 or it[2] > it[1]
             lo = it[2]
-        at += num
-        part += num if num > 1 else 0
-    assert at == count
+    assert sorted(parts) == list(range(len(parts))) and sum(np.isin(items[:, 0], want)) == count
+    if S <= 1024:            # the longer ones first
+        assert (np.diff(((items[:, 3] >> 16) > 1).astype(int)) <= 0).all()
     used = 8 + 8 * count
     assert (lst[used:-8] >= -7).all() and ((lst[used:-8] == 0) | (lst[used:-8] == -7)).all()
 
