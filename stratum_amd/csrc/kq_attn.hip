@@ -759,10 +759,11 @@ extern "C" {
 void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
     z->blocks = (s->T * (s->n_q / s->n_kv) + 15) / 16;
     const int per = s->n_kv * z->blocks;
-    z->budget = (2 * n_cu + per - 1) / per;
+    const int one = (n_cu + per - 1) / per;       // items for a workgroup on each CU
     z->few = 32 * n_cu / per;
-    z->cap = s->S + z->budget;
-    z->parts = 2 * z->budget;
+    const int extra = 2 * one - s->S > one ? 2 * one - s->S : one;
+    z->cap = s->S + extra;
+    z->parts = 2 * extra;                         // (a split sequence has two items or more)
     z->counters = (int64_t)z->parts * per;
 }
 

@@ -24,7 +24,7 @@ constexpr int MOST = (1 << 30) - 1; // of a length
 
 struct PlanArg {
     kq_kv_plan p;
-    int budget, cap, few;           // (kqk_attn_sizes)
+    int cap, few;                   // (kqk_attn_sizes)
     int counters;
     int* items;                     // KQK_ITEM each
     int* count;
@@ -131,7 +131,7 @@ __device__ __forceinline__ void put_item(const PlanArg& a, uint32_t at, int s, u
 }
 
 __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
-    __shared__ uint32_t sm[3][PT / 64][4];
+    __shared__ uint32_t sm[8][PT / 64][4];
     __shared__ uint32_t first_tok[PT], first_page[PT], first_item[PT], s_cached[PT], s_held[PT], s_from[PT],
         s_end[PT], s_fresh[PT], s_part[PT];
     __shared__ bool s_ok[PT];
@@ -141,20 +141,41 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
     Seq q = load_seq(a, tid);
     for (int i = tid; i < a.counters; i += T) a.counter[i] = 0;
     uint32_t share = 0x7fffffc0u;
-    if (a.items && a.budget) {
-        // keys in units of 32, their lower and upper 16 bits
-        uint32_t units[2] = {0, 0}, before[2], all[2];
+    if (a.items) {
+        // The most keys that an item has: with keys / extra or more there are no more than
+        // `extra` items beyond one a sequence.  Keys in units of 32, their lower and upper
+        // 16 bits:
+        uint32_t units[3] = {0, 0, 0}, before[3], all[3];
         for (int s0 = 0; s0 < p.S; s0 += T) {
             const Seq r = s0 ? load_seq(a, s0 + tid) : q;
             const uint32_t n = r.attended ? (r.end - r.from + 31) / 32 : 0;
             units[0] += n & 0xffff;
             units[1] += n >> 16;
+            units[2] += r.attended;
         }
-        wg_scan<2>(units, sm[0], before, all);
+        wg_scan<3>(units, sm[0], before, all);
         const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
-        uint32_t n = (uint32_t)((double)total / (double)a.budget);
-        while ((uint64_t)n * (uint32_t)a.budget < total) n++;
-        share = min(share, max(total * 32 <= (uint64_t)a.few ? 128u : 256u, min(n, 0x3ffffffu) * 32));
+        const uint32_t extra = a.cap - p.S, cap = all[2] + extra;
+        auto over = [&](uint32_t n) {
+            uint32_t x = (uint32_t)((double)total / (double)n);
+            while ((uint64_t)x * n < total) x++;
+            return x;
+        };
+        const uint32_t least = total * 32 <= (uint64_t)a.few ? 4 : 8;
+        uint32_t most = max(least, min(over(extra), 0x3ffffffu));
+        if (p.S <= T) {
+            // fewer, where that gives no more items either, by bisection
+            uint32_t lo = max(least, min(over(cap), most));
+#pragma unroll 1
+            for (int i = 0; i < 5 && lo < most; i++) {
+                const uint32_t mid = (lo + most) / 2;
+                uint32_t per, v[1] = {q.attended ? items_of(q.end - q.from, 32 * mid, &per) : 0}, b1[1], n1[1];
+                wg_scan<1>(v, sm[3 + i], b1, n1);
+                if (n1[0] <= cap) most = mid;
+                else lo = mid + 1;
+            }
+        }
+        share = 32 * most;
     }
     uint32_t tok0 = 0, page0 = 0, taken = 0, shorts = 0, item0 = 0, part0 = 0;
     for (int s0 = 0; s0 < p.S; s0 += T) {
@@ -328,7 +349,6 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
     PlanArg a = {};
     a.p = *p;
     if (p->list) {
-        a.budget = z->budget;
         a.cap = z->cap;
         a.few = z->few;
         a.counters = (int)z->counters;

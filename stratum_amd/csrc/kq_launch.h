@@ -139,9 +139,8 @@ int kqk_launch_verify(const kq_spec_verify* v, void* work, hipStream_t st);
 #define KQK_LIST_HEAD 8
 #define KQK_ITEM 8
 typedef struct {
-    int budget;              /* items beyond one a sequence */
+    int cap;                 /* items at most */
     int few;                 /* keys up to which an item has 128 at least, and 256 beyond */
-    int cap;                 /* S + budget */
     int parts;               /* partial results at most: of sequences with several items */
     int blocks;              /* of query rows, in each sequence and head of keys */
     int64_t counters;
