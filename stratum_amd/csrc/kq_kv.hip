@@ -77,29 +77,26 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 
 // N sums (that stay at 2^32 - 1 from there on) over the lanes before each and over all.
 template <int N>
-__device__ __forceinline__ void wg_scan(const uint32_t (&v)[N], uint32_t (*sm)[4], uint32_t (&before)[N],
+__device__ __forceinline__ void wg_scan(const uint32_t (&v)[N], uint32_t (*sm)[PT / 64], uint32_t (&before)[N],
                                         uint32_t (&all)[N]) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int waves = blockDim.x >> 6;
     uint32_t in[N];
 #pragma unroll
     for (int i = 0; i < N; i++) in[i] = wave_scan(v[i]);
     if (lane == 63)
 #pragma unroll
-        for (int i = 0; i < N; i++) sm[wave][i] = in[i];
+        for (int i = 0; i < N; i++) sm[i][wave] = in[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < N; i++) before[i] = all[i] = 0;
-    for (int w = 0; w < waves; w++)
-#pragma unroll
-        for (int i = 0; i < N; i++) {
-            if (w == wave) before[i] = all[i];
-            all[i] = plus(all[i], sm[w][i]);
-        }
-#pragma unroll
     for (int i = 0; i < N; i++) {
+        // the waves' sums, one a lane, summed in their turn
+        const uint32_t w = wave_scan(lane < waves ? sm[i][lane] : 0);
+        all[i] = (uint32_t)__builtin_amdgcn_readlane((int)w, 63);
+        const uint32_t mine = wave ? (uint32_t)__builtin_amdgcn_readlane((int)w, wave - 1) : 0;
         // (the lane before's inclusive sum: exact also where sums stay at their most)
-        const uint32_t prev = (uint32_t)__shfl_up((int)in[i], 1);
-        before[i] = plus(before[i], lane ? prev : 0);
+        const uint32_t prev = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)in[i], 0x138, 0xf, 0xf, false);
+        before[i] = plus(mine, prev);
     }
 }
 
@@ -131,17 +128,19 @@ __device__ __forceinline__ void put_item(const PlanArg& a, uint32_t at, int s, u
 }
 
 __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
-    __shared__ uint32_t sm[8][PT / 64][4];
+    __shared__ uint32_t sm[8][4][PT / 64];
     __shared__ uint32_t first_tok[PT], first_page[PT], first_item[PT], s_cached[PT], s_held[PT], s_from[PT],
         s_end[PT], s_fresh[PT], s_part[PT];
     __shared__ bool s_ok[PT];
     const kq_kv_plan& p = a.p;
     const int tid = threadIdx.x, T = blockDim.x;
+    const uint32_t many = T * gridDim.x;
+    const bool head = blockIdx.x == 0;          // (the others only help with the tokens)
     const uint32_t room = p.table ? (uint32_t)max(0, *p.n_free) : 0;
     Seq q = load_seq(a, tid);
-    for (int i = tid; i < a.counters; i += T) a.counter[i] = 0;
+    for (int i = tid; head && i < a.counters; i += T) a.counter[i] = 0;
     uint32_t share = 0x7fffffc0u;
-    if (a.items) {
+    if (head && a.items) {
         // The most keys that an item has: with keys / extra or more there are no more than
         // `extra` items beyond one a sequence.  Keys in units of 32, their lower and upper
         // 16 bits:
@@ -156,20 +155,21 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         wg_scan<3>(units, sm[0], before, all);
         const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
         const uint32_t extra = a.cap - p.S, cap = all[2] + extra;
+        // (total / n or a little more: binary32 is off by 2^-22 of it at most)
         auto over = [&](uint32_t n) {
-            uint32_t x = (uint32_t)((double)total / (double)n);
-            while ((uint64_t)x * n < total) x++;
-            return x;
+            return (uint32_t)fminf(ceilf((float)total / (float)n * (1.0f + 0x1p-21f)), 0x1p26f);
         };
         const uint32_t least = total * 32 <= (uint64_t)a.few ? 4 : 8;
-        uint32_t most = max(least, min(over(extra), 0x3ffffffu));
+        uint32_t most = max(least, over(extra));
         if (p.S <= T) {
             // fewer, where that gives no more items either, by bisection
             uint32_t lo = max(least, min(over(cap), most));
 #pragma unroll 1
             for (int i = 0; i < 5 && lo < most; i++) {
                 const uint32_t mid = (lo + most) / 2;
-                uint32_t per, v[1] = {q.attended ? items_of(q.end - q.from, 32 * mid, &per) : 0}, b1[1], n1[1];
+                // (units / mid rounded up, or one more: binary32 is off by 2^-22 of it at most)
+                const float each = ceilf((float)((q.end - q.from + 31) / 32) * (1.0f / (float)mid) * (1.0f + 0x1p-21f));
+                uint32_t v[1] = {q.attended ? max(1u, (uint32_t)each) : 0}, b1[1], n1[1];
                 wg_scan<1>(v, sm[3 + i], b1, n1);
                 if (n1[0] <= cap) most = mid;
                 else lo = mid + 1;
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         wg_scan<2>(v1, sm[1], b1, n1);
         const bool ok = !q.narrow && (q.need == 0 || plus(plus(page0, b1[1]), q.need) <= room);
         const uint32_t from = ok ? q.from : 0, end = ok ? q.end : 0;
-        const uint32_t items = q.attended ? items_of(end - from, share, &per) : 0, parts = items > 1 ? items : 0;
+        const uint32_t items = head && q.attended ? items_of(end - from, share, &per) : 0, parts = items > 1 ? items : 0;
         // (pages run out once: those who get theirs are the first that need any)
         const uint32_t v2[4] = {items, parts, s < p.S && !ok ? 1u : 0u, ok ? q.need : 0u};
         wg_scan<4>(v2, sm[2], b2, n2);
@@ -206,35 +206,45 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         s_end[tid] = end;
         s_fresh[tid] = q.fresh;
         s_ok[tid] = ok;
-        if (s < p.S) {
+        if (head && s < p.S) {
             if (p.start) p.start[s] = (int)(tok0 + b1[0]);
             if (p.lens) p.lens[s] = ok ? (int)q.end : 0;
             if (p.held_out) p.held_out[s] = (int)(q.held + (ok ? q.need : 0));
         }
         __syncthreads();
         // new pages, from the end of the free ones
-        if (p.table)
+        if (head && p.table)
             for (uint32_t e = tid; e < n1[1] && plus(page0, e) < room; e += T) {
                 const int i = owner(first_page, n, e);
                 if (s_ok[i])
                     p.table[(int64_t)(s0 + i) * p.table_stride + s_held[i] + (e - first_page[i])] =
                         p.free_pages[room - 1 - (page0 + e)];
             }
-        // new tokens
+        // new tokens, four a lane at a time, as their pages are a memory's latency away
         if (p.pos || p.slot)
-            for (uint32_t t = tid; t < n1[0] && plus(tok0, t) < (uint32_t)p.N; t += T) {
-                const int i = owner(first_tok, n, t);
-                const uint32_t pos = s_cached[i] + (t - first_tok[i]);
-                if (p.pos) p.pos[tok0 + t] = (int)pos;
-                if (!p.slot) continue;
-                int slot = -1;
-                if (s_ok[i]) {
-                    const uint32_t b = pos / (uint32_t)p.page;
-                    const int page = b < s_held[i] ? p.table[(int64_t)(s0 + i) * p.table_stride + b]
-                                                   : p.free_pages[room - 1 - (page0 + first_page[i] + (b - s_held[i]))];
-                    if ((uint32_t)page < (uint32_t)p.n_pages) slot = page * p.page + (int)(pos - b * (uint32_t)p.page);
+            for (uint32_t t0 = tid + blockIdx.x * T; t0 < n1[0] && plus(tok0, t0) < (uint32_t)p.N; t0 += 4 * many) {
+                uint32_t pos[4], b[4];
+                int page[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t t = t0 + u * many;
+                    if (t >= n1[0]) break;
+                    const int i = owner(first_tok, n, t);
+                    pos[u] = s_cached[i] + (t - first_tok[i]);
+                    b[u] = pos[u] / (uint32_t)p.page;
+                    page[u] = -1;
+                    if (p.slot && s_ok[i])
+                        page[u] = b[u] < s_held[i] ? p.table[(int64_t)(s0 + i) * p.table_stride + b[u]]
+                                                   : p.free_pages[room - 1 - (page0 + first_page[i] + (b[u] - s_held[i]))];
                 }
-                p.slot[tok0 + t] = slot;
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const uint32_t t = t0 + u * many;
+                    if (t >= n1[0] || plus(tok0, t) >= (uint32_t)p.N) break;
+                    if (p.pos) p.pos[tok0 + t] = (int)pos[u];
+                    const bool ok = (uint32_t)page[u] < (uint32_t)p.n_pages;
+                    if (p.slot) p.slot[tok0 + t] = ok ? page[u] * p.page + (int)(pos[u] - b[u] * (uint32_t)p.page) : -1;
+                }
             }
         // the attention's items
         for (uint32_t e = tid; e < n2[1] && item0 + e < (uint32_t)a.cap; e += T) {
@@ -251,7 +261,7 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         taken += n2[3];
         __syncthreads();
     }
-    if (tid == 0) {
+    if (head && tid == 0) {
         if (p.start) p.start[p.S] = (int)tok0;
         if (p.n_free_out) *p.n_free_out = (int)(room - taken);
         if (p.n_short) *p.n_short = (int)shorts;
@@ -263,6 +273,11 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
+// One workgroup a token (several, where tokens are few): its angles' cosines and sines
+// once in LDS, then its heads' rows, `lanes` lanes of four values each, U rows a lane
+// in flight.  The partners of a rotation are read a second time, from the cache.
+constexpr int U = 4;
+
 template <int TYPE>
 __global__ __launch_bounds__(256) void kq_kv_store_kernel(kq_kv_store a, int lanes) {
     __shared__ double cs[KQ_KV_MAX_D / 2], sn[KQ_KV_MAX_D / 2];
@@ -270,75 +285,90 @@ __global__ __launch_bounds__(256) void kq_kv_store_kernel(kq_kv_store a, int lan
     const long tok = blockIdx.x;
     if (a.n_tokens && tok >= *a.n_tokens) return;
     const int half = a.rot / 2, D = c.D;
-    if ((int)threadIdx.x < half) {
-        const double angle = (double)a.pos[tok] * (double)a.freq[threadIdx.x];
-        sincos(angle, &sn[threadIdx.x], &cs[threadIdx.x]);
-    }
-    __syncthreads();
     const long slot = a.slot[tok];
     const bool live = slot >= 0 && slot < (long)c.n_pages * c.page;
     const long page = live ? slot / c.page : 0, at = live ? slot - page * c.page : 0;
-    const int rows = a.n_q + 2 * c.n_kv, per = 64 / lanes * 4;
-    const int j0 = (threadIdx.x & (lanes - 1)) * 4;
-    for (int r0 = blockIdx.y * per; r0 < rows; r0 += gridDim.y * per) {
-        const int r = r0 + (int)threadIdx.x / lanes;
-        const bool on = r < rows && j0 < D;
-        const int head = r < a.n_q ? r : r < a.n_q + c.n_kv ? r - a.n_q : r - a.n_q - c.n_kv;
-        const bool is_q = r < a.n_q, is_v = r >= a.n_q + c.n_kv;
-        const float* const x = is_q ? a.q + tok * a.q_stride + (long)head * D
-                             : is_v ? a.v + tok * a.v_stride + (long)head * D
-                                    : a.k + tok * a.k_stride + (long)head * D;
-        f32x4 y = (f32x4)0.0f;
-        if (on) y = *reinterpret_cast<const f32x4*>(x + j0);
-        // (q_out may be q: a row is one wave's, which reads it before it writes)
-        f32x4 o = y;
-        if (on && !is_v && j0 < a.rot) {
+    const int rows = a.n_q + 2 * c.n_kv, per = 256 / lanes;
+    const int j0 = (threadIdx.x & (lanes - 1)) * 4, r1 = threadIdx.x / lanes;
+    // four partners in a row, or four pairs of neighbours, at 16-byte addresses
+    const bool even = a.interleaved ? a.rot % 4 == 0 : half % 4 == 0;
+    bool first = true;
+    for (int r0 = blockIdx.y * per; r0 < rows; r0 += gridDim.y * per * U) {
+        f32x4 y[U], o[U];
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + e;
-                if (j >= a.rot) continue;
-                const int other = a.interleaved ? j ^ 1 : j < half ? j + half : j - half;
-                o[e] = x[other];
+        for (int u = 0; u < U; u++) {
+            const int r = r0 + u * gridDim.y * per + r1;
+            y[u] = o[u] = (f32x4)0.0f;
+            if (r >= rows || j0 >= D) continue;
+            const float* const x = r < a.n_q           ? a.q + tok * a.q_stride + (long)r * D
+                                   : r < a.n_q + c.n_kv ? a.k + tok * a.k_stride + (long)(r - a.n_q) * D
+                                                        : a.v + tok * a.v_stride + (long)(r - a.n_q - c.n_kv) * D;
+            y[u] = *reinterpret_cast<const f32x4*>(x + j0);
+            if (r >= a.n_q + c.n_kv || j0 >= a.rot) continue;
+            if (a.interleaved) {
+                o[u] = (f32x4){y[u][1], y[u][0], y[u][3], y[u][2]};
+            } else if (even) {
+                o[u] = *reinterpret_cast<const f32x4*>(x + (j0 < half ? j0 + half : j0 - half));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = j0 + e;
+                    if (j < a.rot) o[u][e] = x[j < half ? j + half : j - half];
+                }
             }
         }
-        if (on && !is_v && j0 < a.rot) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int j = j0 + e;
-                if (j >= a.rot) continue;
-                const int i = a.interleaved ? j >> 1 : j < half ? j : j - half;
-                const bool lead = a.interleaved ? !(j & 1) : j < half;
-                const double m = (double)y[e] * cs[i], n = (double)o[e] * sn[i];
-                y[e] = (float)(lead ? m - n : m + n);
+        if (first) {
+            if ((int)threadIdx.x < half) {
+                const double angle = (double)a.pos[tok] * (double)a.freq[threadIdx.x];
+                sincos(angle, &sn[threadIdx.x], &cs[threadIdx.x]);
             }
+            __syncthreads();
+            first = false;
         }
-        if (is_q) {
-            if (on) *reinterpret_cast<f32x4*>(a.q_out + tok * a.q_out_stride + (long)head * D + j0) = y;
-            continue;
-        }
-        const long row = page * c.page_stride + head * c.head_stride + at * c.token_stride + j0;
-        if constexpr (TYPE == KQ_TYPE_I8) {
-            float amax = fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3])));
-            for (int off = 1; off < lanes; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
-            const float scale = __fdiv_rn(amax, 127.0f);
-            const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-            uint32_t w = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                w |= ((uint32_t)min(127, max(-128, __float2int_rn(y[e] * inv))) & 0xffu) << (8 * e);
-            if (on && live) {
-                *reinterpret_cast<uint32_t*>((int8_t*)(is_v ? c.v : c.k) + row) = w;
-                if (j0 == 0)
-                    (is_v ? c.v_scale : c.k_scale)[(page * c.n_kv + head) * c.page + at] = scale;
+        for (int u = 0; u < U; u++) {
+            const int r = r0 + u * gridDim.y * per + r1;
+            const bool on = r < rows && j0 < D;
+            const bool is_q = r < a.n_q, is_v = r >= a.n_q + c.n_kv;
+            const int head = is_q ? r : is_v ? r - a.n_q - c.n_kv : r - a.n_q;
+            if (on && !is_v && j0 < a.rot) {
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int j = j0 + e;
+                    if (j >= a.rot) continue;
+                    const int i = a.interleaved ? j >> 1 : j < half ? j : j - half;
+                    const bool lead = a.interleaved ? !(j & 1) : j < half;
+                    const double m = (double)y[u][e] * cs[i], n = (double)o[u][e] * sn[i];
+                    y[u][e] = (float)(lead ? m - n : m + n);
+                }
             }
-        } else if (on && live) {
-            uint16_t h[4];
+            if (is_q) {
+                if (on) *reinterpret_cast<f32x4*>(a.q_out + tok * a.q_out_stride + (long)head * D + j0) = y[u];
+                continue;
+            }
+            const long row = page * c.page_stride + head * c.head_stride + at * c.token_stride + j0;
+            if constexpr (TYPE == KQ_TYPE_I8) {
+                float amax = fmaxf(fmaxf(fabsf(y[u][0]), fabsf(y[u][1])), fmaxf(fabsf(y[u][2]), fabsf(y[u][3])));
+                for (int off = 1; off < lanes; off <<= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+                const float scale = __fdiv_rn(amax, 127.0f);
+                const float inv = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+                uint32_t w = 0;
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                h[e] = TYPE == KQ_TYPE_F16 ? __half_as_ushort(__float2half_rn(y[e]))
-                                           : __bfloat16_as_ushort(__float2bfloat16(y[e]));
-            *reinterpret_cast<uint2*>((uint16_t*)(is_v ? c.v : c.k) + row) =
-                make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+                for (int e = 0; e < 4; e++)
+                    w |= ((uint32_t)min(127, max(-128, __float2int_rn(y[u][e] * inv))) & 0xffu) << (8 * e);
+                if (on && live) {
+                    *reinterpret_cast<uint32_t*>((int8_t*)(is_v ? c.v : c.k) + row) = w;
+                    if (j0 == 0) (is_v ? c.v_scale : c.k_scale)[(page * c.n_kv + head) * c.page + at] = scale;
+                }
+            } else if (on && live) {
+                uint16_t h[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    h[e] = TYPE == KQ_TYPE_F16 ? __half_as_ushort(__float2half_rn(y[u][e]))
+                                               : __bfloat16_as_ushort(__float2bfloat16(y[u][e]));
+                *reinterpret_cast<uint2*>((uint16_t*)(is_v ? c.v : c.k) + row) =
+                    make_uint2(h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16);
+            }
         }
     }
 }
@@ -356,10 +386,14 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
         a.items = a.count + KQK_LIST_HEAD;
         a.counter = a.items + (long)z->cap * KQK_ITEM;
     }
-    // a lane for each sequence, and for each new token that there may be
-    int lanes = p->S > p->N ? p->S : p->N;
-    lanes = lanes > PT ? PT : (lanes + 63) / 64 * 64;
-    hipLaunchKernelGGL(kq_kv_plan_kernel, dim3(1), dim3((unsigned)lanes), 0, st, a);
+    // A lane for each sequence, and for each four new tokens that there may be; of many
+    // tokens (us of one workgroup / of this: 14119 16.9 / 6.9) several workgroups, each of
+    // which takes the sums for itself, unless the first writes over what they read.
+    int lanes = p->S > p->N / 4 ? p->S : p->N / 4;
+    lanes = lanes > PT ? PT : lanes < 64 ? 64 : (lanes + 63) / 64 * 64;
+    const bool apart = (!p->held_out || p->held_out != p->held) && (!p->n_free_out || p->n_free_out != p->n_free);
+    const int groups = !apart || p->N <= 4096 ? 1 : p->N >= 16 * 2048 ? 16 : p->N / 2048;
+    hipLaunchKernelGGL(kq_kv_plan_kernel, dim3((unsigned)groups), dim3((unsigned)lanes), 0, st, a);
     return (int)hipGetLastError();
 }
 
