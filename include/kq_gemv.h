@@ -660,6 +660,7 @@ typedef struct kq_kv_cache {
 #define KQ_ATTN_MAX_SEQS 65535
 #define KQ_ATTN_MAX_NEW 64          /* KQ_VERIFY_MAX_DRAFT drafted tokens and the one before them */
 #define KQ_ATTN_MAX_HEADS 1024
+#define KQ_ATTN_MAX_WINDOW (1 << 30)
 typedef struct kq_attn_shape {
     int S, T, n_q, n_kv, D, window;
 } kq_attn_shape;
@@ -680,7 +681,7 @@ typedef struct kq_attn_shape {
  *   pos, slot   of each new token: its position, and its slot (-1 where pages are
  *               missing, or its page is not in 0..n_pages-1); N entries at most
  *   n_short     one value: the sequences whose pages are missing
- * Any output may be NULL.  table NULL: no pages are dealt with (free_pages, n_free,
+ * Any output may be NULL; they do not overlap, nor lie in the inputs but as said.  table NULL: no pages are dealt with (free_pages, n_free,
  * held, held_out, n_free_out, slot and n_short are NULL then).  Lengths below 0
  * count as 0, above 2^30 - 1 as that; the new tokens are fewer than 2^31.
  * list (NULL: none, shape unused): kq_kv_list_bytes of device memory, 256-byte

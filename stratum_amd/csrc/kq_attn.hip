@@ -4,8 +4,7 @@
 //
 // The rows of a sequence and a head of keys are its new tokens' queries of the G =
 // n_q / n_kv heads that read it; a workgroup takes 16 of them and an item of the list
-// (a share of the sequence's keys), each of its waves every fourth step of 32 keys (64 of
-// few bytes).  One pass, with a running maximum m and sum l of each row:
+// (a share of the sequence's keys), each of its waves every fourth step of 32 keys.  One pass, with a running maximum m and sum l of each row:
 //   S^T = K Q^T   16 keys x 16 rows a matrix instruction, K as it lies in the cache
 //                 (a lane has 8 values of one key), Q^T from LDS
 //   p = 2^(S - m), in the layout that S^T has: 8 keys of a row a lane, which is that
@@ -50,7 +49,8 @@ struct AttnArg {
     int* counter;
     float* part;                // partial results: parts x n_kv x R rows of D
     float2* ml;                 // and their maximum and sum
-    int64_t page_b, head_b, tok_b, q_stride, out_stride;      // cache strides in bytes
+    int64_t page_b, head_b, q_stride, out_stride;             // cache strides in bytes
+    uint32_t tok_b, page_s;     // page_s: scales of a page
     uint64_t div, kv_div, blocks_div;    // page / 16, n_kv and 8 blocks by multiplication
     float qscale;               // scale log2 e
     int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts, blocks;
@@ -130,8 +130,6 @@ void kq_attn_kernel(const AttnArg a) {
     constexpr int NP = TYPE == KQ_TYPE_BF16 ? 3 : 2;      // numbers for a query or weight
     constexpr int ES = TYPE == KQ_TYPE_I8 ? 1 : 2;
     constexpr int NCH = DM / 32;                          // steps of 32 values of the first product
-    // tiles of 32 keys in a step: two where one has few bytes to wait for
-    constexpr int NS = DM * ES <= 128 ? 2 : 1, KEYS = 32 * NS;
     constexpr bool WIDE = TYPE == KQ_TYPE_I8 && EXACT;    // int8 keys in loads of 16
     constexpr int W = DM >= 128 ? 8 : 4;                  // values a lane of a key in the second
     constexpr int NB = DM / (16 * W);
@@ -154,9 +152,10 @@ void kq_attn_kernel(const AttnArg a) {
     int s = (int)((uint64_t)(uint32_t)pair * a.kv_div >> 40);
     const int h = pair - s * a.n_kv;
     int k0 = 0, k1, num = 1, idx = 0, part = 0, row0, n, len;
-    if (s >= (a.items ? min(a.cap, *a.count) : a.S)) return;
     if (a.items) {
-        const int* const it = a.items + s * KQK_ITEM;
+        // (the item is read with the number of items, not after it: the list reaches to cap)
+        const int* const it = a.items + min(s, a.cap - 1) * KQK_ITEM;
+        const int at = s;
         s = it[0];
         k0 = it[1];
         k1 = it[2];
@@ -166,9 +165,11 @@ void kq_attn_kernel(const AttnArg a) {
         row0 = it[5];
         n = it[6];
         len = it[7];
-        if (s < 0 || s >= a.S || k0 < 0 || num < 1 || (num > 1 && (part < 0 || idx >= num || part > a.parts - num)))
+        if ((at >= min(a.cap, *a.count)) | (s < 0) | (s >= a.S) | (k0 < 0) | (num < 1) |
+            ((num > 1) & ((part < 0) | (idx >= num) | (part > a.parts - num))))
             return;
     } else {
+        if (s >= a.S) return;
         row0 = a.start ? a.start[s] : s;
         n = a.start ? a.start[s + 1] - row0 : 1;
         k1 = len = a.lens[s];
@@ -213,27 +214,27 @@ void kq_attn_kernel(const AttnArg a) {
         }
 
         // ---- where a step's keys lie
-        int pg[2 * NS];                     // pages of the next step's keys
+        int pg[2];                     // pages of the next step's keys
         auto fetch = [&](int kb) {
 #pragma unroll
-            for (int t = 0; t < 2 * NS; t++) {
+            for (int t = 0; t < 2; t++) {
                 uint32_t b;
                 if constexpr (TILED) b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
                 else b = (uint32_t)(kb + 16 * t + c) / (uint32_t)a.page;
                 pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
             }
         };
-        u32x4 kr[2 * NS][WIDE ? NCH / 2 : NCH], vr[8 * NS][NB];
-        float ksr[8 * NS], vsr[8 * NS];
-        bool have[2 * NS];                  // the keys' pages are pages
-        const uint8_t* vp[8 * NS];
-        int64_t sp[2 * NS];
-        const uint32_t klane = (TILED ? c * (uint32_t)a.tok_b : 0u) + (WIDE ? 16 : 8 * ES) * g;
-        const uint32_t vlane = (TILED ? 4 * g * (uint32_t)a.tok_b : 0u) + W * ES * c;
+        u32x4 kr[2][WIDE ? NCH / 2 : NCH], vr[8][NB];
+        float ksr[8], vsr[8];
+        bool have[2];                  // the keys' pages are pages
+        const uint8_t* vp[8];
+        int64_t sp[2];
+        const uint32_t klane = (TILED ? c * a.tok_b : 0u) + (WIDE ? 16 : 8 * ES) * g;
+        const uint32_t vlane = (TILED ? 4 * g * a.tok_b : 0u) + W * ES * c;
         auto octet = [&](int ch) { return EXACT || 32 * ch + 8 * g < D; };
         auto load_k = [&](int kb) {
 #pragma unroll
-            for (int t = 0; t < 2 * NS; t++) {
+            for (int t = 0; t < 2; t++) {
                 // (a key that is not there is read as the first one of the first page)
                 int page = TILED ? uniform(pg[t]) : pg[t], at;
                 have[t] = (uint32_t)page < (uint32_t)a.n_pages;
@@ -245,10 +246,10 @@ void kq_attn_kernel(const AttnArg a) {
                     at = (int)((uint32_t)(kb + 16 * t + c) % (uint32_t)a.page);
                 }
                 at = have[t] ? at : 0;
-                const int64_t o = page * a.page_b + at * a.tok_b;
+                const int64_t o = (uint32_t)page * a.page_b + (int64_t)((uint64_t)(uint32_t)at * a.tok_b);
 #pragma unroll
                 for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + (TILED ? o + j * a.tok_b : (int64_t)__shfl(o, 4 * g + j));
-                sp[t] = ((int64_t)page * a.n_kv + h) * a.page + at;
+                sp[t] = (int64_t)((uint64_t)(uint32_t)page * a.page_s) + (h * a.page + at);
 #pragma unroll
                 for (int ch = 0; ch < NCH; ch++) {
                     if (!EXACT && 32 * ch >= D) continue;
@@ -274,7 +275,7 @@ void kq_attn_kernel(const AttnArg a) {
         };
         auto load_v = [&]() {
 #pragma unroll
-            for (int j = 0; j < 8 * NS; j++)
+            for (int j = 0; j < 8; j++)
 #pragma unroll
                 for (int b = 0; b < NB; b++) {
                     const uint8_t* const x = vp[j] + (EXACT || W * c + 16 * W * b < D ? vlane + 16 * W * ES * b
@@ -291,7 +292,7 @@ void kq_attn_kernel(const AttnArg a) {
                 }
             if constexpr (TYPE == KQ_TYPE_I8) {
 #pragma unroll
-                for (int t = 0; t < 2 * NS; t++) {
+                for (int t = 0; t < 2; t++) {
                     if constexpr (TILED) {
                         const F4 x = *reinterpret_cast<const F4*>(a.vs + sp[t] + 4 * g);
 #pragma unroll
@@ -303,12 +304,12 @@ void kq_attn_kernel(const AttnArg a) {
             }
         };
 
-        int kb = k0 + KEYS * wave;
+        int kb = k0 + 32 * wave;
         if (kb < k1) {
             fetch(kb);
             load_k(kb);
             load_v();
-            if (kb + KEYS * NW < k1) fetch(kb + KEYS * NW);
+            if (kb + 32 * NW < k1) fetch(kb + 32 * NW);
         }
 
         u32x4* const ql = reinterpret_cast<u32x4*>(lds);
@@ -370,26 +371,26 @@ void kq_attn_kernel(const AttnArg a) {
 
         // ---- steps
 #pragma unroll 1
-        for (; kb < k1; kb += KEYS * NW) {
-            bool ok[2 * NS], all_ok = true;
+        for (; kb < k1; kb += 32 * NW) {
+            bool ok[2], all_ok = true;
 #pragma unroll
-            for (int t = 0; t < 2 * NS; t++) {
+            for (int t = 0; t < 2; t++) {
                 ok[t] = have[t];
                 all_ok &= ok[t];
             }
-            const bool full = kb >= all_lo && kb + KEYS <= all_hi && (TILED ? all_ok : __all(all_ok));
+            const bool full = kb >= all_lo && kb + 32 <= all_hi && (TILED ? all_ok : __all(all_ok));
             // (queries are read in each step: the compiler would keep them in registers)
             uint32_t qat = WIDE ? 32 * g + c : lane;
             asm volatile("" : "+v"(qat));
-            f32x4 sc[2 * NS];
+            f32x4 sc[2];
 #pragma unroll
-            for (int t = 0; t < 2 * NS; t++) sc[t] = (f32x4)0.0f;
+            for (int t = 0; t < 2; t++) sc[t] = (f32x4)0.0f;
 #pragma unroll
             for (int ch = 0; ch < NCH; ch++) {
                 if (!EXACT && 32 * ch >= D) continue;
-                u32x4 x[2 * NS];
+                u32x4 x[2];
 #pragma unroll
-                for (int t = 0; t < 2 * NS; t++) {
+                for (int t = 0; t < 2; t++) {
                     if constexpr (TYPE == KQ_TYPE_I8) {
                         const uint32_t y0 = WIDE ? kr[t][ch / 2][2 * (ch & 1)] : kr[t][ch][0];
                         const uint32_t y1 = WIDE ? kr[t][ch / 2][2 * (ch & 1) + 1] : kr[t][ch][1];
@@ -408,48 +409,48 @@ void kq_attn_kernel(const AttnArg a) {
                 for (int j = 0; j < NP; j++) {
                     const u32x4 y = ql[(j * (DM / 8) + (WIDE ? 8 * (ch / 2) + (ch & 1) : 4 * ch)) * 16 + qat];
 #pragma unroll
-                    for (int t = 0; t < 2 * NS; t++) sc[t] = mfma<NP>(x[t], y, sc[t]);
+                    for (int t = 0; t < 2; t++) sc[t] = mfma<NP>(x[t], y, sc[t]);
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-            float kscale[8 * NS], vscale[8 * NS];
+            float kscale[8], vscale[8];
             if constexpr (TYPE == KQ_TYPE_I8) {
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++) {
+                for (int j = 0; j < 8; j++) {
                     kscale[j] = TILED ? ksr[j] : __shfl(ksr[j >> 2], 4 * g + (j & 3));
                     vscale[j] = TILED ? vsr[j] : __shfl(vsr[j >> 2], 4 * g + (j & 3));
                 }
             }
             // which of the lane's keys are there at all, bit j: key 16 (j / 4) + 4 g + j % 4
-            uint32_t there = (1u << 8 * NS) - 1;
+            uint32_t there = 0xff;
             if (!full) {
                 uint32_t p = 0;
 #pragma unroll
-                for (int t = 0; t < 2 * NS; t++)
+                for (int t = 0; t < 2; t++)
                     p |= (TILED ? (ok[t] ? 15u : 0u) : (uint32_t)(__ballot(ok[t]) >> (4 * g)) & 15u) << (4 * t);
                 there = 0;
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++) {
+                for (int j = 0; j < 8; j++) {
                     const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
                     if (key < k1 && (p >> j & 1)) there |= 1u << j;
                 }
                 if constexpr (TYPE == KQ_TYPE_I8) {
 #pragma unroll
-                    for (int j = 0; j < 8 * NS; j++) vscale[j] = there >> j & 1 ? vscale[j] : 0.0f;
+                    for (int j = 0; j < 8; j++) vscale[j] = there >> j & 1 ? vscale[j] : 0.0f;
                 }
             }
             // the next step's keys are asked for as soon as this one's are used
-            const int nb = kb + KEYS * NW;
+            const int nb = kb + 32 * NW;
             if (nb < k1) {
                 load_k(nb);
-                if (nb + KEYS * NW < k1) fetch(nb + KEYS * NW);
+                if (nb + 32 * NW < k1) fetch(nb + 32 * NW);
             }
             // weights
             if constexpr (TYPE == KQ_TYPE_I8) {
                 // the sums are kept times a power of two that is near the largest scale so far
                 float top = fabsf(vscale[0]);
 #pragma unroll
-                for (int j = 1; j < 8 * NS; j++) top = fmaxf(top, fabsf(vscale[j]));
+                for (int j = 1; j < 8; j++) top = fmaxf(top, fabsf(vscale[j]));
                 const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
                 if (e > ve) {
                     const float f = ve ? __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23) : 0.0f;
@@ -461,25 +462,25 @@ void kq_attn_kernel(const AttnArg a) {
                 }
                 const float f = __uint_as_float((uint32_t)(254 - max(1, ve)) << 23);
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++) vscale[j] *= f;
+                for (int j = 0; j < 8; j++) vscale[j] *= f;
             }
-            float x[8 * NS];
+            float x[8];
 #pragma unroll
-            for (int j = 0; j < 8 * NS; j++) {
+            for (int j = 0; j < 8; j++) {
                 x[j] = sc[j >> 2][j & 3];
                 if constexpr (NP == 2) x[j] *= inv;
                 if constexpr (TYPE == KQ_TYPE_I8) x[j] *= kscale[j];
             }
             if (!full) {
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++) {
+                for (int j = 0; j < 8; j++) {
                     const int key = kb + 16 * (j >> 2) + 4 * g + (j & 3);
                     x[j] = key >= lo && key < hi && (there >> j & 1) ? x[j] : -INFINITY;
                 }
             }
             float top = x[0];
 #pragma unroll
-            for (int j = 1; j < 8 * NS; j++) top = fmaxf(top, x[j]);
+            for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
             top = max4(top);
             // (2^5 above the maximum that the weights are taken from before that is moved)
             if (__any(top > m + 5.0f)) {
@@ -493,10 +494,10 @@ void kq_attn_kernel(const AttnArg a) {
             }
             // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
             // with int8 values' scales below 2^16)
-            u32x4 w[NS][NP];
+            u32x4 w[NP];
             const float base = (m == -INFINITY ? 0.0f : m) - (NP == 2 ? 9.0f : 0.0f);
 #pragma unroll
-            for (int j = 0; j < 8 * NS; j += 2) {
+            for (int j = 0; j < 8; j += 2) {
                 float p = exp2_(x[j] - base), q = exp2_(x[j + 1] - base);
                 l += p + q;
                 if constexpr (TYPE == KQ_TYPE_I8) {
@@ -506,13 +507,13 @@ void kq_attn_kernel(const AttnArg a) {
                 uint32_t o[NP];
                 split<NP>(p, q, o);
 #pragma unroll
-                for (int e = 0; e < NP; e++) w[j >> 3][e][j >> 1 & 3] = o[e];
+                for (int e = 0; e < NP; e++) w[e][j >> 1] = o[e];
             }
             __builtin_amdgcn_sched_barrier(0);
             // values
             if (!full) {
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++) {
+                for (int j = 0; j < 8; j++) {
                     const uint32_t keep = there >> j & 1 ? 0xffffffffu : 0u;
 #pragma unroll
                     for (int b = 0; b < NB; b++)
@@ -523,7 +524,7 @@ void kq_attn_kernel(const AttnArg a) {
             if (ES == 2 && careful) {
                 constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
 #pragma unroll
-                for (int j = 0; j < 8 * NS; j++)
+                for (int j = 0; j < 8; j++)
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -538,20 +539,17 @@ void kq_attn_kernel(const AttnArg a) {
                 if (!EXACT && 16 * W * b >= D) continue;
 #pragma unroll
                 for (int t = 0; t < W; t++) {
+                    u32x4 v;
 #pragma unroll
-                    for (int i = 0; i < NS; i++) {
-                        u32x4 v;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const u32x4 v0 = vr[8 * i + 2 * j][b], v1 = vr[8 * i + 2 * j + 1][b];
-                            if constexpr (ES == 2)
-                                v[j] = perm(v1[t >> 1], v0[t >> 1], t & 1 ? 0x07060302 : 0x05040100);
-                            else
-                                v[j] = halves(perm(v1[t >> 2], v0[t >> 2], 0x0c000c00u | (t & 3) | (4 + (t & 3)) << 16));
-                        }
-#pragma unroll
-                        for (int j = 0; j < NP; j++) acc[b][t] = mfma<NP>(v, w[i][j], acc[b][t]);
+                    for (int j = 0; j < 4; j++) {
+                        const u32x4 v0 = vr[2 * j][b], v1 = vr[2 * j + 1][b];
+                        if constexpr (ES == 2)
+                            v[j] = perm(v1[t >> 1], v0[t >> 1], t & 1 ? 0x07060302 : 0x05040100);
+                        else
+                            v[j] = halves(perm(v1[t >> 2], v0[t >> 2], 0x0c000c00u | (t & 3) | (4 + (t & 3)) << 16));
                     }
+#pragma unroll
+                    for (int j = 0; j < NP; j++) acc[b][t] = mfma<NP>(v, w[j], acc[b][t]);
                     // (in few registers: the compiler would make all operands first)
                     if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
                 }
@@ -630,7 +628,7 @@ void kq_attn_kernel(const AttnArg a) {
             for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
                 const int page = table[key / a.page];
                 if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + key % a.page * a.tok_b + 2 * d);
+                const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + (int64_t)(key % a.page) * a.tok_b + 2 * d);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const float v = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
@@ -790,7 +788,8 @@ int kqk_launch_attn(const kq_paged_attn* p, const kqk_attn_sizes* z, void* work,
     a.lens = p->lens;
     a.page_b = c.page_stride * es;
     a.head_b = c.head_stride * es;
-    a.tok_b = c.token_stride * es;
+    a.tok_b = (uint32_t)c.token_stride * es;
+    a.page_s = (uint32_t)c.n_kv * c.page;
     a.q_stride = p->q_stride;
     a.out_stride = p->out_stride;
     a.qscale = (float)(p->scale * 1.4426950408889634);

@@ -56,7 +56,7 @@ static int shape_check(const kq_attn_shape* s, const char* who) {
         return kq_fail("%s: %d heads of queries, %d of keys", who, s->n_q, s->n_kv);
     if (s->D < 8 || s->D > KQ_KV_MAX_D || s->D % 8)
         return kq_fail("%s: D=%d (a multiple of 8 up to %d)", who, s->D, KQ_KV_MAX_D);
-    if (s->window < 0) return kq_fail("%s: window %d", who, s->window);
+    if (s->window < 0 || s->window > KQ_ATTN_MAX_WINDOW) return kq_fail("%s: window %d", who, s->window);
     return 0;
 }
 

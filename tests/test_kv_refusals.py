@@ -34,7 +34,7 @@ def shape(**kw):
 SHAPES = [(dict(S=0), "S=0"), (dict(S=65536), "S=65536"), (dict(T=0), "T=0"), (dict(T=65), "T=65"),
           (dict(n_q=0), "0 heads"), (dict(n_kv=0), "0 of keys"), (dict(n_kv=3), "3 of keys"), (dict(n_q=2048), "2048"),
           (dict(n_kv=-2), "-2 of keys"), (dict(D=0), "D=0"), (dict(D=60), "D=60"), (dict(D=264), "D=264"),
-          (dict(window=-1), "window")]
+          (dict(window=-1), "window"), (dict(window=(1 << 30) + 1), "window")]
 
 
 @pytest.mark.parametrize("kw,word", SHAPES)
