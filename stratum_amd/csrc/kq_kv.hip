@@ -100,23 +100,38 @@ __device__ __forceinline__ void wg_scan(const uint32_t (&v)[N], uint32_t (*sm)[P
     }
 }
 
-// The last i < n with first[i] <= v (first[0] is 0, the values ascend).
-__device__ __forceinline__ int owner(const uint32_t* first, int n, uint32_t v) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= v) lo = mid;
-        else hi = mid;
+// The last i < n with first[i] <= v (first[0] is 0, the values ascend), of K values at
+// once, whose steps wait for LDS together.
+template <int K>
+__device__ __forceinline__ void owners(const uint32_t* first, int n, const uint32_t (&v)[K], int (&at)[K]) {
+#pragma unroll
+    for (int k = 0; k < K; k++) at[k] = 0;
+    for (int step = n > 1 ? 1 << (31 - __clz(n - 1)) : 0; step; step >>= 1) {
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int mid = at[k] + step;
+            const uint32_t f = first[min(mid, n - 1)];
+            at[k] = mid < n && f <= v[k] ? mid : at[k];
+        }
     }
-    return lo;
 }
+__device__ __forceinline__ int owner(const uint32_t* first, int n, uint32_t v) {
+    const uint32_t w[1] = {v};
+    int at[1];
+    owners<1>(first, n, w, at);
+    return at[0];
+}
+
+// An item's keys are a multiple of 128 (a step of 32 for each of four waves), but for a
+// sequence's last.
+constexpr uint32_t ROUND = 128;
 
 // How many items keys take where one has at most `share`, and the keys of each.
 __device__ __forceinline__ uint32_t items_of(uint32_t keys, uint32_t share, uint32_t* per) {
     *per = max(keys, 1u);
     if (keys <= share) return 1;
     const uint32_t n = (keys + share - 1) / share;
-    *per = ((keys + n - 1) / n + 31) & ~31u;
+    *per = ((keys + n - 1) / n + ROUND - 1) / ROUND * ROUND;
     return (keys + *per - 1) / *per;
 }
 
@@ -139,15 +154,15 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
     const uint32_t room = p.table ? (uint32_t)max(0, *p.n_free) : 0;
     Seq q = load_seq(a, tid);
     for (int i = tid; head && i < a.counters; i += T) a.counter[i] = 0;
-    uint32_t share = 0x7fffffc0u;
+    uint32_t share = 0;
     if (head && a.items) {
         // The most keys that an item has: with keys / extra or more there are no more than
-        // `extra` items beyond one a sequence.  Keys in units of 32, their lower and upper
-        // 16 bits:
+        // `extra` items beyond one a sequence.  Keys in units of ROUND, their lower and
+        // upper 16 bits:
         uint32_t units[3] = {0, 0, 0}, before[3], all[3];
         for (int s0 = 0; s0 < p.S; s0 += T) {
             const Seq r = s0 ? load_seq(a, s0 + tid) : q;
-            const uint32_t n = r.attended ? (r.end - r.from + 31) / 32 : 0;
+            const uint32_t n = r.attended ? (r.end - r.from + ROUND - 1) / ROUND : 0;
             units[0] += n & 0xffff;
             units[1] += n >> 16;
             units[2] += r.attended;
@@ -155,27 +170,30 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         wg_scan<3>(units, sm[0], before, all);
         const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
         const uint32_t extra = a.cap - p.S, cap = all[2] + extra;
-        // (total / n or a little more: binary32 is off by 2^-22 of it at most)
-        auto over = [&](uint32_t n) {
-            return (uint32_t)fminf(ceilf((float)total / (float)n * (1.0f + 0x1p-21f)), 0x1p26f);
+        // x / n rounded up, or a little more (x past 2^24)
+        auto over = [](uint64_t x, uint32_t n) {
+            uint32_t y = (uint32_t)((float)x / (float)n);
+            while ((uint64_t)y * n < x) y++;
+            return y;
         };
-        const uint32_t least = total * 32 <= (uint64_t)a.few ? 4 : 8;
-        uint32_t most = max(least, over(extra));
-        if (p.S <= T) {
-            // fewer, where that gives no more items either, by bisection
-            uint32_t lo = max(least, min(over(cap), most));
+        const uint32_t least = total * ROUND <= (uint64_t)a.few ? 1 : 2;
+        uint32_t most = max(least, over(total, extra));
+        if (p.S <= 64) {
+            // Fewer, where that gives no more items either, by bisection (0.6 us a step where
+            // there are several waves, and with many sequences little to gain; 64 ragged
+            // streams' attention takes 103 us for 108 with it).
+            const uint32_t mine = q.attended ? (q.end - q.from + ROUND - 1) / ROUND : 0;
+            uint32_t lo = max(least, min(over(total, cap), most));
 #pragma unroll 1
             for (int i = 0; i < 5 && lo < most; i++) {
                 const uint32_t mid = (lo + most) / 2;
-                // (units / mid rounded up, or one more: binary32 is off by 2^-22 of it at most)
-                const float each = ceilf((float)((q.end - q.from + 31) / 32) * (1.0f / (float)mid) * (1.0f + 0x1p-21f));
-                uint32_t v[1] = {q.attended ? max(1u, (uint32_t)each) : 0}, b1[1], n1[1];
+                uint32_t v[1] = {q.attended ? max(1u, over(mine, mid)) : 0}, b1[1], n1[1];
                 wg_scan<1>(v, sm[3 + i], b1, n1);
                 if (n1[0] <= cap) most = mid;
                 else lo = mid + 1;
             }
         }
-        share = 32 * most;
+        share = min(most, 0x7fffffu) * ROUND;
     }
     uint32_t tok0 = 0, page0 = 0, taken = 0, shorts = 0, item0 = 0, part0 = 0;
     for (int s0 = 0; s0 < p.S; s0 += T) {
@@ -223,14 +241,16 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         // new tokens, four a lane at a time, as their pages are a memory's latency away
         if (p.pos || p.slot)
             for (uint32_t t0 = tid + blockIdx.x * T; t0 < n1[0] && plus(tok0, t0) < (uint32_t)p.N; t0 += 4 * many) {
-                uint32_t pos[4], b[4];
-                int page[4];
+                uint32_t tok[4], pos[4], b[4];
+                int page[4], at[4];
+#pragma unroll
+                for (int u = 0; u < 4; u++) tok[u] = min(t0 + u * many, n1[0] - 1);
+                owners<4>(first_tok, n, tok, at);
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
-                    const uint32_t t = t0 + u * many;
-                    if (t >= n1[0]) break;
-                    const int i = owner(first_tok, n, t);
-                    pos[u] = s_cached[i] + (t - first_tok[i]);
+                    if (t0 + u * many >= n1[0]) break;
+                    const int i = at[u];
+                    pos[u] = s_cached[i] + (tok[u] - first_tok[i]);
                     b[u] = pos[u] / (uint32_t)p.page;
                     page[u] = -1;
                     if (p.slot && s_ok[i])
@@ -386,11 +406,11 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
         a.items = a.count + KQK_LIST_HEAD;
         a.counter = a.items + (long)z->cap * KQK_ITEM;
     }
-    // A lane for each sequence, and for each four new tokens that there may be; of many
+    // A lane for each sequence, and for each new token that there may be; of many
     // tokens (us of one workgroup / of this: 14119 16.9 / 6.9) several workgroups, each of
     // which takes the sums for itself, unless the first writes over what they read.
-    int lanes = p->S > p->N / 4 ? p->S : p->N / 4;
-    lanes = lanes > PT ? PT : lanes < 64 ? 64 : (lanes + 63) / 64 * 64;
+    int lanes = p->S > p->N ? p->S : p->N;
+    lanes = lanes > PT ? PT : (lanes + 63) / 64 * 64;
     const bool apart = (!p->held_out || p->held_out != p->held) && (!p->n_free_out || p->n_free_out != p->n_free);
     const int groups = !apart || p->N <= 4096 ? 1 : p->N >= 16 * 2048 ? 16 : p->N / 2048;
     hipLaunchKernelGGL(kq_kv_plan_kernel, dim3((unsigned)groups), dim3((unsigned)lanes), 0, st, a);
