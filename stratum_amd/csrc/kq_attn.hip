@@ -187,7 +187,7 @@ void kq_attn_kernel(const AttnArg a) {
     int lo, hi;                             // the keys that a lane's row sees
     float m, l;
     f32x4 acc[NB][W];
-    int ve = 0;                             // int8: the sums' exponent
+    int ve;                                 // int8: the sums' exponent
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
     // number all are taken again without such values, which are then added alone.
@@ -360,7 +360,7 @@ void kq_attn_kernel(const AttnArg a) {
         const float inv = NP == 2 ? s_inv[c] : 1.0f;
         m = -INFINITY;
         l = 0.0f;
-        ve = 0;
+        ve = 1;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -448,19 +448,23 @@ void kq_attn_kernel(const AttnArg a) {
             // weights
             if constexpr (TYPE == KQ_TYPE_I8) {
                 // the sums are kept times a power of two that is near the largest scale so far
-                float top = fabsf(vscale[0]);
+                // (but for infinite ones, of keys that not all rows may see)
+                float top = 0.0f;
 #pragma unroll
-                for (int j = 1; j < 8; j++) top = fmaxf(top, fabsf(vscale[j]));
+                for (int j = 0; j < 8; j++) {
+                    const float v = fabsf(vscale[j]);
+                    top = fmaxf(top, full || v < INFINITY ? v : 0.0f);
+                }
                 const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
                 if (e > ve) {
-                    const float f = ve ? __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23) : 0.0f;
+                    const float f = __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23);
                     ve = e;
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
                         for (int t = 0; t < W; t++) acc[b][t] *= f;
                 }
-                const float f = __uint_as_float((uint32_t)(254 - max(1, ve)) << 23);
+                const float f = __uint_as_float((uint32_t)(254 - ve) << 23);
 #pragma unroll
                 for (int j = 0; j < 8; j++) vscale[j] *= f;
             }
@@ -501,8 +505,9 @@ void kq_attn_kernel(const AttnArg a) {
                 float p = exp2_(x[j] - base), q = exp2_(x[j + 1] - base);
                 l += p + q;
                 if constexpr (TYPE == KQ_TYPE_I8) {
-                    p *= vscale[j];
-                    q *= vscale[j + 1];
+                    // (a hidden key's scale may be no number)
+                    p = full || x[j] != -INFINITY ? p * vscale[j] : 0.0f;
+                    q = full || x[j + 1] != -INFINITY ? q * vscale[j + 1] : 0.0f;
                 }
                 uint32_t o[NP];
                 split<NP>(p, q, o);
@@ -588,7 +593,7 @@ void kq_attn_kernel(const AttnArg a) {
             s_all[c] = make_float2(top, sum);
         }
         float f = exp2_(m - base);
-        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)max(1, ve) << 23);
+        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)ve << 23);
         if (c < live) {
 #pragma unroll
             for (int b = 0; b < NB; b++)

@@ -252,6 +252,31 @@ def test_many_sequences():
     both(Case(5, K.TYPE_F16, lens, np.ones(700, int), 8, 2, 64))
 
 
+def test_more_sequences_than_the_plan_has_lanes():
+    """Sums over sequences in rounds; short ones, and a few long ones that are split."""
+    g = np.random.default_rng(40)
+    lens = g.integers(1, 30, 2300)
+    lens[[5, 1100, 2299]] = 5000, 3000, 700
+    c = Case(41, K.TYPE_F16, lens, np.ones(2300, int), 2, 1, 64)
+    c.check(c.run(True))
+
+
+@pytest.mark.parametrize("lo,hi", [(1e-40, 2e-38), (3e-39, 1e-36), (1e-30, 1e30)])
+def test_int8_scales_of_all_sizes(lo, hi):
+    """Values' scales below the normal range, and far apart, in either order over the keys."""
+    for s1, s2 in ((lo, hi), (hi, lo)):
+        c = Case(42, K.TYPE_I8, [1000, 140], [1, 2], 4, 2, 128, qscale=0.3)
+        for s in range(2):
+            page, at = c.places(s)
+            f = np.where(np.arange(len(at)) < len(at) // 2, s1, s2).astype(np.float32)
+            p, a = torch.from_numpy(page).cuda(), torch.from_numpy(at).cuda()
+            new = torch.from_numpy(f).cuda().unsqueeze(1) * c.sc[1][p, :, a]
+            old = c.sc[1][p, :, a]
+            c.rows[s][1] *= (new.double() / old.double()).t().unsqueeze(-1)
+            c.sc[1][p, :, a] = new
+        both(c)
+
+
 def test_one_row_each_without_offsets():
     c = Case(6, K.TYPE_BF16, [3, 50, 64, 900], [1, 1, 1, 1], 8, 4, 128, pad_rows=0)
     for listed in (False, True):
@@ -333,6 +358,20 @@ def test_what_a_token_does_not_see_does_not_reach_it(t, bad, n_q):
         if bad != bad:
             for s, i in skip:
                 assert torch.isnan(got[c.start[s] + i]).all()
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+def test_scales_of_hidden_keys_do_not_reach_a_token(bad):
+    """The same of an int8 cache's scales, of keys, of values and of both."""
+    for which in ((0,), (1,), (0, 1)):
+        c = Case(24, K.TYPE_I8, [50, 400], [6, 5], 4, 2, 128, window=100)
+        for s, places in ((0, (46, 48)), (1, (397, 290, 299, 60))):
+            page, at = c.places(s)
+            for j in which:
+                for e in places:
+                    c.sc[j][int(page[e]), :, int(at[e])] = bad
+        skip = {(0, i) for i in range(2, 6)} | {(1, i) for i in (0, 1, 2, 3, 4) if i >= 2 or 296 + i <= 299}
+        both(c, skip=skip)
 
 
 def test_infinite_values_that_are_seen():
