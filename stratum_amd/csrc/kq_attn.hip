@@ -4,7 +4,8 @@
 //
 // The rows of a sequence and a head of keys are its new tokens' queries of the G =
 // n_q / n_kv heads that read it; a workgroup takes 16 of them and an item of the list
-// (a share of the sequence's keys), each of its waves every fourth step of 32 keys.  One pass, with a running maximum m and sum l of each row:
+// (a share of the sequence's keys), each of its waves every fourth step of 32 keys.  One
+// pass, with a running maximum m and sum l of each row:
 //   S^T = K Q^T   16 keys x 16 rows a matrix instruction, K as it lies in the cache
 //                 (a lane has 8 values of one key), Q^T from LDS
 //   p = 2^(S - m), in the layout that S^T has: 8 keys of a row a lane, which is that
@@ -17,6 +18,14 @@
 // power of two a row, weights times 2^9) where keys are binary16 or int8, as three
 // bfloat16 numbers (24 bits) where they are bfloat16.  Matrix work is far from full,
 // so that the further products are free.
+// Long caches are bound by memory (16 / 8 heads of 128, binary16, 16 sequences of 8192:
+// 101 us, 5.3 TB/s; 24 / 4 of 256, bfloat16, 64 of 8192: 375 us, 5.7), short ones by a
+// chain of latencies: item, pages, keys, a step, the join of waves (one sequence of 32:
+// 5.8 us, heads of 256 7.8), and 4 to 5 us for a join of items.  Two tiles of 16 rows a
+// wave share a step's operands but take all of a SIMD's registers: 8 sequences of 8 new
+// tokens, 24 / 4 heads of 256, of 32 / 1000 to 4000 / 4096 keys took 14 / 64 / 57 us for
+// 9 / 50 / 71 of one; 8 waves a workgroup 96 us for 82 with 200 sequences of 500 keys, and
+// no less with few.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -49,8 +58,9 @@ struct AttnArg {
     int* counter;
     float* part;                // partial results: parts x n_kv x R rows of D
     float2* ml;                 // and their maximum and sum
-    int64_t page_b, head_b, q_stride, out_stride;             // cache strides in bytes
-    uint32_t tok_b, page_s;     // page_s: scales of a page
+    int64_t q_stride, out_stride;
+    int64_t page_b, head_b;     // cache strides in bytes
+    uint32_t tok_b, page_s;     // (page_s: scales of a page)
     uint64_t div, kv_div, blocks_div;    // page / 16, n_kv and 8 blocks by multiplication
     float qscale;               // scale log2 e
     int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts, blocks;
@@ -248,7 +258,8 @@ void kq_attn_kernel(const AttnArg a) {
                 at = have[t] ? at : 0;
                 const int64_t o = (uint32_t)page * a.page_b + (int64_t)((uint64_t)(uint32_t)at * a.tok_b);
 #pragma unroll
-                for (int j = 0; j < 4; j++) vp[4 * t + j] = vh + (TILED ? o + j * a.tok_b : (int64_t)__shfl(o, 4 * g + j));
+                for (int j = 0; j < 4; j++)
+                    vp[4 * t + j] = vh + (TILED ? o + j * a.tok_b : (int64_t)__shfl(o, 4 * g + j));
                 sp[t] = (int64_t)((uint64_t)(uint32_t)page * a.page_s) + (h * a.page + at);
 #pragma unroll
                 for (int ch = 0; ch < NCH; ch++) {
@@ -672,7 +683,9 @@ void kq_attn_kernel(const AttnArg a) {
         const uint64_t x = __hip_atomic_load(static_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         return make_float2(__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32)));
     };
-    // JU quads of JN results that a lane has in flight
+    // JU quads of JN results that a lane has in flight.  By eights where there are more than
+    // FLAT quads (of 6 rows of 256, 16 parts: all at once 18 us a call, by eights 24; 64
+    // parts: 46 and 40).
     constexpr int JU = 2, JN = 8, FLAT = 12288;
     // n results, `by` apart from slot `from` on, to the first's place or, `end`, to out
     auto join = [&](int from, int by, int of, bool end) {
@@ -762,6 +775,12 @@ extern "C" {
 void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
     z->blocks = (s->T * (s->n_q / s->n_kv) + 15) / 16;
     const int per = s->n_kv * z->blocks;
+    // Two workgroups on each CU, in one round, where sequences are few (8 of 8192 keys, 16 / 8
+    // heads of 128, 320 / 448 / 512 / 576 workgroups: 65 / 56 / 55 / 63 us; one of 32768, heads
+    // of 256, 256 / 512: 39 / 43); beyond, one on each more than there are sequences (64 ragged
+    // ones, 400 / 500 / 756: 114 / 100 / 103).  128 keys an item where that is a workgroup on
+    // every fourth CU at most, 256 otherwise (one sequence, heads of 256, of 1024: 13.2 / 17.1,
+    // of 4096: 20.0 / 18.3).
     const int one = (n_cu + per - 1) / per;       // items for a workgroup on each CU
     z->few = 32 * n_cu / per;
     const int extra = 2 * one - s->S > one ? 2 * one - s->S : one;

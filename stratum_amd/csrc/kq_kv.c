@@ -103,6 +103,13 @@ int kq_kv_plan_dev(const kq_kv_plan* in, kq_stream stream) {
                                 p.n_free_out, p.start, p.lens, p.pos, p.slot, p.n_short};
     for (unsigned i = 0; i < sizeof ints / sizeof *ints; i++)
         if (misaligned(ints[i], 4)) return kq_fail("%s: operands must be 4-byte aligned", who);
+    /* inputs, then outputs, which may be held and n_free where they are held_out and n_free_out */
+    const void* const in_out[] = {p.cached, p.n_new, p.free_pages, p.held, p.n_free, p.held_out, p.n_free_out,
+                                  p.table, p.start, p.lens, p.pos, p.slot, p.n_short};
+    for (unsigned i = 0; i < sizeof in_out / sizeof *in_out; i++)
+        for (unsigned j = i < 5 ? 5 : i + 1; j < sizeof in_out / sizeof *in_out; j++)
+            if (in_out[i] && in_out[i] == in_out[j] && !(i == 3 && j == 5) && !(i == 4 && j == 6))
+                return kq_fail("%s: an output is another operand's buffer", who);
     memset(&z, 0, sizeof z);
     if (p.list) {
         if (shape_check(&p.shape, who)) return -1;

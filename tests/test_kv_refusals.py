@@ -50,8 +50,9 @@ def test_shapes(kw, word):
 
 
 def plan(**kw):
-    a = dict(S=2, page=16, n_pages=100, cached_ptr=P, new_ptr=P, table_ptr=P, table_stride=10, free_ptr=P, n_free_ptr=P,
-             lens_ptr=P, start_ptr=P, N=8, pos_ptr=P, slot_ptr=P)
+    at = [P * i for i in range(1, 10)]
+    a = dict(S=2, page=16, n_pages=100, cached_ptr=at[0], new_ptr=at[1], table_ptr=at[2], table_stride=10, free_ptr=at[3],
+             n_free_ptr=at[4], lens_ptr=at[5], start_ptr=at[6], N=8, pos_ptr=at[7], slot_ptr=at[8])
     a.update(kw)
     return K.kv_plan(**a)
 
@@ -67,6 +68,9 @@ def plan(**kw):
     (dict(N=0), "N=0"), (dict(N=-1), "N=-1"), (dict(cached_ptr=P + 2), "aligned"), (dict(slot_ptr=P + 1), "aligned"),
     (dict(n_free_ptr=P + 2), "aligned"), (dict(short_ptr=P + 2), "aligned"),
     (dict(list_ptr=P, list_bytes=1 << 40, shape=shape(S=3)), "shape of S=3"),
+    (dict(lens_ptr=P), "another operand"), (dict(held_out_ptr=P), "another operand"), (dict(n_free_out_ptr=4 * P), "another operand"),
+    (dict(held_ptr=10 * P, held_out_ptr=5 * P), "another operand"), (dict(slot_ptr=8 * P), "another operand"),
+    (dict(short_ptr=3 * P), "another operand"), (dict(start_ptr=2 * P), "another operand"),
 ])
 def test_plan_refuses(kw, word):
     refused(K.lib().kq_kv_plan_dev(ctypes.byref(plan(**kw)), None), word)
