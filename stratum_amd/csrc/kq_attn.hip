@@ -776,14 +776,17 @@ void kqk_attn_plan(const kq_attn_shape* s, int n_cu, kqk_attn_sizes* z) {
     z->blocks = (s->T * (s->n_q / s->n_kv) + 15) / 16;
     const int per = s->n_kv * z->blocks;
     // Two workgroups on each CU, in one round, where sequences are few (8 of 8192 keys, 16 / 8
-    // heads of 128, 320 / 448 / 512 / 576 workgroups: 65 / 56 / 55 / 63 us; one of 32768, heads
-    // of 256, 256 / 512: 39 / 43); beyond, one on each more than there are sequences (64 ragged
-    // ones, 400 / 500 / 756: 114 / 100 / 103).  128 keys an item where that is a workgroup on
-    // every fourth CU at most, 256 otherwise (one sequence, heads of 256, of 1024: 13.2 / 17.1,
-    // of 4096: 20.0 / 18.3).
+    // heads of 128, 320 / 448 / 512 / 576 workgroups: 65 / 56 / 55 / 63 us), one with heads
+    // past 128 values, of which the join of more is longer (heads of 256, 256 / 512
+    // workgroups: one of 32768 39 / 43.6, 8 of 8192 59 / 65, 8 of 500 to 20000 51 / 56; int8
+    // heads of 128 are the other way, 46 / 34); beyond, one on each more than there are
+    // sequences (64 ragged ones, 400 / 500 / 756: 114 / 100 / 103).  128 keys an item where
+    // that is a workgroup on every fourth CU at most, 256 otherwise (one sequence, heads of
+    // 256, of 1024: 13.2 / 17.1, of 4096: 20.0 / 18.3).
     const int one = (n_cu + per - 1) / per;       // items for a workgroup on each CU
     z->few = 32 * n_cu / per;
-    const int extra = 2 * one - s->S > one ? 2 * one - s->S : one;
+    const int few = s->D > 128 && 8 * s->S <= one ? one : 2 * one;
+    const int extra = few - s->S > one || few == one ? few - s->S : one;
     z->cap = s->S + extra;
     z->parts = 2 * extra;                         // (a split sequence has two items or more)
     z->counters = (int64_t)z->parts * per;
