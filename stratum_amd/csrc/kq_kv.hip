@@ -171,8 +171,10 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
         wg_scan<3>(units, sm[0], before, all);
         const uint64_t total = ((uint64_t)all[1] << 16) + all[0];
         const uint32_t extra = a.cap - p.S, cap = all[2] + extra;
-        // x / n rounded up, or a little more (x past 2^24)
+        // x / n rounded up, or a little more (x past 2^24), and 2^26 where it is above, which
+        // is more units than a sequence has
         auto over = [](uint64_t x, uint32_t n) {
+            if (x >= (uint64_t)n << 26) return 1u << 26;
             uint32_t y = (uint32_t)((float)x / (float)n);
             while ((uint64_t)y * n < x) y++;
             return y;
@@ -194,7 +196,7 @@ __global__ __launch_bounds__(PT) void kq_kv_plan_kernel(const PlanArg a) {
                 else lo = mid + 1;
             }
         }
-        share = min(most, 0x7fffffu) * ROUND;
+        share = min(most, 0x1ffffffu) * ROUND;
     }
     uint32_t tok0 = 0, page0 = 0, taken = 0, shorts = 0, item0 = 0, part0 = 0;
     for (int s0 = 0; s0 < p.S; s0 += T) {

@@ -216,6 +216,22 @@ def test_list(S, T, n_kv, window, longest, new):
     assert (lst[used:-8] >= -7).all() and ((lst[used:-8] == 0) | (lst[used:-8] == -7)).all()
 
 
+@pytest.mark.parametrize("S", [3, 1000])
+def test_list_of_the_longest_lengths(S):
+    """Lengths above 2^30 - 1 count as that; as many keys as a list may have to share out."""
+    shape = K.attn_shape(S, 1, 1024, 1024, 128)
+    nb = K.kv_list_bytes(shape)
+    lst, cached, lens = torch.empty(nb // 4, dtype=torch.int32, device="cuda"), ints(np.full(S, 2 ** 31 - 1)), ints(np.zeros(S))
+    K.kv_plan_dev(K.kv_plan(S, 16, 1, cached.data_ptr(), lens_ptr=lens.data_ptr(), shape=shape, list_ptr=lst.data_ptr(),
+                            list_bytes=nb), st())
+    torch.cuda.synchronize()
+    assert (lens == 2 ** 30).all()
+    lst = lst.cpu().numpy()
+    items = lst[8:8 + 8 * lst[0]].reshape(-1, 8).astype(np.int64)
+    assert lst[0] <= S + 1 and sorted(set(items[:, 0])) == list(range(S))
+    assert (items[:, 2] - items[:, 1]).sum() == S * 2 ** 30
+
+
 def test_plan_captured():
     """A replayed graph of the call follows its lengths."""
     S, page = 70, 16
