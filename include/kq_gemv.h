@@ -752,7 +752,7 @@ int kq_kv_store_dev(const kq_kv_store* a, kq_stream stream);
  *   out = sum_j p_j v_j,  p = softmax over the keys j that the token sees of scale q . k_j
  * q and out: N rows of n_q heads of D binary32 values, q_stride and out_stride
  * elements apart (0: n_q * D; multiples of 4), 16-byte aligned; they do not overlap.
- * table: S rows of table_stride page numbers.  Keys past the table, and keys
+ * table: S rows of table_stride page numbers.  Keys past the table, past 2^31 - 2^16, and keys
  * on pages outside 0..n_pages-1, are not seen; a token that sees no key gets zeros.
  * What a token does not see does not reach it, whatever it holds.  Sequences of more
  * than T new tokens, rows of none and rows outside 0..N-1 are left as they are.

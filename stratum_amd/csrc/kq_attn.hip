@@ -63,7 +63,7 @@ struct AttnArg {
     uint32_t tok_b, page_s;     // (page_s: scales of a page)
     uint64_t div, kv_div, blocks_div;    // page / 16, n_kv and 8 blocks by multiplication
     float qscale;               // scale log2 e
-    int S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts, blocks;
+    int div_shift, S, T, G, R, n_kv, D, window, N, page, n_pages, table_stride, cap, parts, blocks;
 };
 
 __device__ __forceinline__ uint32_t perm(uint32_t hi, uint32_t lo, uint32_t sel) {
@@ -229,7 +229,7 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
             for (int t = 0; t < 2; t++) {
                 uint32_t b;
-                if constexpr (TILED) b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                if constexpr (TILED) b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> a.div_shift);
                 else b = (uint32_t)(kb + 16 * t + c) / (uint32_t)a.page;
                 pg[t] = b < (uint32_t)a.table_stride ? table[b] : -1;
             }
@@ -250,7 +250,7 @@ void kq_attn_kernel(const AttnArg a) {
                 have[t] = (uint32_t)page < (uint32_t)a.n_pages;
                 page = have[t] ? page : 0;
                 if constexpr (TILED) {
-                    const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> 40);
+                    const uint32_t b = (uint32_t)(((uint64_t)(uint32_t)(kb / 16 + t) * a.div) >> a.div_shift);
                     at = kb + 16 * t - (int)(b * (uint32_t)a.page);
                 } else {
                     at = (int)((uint32_t)(kb + 16 * t + c) % (uint32_t)a.page);
@@ -835,9 +835,12 @@ int kqk_launch_attn(const kq_paged_attn* p, const kqk_attn_sizes* z, void* work,
     a.parts = z->parts;
     const bool tiled = c.page % 16 == 0;
     if (tiled) {
-        // (b d = 2^40 + e with e < d = page / 16 <= 2^12: tiles below 2^27 are divided exactly)
+        // div d = 2^shift + e with e < d = page / 16 and 2^27 d <= 2^shift < 2^28 d: tiles below
+        // 2^27 (keys below 2^31) are divided exactly, their products below 2^56
         const uint64_t d = c.page / 16;
-        a.div = (((uint64_t)1 << 40) + d - 1) / d;
+        a.div_shift = 27;
+        while ((uint64_t)1 << (a.div_shift - 27) < d) a.div_shift++;
+        a.div = (((uint64_t)1 << a.div_shift) + d - 1) / d;
     }
     if (p->list) {
         a.count = (const int*)p->list;

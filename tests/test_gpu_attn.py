@@ -416,6 +416,23 @@ def test_past_32_bits():
     both(c)
 
 
+@pytest.mark.parametrize("page", [16, 32, 48, 112, 128])
+@pytest.mark.parametrize("t", [K.TYPE_F16, K.TYPE_I8])
+def test_long_tables(t, page):
+    """Keys past the first 2^24 pages of a table, of which a window hides those before: the same bits as of
+    a table of the last pages, with as many keys fewer."""
+    c = Case(24, t, [5 * page + 3], [2], 4, 2, 64, page=page, window=2 * page + 5)
+    want = c.run(False)
+    c.check(want)
+    before = (2 ** 31 - 2 ** 17 - 8 * page) // page // 32 * 32 if page > 112 else 2 ** 24
+    tail = c.table
+    c.table = np.zeros((1, before + tail.shape[1]), np.int32)
+    c.table[0, before:] = tail
+    c.lens = c.lens + before * page
+    del c.d
+    assert torch.equal(torch.nan_to_num(want), torch.nan_to_num(c.run(False)))
+
+
 def test_repeatable_and_equal_in_a_batch():
     """The same bits from call to call, also where sequences are split."""
     c = Case(22, K.TYPE_F16, [9000, 300, 40], [1, 2, 1], 24, 4, 256)
