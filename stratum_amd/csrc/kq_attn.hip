@@ -201,6 +201,8 @@ void kq_attn_kernel(const AttnArg a) {
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
     // number all are taken again without such values, which are then added alone.
+    // So are sums past 2^96, of large bfloat16 values, with weights (and their sum)
+    // times 2^-40: 2^30 values of any size stay finite, where the result is.
     bool careful = false;
 #pragma unroll 1
     while (true) {
@@ -510,7 +512,7 @@ void kq_attn_kernel(const AttnArg a) {
             // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
             // with int8 values' scales below 2^16)
             u32x4 w[NP];
-            const float base = (m == -INFINITY ? 0.0f : m) - (NP == 2 ? 9.0f : 0.0f);
+            const float base = (m == -INFINITY ? 0.0f : m) - (NP == 2 ? 9.0f : careful ? -40.0f : 0.0f);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
                 float p = exp2_(x[j] - base), q = exp2_(x[j + 1] - base);
@@ -580,12 +582,13 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                 for (int t = 0; t < W; t++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) none = fmaf(acc[b][t][i], 0.0f, none);
+                    for (int i = 0; i < 4; i++) none = fmaf(acc[b][t][i], 0x1p32f, none);
         }
         // (a barrier: queries have been read)
-        if (!__syncthreads_or(none != 0.0f) || careful) break;
+        if (!__syncthreads_or(!__builtin_isfinite(none)) || careful) break;
         careful = true;
     }
+    if (NP == 3 && careful && m != -INFINITY) m += 40.0f;         // (what the weights were taken from)
 
     // ---- the waves' sums
     l = sum4(l);

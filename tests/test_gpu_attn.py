@@ -416,6 +416,21 @@ def test_past_32_bits():
     both(c)
 
 
+@pytest.mark.parametrize("lens,new", [([200, 33, 9000], [2, 1, 1]), ([20000, 5], [1, 3])])
+@pytest.mark.parametrize("size", [1e27, 3e33, 7e37])
+def test_large_bfloat16_values(lens, new, size):
+    """Sums of weights up to 2^5 and values near the type's largest pass binary32's range; their quotient does
+    not.  One sequence has large values in the last keys only, so that its shares differ in how they are summed."""
+    c = Case(25, K.TYPE_BF16, lens, new, 8, 2, 64)
+    for s in range(len(lens)):
+        x = c.rows[s].float()
+        x[1] = (x[1].clamp(-4, 4) * size)
+        if s == 0:
+            x[1, :, :lens[0] // 2] /= 1e20
+        c.put(s, x)
+    both(c)
+
+
 @pytest.mark.parametrize("page", [16, 32, 48, 112, 128])
 @pytest.mark.parametrize("t", [K.TYPE_F16, K.TYPE_I8])
 def test_long_tables(t, page):
