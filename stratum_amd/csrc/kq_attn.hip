@@ -197,7 +197,7 @@ void kq_attn_kernel(const AttnArg a) {
     int lo, hi;                             // the keys that a lane's row sees
     float m, l;
     f32x4 acc[NB][W];
-    int ve;                                 // int8: the sums' exponent
+    int ve;                                 // int8: the exponent of the lane's row of sums
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
     // number all are taken again without such values, which are then added alone.
@@ -459,28 +459,6 @@ void kq_attn_kernel(const AttnArg a) {
                 if (nb + 32 * NW < k1) fetch(nb + 32 * NW);
             }
             // weights
-            if constexpr (TYPE == KQ_TYPE_I8) {
-                // the sums are kept times a power of two that is near the largest scale so far
-                // (but for infinite ones, of keys that not all rows may see)
-                float top = 0.0f;
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const float v = fabsf(vscale[j]);
-                    top = fmaxf(top, full || v < INFINITY ? v : 0.0f);
-                }
-                const int e = min(253, uniform((int)(__float_as_uint(max4(top)) >> 23)));
-                if (e > ve) {
-                    const float f = __uint_as_float((uint32_t)max(0, 127 + ve - e) << 23);
-                    ve = e;
-#pragma unroll
-                    for (int b = 0; b < NB; b++)
-#pragma unroll
-                        for (int t = 0; t < W; t++) acc[b][t] *= f;
-                }
-                const float f = __uint_as_float((uint32_t)(254 - ve) << 23);
-#pragma unroll
-                for (int j = 0; j < 8; j++) vscale[j] *= f;
-            }
             float x[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -508,6 +486,27 @@ void kq_attn_kernel(const AttnArg a) {
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int t = 0; t < W; t++) acc[b][t] *= f;
+            }
+            if constexpr (TYPE == KQ_TYPE_I8) {
+                // a row's sums are kept times a power of two that is near the largest scale so
+                // far of the keys that it sees (every lane of a row has the same)
+                float big = 0.0f;
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    big = fmaxf(big, full || x[j] != -INFINITY ? fabsf(vscale[j]) : 0.0f);
+                const int e = min(253, (int)(__float_as_uint(max4(big)) >> 23));
+                if (__any(e > ve)) {
+                    const int top = max(e, ve);
+                    const float f = __uint_as_float((uint32_t)max(0, 127 + ve - top) << 23);
+                    ve = top;
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+#pragma unroll
+                        for (int t = 0; t < W; t++) acc[b][t] *= f;
+                }
+                const float f = __uint_as_float((uint32_t)(254 - ve) << 23);
+#pragma unroll
+                for (int j = 0; j < 8; j++) vscale[j] *= f;
             }
             // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
             // with int8 values' scales below 2^16)

@@ -595,3 +595,23 @@ def test_decode_steps(t, listed):
         for s in range(S):
             past[s] = past[s][:cached[s] + keep[s]]
         cached = cached + keep
+
+
+def scale_values(c, s, keys, f):
+    """The value scales of these keys of sequence s times f (one factor, or one a key)."""
+    page, at = c.places(s)
+    for e, x in zip(keys, np.broadcast_to(f, len(keys))):
+        old = c.sc[1][int(page[e]), :, int(at[e])].clone()
+        new = old * float(x)
+        c.sc[1][int(page[e]), :, int(at[e])] = new
+        c.rows[s][1][:, e] *= (new.double() / old.double()).unsqueeze(-1)
+
+
+@pytest.mark.parametrize("size", [1e5, 1e10, 1e30])
+@pytest.mark.parametrize("n_q,n_kv,D,page", [(4, 2, 128, 16), (12, 2, 80, 7), (2, 1, 256, 32)])
+def test_finite_scales_of_hidden_keys_do_not_reach_a_token(n_q, n_kv, D, page, size):
+    """Large value scales of later tokens and of tokens before a window: the bound knows only those that are seen."""
+    c = Case(26, K.TYPE_I8, [50, 400], [6, 5], n_q, n_kv, D, page, window=100)
+    for s, places in ((0, (46, 48)), (1, (397, 290, 299, 60))):
+        scale_values(c, s, places, size)
+    both(c)
