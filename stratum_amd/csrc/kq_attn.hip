@@ -197,7 +197,8 @@ void kq_attn_kernel(const AttnArg a) {
     int lo, hi;                             // the keys that a lane's row sees
     float m, l;
     f32x4 acc[NB][W];
-    int ve;                                 // int8: the exponent of the lane's row of sums
+    constexpr int VE0 = 11;                 // int8: the sums are acc 2^(ve - 137), of one ve a row
+    int ve;
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
     // number all are taken again without such values, which are then added alone.
@@ -373,7 +374,7 @@ void kq_attn_kernel(const AttnArg a) {
         const float inv = NP == 2 ? s_inv[c] : 1.0f;
         m = -INFINITY;
         l = 0.0f;
-        ve = 1;
+        ve = VE0;
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -477,26 +478,47 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
             for (int j = 1; j < 8; j++) top = fmaxf(top, x[j]);
             top = max4(top);
-            // (2^5 above the maximum that the weights are taken from before that is moved)
+            // (2^5 above the maximum that the weights are taken from before that is moved; int8: by
+            // whole steps, which the exponent takes)
             if (__any(top > m + 5.0f)) {
-                const float nm = fmaxf(m, top), f = nm == -INFINITY ? 1.0f : exp2_(m - nm);
-                m = nm;
+                const float nm = fmaxf(m, TYPE == KQ_TYPE_I8 ? ceilf(top) : top);
+                float f = nm == -INFINITY ? 1.0f : exp2_(m - nm);
                 l *= f;
+                if constexpr (TYPE == KQ_TYPE_I8) {
+                    const int e = ve - (int)fminf(nm - m, 1000.0f);
+                    ve = max(e, VE0);
+                    f = __uint_as_float((uint32_t)max(0, 127 + e - ve) << 23);
+                }
+                m = nm;
 #pragma unroll
                 for (int b = 0; b < NB; b++)
 #pragma unroll
                     for (int t = 0; t < W; t++) acc[b][t] *= f;
             }
+            // binary16: times 2^9, which leaves with the division by the sum; int8: times 2^-6, so
+            // that weights up to 2^5 times their values' scales stay finite
+            const float base =
+                (m == -INFINITY ? 0.0f : m) - (TYPE == KQ_TYPE_I8 ? -6.0f : NP == 2 ? 9.0f : careful ? -40.0f : 0.0f);
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                p[j] = exp2_(x[j] - base);
+                p[j + 1] = exp2_(x[j + 1] - base);
+                l += p[j] + p[j + 1];
+            }
             if constexpr (TYPE == KQ_TYPE_I8) {
-                // a row's sums are kept times a power of two that is near the largest scale so
-                // far of the keys that it sees (every lane of a row has the same)
+                // A row's sums are those of weights times scales, in units of a power of two that
+                // puts the largest of these so far (of the keys that the row sees) from 2^10 to
+                // 2^15.  (A hidden key's scale may be no number.)
                 float big = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 8; j++)
-                    big = fmaxf(big, full || x[j] != -INFINITY ? fabsf(vscale[j]) : 0.0f);
+                for (int j = 0; j < 8; j++) {
+                    p[j] = full || x[j] != -INFINITY ? p[j] * vscale[j] : 0.0f;
+                    big = fmaxf(big, fabsf(p[j]));
+                }
                 const int e = min(253, (int)(__float_as_uint(max4(big)) >> 23));
-                if (__any(e > ve)) {
-                    const int top = max(e, ve);
+                if (__any(e > ve + 4)) {
+                    const int top = e > ve + 4 ? e : ve;
                     const float f = __uint_as_float((uint32_t)max(0, 127 + ve - top) << 23);
                     ve = top;
 #pragma unroll
@@ -504,25 +526,15 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                         for (int t = 0; t < W; t++) acc[b][t] *= f;
                 }
-                const float f = __uint_as_float((uint32_t)(254 - ve) << 23);
+                const float f = __uint_as_float((uint32_t)(264 - ve) << 23);
 #pragma unroll
-                for (int j = 0; j < 8; j++) vscale[j] *= f;
+                for (int j = 0; j < 8; j++) p[j] *= f;
             }
-            // binary16: times 2^9, which leaves with the division by the sum (2^15 at most,
-            // with int8 values' scales below 2^16)
             u32x4 w[NP];
-            const float base = (m == -INFINITY ? 0.0f : m) - (NP == 2 ? 9.0f : careful ? -40.0f : 0.0f);
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                float p = exp2_(x[j] - base), q = exp2_(x[j + 1] - base);
-                l += p + q;
-                if constexpr (TYPE == KQ_TYPE_I8) {
-                    // (a hidden key's scale may be no number)
-                    p = full || x[j] != -INFINITY ? p * vscale[j] : 0.0f;
-                    q = full || x[j + 1] != -INFINITY ? q * vscale[j + 1] : 0.0f;
-                }
                 uint32_t o[NP];
-                split<NP>(p, q, o);
+                split<NP>(p[j], p[j + 1], o);
 #pragma unroll
                 for (int e = 0; e < NP; e++) w[e][j >> 1] = o[e];
             }
@@ -606,7 +618,7 @@ void kq_attn_kernel(const AttnArg a) {
             s_all[c] = make_float2(top, sum);
         }
         float f = exp2_(m - base);
-        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)ve << 23);
+        if constexpr (TYPE == KQ_TYPE_I8) f *= __uint_as_float((uint32_t)(ve - 10) << 23);
         if (c < live) {
 #pragma unroll
             for (int b = 0; b < NB; b++)

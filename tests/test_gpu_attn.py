@@ -615,3 +615,77 @@ def test_finite_scales_of_hidden_keys_do_not_reach_a_token(n_q, n_kv, D, page, s
     for s, places in ((0, (46, 48)), (1, (397, 290, 299, 60))):
         scale_values(c, s, places, size)
     both(c)
+
+
+def check_int8(c, out):
+    """The module's bound with the loss of an int8 cache's weights taken at what they multiply.  A weight times
+    its value's scale is two binary16 numbers of a power of two that puts the row's largest such product from
+    2^10 on, so that 2^-25 / 2^10 = 2^-35 of that one goes missing at most, times 128: L 2^-28 max p s in all."""
+    G, D = c.n_q // c.n_kv, c.D
+    got = out[:, :c.n_q * D].double().view(c.N, c.n_q, D)
+    for s in range(c.S):
+        page, at = c.places(s)
+        p_, a_ = torch.from_numpy(page).cuda(), torch.from_numpy(at).cuda()
+        scales = c.sc[1][p_, :, a_].double().t().abs()
+        for i in range(int(c.new[s])):
+            r = int(c.start[s]) + i
+            keys = torch.from_numpy(c.seen(s, i)).cuda()
+            k, v = c.rows[s][0][:, keys], c.rows[s][1][:, keys]
+            q = c.q[r, :c.n_q * D].double().view(c.n_kv, G, D) * float(np.float32(c.scale))
+            x = torch.matmul(q, k.transpose(1, 2).contiguous())
+            X = torch.matmul(q.abs(), k.abs().transpose(1, 2).contiguous())
+            p = torch.softmax(x, -1)
+            want, pv = torch.matmul(p, v).reshape(c.n_q, D), torch.matmul(p, v.abs()).reshape(c.n_q, D)
+            e = X.amax(-1) * (2.0 ** -21 + (D + 8) * U) + 4 * U * x.abs().amax(-1) + \
+                2.0 ** -38 * q.abs().amax(-1) * k.abs().sum(-1).amax(-1, keepdim=True)
+            ps = (p * scales[:, keys].unsqueeze(1)).amax(-1).reshape(c.n_q, 1)
+            tol = pv * (2 * e.reshape(c.n_q, 1) + 2.0 ** -20 + (4 * len(keys) + 200) * U) + len(keys) * 2.0 ** -28 * ps + 2.0 ** -126
+            bad = ~((got[r] - want).abs() <= tol)
+            assert not bad.any(), (s, i, int(bad.sum()), float((got[r] - want).abs().max()), float(tol.max()))
+
+
+def steer(c, scores):
+    """Keys become multiples of one vector, queries all ones, so that sequence s's scores are those given."""
+    c.q.fill_(1.0)
+    g = torch.Generator(device="cuda").manual_seed(27)
+    for s, x in enumerate(scores):
+        L = int(c.lens[s])
+        y = torch.randn(2, c.n_kv, L, c.D, generator=g, device="cuda")
+        y[0] = (torch.from_numpy(np.asarray(x, dtype=np.float32)).cuda() / (c.D * c.scale)).view(1, L, 1)
+        c.put(s, y)
+
+
+@pytest.mark.parametrize("size", [2.0 ** 30, 2.0 ** 40, 2.0 ** 70, 2.0 ** 100])
+@pytest.mark.parametrize("D,page", [(128, 16), (80, 7), (256, 32), (64, 16)])
+def test_int8_scales_under_small_weights(D, page, size):
+    """Values of large scales whose keys have scores of -50 beside others of about 0: first, last, a step of keys
+    at once, and before a window, where the maximum moves past them."""
+    lens = [40, 700, 300, 3000]
+    at = [[3], [0, 699], list(range(32)), list(range(64, 96)) + [2999]]
+    c = Case(28, K.TYPE_I8, lens, [1, 2, 1, 3], 6, 2, D, page)
+    g = np.random.default_rng(29)
+    scores = [0.3 * g.standard_normal(n) for n in lens]
+    for x, j in zip(scores, at):
+        x[j] = -50.0
+    steer(c, scores)
+    for s in range(4):
+        scale_values(c, s, at[s], size)
+    for listed in (False, True):
+        check_int8(c, c.run(listed))
+
+
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("D,page", [(128, 16), (72, 5), (256, 16)])
+def test_int8_scales_of_any_size_under_any_weight(D, page, T):
+    """Scores of -40 to 40 and scales from 2^-50 to 2^50, in any order, rising and falling against each other."""
+    lens = [90, 33, 500, 6000, 400, 400]
+    c = Case(30, K.TYPE_I8, lens, [1, 1, T, T, T, T], 4, 2, D, page, window=350)
+    g = np.random.default_rng(31)
+    scores, scales = [g.uniform(-40, 40, n) for n in lens], [2.0 ** g.uniform(-50, 50, n) for n in lens]
+    scores[4], scales[4] = np.linspace(-60, 60, 400), 2.0 ** np.linspace(80, -80, 400)
+    scores[5], scales[5] = np.linspace(60, -60, 400), 2.0 ** np.linspace(-80, 80, 400)
+    steer(c, scores)
+    for s, n in enumerate(lens):
+        scale_values(c, s, range(n), scales[s])
+    for listed in (False, True):
+        check_int8(c, c.run(listed))
