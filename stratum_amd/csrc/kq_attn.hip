@@ -603,6 +603,15 @@ void kq_attn_kernel(const AttnArg a) {
 
     // ---- the waves' sums
     l = sum4(l);
+    if constexpr (TYPE == KQ_TYPE_I8) {
+        // (where products pass 2^33, sums of them and of weights times 2^-64: 2^30 values of any
+        // scale stay finite, where the result is)
+        if (ve > 160) {
+            ve -= 64;
+            l *= 0x1p-64f;
+            m += 64.0f;
+        }
+    }
     if (g == 0) s_ml[wave][c] = make_float2(m, l);
     __syncthreads();
     float* const ol = reinterpret_cast<float*>(lds);

@@ -689,3 +689,21 @@ def test_int8_scales_of_any_size_under_any_weight(D, page, T):
         scale_values(c, s, range(n), scales[s])
     for listed in (False, True):
         check_int8(c, c.run(listed))
+
+
+@pytest.mark.parametrize("lens,new", [([200, 33, 9000], [2, 1, 1]), ([20000, 5], [1, 3])])
+@pytest.mark.parametrize("size", [1e27, 3e33, 7e37])
+def test_large_int8_scales(lens, new, size):
+    """Sums of weights and values of scales near binary32's largest pass its range; their quotient does not.  One
+    sequence has large values in the last keys only, so that its shares differ in how they are summed."""
+    c = Case(32, K.TYPE_I8, lens, new, 8, 2, 64)
+    for s in range(len(lens)):
+        x = c.rows[s].float()
+        x[1] = x[1].clamp(-4, 4) * size
+        if s == 0:
+            x[1, :, :lens[0] // 2] /= 1e20
+        c.put(s, x)
+    for listed in (False, True):
+        out = c.run(listed)
+        c.check(out)
+        check_int8(c, out)
