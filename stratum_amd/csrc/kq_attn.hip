@@ -202,9 +202,12 @@ void kq_attn_kernel(const AttnArg a) {
     // An infinity or NaN among the values would reach rows that do not see its key, and
     // an infinity as NaN those that do, as 0 times itself.  Where a sum ends as no
     // number all are taken again without such values, which are then added alone.
-    // So are sums past 2^96, of large bfloat16 values, with weights (and their sum)
-    // times 2^-40: 2^30 values of any size stay finite, where the result is.
-    bool careful = false;
+    // So are sums past 2^96, of large bfloat16 values, and rows in which they are that still
+    // once more, with weights (and their sum) times 2^-40: 2^30 values of any size stay
+    // finite, where the result is.  (Rows of other sums keep theirs, as 2^-40 costs small
+    // values bits.)
+    int pass = 0;
+    float less = 0.0f;
 #pragma unroll 1
     while (true) {
         // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
@@ -498,7 +501,7 @@ void kq_attn_kernel(const AttnArg a) {
             // binary16: times 2^9, which leaves with the division by the sum; int8: times 2^-6, so
             // that weights up to 2^5 times their values' scales stay finite
             const float base =
-                (m == -INFINITY ? 0.0f : m) - (TYPE == KQ_TYPE_I8 ? -6.0f : NP == 2 ? 9.0f : careful ? -40.0f : 0.0f);
+                (m == -INFINITY ? 0.0f : m) - (TYPE == KQ_TYPE_I8 ? -6.0f : NP == 2 ? 9.0f : -less);
             float p[8];
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
@@ -550,7 +553,7 @@ void kq_attn_kernel(const AttnArg a) {
                         for (int e = 0; e < VW; e++) vr[j][b][e] &= keep;
                 }
             }
-            if (ES == 2 && careful) {
+            if (ES == 2 && pass) {
                 constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -595,11 +598,12 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) none = fmaf(acc[b][t][i], 0x1p32f, none);
         }
+        const bool bad = c < live && !__builtin_isfinite(none);
         // (a barrier: queries have been read)
-        if (!__syncthreads_or(!__builtin_isfinite(none)) || careful) break;
-        careful = true;
+        if (!__syncthreads_or(bad) || pass == NP - 1) break;
+        if (++pass == 2) less = max4(bad ? 40.0f : 0.0f);
     }
-    if (NP == 3 && careful && m != -INFINITY) m += 40.0f;         // (what the weights were taken from)
+    if (NP == 3 && m != -INFINITY) m += less;               // (what the weights were taken from)
 
     // ---- the waves' sums
     l = sum4(l);
@@ -660,7 +664,7 @@ void kq_attn_kernel(const AttnArg a) {
         f32x4 y = *reinterpret_cast<const f32x4*>(ol + r * OS + d);
 #pragma unroll
         for (int i = 1; i < NW; i++) y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
-        if (ES == 2 && careful) {
+        if (ES == 2 && pass) {
             // values that are no numbers, for the rows that see them
             const int last = len - n + (first + r) / G, end = min(last + 1, k1);
 #pragma unroll 1

@@ -707,3 +707,18 @@ def test_large_int8_scales(lens, new, size):
         out = c.run(listed)
         c.check(out)
         check_int8(c, out)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf"), 3e38])
+@pytest.mark.parametrize("n_q,D,page", [(4, 128, 16), (12, 80, 7), (2, 256, 16)])
+def test_hidden_values_do_not_cost_small_ones_bits(n_q, D, page, bad):
+    """bfloat16 values of 1e-30 beside infinities, NaN and values near the largest that tokens do not see."""
+    c = Case(33, K.TYPE_BF16, [50, 400], [6, 5], n_q, 2, D, page, window=100)
+    for s, places in ((0, (46, 48)), (1, (397, 290, 299, 60))):
+        x = c.rows[s].float()
+        x[1] *= 1e-30
+        x[1][:, list(places)] = bad
+        c.put(s, x)
+    # tokens 44.. of 50 and 395.. of 400; the windows start at 0 and 296..300
+    skip = {(0, i) for i in range(2, 6)} | {(1, i) for i in (0, 1, 2, 3, 4) if i >= 2 or 296 + i <= 299}
+    both(c, skip=skip if not bad == 3e38 else ())
