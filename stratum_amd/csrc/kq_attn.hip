@@ -112,11 +112,6 @@ __device__ __forceinline__ uint32_t halves(uint32_t u) {
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u ^ 0x64806480u) - off);
 }
 
-template <int TYPE>
-__device__ __forceinline__ float value(uint32_t u) {
-    return TYPE == KQ_TYPE_F16 ? __half2float(__ushort_as_half((unsigned short)u)) : __uint_as_float(u << 16);
-}
-
 template <int NP>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     if constexpr (NP == 2)
@@ -149,7 +144,8 @@ void kq_attn_kernel(const AttnArg a) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[QB > OB ? QB : OB];
     __shared__ float2 s_ml[NW][16], s_all[16];
     __shared__ float s_inv[16];
-    __shared__ int s_last;
+    __shared__ int s_last, s_odd[NW][2];
+    __shared__ uint32_t s_inf[ES == 2 ? DM : 1];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int c = lane & 15, g = lane >> 4, D = EXACT ? DM : a.D, G = a.G;
@@ -206,8 +202,10 @@ void kq_attn_kernel(const AttnArg a) {
     // once more, with weights (and their sum) times 2^-40: 2^30 values of any size stay
     // finite, where the result is.  (Rows of other sums keep theirs, as 2^-40 costs small
     // values bits.)
+    // Rows whose weights' sum is no number stay as they are: so are all of their sums.
     int pass = 0;
     float less = 0.0f;
+    int odd0 = 0x7fffffff, odd1 = 0;        // keys among which are this wave's with such values
 #pragma unroll 1
     while (true) {
         // ---- queries: as 16-bit numbers in LDS, in the right operand's layout
@@ -554,17 +552,29 @@ void kq_attn_kernel(const AttnArg a) {
                 }
             }
             if (ES == 2 && pass) {
-                constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
+                // (an exponent of ones plus one is the sign's bit)
+                constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80, ONE = 0x8000 - NONE;
+                uint32_t sum = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++)
 #pragma unroll
                     for (int b = 0; b < NB; b++)
 #pragma unroll
-                        for (int e = 0; e < VW; e++) {
-                            const uint32_t v = vr[j][b][e];
-                            if ((v & 0x7fff) >= NONE) vr[j][b][e] &= 0xffff0000u;
-                            if ((v >> 16 & 0x7fff) >= NONE) vr[j][b][e] &= 0xffffu;
-                        }
+                        for (int e = 0; e < VW; e++) sum |= (vr[j][b][e] & 0x7fff7fffu) + ONE * 0x10001u;
+                if (__any((sum & 0x80008000u) != 0)) {
+                    odd0 = min(odd0, kb);
+                    odd1 = kb + 32;
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+#pragma unroll
+                        for (int b = 0; b < NB; b++)
+#pragma unroll
+                            for (int e = 0; e < VW; e++) {
+                                const uint32_t v = vr[j][b][e];
+                                if ((v & 0x7fff) >= NONE) vr[j][b][e] &= 0xffff0000u;
+                                if ((v >> 16 & 0x7fff) >= NONE) vr[j][b][e] &= 0xffffu;
+                            }
+                }
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -598,7 +608,8 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
                     for (int i = 0; i < 4; i++) none = fmaf(acc[b][t][i], 0x1p32f, none);
         }
-        const bool bad = c < live && !__builtin_isfinite(none);
+        const float sum = sum4(l);
+        const bool bad = c < live && __builtin_isfinite(sum) && !__builtin_isfinite(none);
         // (a barrier: queries have been read)
         if (!__syncthreads_or(bad) || pass == NP - 1) break;
         if (++pass == 2) less = max4(bad ? 40.0f : 0.0f);
@@ -617,6 +628,13 @@ void kq_attn_kernel(const AttnArg a) {
         }
     }
     if (g == 0) s_ml[wave][c] = make_float2(m, l);
+    if (ES == 2 && pass) {
+        if (lane == 0) {
+            s_odd[wave][0] = odd0;
+            s_odd[wave][1] = odd1;
+        }
+        if (tid < D) s_inf[tid] = 0;
+    }
     __syncthreads();
     float* const ol = reinterpret_cast<float*>(lds);
     const int quads = D / 4;
@@ -643,6 +661,61 @@ void kq_attn_kernel(const AttnArg a) {
                             (f32x4){acc[b][t][i], acc[b][t + 1][i], acc[b][t + 2][i], acc[b][t + 3][i]} * f;
         }
     }
+    if (ES == 2 && pass) {
+        // Which rows see infinities and NaN of a place in a row of values: bit r of s_inf for +inf,
+        // 16 + r for -inf, both for NaN.  A lane has eight places of every (2048 / D)th key, eight of them
+        // in flight (a lane's keys one by one: one sequence of 32768, heads of 256, with NaN in one
+        // key's values took 372 us for 52, 31 ms for 1.6 without a list).
+        int from = 0x7fffffff, to = 0;
+#pragma unroll
+        for (int i = 0; i < NW; i++) {
+            from = min(from, s_odd[i][0]);
+            to = max(to, s_odd[i][1]);
+        }
+        to = min(to, k1);
+        constexpr int KU = 8;
+        constexpr uint32_t NONE = TYPE == KQ_TYPE_F16 ? 0x7c00 : 0x7f80;
+        const int pieces = D / 8, by = 64 * NW / pieces, piece = tid % pieces, old = len - n;
+        uint32_t inf[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) inf[e] = 0;
+#pragma unroll 1
+        for (int64_t key0 = (int64_t)from + tid / pieces; key0 < to && tid < pieces * by; key0 += KU * by) {
+            int page[KU];
+            u32x4 v[KU];
+#pragma unroll
+            for (int u = 0; u < KU; u++) page[u] = table[(uint32_t)min(key0 + u * by, (int64_t)to - 1) / (uint32_t)a.page];
+#pragma unroll
+            for (int u = 0; u < KU; u++) {
+                const uint32_t key = (uint32_t)min(key0 + u * by, (int64_t)to - 1);
+                const bool there = (uint32_t)page[u] < (uint32_t)a.n_pages;
+                v[u] = *reinterpret_cast<const u32x4*>(vh + (there ? page[u] : 0) * a.page_b +
+                                                       (int64_t)((uint64_t)(key % (uint32_t)a.page) * a.tok_b) + 16 * piece);
+                if (!there) v[u] = (u32x4)0u;
+            }
+#pragma unroll
+            for (int u = 0; u < KU; u++) {
+                uint32_t sum = 0;
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum |= (v[u][e] & 0x7fff7fffu) + (0x8000 - NONE) * 0x10001u;
+                if (!(sum & 0x80008000u)) continue;
+                // rows lo..hi - 1 see the key (the last one again, where there are fewer)
+                const int rel = (int)min(key0 + u * by, (int64_t)to - 1) - old;
+                const int lo = min(max(rel <= 0 ? 0 : rel * G - first, 0), 16);
+                const int hi = !a.window || rel + a.window >= n ? 16 : min(max(max(rel + a.window, 0) * G - first, 0), 16);
+                const uint32_t rows = (1u << max(hi, lo)) - (1u << lo);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const uint32_t x = v[u][e >> 1] >> 16 * (e & 1) & 0xffff, y = x & 0x7fff;
+                    if (y == NONE) inf[e] |= rows << (x == y ? 0 : 16);
+                    if (y > NONE) inf[e] |= rows * 0x10001u;
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (inf[e]) atomicOr(&s_inf[8 * piece + e], inf[e]);
+    }
     __syncthreads();
     auto store_out = [&](int r, int d, f32x4 y) {
         const int64_t tok = (int64_t)row0 + (first + r) / G;
@@ -665,18 +738,11 @@ void kq_attn_kernel(const AttnArg a) {
 #pragma unroll
         for (int i = 1; i < NW; i++) y += *reinterpret_cast<const f32x4*>(ol + (i * 16 + r) * OS + d);
         if (ES == 2 && pass) {
-            // values that are no numbers, for the rows that see them
-            const int last = len - n + (first + r) / G, end = min(last + 1, k1);
-#pragma unroll 1
-            for (int key = max(k0, a.window ? last + 1 - a.window : 0); key < end; key++) {
-                const int page = table[key / a.page];
-                if ((uint32_t)page >= (uint32_t)a.n_pages) continue;
-                const u32x2 u = *reinterpret_cast<const u32x2*>(vh + page * a.page_b + (int64_t)(key % a.page) * a.tok_b + 2 * d);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float v = value<TYPE>(u[i >> 1] >> 16 * (i & 1));
-                    y[i] += __builtin_isfinite(v) ? 0.0f : v;
-                }
+            for (int i = 0; i < 4; i++) {
+                const uint32_t x = s_inf[d + i] >> r;
+                if (x & 1) y[i] += INFINITY;
+                if (x & 0x10000) y[i] -= INFINITY;
             }
         }
         const float2 all = s_all[r];

@@ -722,3 +722,38 @@ def test_hidden_values_do_not_cost_small_ones_bits(n_q, D, page, bad):
     # tokens 44.. of 50 and 395.. of 400; the windows start at 0 and 296..300
     skip = {(0, i) for i in range(2, 6)} | {(1, i) for i in (0, 1, 2, 3, 4) if i >= 2 or 296 + i <= 299}
     both(c, skip=skip if not bad == 3e38 else ())
+
+
+@pytest.mark.parametrize("t", [K.TYPE_F16, K.TYPE_BF16])
+@pytest.mark.parametrize("n_q,n_kv,D,page,T,window", [(4, 2, 128, 16, 4, 0), (24, 2, 256, 16, 5, 90), (15, 3, 80, 7, 3, 40),
+                                                      (2, 2, 64, 32, 1, 0), (33, 1, 72, 5, 9, 500), (6, 1, 248, 48, 7, 1)])
+def test_infinities_and_nan_anywhere(t, n_q, n_kv, D, page, T, window):
+    """Values that are no numbers in places far apart: those that a token sees give an infinity, or NaN of NaN or of
+    both signs, in their place of the row; the others are within the bound."""
+    lens = [T, 33 + T, 260, 5000]
+    c = Case(34, t, lens, [T] * 4, n_q, n_kv, D, page, window=window)
+    g = np.random.default_rng(35)
+    for s, n in enumerate(lens):
+        x = c.rows[s].float()
+        for e in range(12):
+            x[1, g.integers(n_kv), g.choice([0, n // 3, n - 1, n - 1 - g.integers(T), g.integers(n)]), g.integers(D)] = float(
+                g.choice(["inf", "-inf", "nan"]))
+        c.put(s, x)
+    special = [r[1].clone() for r in c.rows]
+    for r in c.rows:
+        r[1] = torch.nan_to_num(r[1], 0.0, 0.0, 0.0)
+    for listed in (False, True):
+        out = c.run(listed)
+        for s, n in enumerate(lens):
+            for i in range(T):
+                keys, r = torch.from_numpy(c.seen(s, i)).cuda(), int(c.start[s]) + i
+                v = special[s][:, keys]
+                y = torch.where(torch.isfinite(v), torch.zeros_like(v), v).sum(1)         # inf - inf and NaN: NaN
+                y = y.repeat_interleave(n_q // n_kv, 0).reshape(-1)
+                got, odd = out[r, :n_q * D], y != 0
+                assert torch.equal(torch.nan_to_num(got[odd].double(), 1e300), torch.nan_to_num(y[odd], 1e300)), (s, i)
+                # (in the others the sums of finite values: here those take the places of these as well)
+                q = c.q[r, :n_q * D].double().view(n_kv, n_q // n_kv, D) * float(np.float32(c.scale))
+                x = torch.matmul(q, c.rows[s][0][:, keys].transpose(1, 2).contiguous())
+                got[odd] = torch.matmul(torch.softmax(x, -1), c.rows[s][1][:, keys]).reshape(-1)[odd].float()
+        c.check(out)
