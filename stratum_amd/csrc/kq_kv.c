@@ -60,12 +60,12 @@ static int shape_check(const kq_attn_shape* s, const char* who) {
     return 0;
 }
 
-static int sizes(const kq_attn_shape* s, const char* who, kqk_attn_sizes* z) {
+static int sizes(const kq_attn_shape* s, int listed, const char* who, kqk_attn_sizes* z) {
     int n_cu;
     if (kq_device(&n_cu)) return -1;
     kqk_attn_plan(s, n_cu, z);
     /* a launch's lanes are counted in 32 bits */
-    if ((int64_t)z->cap * s->n_kv * z->blocks > 1 << 22)
+    if ((int64_t)(listed ? z->cap : s->S) * s->n_kv * z->blocks > 1 << 22)
         return kq_fail("%s: %d sequences x %d heads x %d rows are too many for one call", who, s->S,
                        s->n_kv, s->T * (s->n_q / s->n_kv));
     return 0;
@@ -79,7 +79,7 @@ static int64_t list_bytes(const kqk_attn_sizes* z) {
 
 int64_t kq_kv_list_bytes(const kq_attn_shape* s) {
     kqk_attn_sizes z;
-    if (shape_check(s, "kq_kv_list_bytes") || sizes(s, "kq_kv_list_bytes", &z)) return -1;
+    if (shape_check(s, "kq_kv_list_bytes") || sizes(s, 1, "kq_kv_list_bytes", &z)) return -1;
     return list_bytes(&z);
 }
 
@@ -114,7 +114,7 @@ int kq_kv_plan_dev(const kq_kv_plan* in, kq_stream stream) {
     if (p.list) {
         if (shape_check(&p.shape, who)) return -1;
         if (p.shape.S != p.S) return kq_fail("%s: S=%d, shape of S=%d", who, p.S, p.shape.S);
-        if (sizes(&p.shape, who, &z)) return -1;
+        if (sizes(&p.shape, 1, who, &z)) return -1;
         if (misaligned(p.list, 256) || p.list_bytes < list_bytes(&z))
             return kq_fail("%s: list of %lld bytes, 256-byte aligned, needed", who, (long long)list_bytes(&z));
     }
@@ -162,7 +162,7 @@ int64_t kq_paged_attn_workspace_bytes(const kq_attn_shape* s) {
     static const char who[] = "kq_paged_attn_workspace_bytes";
     kqk_attn_sizes z;
     int n_cu;
-    if (shape_check(s, who) || sizes(s, who, &z) || kq_device(&n_cu)) return -1;
+    if (shape_check(s, who) || sizes(s, 1, who, &z) || kq_device(&n_cu)) return -1;
     return kqk_attn_workspace(s, n_cu);
 }
 
@@ -190,7 +190,7 @@ int kq_paged_attn_dev(const kq_paged_attn* in, void* work, int64_t work_bytes, k
     if (!a.out_stride) a.out_stride = n;
     if (a.q_stride < n || a.out_stride < n || (a.q_stride | a.out_stride) % 4)
         return kq_fail("%s: row strides %lld, %lld", who, (long long)a.q_stride, (long long)a.out_stride);
-    if (sizes(&a.shape, who, &z) || kq_device(&n_cu)) return -1;
+    if (sizes(&a.shape, a.list != NULL, who, &z) || kq_device(&n_cu)) return -1;
     if (a.list) {
         if (misaligned(a.list, 256) || a.list_bytes < list_bytes(&z))
             return kq_fail("%s: list of %lld bytes, 256-byte aligned, needed", who, (long long)list_bytes(&z));

@@ -757,3 +757,14 @@ def test_infinities_and_nan_anywhere(t, n_q, n_kv, D, page, T, window):
                 x = torch.matmul(q, c.rows[s][0][:, keys].transpose(1, 2).contiguous())
                 got[odd] = torch.matmul(torch.softmax(x, -1), c.rows[s][1][:, keys]).reshape(-1)[odd].float()
         c.check(out)
+
+
+def test_as_many_blocks_of_rows_as_a_launch_takes():
+    """2^22 workgroups are a call without a list; the list of as many sequences would have one item more."""
+    c = Case(37, K.TYPE_F16, np.arange(1024) % 40 + 1, np.ones(1024, int), 1024, 1, 8, T=64)
+    c.check(c.run(False))
+    with pytest.raises(RuntimeError, match="too many"):
+        K.kv_list_bytes(c.shape())
+    c.T, c.S = 64, 1025
+    with pytest.raises(RuntimeError, match="too many"):
+        c.run(False)
