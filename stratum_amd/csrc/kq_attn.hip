@@ -105,8 +105,8 @@ __device__ __forceinline__ void split(float a, float b, uint32_t* o) {
     }
 }
 
-// Bytes e and e + 1 of x, and byte e of x and of y, as binary16 integers: 1024 + 128
-// + the value by its bits, less 1152.
+// Two int8 values, in the lower bytes of a register's halves, as binary16 numbers: 1024
+// + 128 + the value by its bits, less 1152.
 __device__ __forceinline__ uint32_t halves(uint32_t u) {
     const f16x2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
     return __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, u ^ 0x64806480u) - off);
@@ -946,7 +946,8 @@ int kqk_launch_attn(const kq_paged_attn* p, const kqk_attn_sizes* z, void* work,
     const Kernel k = c.type == KQ_TYPE_F16    ? pick<KQ_TYPE_F16>(s.D, tiled)
                      : c.type == KQ_TYPE_BF16 ? pick<KQ_TYPE_BF16>(s.D, tiled)
                                               : pick<KQ_TYPE_I8>(s.D, tiled);
-    // (below 2^23 workgroups, n_kv and blocks at most 2^10 and 2^8: exact)
+    // A number x divided by d as x ceil(2^40 / d) 2^-40 is exact where x d < 2^40: here d = n_kv is at most
+    // 2^10, or 8 blocks at most 2^15 (64 tokens of 1024 heads are 2^12 blocks), and x below 2^23.
     a.blocks = z->blocks;
     a.kv_div = (((uint64_t)1 << 40) + s.n_kv - 1) / s.n_kv;
     a.blocks_div = (((uint64_t)1 << 40) + 8 * z->blocks - 1) / (8 * z->blocks);

@@ -768,3 +768,10 @@ def test_as_many_blocks_of_rows_as_a_launch_takes():
     c.T, c.S = 64, 1025
     with pytest.raises(RuntimeError, match="too many"):
         c.run(False)
+
+
+@pytest.mark.parametrize("t,S,T,n_q,n_kv,D,page", [(K.TYPE_F16, 2, 64, 1024, 1, 8, 16), (K.TYPE_I8, 3, 64, 300, 1, 64, 16),
+                                                   (K.TYPE_BF16, 2, 50, 700, 2, 16, 7)])
+def test_thousands_of_rows_of_one_head(t, S, T, n_q, n_kv, D, page):
+    """64 new tokens of many heads over one head of keys: up to 4096 blocks of rows."""
+    both(Case(36, t, [90, 700, 64][:S], [T, T - 1, 1][:S], n_q, n_kv, D, page, T=T))
