@@ -176,7 +176,8 @@ int kq_paged_attn_dev(const kq_paged_attn* in, void* work, int64_t work_bytes, k
     if (a.shape.n_kv != a.cache.n_kv || a.shape.D != a.cache.D)
         return kq_fail("%s: shape of %d heads of %d, cache of %d of %d", who, a.shape.n_kv, a.shape.D,
                        a.cache.n_kv, a.cache.D);
-    if (!isfinite(a.scale)) return kq_fail("%s: scale %g", who, (double)a.scale);
+    /* (the kernel's scores are powers of two) */
+    if (!isfinite((float)(a.scale * 1.4426950408889634))) return kq_fail("%s: scale %g", who, (double)a.scale);
     if (a.N < 1) return kq_fail("%s: N=%d", who, a.N);
     if (!a.q || !a.out || !a.table || !a.lens) return kq_fail("%s: NULL pointer", who);
     if (a.q == a.out) return kq_fail("%s: q and out are one buffer", who);

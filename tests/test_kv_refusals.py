@@ -136,3 +136,8 @@ def attn(**kw):
 ])
 def test_attn_refuses(kw, word):
     refused(K.lib().kq_paged_attn_dev(ctypes.byref(attn(**kw)), None, 0, None), word)
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3e38, 3.4028234e38])
+def test_attn_refuses_scales_that_pass_the_range_times_log2_e(scale):
+    refused(K.lib().kq_paged_attn_dev(ctypes.byref(attn(scale=scale)), None, 0, None), "scale")
