@@ -17,6 +17,8 @@ the base they are taken from, so it is no less than the base's) and of the large
 scale go missing at most, times a value each: L 2^-34 max|v| in all.  Queries likewise: two
 binary16 numbers of the row times a power of two that puts its largest from 2^13 on, so
 2^-25 / 2^13 = 2^-38 of that one, times sum |scale k_d|, is added to e."""
+import copy
+
 import numpy as np
 import pytest
 
@@ -775,3 +777,16 @@ def test_as_many_blocks_of_rows_as_a_launch_takes():
 def test_thousands_of_rows_of_one_head(t, S, T, n_q, n_kv, D, page):
     """64 new tokens of many heads over one head of keys: up to 4096 blocks of rows."""
     both(Case(36, t, [90, 700, 64][:S], [T, T - 1, 1][:S], n_q, n_kv, D, page, T=T))
+
+
+def test_a_sequence_alone_and_in_a_batch():
+    """The same keys and queries, whose shares are others alone than in a batch: within the bound both ways."""
+    c = Case(38, K.TYPE_F16, [9000, 300, 40], [1, 2, 1], 24, 4, 256)
+    c.check(c.run(True))
+    for s in range(3):
+        one, r = copy.copy(c), int(c.start[s])
+        del one.d
+        one.S, one.N, one.rows = 1, int(c.new[s]), c.rows[s:s + 1]
+        one.lens, one.new, one.table = c.lens[s:s + 1], c.new[s:s + 1], c.table[s:s + 1]
+        one.start, one.q = np.array([0, c.new[s]]), c.q[r:r + one.N].clone()
+        both(one)
