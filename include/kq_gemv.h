@@ -638,9 +638,9 @@ int kq_spec_verify_dev(const kq_spec_verify* v, void* work, int64_t work_bytes, 
  * D values each (D % 8 == 0, at most 256; n_pages * page < 2^31).  The row of
  * token t of page p for head h starts p * page_stride + h * head_stride +
  * t * token_stride elements behind k and v (0: D, page rows, n_kv heads; a multiple
- * of 8 otherwise, between tokens at most KQ_KV_MAX_TOKEN_STRIDE), which are 16-byte aligned.  KQ_TYPE_F16, KQ_TYPE_BF16, or
- * KQ_TYPE_I8: a row is int8 times its scale, k_scale and v_scale being n_pages x
- * n_kv x page binary32 values. */
+ * of 8 otherwise, between tokens at most KQ_KV_MAX_TOKEN_STRIDE), which are 16-byte
+ * aligned.  KQ_TYPE_F16, KQ_TYPE_BF16, or KQ_TYPE_I8: a row is int8 times its scale,
+ * k_scale and v_scale being n_pages x n_kv x page binary32 values. */
 #define KQ_TYPE_I8      24      /* of caches only */
 #define KQ_KV_MAX_D     256
 #define KQ_KV_MAX_TOKEN_STRIDE (1 << 24)
@@ -681,8 +681,10 @@ typedef struct kq_attn_shape {
  *   pos, slot   of each new token: its position, and its slot (-1 where pages are
  *               missing, or its page is not in 0..n_pages-1); N entries at most
  *   n_short     one value: the sequences whose pages are missing
- * Any output may be NULL; they do not overlap, nor lie in the inputs but as said.  table NULL: no pages are dealt with (free_pages, n_free,
- * held, held_out, n_free_out, slot and n_short are NULL then).  Lengths below 0
+ * Any output may be NULL; they do not overlap, nor lie in the inputs but as said
+ * (with held_out over held or n_free_out over n_free, more than 4096 new tokens take
+ * one workgroup, otherwise several).  table NULL: no pages are dealt with (free_pages,
+ * n_free, held, held_out, n_free_out, slot and n_short are NULL then).  Lengths below 0
  * count as 0, above 2^30 - 1 as that; the new tokens are fewer than 2^31.
  * list (NULL: none, shape unused): kq_kv_list_bytes of device memory, 256-byte
  * aligned, filled for kq_paged_attn_dev calls of this shape (whose S is the
@@ -752,13 +754,21 @@ int kq_kv_store_dev(const kq_kv_store* a, kq_stream stream);
  *   out = sum_j p_j v_j,  p = softmax over the keys j that the token sees of scale q . k_j
  * q and out: N rows of n_q heads of D binary32 values, q_stride and out_stride
  * elements apart (0: n_q * D; multiples of 4), 16-byte aligned; they do not overlap.
- * table: S rows of table_stride page numbers.  Keys past the table, past 2^31 - 2^16, and keys
- * on pages outside 0..n_pages-1, are not seen; a token that sees no key gets zeros.
- * What a token does not see does not reach it, whatever it holds.  Sequences of more
- * than T new tokens, rows of none and rows outside 0..N-1 are left as they are.
- * Queries and weights enter the products with 22 bits or more (of values below 2^-17 of
- * a head's largest query, or of a row's largest weight, fewer), keys and values as
- * they are; sums are binary32.
+ * scale is finite, also times log2 e.
+ * table: S rows of table_stride page numbers.  Keys past the table, past 2^31 - 2^16,
+ * and keys on pages outside 0..n_pages-1, are not seen; a token that sees no key, or
+ * only keys of scores -inf, gets zeros.  What a token does not see does not reach it,
+ * whatever it holds.  Sequences of more than T new tokens, rows of none and rows
+ * outside 0..N-1 are left as they are.
+ * Keys and values enter the products as they are, sums are binary32.  Queries and
+ * weights have 24 bits where the cache is bfloat16, 22 where it is binary16 or int8:
+ * queries down to 2^-16 of a head's largest, weights down to 2^-12 of a row's largest,
+ * with int8 weights times their values' scales down to 2^-13 of a row's largest of
+ * these.  (What is smaller is off by up to 2^-38, 2^-34 or 2^-35 of the largest.)
+ * Weights below 2^-120 of a row's largest count as 0.  Where bfloat16 values are so
+ * large that a row's sums pass 2^96, weights below 2^-86 do, and values below 2^-62
+ * lose bits.  Infinities and NaN among a 16-bit cache's values, hidden ones as well,
+ * cost their sequence a second reading of its keys.
  * list: as kq_kv_plan_dev wrote it for this shape and these lengths, NULL: a
  * workgroup takes a whole sequence (short ones; with few and long ones most of the
  * device idles).  Calls that share a list must not overlap in time, nor calls that

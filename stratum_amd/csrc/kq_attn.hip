@@ -14,18 +14,19 @@
 //   O^T = V^T P^T a lane loads 8 (or 4) neighbouring values of those 8 keys; an
 //                 operand for value t of each is one byte permutation a register
 // so that keys and values go from memory to registers and matrix cores without LDS.
-// Queries and weights are binary32: as two binary16 numbers (22 bits, queries with a
-// power of two a row, weights times 2^9) where keys are binary16 or int8, as three
-// bfloat16 numbers (24 bits) where they are bfloat16.  Matrix work is far from full,
-// so that the further products are free.
+// Queries and weights are rounded to two binary16 numbers (22 bits: queries with a power
+// of two a row, weights times 2^9, with int8 weights times their values' scales and a
+// power of two a row) where keys are binary16 or int8, to three bfloat16 numbers (24
+// bits) where they are bfloat16.  Matrix work is far from full, so that the further
+// products are free.
 // Long caches are bound by memory (16 / 8 heads of 128, binary16, 16 sequences of 8192:
 // 101 us, 5.3 TB/s; 24 / 4 of 256, bfloat16, 64 of 8192: 375 us, 5.7), short ones by a
 // chain of latencies: item, pages, keys, a step, the join of waves (one sequence of 32:
-// 5.8 us, heads of 256 7.8), and 4 to 5 us for a join of items.  Two tiles of 16 rows a
+// 5.9 us, heads of 256 7.8), and 4 to 5 us for a join of items.  Two tiles of 16 rows a
 // wave share a step's operands but take all of a SIMD's registers: 8 sequences of 8 new
-// tokens, 24 / 4 heads of 256, of 32 / 1000 to 4000 / 4096 keys took 14 / 64 / 57 us for
-// 9 / 50 / 71 of one; 8 waves a workgroup 96 us for 82 with 200 sequences of 500 keys, and
-// no less with few.
+// tokens, 24 / 4 heads of 256, of 32 / 1000 to 4000 / 4096 keys took 14 / 64 / 57 us, which
+// one takes in 9.5 / 43 / 56 to 60 (with 32 keys a step; 9 / 50 / 71 before).  8 waves a
+// workgroup took 96 us for 82 with 200 sequences of 500 keys, and no less with few.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>

@@ -14,11 +14,11 @@ namespace {
 
 // ------------------------------------------------------------------ plan
 //
-// One workgroup: a sequence a lane (more in rounds), sums over them by lanes' shifts,
-// then new pages, new tokens and the attention's items over all lanes, each of which
-// finds its sequence by bisection in LDS.  A chain of latencies bounds it: lengths,
-// sums, the pages that slots lie on (one sequence 5.0 us, 256 of up to four new tokens 8.6,
-// with a list; 1.7 of it the launch).
+// One workgroup, or up to 16 for the slots of more than 4096 new tokens: a sequence a
+// lane (more in rounds), sums over them by lanes' shifts, then new pages, new tokens and the
+// attention's items over all lanes, each of which finds its sequence by bisection in LDS.
+// A chain of latencies bounds it: lengths, sums, the pages that slots lie on (one
+// sequence 5.0 us, 256 of up to four new tokens 8.6, with a list; 1.7 of it the launch).
 
 constexpr int PT = 1024;            // lanes at most
 constexpr int MOST = (1 << 30) - 1; // of a length
@@ -299,9 +299,9 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 // One workgroup a token (several, where tokens are few): its angles' cosines and sines
 // once in LDS, then its heads' rows, `lanes` lanes of four values each, U rows a lane
 // in flight.  The partners of a rotation are read a second time, from the cache.
-// Memory bounds many tokens (4096 of 16 + 2 x 8 heads of 128 to bfloat16: 26 us, 4.5 TB/s,
-// binary64 products about half of the instructions' time), one launch few (one of 24 + 2 x
-// 4 heads of 256: 3.9 us).
+// Memory bounds many tokens (4096 of 16 + 2 x 8 heads of 128 to bfloat16: 26 us, 4.5 TB/s;
+// a SIMD's binary64 products, sums and conversions are 1152 of 7400 instructions, at 8 clocks a sixth of
+// the time), one launch few (one of 24 + 2 x 4 heads of 256: 3.9 us).
 constexpr int U = 4;
 
 template <int TYPE>
@@ -414,7 +414,8 @@ extern "C" int kqk_launch_kv_plan(const kq_kv_plan* p, const kqk_attn_sizes* z, 
     }
     // A lane for each sequence, and for each new token that there may be; of many
     // tokens (14119: one workgroup 17 us, this 8.6) several workgroups, each of
-    // which takes the sums for itself, unless the first writes over what they read.
+    // which takes the sums for itself, unless the first writes over what they read
+    // (`held` and n_free in place: 17 us).
     int lanes = p->S > p->N ? p->S : p->N;
     lanes = lanes > PT ? PT : (lanes + 63) / 64 * 64;
     const bool apart = (!p->held_out || p->held_out != p->held) && (!p->n_free_out || p->n_free_out != p->n_free);
