@@ -765,8 +765,8 @@ int kq_kv_store_dev(const kq_kv_store* a, kq_stream stream);
  * queries down to 2^-16 of a head's largest, weights down to 2^-12 of a row's largest,
  * with int8 weights times their values' scales down to 2^-13 of a row's largest of
  * these.  (What is smaller is off by up to 2^-38, 2^-34 or 2^-35 of the largest.)
- * Weights below 2^-120 of a row's largest count as 0.  Where bfloat16 values are so
- * large that a row's sums pass 2^96, weights below 2^-86 do, and values below 2^-62
+ * Weights below 2^-120 of a row's largest may count as 0.  Where bfloat16 values are
+ * so large that a row's sums pass 2^96, weights below 2^-86 may, and values below 2^-62
  * lose bits.  Infinities and NaN among a 16-bit cache's values, hidden ones as well,
  * cost their sequence a second reading of its keys.
  * list: as kq_kv_plan_dev wrote it for this shape and these lengths, NULL: a
